@@ -41,6 +41,16 @@ int bmk_launch_argmax(const bmk_launch_t* a);
 int bmk_launch_matmul_f32(const bmk_launch_t* a);
 int bmk_launch_matmul_bf16(const bmk_launch_t* a);
 int bmk_launch_matmul_fp16(const bmk_launch_t* a);
+int bmk_launch_quantize_rows_i8(const bmk_launch_t* a);
+int bmk_launch_quantize_rows_i8_bf16(const bmk_launch_t* a);
+int bmk_launch_dequantize_rows_i8(const bmk_launch_t* a);
+int bmk_launch_dequantize_rows_i8_bf16(const bmk_launch_t* a);
+int bmk_launch_rmsnorm_i8(const bmk_launch_t* a);
+int bmk_launch_rmsnorm_i8_bf16(const bmk_launch_t* a);
+int bmk_launch_swiglu_i8(const bmk_launch_t* a);
+int bmk_launch_swiglu_i8_bf16(const bmk_launch_t* a);
+int bmk_launch_matmul_i8(const bmk_launch_t* a);
+int bmk_launch_matmul_i8_bf16(const bmk_launch_t* a);
 }
 
 #define B(i) (1u << (i))
@@ -140,5 +150,20 @@ extern "C" const bmk_desc_t bmk_table[] = {
     {"matmul_forward_fp16_tiled", 5, B(4), B(3), bmk_launch_matmul_fp16, 0},
     /* new: greedy pick on the device (reference tools/run.c:56-60); {values, out int, params{n}} */
     {"argmax_f32", 3, B(2), B(1), bmk_launch_argmax, 0},
+    /* new: the 8-bit integer path (codes with one scale a row); _bf16: bf16 source, branch, products or output */
+    /* {src, codes, scale, params{M,C,lds,ldq}} and back {codes, scale, dst, params{M,C,ldq,ldd}} */
+    {"quantize_rows_i8", 4, B(3), B(1) | B(2), bmk_launch_quantize_rows_i8, 0},
+    {"quantize_rows_i8_bf16", 4, B(3), B(1) | B(2), bmk_launch_quantize_rows_i8_bf16, 0},
+    {"dequantize_rows_i8", 4, B(3), B(2), bmk_launch_dequantize_rows_i8, 0},
+    {"dequantize_rows_i8_bf16", 4, B(3), B(2), bmk_launch_dequantize_rows_i8_bf16, 0},
+    /* {x, residual, weight, sum, codes, scale, params{N,C,ldq,has_residual}, eps} */
+    {"rmsnorm_forward_i8", 8, B(6) | B(7), B(3) | B(4) | B(5), bmk_launch_rmsnorm_i8, 0},
+    {"rmsnorm_forward_i8_bf16", 8, B(6) | B(7), B(3) | B(4) | B(5), bmk_launch_rmsnorm_i8_bf16, 0},
+    /* {gate, up, codes, scale, params{N,H,ld,ldq}} */
+    {"swiglu_forward_i8", 5, B(4), B(2) | B(3), bmk_launch_swiglu_i8, 0},
+    {"swiglu_forward_i8_bf16", 5, B(4), B(2) | B(3), bmk_launch_swiglu_i8_bf16, 0},
+    /* {codes, scale, weight codes, weight scale, bias, out, params{BT,C,OC,has_bias,lda,ldw,ldo}} */
+    {"matmul_forward_i8", 7, B(6), B(5), bmk_launch_matmul_i8, 0},
+    {"matmul_forward_i8_bf16", 7, B(6), B(5), bmk_launch_matmul_i8_bf16, 0},
     {nullptr, 0, 0, 0, nullptr, 0},
 };

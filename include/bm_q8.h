@@ -42,6 +42,44 @@
  *                        (bf16 32x32x16 MFMAs, workgroups x 4 waves x iters x 8 per launch;
  *                        mode 0 register operands, 1 operands read from LDS as the prefill
  *                        GEMM's 2x2 wave tile reads them; the matrix-core ceilings)
+ *
+ * The 8-bit integer path: activations with one scale a token, weights with one
+ * scale an output channel, products on the int8 matrix cores.  A matrix of
+ * codes is int8 [rows][ld], rows on 16-byte boundaries (ld a multiple of 16,
+ * the offset too), each row, the last one included, C codes rounded up to
+ * whole 16-byte groups; the kernels that make codes write zeros behind the
+ * C-th, up to that group's end, and nothing past it.  Row p of C values has
+ * top = max |p|, inv = 127 / top, codes round-to-even(p * inv) in -127 .. 127
+ * and scale top / 127, each step in fp32.  A row of zeros, or whose top is
+ * under 3.8e-37, has zero codes and the scale 0; a row that holds a NaN or an
+ * infinity has zero codes and the scale NaN.  Row counts may be 0 (nothing is
+ * done); rows past them are left as they are.  Inputs and outputs may not
+ * overlap but where stated.  A _bf16 name takes or gives bf16 where "T" stands,
+ * the plain name f32.
+ *   "quantize_rows_i8", "quantize_rows_i8_bf16"
+ *                        {src T [M][lds], codes [M][ldq], scale f32 [M],
+ *                         params int{M, C, lds, ldq}}
+ *   "dequantize_rows_i8", "dequantize_rows_i8_bf16"
+ *                        {codes [M][ldq], scale f32 [M], dst T [M][ldd],
+ *                         params int{M, C, ldq, ldd}}: code * scale (bf16: rounded to nearest even)
+ *   "rmsnorm_forward_i8", "rmsnorm_forward_i8_bf16"
+ *                        {x T [N][C], residual f32 [N][C], weight f32 [C], sum f32 [N][C],
+ *                         codes [N][ldq], scale f32 [N], params int{N, C, ldq, has_residual},
+ *                         eps f32}: sum = x + residual, p = sum * weight (fp32 products), the codes
+ *                         and scale of p / sqrt(mean sum^2 + eps); sum may be the residual's (or an
+ *                         f32 x's) own buffer.  With has_residual 0, x takes the sum's place and
+ *                         buffers 1 and 3 are not touched (bind any)
+ *   "swiglu_forward_i8", "swiglu_forward_i8_bf16"
+ *                        {gate T [N][ld], up T [N][ld], codes [N][ldq], scale f32 [N],
+ *                         params int{N, H, ld, ldq}}: p = gate / (1 + exp(-gate)) * up; a stacked
+ *                         gate|up product goes in as one buffer at two offsets, ld = 2 H
+ *   "matmul_forward_i8", "matmul_forward_i8_bf16"
+ *                        {codes [BT][lda], scale f32 [BT], weight codes [OC][ldw], scale f32 [OC],
+ *                         bias f32 [OC], out T [BT][ldo],
+ *                         params int{BT, C, OC, has_bias, lda, ldw, ldo}}: the sum over C of the code
+ *                         products, exact in 32 bits (C below 131072; codes may be -128), times the
+ *                         row's scale, times the channel's, plus the bias (has_bias 0: bind any),
+ *                         each step in fp32; what lies in a row behind its C codes does not matter
  */
 #ifndef BM_Q8_H
 #define BM_Q8_H
