@@ -3,9 +3,24 @@
  * i8_gemm.hip — the product of 8-bit codes (matmul_forward_i8, _bf16) on gfx950 int8 MFMA:
  *   out[m][n] = (sum_k a[m][k] * w[n][k]) * sa[m] * sw[n] + bias[n]
  * The sum is exact in 32-bit integers (fewer than 2^17 columns: 2^17 products
- * of at most 2^14 would pass 2^31); it is converted once, multiplied by the
- * row's scale, then by the column's (each rounding to fp32), the bias added, and
- * for bf16 outputs rounded once more.
+ * of at most 2^14 would pass 2^31), so neither tiles nor the split of a sum
+ * change a result.  It is converted once, multiplied by the row's scale, then
+ * by the column's (each rounding to fp32), the bias added, and for bf16
+ * outputs rounded once more.
+ *
+ * All forms use v_mfma_i32_16x16x64_i8, with the weights as its first operand:
+ * a lane then holds four neighbouring outputs of one row.  The 32 x 32 x 32 form
+ * is slower on this part (registers only, all CUs, codes of a normal
+ * distribution: 2.6 against 4.1 POP/s).
+ *   k_i8_few   up to 16 rows: weights straight into registers, the sum split over four waves (HBM, or a launch's latency)
+ *   k_i8_tile  tiles of 32 x 32 to 128 x 128 through LDS, four waves
+ *   k_i8_pair  256 x 256, eight waves in two groups that take turns at the matrix cores and at LDS
+ * Operands go to LDS by global_load_lds, which writes 16 bytes a lane at
+ * consecutive addresses, so a row's 16-byte groups are permuted on the source
+ * side (group_key), such that the 16 rows of a fragment lie in different banks.
+ * Rows past M or OC repeat the last one and groups past C the last one; the
+ * first feed nothing stored, and the tokens' codes past C are zeroed in
+ * registers (what the weights hold there is then multiplied by zero).
  */
 #include "i8_common.h"
 
@@ -14,9 +29,18 @@ namespace {
 using namespace bmk;
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(1))) void gvoid;
+typedef __attribute__((address_space(3))) void lvoid;
 
 constexpr int MAX_C = (1 << 17) - 1;
+constexpr int XCDS = 8;
+constexpr int CUS = 256;
+constexpr int MAX_GRID_X = 1 << 20;
 
 struct GemmArgs {
     const unsigned char* a;
@@ -26,19 +50,28 @@ struct GemmArgs {
     const float* bias;
     void* out;
     size_t lda, ldw, ldo;
-    int M, C, OC, tiles_n;
+    int M, C, OC, tiles_m, tiles_n;
 };
 
-template <bool BF16>
-__device__ __forceinline__ void store1(const GemmArgs& g, int m, int n, int acc) {
-    float v = (float)acc * g.sa[m] * g.sw[n];
-    if (g.bias) v += g.bias[n];
-    const size_t at = (size_t)m * g.ldo + n;
-    if (BF16) ((unsigned short*)g.out)[at] = __builtin_bit_cast(unsigned short, (__bf16)v);
-    else ((float*)g.out)[at] = v;
+__device__ __forceinline__ int workgroup() { return (int)(blockIdx.y * gridDim.x + blockIdx.x); }
+
+/* This workgroup's tile, or false for one past the last.  Workgroups are dealt
+ * to the XCDs in turn, and every XCD takes a run of neighbouring tiles (four
+ * tile rows wide), which share operands in its L2. */
+__device__ __forceinline__ bool tile_of(const GemmArgs& g, int& tm, int& tn) {
+    const int total = g.tiles_m * g.tiles_n;
+    int b = workgroup();
+    if (b >= total) return false;
+    const int per = total / XCDS, x = b % XCDS;
+    b = x * per + min(x, total - per * XCDS) + b / XCDS;
+    constexpr int GM = 4;
+    const int span = GM * g.tiles_n, grp = b / span, in = b - grp * span, gm = min(GM, g.tiles_m - grp * GM);
+    tm = grp * GM + in % gm;
+    tn = in / gm;
+    return true;
 }
 
-/* the first n bytes (1 .. 15) of a 16-byte group, zeros behind them */
+/* the first n bytes of a 16-byte group (all from n = 16 on), zeros behind them */
 __device__ __forceinline__ i32x4 head_bytes(i32x4 v, int n) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -49,46 +82,475 @@ __device__ __forceinline__ i32x4 head_bytes(i32x4 v, int n) {
     return v;
 }
 
-constexpr int NT = 256;
+__device__ __forceinline__ unsigned int pk(float lo, float hi) {
+    return __builtin_bit_cast(unsigned int, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
+}
 
-/* 64 x 64 outputs a workgroup, four waves of 32 x 32, 64 columns a step through LDS. */
-template <bool BF16>
-__global__ __launch_bounds__(NT) void k_i8_gemm(GemmArgs g) {
-    constexpr int LD = 80; /* LDS row of 64 codes, padded against bank conflicts */
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2][64 * LD];
-    const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
-    const int tm = blockIdx.x / g.tiles_n, tn = blockIdx.x - tm * g.tiles_n;
-    const int m0 = tm * 64, n0 = tn * 64, wm = 32 * (wave & 1), wn = 32 * (wave >> 1);
-    const int r = t >> 2, c = 16 * (t & 3);
-    const unsigned char* ap = g.a + (size_t)min(m0 + r, g.M - 1) * g.lda;
-    const unsigned char* wp = g.w + (size_t)min(n0 + r, g.OC - 1) * g.ldw;
-    i32x16 acc;
+/* 16 or 8 bytes to an address on an output element's boundary */
+template <bool BF16, class T>
+__device__ __forceinline__ void store_vec(void* out, size_t at, T v) {
+    if (BF16) __builtin_memcpy(__builtin_assume_aligned((unsigned short*)out + at, 2), &v, sizeof v);
+    else __builtin_memcpy(__builtin_assume_aligned((float*)out + at, 4), &v, sizeof v);
+}
+
+/* Scales, bias and store of TM x TN 16 x 16 sums: lane l holds row l % 16,
+ * columns 4 (l / 16) .. + 3 of each.  Pairs of bf16 tiles swap 16-lane halves
+ * first, so that a lane stores 8 neighbours: 64 bytes a row and instruction. */
+template <int TM, int TN, bool BF16>
+__device__ __forceinline__ void store_tile(const GemmArgs& g, const i32x4 (&acc)[TM][TN], int m0, int n0) {
+    const int lane = threadIdx.x & 63, q = lane >> 4;
+    f32x4 sw[TN], bv[TN];
 #pragma unroll
-    for (int i = 0; i < 16; i++) acc[i] = 0;
-    for (int k = 0; k < g.C; k += 64) {
-        const int left = g.C - (k + c); /* codes of this thread's group that the row has; past them zeros */
-        i32x4 av = {0, 0, 0, 0}, wv = {0, 0, 0, 0};
-        if (left > 0) {
-            av = *(const i32x4*)(ap + k + c);
-            wv = *(const i32x4*)(wp + k + c);
-            if (left < 16) av = head_bytes(av, left);
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int n = min(n0 + 16 * j + 4 * q + r, g.OC - 1);
+            sw[j][r] = g.sw[n];
+            bv[j][r] = g.bias ? g.bias[n] : -0.0f; /* nothing to add: v + -0 is v for every v */
         }
-        __syncthreads();
-        *(i32x4*)&lds[0][r * LD + c] = av;
-        *(i32x4*)&lds[1][r * LD + c] = wv;
-        __syncthreads();
+    float sa[TM];
 #pragma unroll
-        for (int kk = 0; kk < 64; kk += 32) {
-            const int at = (lane & 31) * LD + kk + 16 * (lane >> 5);
-            acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(*(const i32x4*)&lds[0][wm * LD + at],
-                                                        *(const i32x4*)&lds[1][wn * LD + at], acc, 0, 0, 0);
+    for (int i = 0; i < TM; i++) sa[i] = g.sa[min(m0 + 16 * i + (lane & 15), g.M - 1)];
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+        const int m = m0 + 16 * i + (lane & 15);
+        const size_t row = (size_t)m * g.ldo;
+        f32x4 v[TN];
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[j][r] = (float)acc[i][j][r] * sa[i] * sw[j][r] + bv[j][r];
+        if (n0 + 16 * TN <= g.OC) {
+            if (BF16) {
+#pragma unroll
+                for (int j = 0; j + 1 < TN; j += 2) {
+                    const u32x2 x = __builtin_amdgcn_permlane16_swap(pk(v[j][0], v[j][1]), pk(v[j + 1][0], v[j + 1][1]),
+                                                                     false, false);
+                    const u32x2 y = __builtin_amdgcn_permlane16_swap(pk(v[j][2], v[j][3]), pk(v[j + 1][2], v[j + 1][3]),
+                                                                     false, false);
+                    if (m < g.M)
+                        store_vec<BF16>(g.out, row + n0 + 16 * (j + (q & 1)) + 8 * (q >> 1), u32x4{x[0], y[0], x[1], y[1]});
+                }
+                if (TN % 2 && m < g.M)
+                    store_vec<BF16>(g.out, row + n0 + 16 * (TN - 1) + 4 * q,
+                                    u32x2{pk(v[TN - 1][0], v[TN - 1][1]), pk(v[TN - 1][2], v[TN - 1][3])});
+            } else {
+#pragma unroll
+                for (int j = 0; j < TN; j++)
+                    if (m < g.M) store_vec<BF16>(g.out, row + n0 + 16 * j + 4 * q, v[j]);
+            }
+        } else if (m < g.M) {
+#pragma unroll
+            for (int j = 0; j < TN; j++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int n = n0 + 16 * j + 4 * q + r;
+                    if (n >= g.OC) continue;
+                    if (BF16) ((unsigned short*)g.out)[row + n] = __builtin_bit_cast(unsigned short, (__bf16)v[j][r]);
+                    else ((float*)g.out)[row + n] = v[j][r];
+                }
         }
     }
-    const int n = n0 + wn + (lane & 31);
+}
+
+template <int TM, int TN>
+__device__ __forceinline__ void clear(i32x4 (&acc)[TM][TN]) {
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int m = m0 + wm + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-        if (m < g.M && n < g.OC) store1<BF16>(g, m, n, acc[i]);
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++) acc[i][j] = i32x4{0, 0, 0, 0};
+}
+
+/* ------------------------------------------------------------------ */
+/* up to 16 rows */
+
+constexpr int FEW_KP = 4; /* waves along the sum */
+
+/* 16 * TN outputs a workgroup; wave p takes every fourth slice of 64 columns
+ * from p on, U slices' loads in flight, so that a workgroup reads 256
+ * neighbouring bytes of a row at once.  The partial sums meet in LDS.
+ * (One wave along the sum or sixteen instead of four: 2.8 and 2.4 against 2.4 us
+ * for 576 -> 1536, 5.2 and 3.5 against 3.4 for 2560 -> 960, one row each;
+ * 9.3 and 14.9 against 9.2 for 8 rows of 960 -> 49152.) */
+template <int TN, int U, bool BF16>
+__global__ __launch_bounds__(64 * FEW_KP) void k_i8_few(GemmArgs g) {
+    __shared__ __attribute__((aligned(16))) i32x4 part[FEW_KP * TN * 64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int tile = workgroup();
+    if (tile >= g.tiles_n) return;
+    const int n0 = tile * 16 * TN;
+    const int c = 16 * (lane >> 4), last = 16 * ((g.C - 1) >> 4), slices = (g.C + 63) >> 6;
+    const unsigned char* ap = g.a + (size_t)min(lane & 15, g.M - 1) * g.lda;
+    const unsigned char* wp[TN];
+#pragma unroll
+    for (int j = 0; j < TN; j++) wp[j] = g.w + (size_t)min(n0 + 16 * j + (lane & 15), g.OC - 1) * g.ldw;
+    i32x4 acc[1][TN];
+    clear(acc);
+    for (int s = wave; s < slices; s += FEW_KP * U) {
+        i32x4 a[U], w[U][TN];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int k = min(64 * (s + FEW_KP * u) + c, last);
+#pragma unroll
+            for (int j = 0; j < TN; j++) w[u][j] = *(const i32x4*)(wp[j] + k);
+            a[u] = *(const i32x4*)(ap + k);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int left = g.C - 64 * (s + FEW_KP * u) - c;
+            if (left < 16) a[u] = head_bytes(a[u], left);
+#pragma unroll
+            for (int j = 0; j < TN; j++)
+                acc[0][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][j], a[u], acc[0][j], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < TN; j++) part[(wave * TN + j) * 64 + lane] = acc[0][j];
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int p = 1; p < FEW_KP; p++) acc[0][j] += part[(p * TN + j) * 64 + lane];
+    store_tile<1, TN, BF16>(g, acc, 0, n0);
+}
+
+/* ------------------------------------------------------------------ */
+/* LDS stages */
+
+/* Of a row of BK / 16 groups, group c lies at place c ^ group_key(row).  A
+ * fragment's read takes, in each of its four passes of 16 lanes, rows r, r + 1,
+ * r + 2, r + 3 of two quads at group c and of the other two at c + 1; the keys
+ * put these 16 groups in 16 different places of 256 bytes (64 banks). */
+template <int BK>
+__device__ __forceinline__ int group_key(int row) {
+    static_assert(BK == 64 || BK == 128, "");
+    return BK == 64 ? (0x78 >> (2 * ((row >> 2) & 3))) & 3 : (row >> 1) & 7;
+}
+
+/* keeps memory accesses on their side; no instruction */
+__device__ __forceinline__ void fence() { asm volatile("" ::: "memory"); }
+
+/* waits until at most VM of this wave's loads are under way (and, with LDS, none of its LDS accesses) */
+template <int VM, bool LDS>
+__device__ __forceinline__ void wait_loads() {
+    static_assert(VM < 64, "six bits");
+    __builtin_amdgcn_s_waitcnt((LDS ? 0x070 : 0xF70) | (VM & 15) | ((VM >> 4) << 14));
+}
+
+__device__ __forceinline__ void barrier() {
+    fence();
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    fence();
+}
+
+constexpr int RING = 4; /* stages of a tile's ring */
+
+/* MW x NW waves of TM x TN 16 x 16 tiles, stages of BK columns, a ring of four:
+ * while a stage is multiplied, the first fragments of the next are read and
+ * three more are on their way.  A stage's buffer is requested again at the one
+ * barrier behind which every wave has read it. */
+template <int MW, int NW, int TM, int TN, int BK, bool BF16>
+__global__ __launch_bounds__(64 * MW * NW, 2) void k_i8_tile(GemmArgs g) {
+    constexpr int W = MW * NW, BM = 16 * TM * MW, BN = 16 * TN * NW, SB = (BM + BN) * BK;
+    constexpr int CPR = BK / 16, RPI = 1024 / BK, NI = SB / 1024 / W, S = BK / 64;
+    static_assert(SB % (1024 * W) == 0 && BM % (RPI * W) == 0, "whole loads, each of one operand");
+    __shared__ __attribute__((aligned(16))) unsigned char s0[SB], s1[SB], s2[SB], s3[SB];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    int tm, tn;
+    if (!tile_of(g, tm, tn)) return;
+    const int m0 = tm * BM, n0 = tn * BN;
+    const int wm = (wave % MW) * 16 * TM, wn = (wave / MW) * 16 * TN;
+    const int last16 = 16 * ((g.C - 1) >> 4), stages = (g.C + BK - 1) / BK, last = stages - 1;
+    /* this lane's rows and groups of the loads: load i fills 1 KB, RPI rows */
+    const unsigned char* rp[NI];
+    int ck[NI];
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+        const int row = (i * W + wave) * RPI + lane / CPR;
+        ck[i] = 16 * ((lane % CPR) ^ group_key<BK>(row));
+        rp[i] = i * W * RPI < BM ? g.a + (size_t)min(m0 + row, g.M - 1) * g.lda
+                                 : g.w + (size_t)min(n0 + row - BM, g.OC - 1) * g.ldw;
+    }
+    auto request = [&](int stage, unsigned char* buf) {
+#pragma unroll
+        for (int i = 0; i < NI; i++)
+            __builtin_amdgcn_global_load_lds((const gvoid*)(rp[i] + min(stage * BK + ck[i], last16)),
+                                             (lvoid*)(buf + (i * W + wave) * 1024), 16, 0, 0);
+    };
+    i32x4 acc[TM][TN];
+    clear(acc);
+    struct Frag {
+        i32x4 a[TM], b[TN];
+    };
+    int fo[S]; /* this lane's place in a fragment of slice s */
+#pragma unroll
+    for (int s = 0; s < S; s++) fo[s] = (lane & 15) * BK + (((4 * s + (lane >> 4)) ^ group_key<BK>(lane & 15)) << 4);
+    auto read = [&](const unsigned char* buf, int s, Frag& f) {
+#pragma unroll
+        for (int j = 0; j < TN; j++) f.b[j] = *(const i32x4*)(buf + (BM + wn + 16 * j) * BK + fo[s]);
+#pragma unroll
+        for (int i = 0; i < TM; i++) f.a[i] = *(const i32x4*)(buf + (wm + 16 * i) * BK + fo[s]);
+    };
+    auto multiply = [&](const Frag& f) {
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+#pragma unroll
+            for (int j = 0; j < TN; j++)
+                acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.b[j], f.a[i], acc[i][j], 0, 0, 0);
+    };
+    /* stage `stage` out of buf, its first slice in f already; leaves the next stage's first slice there */
+    auto body = [&](int stage, Frag& f, unsigned char* buf, const unsigned char* next) {
+        Frag h;
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            Frag& to = s & 1 ? f : h;
+            if (s + 1 < S) {
+                read(buf, s + 1, to);
+            } else {
+                wait_loads<(RING - 2) * NI, true>(); /* the next stage has landed, this one has been read */
+                barrier();
+                request(stage + RING, buf);
+                read(next, 0, to);
+            }
+            multiply(s & 1 ? h : f);
+        }
+        if (S & 1) f = h;
+    };
+    Frag f;
+    request(0, s0);
+    request(1, s1);
+    request(2, s2);
+    request(3, s3);
+    wait_loads<(RING - 1) * NI, false>();
+    barrier();
+    read(s0, 0, f);
+    int stage = 0;
+    for (; stage + RING <= last; stage += RING) { /* one way out: a loop left in its middle costs the sums copies */
+        body(stage, f, s0, s1);
+        body(stage + 1, f, s1, s2);
+        body(stage + 2, f, s2, s3);
+        body(stage + 3, f, s3, s0);
+    }
+    const unsigned char* end = s0;
+    if (stage < last) {
+        body(stage, f, s0, s1);
+        end = s1;
+    }
+    if (stage + 1 < last) {
+        body(stage + 1, f, s1, s2);
+        end = s2;
+    }
+    if (stage + 2 < last) {
+        body(stage + 2, f, s2, s3);
+        end = s3;
+    }
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+        if (s) read(end, s, f);
+        const int left = g.C - last * BK - 64 * s - 16 * (lane >> 4);
+        if (left < 16) {
+#pragma unroll
+            for (int i = 0; i < TM; i++) f.a[i] = head_bytes(f.a[i], left);
+        }
+        multiply(f);
+    }
+    wait_loads<0, true>(); /* nothing may land in the LDS of the workgroup after this one */
+    store_tile<TM, TN, BF16>(g, acc, m0 + wm, n0 + wn);
+}
+
+/* ------------------------------------------------------------------ */
+/* 256 x 256 */
+
+constexpr int PAIR_RING = 5;
+constexpr size_t PAIR_MAX_LD = (size_t)1 << 23; /* 256 rows of it stay inside 32-bit offsets */
+
+/* Eight waves of 128 x 64 (2 x 4), two on each SIMD, in two groups of four a
+ * half turn apart: while one group's 16 MFMAs of a half stage run, the other
+ * reads the fragments of its next, and a barrier ends each turn.  What bounds
+ * it: LDS (96 KB read and 32 KB written of a stage's 64 columns) and, on every CU
+ * at once, the part's power: 4096 x 4096 x 8192 takes 97 us on zeros and 125 on
+ * codes of a normal distribution.  Against it: the whole workgroup
+ * in step and fragments read as they are used 173 us; four waves of 128 x 128 142; turns
+ * without fragments read ahead 132; a ring of four stages 129.
+ * A stage of 64 columns is 32 KB; the ring of five fills the CU's LDS, and four
+ * stages are under way or landed while one is multiplied. */
+template <bool BF16>
+__global__ __launch_bounds__(512, 2) void k_i8_pair(GemmArgs g) {
+    constexpr int W = 8, MW = 2, TM = 8, TN = 4, HM = TM / 2, BM = 256, BN = 256, BK = 64, SB = (BM + BN) * BK;
+    constexpr int NI = SB / 1024 / W;
+    __shared__ __attribute__((aligned(16))) unsigned char s0[SB], s1[SB], s2[SB], s3[SB], s4[SB];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    int tm, tn;
+    if (!tile_of(g, tm, tn)) return;
+    const int m0 = tm * BM, n0 = tn * BN;
+    const int wm = (wave % MW) * 16 * TM, wn = (wave / MW) * 16 * TN;
+    const int last16 = 16 * ((g.C - 1) >> 4), stages = (g.C + BK - 1) / BK, last = stages - 1;
+    const int group = 16 * ((lane & 3) ^ group_key<BK>(lane >> 2));
+    const unsigned char* ab = g.a + (size_t)m0 * g.lda;
+    const unsigned char* wb = g.w + (size_t)n0 * g.ldw;
+    unsigned int ro[NI]; /* this lane's rows, in bytes from the tile's first */
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+        const int row = (i * W + wave) * 16 + (lane >> 2);
+        ro[i] = i * W * 16 < BM ? min(row, g.M - 1 - m0) * (unsigned int)g.lda
+                                : min(row - BM, g.OC - 1 - n0) * (unsigned int)g.ldw;
+    }
+    auto request = [&](int stage, unsigned char* buf) {
+        const unsigned int k = min(stage * BK + group, last16);
+#pragma unroll
+        for (int i = 0; i < NI; i++)
+            __builtin_amdgcn_global_load_lds((const gvoid*)((i * W * 16 < BM ? ab : wb) + (ro[i] + k)),
+                                             (lvoid*)(buf + (i * W + wave) * 1024), 16, 0, 0);
+    };
+    i32x4 acc[TM][TN];
+    clear(acc);
+    const int fo = (lane & 15) * BK + (((lane >> 4) ^ group_key<BK>(lane & 15)) << 4);
+    struct Cols {
+        i32x4 v[TN];
+    };
+    struct Rows {
+        i32x4 v[HM];
+    };
+    Cols b0, b1; /* weights of this stage and the next, in turn */
+    Rows a0, a1; /* the wave's upper and lower half of rows */
+    auto read_cols = [&](const unsigned char* buf, Cols& b) {
+#pragma unroll
+        for (int j = 0; j < TN; j++) b.v[j] = *(const i32x4*)(buf + (BM + wn + 16 * j) * BK + fo);
+    };
+    auto read_rows = [&](const unsigned char* buf, int half, Rows& a) {
+#pragma unroll
+        for (int i = 0; i < HM; i++) a.v[i] = *(const i32x4*)(buf + (wm + 16 * (i + half * HM)) * BK + fo);
+    };
+    auto multiply = [&](const Rows& a, const Cols& b, int half) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < HM; i++)
+#pragma unroll
+            for (int j = 0; j < TN; j++)
+                acc[i + half * HM][j] =
+                    __builtin_amdgcn_mfma_i32_16x16x64_i8(b.v[j], a.v[i], acc[i + half * HM][j], 0, 0, 0);
+        __builtin_amdgcn_s_setprio(0);
+    };
+    /* Turns are counted by barriers: the first group reads for a stage's second
+     * half in turn 4s and for stage s + 1 in turn 4s + 2, the other group a
+     * turn later.  So stage s + 1 has to have landed for all before turn
+     * 4s + 2 (each wave waits for its own part in its first reads of stage s),
+     * and stage s has been read by all, the reads waited for, before turn 4s + 5:
+     * its buffer is requested again in the second reads of stage s + 1, turn 4s + 6
+     * at the earliest. */
+    auto body = [&](int stage, const unsigned char* buf, const unsigned char* next, unsigned char* before, const Cols& b,
+                    Cols& bn) {
+        read_rows(buf, 1, a1);
+        wait_loads<(PAIR_RING - 3) * NI, false>();
+        barrier();
+        multiply(a0, b, 0);
+        barrier();
+        read_cols(next, bn);
+        read_rows(next, 0, a0);
+        request(stage + PAIR_RING - 1, before);
+        barrier();
+        multiply(a1, b, 1);
+        barrier();
+    };
+    request(0, s0);
+    request(1, s1);
+    request(2, s2);
+    request(3, s3);
+    wait_loads<(PAIR_RING - 2) * NI, false>();
+    barrier();
+    read_cols(s0, b0);
+    read_rows(s0, 0, a0);
+    if (wave >= W / 2) barrier(); /* the half turn */
+    int stage = 0;
+    for (; stage + PAIR_RING <= last; stage += PAIR_RING) {
+        body(stage, s0, s1, s4, b0, b1);
+        body(stage + 1, s1, s2, s0, b1, b0);
+        body(stage + 2, s2, s3, s1, b0, b1);
+        body(stage + 3, s3, s4, s2, b1, b0);
+        body(stage + 4, s4, s0, s3, b0, b1);
+        b0 = b1;
+    }
+    const unsigned char* end = s0;
+    if (stage < last) {
+        body(stage, s0, s1, s4, b0, b1);
+        b0 = b1;
+        end = s1;
+    }
+    if (stage + 1 < last) {
+        body(stage + 1, s1, s2, s0, b0, b1);
+        b0 = b1;
+        end = s2;
+    }
+    if (stage + 2 < last) {
+        body(stage + 2, s2, s3, s1, b0, b1);
+        b0 = b1;
+        end = s3;
+    }
+    if (stage + 3 < last) {
+        body(stage + 3, s3, s4, s2, b0, b1);
+        b0 = b1;
+        end = s4;
+    }
+    read_rows(end, 1, a1);
+    const int left = g.C - last * BK - 16 * (lane >> 4);
+    if (left < 16) {
+#pragma unroll
+        for (int i = 0; i < HM; i++) {
+            a0.v[i] = head_bytes(a0.v[i], left);
+            a1.v[i] = head_bytes(a1.v[i], left);
+        }
+    }
+    multiply(a0, b0, 0);
+    multiply(a1, b0, 1);
+    if (wave < W / 2) barrier();
+    wait_loads<0, true>(); /* nothing may land in the LDS of the workgroup after this one */
+    store_tile<TM, TN, BF16>(g, acc, m0 + wm, n0 + wn);
+}
+
+/* ------------------------------------------------------------------ */
+
+long tiles(int n, int t) { return ((long)n + t - 1) / t; }
+
+template <bool BF16>
+void launch(GemmArgs g, hipStream_t s) {
+    auto grid = [&](int bm, int bn) {
+        g.tiles_m = (int)tiles(g.M, bm);
+        g.tiles_n = (int)tiles(g.OC, bn);
+        const long n = (long)g.tiles_m * g.tiles_n;
+        return n <= MAX_GRID_X ? dim3((unsigned)n) : dim3(MAX_GRID_X, (unsigned)tiles((int)n, MAX_GRID_X));
+    };
+    if (g.M <= 16) {
+        if (g.M > 8 && g.OC >= 16384) {
+            const dim3 d = grid(16, 64);
+            hipLaunchKernelGGL((k_i8_few<4, 4, BF16>), d, dim3(64 * FEW_KP), 0, s, g);
+        } else {
+            const dim3 d = grid(16, 16);
+            hipLaunchKernelGGL((k_i8_few<1, 2, BF16>), d, dim3(64 * FEW_KP), 0, s, g);
+        }
+        return;
+    }
+    const long big = tiles(g.M, 256) * tiles(g.OC, 256), rounds = (big + CUS - 1) / CUS;
+    if (big * 100 >= rounds * CUS * 65 && g.lda <= PAIR_MAX_LD && g.ldw <= PAIR_MAX_LD) {
+        const dim3 d = grid(256, 256);
+        hipLaunchKernelGGL(k_i8_pair<BF16>, d, dim3(512), 0, s, g);
+    } else if (tiles(g.M, 128) * tiles(g.OC, 128) >= CUS) {
+        const dim3 d = grid(128, 128);
+        hipLaunchKernelGGL((k_i8_tile<2, 2, 4, 4, 64, BF16>), d, dim3(256), 0, s, g);
+    } else if (tiles(g.M, 128) * tiles(g.OC, 64) >= CUS) {
+        const dim3 d = grid(128, 64);
+        hipLaunchKernelGGL((k_i8_tile<2, 2, 4, 2, 64, BF16>), d, dim3(256), 0, s, g);
+    } else if (tiles(g.M, 64) * tiles(g.OC, 64) >= CUS) {
+        const dim3 d = grid(64, 64);
+        hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 128, BF16>), d, dim3(256), 0, s, g);
+    } else if (tiles(g.M, 32) * tiles(g.OC, 64) >= CUS) {
+        const dim3 d = grid(32, 64);
+        hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 2, 128, BF16>), d, dim3(256), 0, s, g);
+    } else {
+        const dim3 d = grid(32, 32);
+        hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 1, 128, BF16>), d, dim3(256), 0, s, g);
     }
 }
 
@@ -125,12 +587,8 @@ int launch_matmul_i8(const bmk_launch_t* a, bool bf16) {
     g.M = BT;
     g.C = C;
     g.OC = OC;
-    g.tiles_n = (OC + 63) / 64;
-    const size_t tiles = (size_t)((BT + 63) / 64) * (size_t)g.tiles_n;
-    BMK_REQUIRE(tiles <= (1u << 24) - 1, "matmul_forward_i8: BT=%d x OC=%d is too large for one launch", BT, OC);
-    const dim3 grid((unsigned)tiles);
-    if (bf16) hipLaunchKernelGGL(k_i8_gemm<true>, grid, dim3(NT), 0, a->stream, g);
-    else hipLaunchKernelGGL(k_i8_gemm<false>, grid, dim3(NT), 0, a->stream, g);
+    if (bf16) launch<true>(g, a->stream);
+    else launch<false>(g, a->stream);
     BMK_LAUNCH_CHECK();
     return 0;
 }
