@@ -12,8 +12,8 @@
  * a lane then holds four neighbouring outputs of one row.  The 32 x 32 x 32 form
  * is slower on this part (registers only, all CUs, codes of a normal
  * distribution: 2.6 against 4.1 POP/s).
- *   k_i8_few   up to 16 rows: weights straight into registers, the sum split over four waves (HBM, or a launch's latency)
- *   k_i8_tile  tiles of 32 x 32 to 128 x 128 through LDS, four waves
+ *   k_i8_few   up to 16 rows, or few outputs: operands straight into registers, the sum split over four waves
+ *   k_i8_tile  tiles of 32 x 32 to 128 x 128 through LDS, four or eight waves
  *   k_i8_pair  256 x 256, eight waves in two groups that take turns at the matrix cores and at LDS
  * Operands go to LDS by global_load_lds, which writes 16 bytes a lane at
  * consecutive addresses, so a row's 16-byte groups are permuted on the source
@@ -164,40 +164,39 @@ __device__ __forceinline__ void clear(i32x4 (&acc)[TM][TN]) {
 /* ------------------------------------------------------------------ */
 /* up to 16 rows */
 
-constexpr int FEW_KP = 4; /* waves along the sum */
-
-/* 16 * TN outputs a workgroup; wave p takes every fourth slice of 64 columns
- * from p on, U slices' loads in flight, so that a workgroup reads 256
+/* 16 x 16 TN outputs a workgroup; wave p of KP takes every KP-th slice of 64
+ * columns from p on, U slices' loads in flight, so that a workgroup reads 64 KP
  * neighbouring bytes of a row at once.  The partial sums meet in LDS.
- * (One wave along the sum or sixteen instead of four: 2.8 and 2.4 against 2.4 us
- * for 576 -> 1536, 5.2 and 3.5 against 3.4 for 2560 -> 960, one row each;
- * 9.3 and 14.9 against 9.2 for 8 rows of 960 -> 49152.) */
-template <int TN, int U, bool BF16>
-__global__ __launch_bounds__(64 * FEW_KP) void k_i8_few(GemmArgs g) {
-    __shared__ __attribute__((aligned(16))) i32x4 part[FEW_KP * TN * 64];
+ * What bounds it: reading the weights (8 x 960 -> 49152 9.2 us, 5.1 TB/s from the
+ * Infinity Cache), with few outputs the reads of one CU (5 x 8192 -> 500 7.2 us on
+ * 32 CUs), else the launch (1 x 960 -> 5120 2.9 us).  Four waves along the sum: one
+ * took 5.2 us for 1 x 2560 -> 960, sixteen 4.2, four 3.8 (8 x 960 -> 49152 9.3 / 15 / 9.2). */
+template <int KP, int TN, int U, bool BF16>
+__global__ __launch_bounds__(64 * KP) void k_i8_few(GemmArgs g) {
+    __shared__ __attribute__((aligned(16))) i32x4 part[KP * TN * 64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int tile = workgroup();
-    if (tile >= g.tiles_n) return;
-    const int n0 = tile * 16 * TN;
+    int tm, tn;
+    if (!tile_of(g, tm, tn)) return;
+    const int m0 = tm * 16, n0 = tn * 16 * TN;
     const int c = 16 * (lane >> 4), last = 16 * ((g.C - 1) >> 4), slices = (g.C + 63) >> 6;
-    const unsigned char* ap = g.a + (size_t)min(lane & 15, g.M - 1) * g.lda;
+    const unsigned char* ap = g.a + (size_t)min(m0 + (lane & 15), g.M - 1) * g.lda;
     const unsigned char* wp[TN];
 #pragma unroll
     for (int j = 0; j < TN; j++) wp[j] = g.w + (size_t)min(n0 + 16 * j + (lane & 15), g.OC - 1) * g.ldw;
     i32x4 acc[1][TN];
     clear(acc);
-    for (int s = wave; s < slices; s += FEW_KP * U) {
+    for (int s = wave; s < slices; s += KP * U) {
         i32x4 a[U], w[U][TN];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int k = min(64 * (s + FEW_KP * u) + c, last);
+            const int k = min(64 * (s + KP * u) + c, last);
 #pragma unroll
             for (int j = 0; j < TN; j++) w[u][j] = *(const i32x4*)(wp[j] + k);
             a[u] = *(const i32x4*)(ap + k);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int left = g.C - 64 * (s + FEW_KP * u) - c;
+            const int left = g.C - 64 * (s + KP * u) - c;
             if (left < 16) a[u] = head_bytes(a[u], left);
 #pragma unroll
             for (int j = 0; j < TN; j++)
@@ -211,8 +210,8 @@ __global__ __launch_bounds__(64 * FEW_KP) void k_i8_few(GemmArgs g) {
 #pragma unroll
     for (int j = 0; j < TN; j++)
 #pragma unroll
-        for (int p = 1; p < FEW_KP; p++) acc[0][j] += part[(p * TN + j) * 64 + lane];
-    store_tile<1, TN, BF16>(g, acc, 0, n0);
+        for (int p = 1; p < KP; p++) acc[0][j] += part[(p * TN + j) * 64 + lane];
+    store_tile<1, TN, BF16>(g, acc, m0, n0);
 }
 
 /* ------------------------------------------------------------------ */
@@ -246,18 +245,23 @@ __device__ __forceinline__ void barrier() {
     fence();
 }
 
-constexpr int RING = 4; /* stages of a tile's ring */
+constexpr int RING = 3; /* stages of a tile's ring */
 
-/* MW x NW waves of TM x TN 16 x 16 tiles, stages of BK columns, a ring of four:
- * while a stage is multiplied, the first fragments of the next are read and
- * three more are on their way.  A stage's buffer is requested again at the one
- * barrier behind which every wave has read it. */
+/* MW x NW waves of TM x TN 16 x 16 tiles, stages of BK columns, a ring of
+ * three: while a stage is multiplied, the first fragments of the next are read
+ * and two more are on their way.  A stage's buffer is requested again at the
+ * one barrier behind which every wave has read it.
+ * What bounds it: a workgroup's chain of load, barrier and fragment reads (a CU
+ * moves 40 KB/us into LDS this way; its matrix cores would take twice that).  us at
+ * 2048 x 2048 x 2048 / 4096 x 2560 x 960 / 1024 x 4096 x 4096, tiles of 128 x 128: eight
+ * waves over 128 columns a stage 12.5 / 14.1 / 21; over 64 13.4 / 16.3 / 24; four waves
+ * 13.7 / 16 / 24; a ring of two 13.2 / 17.2 / 28, of four over 64 14.3 / 18 / 26. */
 template <int MW, int NW, int TM, int TN, int BK, bool BF16>
 __global__ __launch_bounds__(64 * MW * NW, 2) void k_i8_tile(GemmArgs g) {
     constexpr int W = MW * NW, BM = 16 * TM * MW, BN = 16 * TN * NW, SB = (BM + BN) * BK;
     constexpr int CPR = BK / 16, RPI = 1024 / BK, NI = SB / 1024 / W, S = BK / 64;
     static_assert(SB % (1024 * W) == 0 && BM % (RPI * W) == 0, "whole loads, each of one operand");
-    __shared__ __attribute__((aligned(16))) unsigned char s0[SB], s1[SB], s2[SB], s3[SB];
+    __shared__ __attribute__((aligned(16))) unsigned char s0[SB], s1[SB], s2[SB];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     int tm, tn;
     if (!tile_of(g, tm, tn)) return;
@@ -316,6 +320,14 @@ __global__ __launch_bounds__(64 * MW * NW, 2) void k_i8_tile(GemmArgs g) {
                 read(next, 0, to);
             }
             multiply(s & 1 ? h : f);
+            /* the reads and requests between the MFMAs, not behind them */
+#pragma unroll
+            for (int i = 0; i < TM + TN; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, TM * TN > TM + TN ? TM * TN / (TM + TN) : 1, 0); /* MFMA */
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                                       /* LDS read */
+                if (i % 2 == 0 && i / 2 < NI) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);             /* load */
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
         if (S & 1) f = h;
     };
@@ -323,7 +335,6 @@ __global__ __launch_bounds__(64 * MW * NW, 2) void k_i8_tile(GemmArgs g) {
     request(0, s0);
     request(1, s1);
     request(2, s2);
-    request(3, s3);
     wait_loads<(RING - 1) * NI, false>();
     barrier();
     read(s0, 0, f);
@@ -331,8 +342,7 @@ __global__ __launch_bounds__(64 * MW * NW, 2) void k_i8_tile(GemmArgs g) {
     for (; stage + RING <= last; stage += RING) { /* one way out: a loop left in its middle costs the sums copies */
         body(stage, f, s0, s1);
         body(stage + 1, f, s1, s2);
-        body(stage + 2, f, s2, s3);
-        body(stage + 3, f, s3, s0);
+        body(stage + 2, f, s2, s0);
     }
     const unsigned char* end = s0;
     if (stage < last) {
@@ -342,10 +352,6 @@ __global__ __launch_bounds__(64 * MW * NW, 2) void k_i8_tile(GemmArgs g) {
     if (stage + 1 < last) {
         body(stage + 1, f, s1, s2);
         end = s2;
-    }
-    if (stage + 2 < last) {
-        body(stage + 2, f, s2, s3);
-        end = s3;
     }
 #pragma unroll
     for (int s = 0; s < S; s++) {
@@ -512,6 +518,8 @@ __global__ __launch_bounds__(512, 2) void k_i8_pair(GemmArgs g) {
 
 /* ------------------------------------------------------------------ */
 
+constexpr int FILL = 150; /* tiles a launch wants at least */
+
 long tiles(int n, int t) { return ((long)n + t - 1) / t; }
 
 template <bool BF16>
@@ -522,30 +530,41 @@ void launch(GemmArgs g, hipStream_t s) {
         const long n = (long)g.tiles_m * g.tiles_n;
         return n <= MAX_GRID_X ? dim3((unsigned)n) : dim3(MAX_GRID_X, (unsigned)tiles((int)n, MAX_GRID_X));
     };
-    if (g.M <= 16) {
-        if (g.M > 8 && g.OC >= 16384) {
+    /* up to 16 rows, or few outputs in all (64 tiles of 32 x 32: 17 x 960 x 960 2.9 us against 4.2 in those, 100 x
+     * 8000 x 50 7.2 / 9.0, 64 x 2560 x 960 4.6 / 5.1; with 320 tiles, 48 x 960 x 5120, 4.5 / 4.0) */
+    if (g.M <= 16 || tiles(g.M, 32) * tiles(g.OC, 32) <= 64) {
+        /* more than 8 rows over many outputs share their rows' reads: 16 x 4096 x 16384 17.5 us / 13.9 with four
+         * tiles a wave, 16 x 960 x 49152 10.2 / 9.6; 16 x 8192 x 8192 16.9 / 20.9 */
+        if (g.M > 8 && g.M <= 16 && g.OC >= 16384) {
             const dim3 d = grid(16, 64);
-            hipLaunchKernelGGL((k_i8_few<4, 4, BF16>), d, dim3(64 * FEW_KP), 0, s, g);
+            hipLaunchKernelGGL((k_i8_few<4, 4, 4, BF16>), d, dim3(256), 0, s, g);
         } else {
             const dim3 d = grid(16, 16);
-            hipLaunchKernelGGL((k_i8_few<1, 2, BF16>), d, dim3(64 * FEW_KP), 0, s, g);
+            hipLaunchKernelGGL((k_i8_few<4, 1, 2, BF16>), d, dim3(256), 0, s, g);
         }
         return;
     }
+    /* 256 x 256 where its last round fills the CUs well enough: 4096 x 960 x 5120 (320 tiles, 62%) 38.5 us against 40.3 in
+     * 128 x 128 tiles, 1024 x 4096 x 4096 (64 tiles, 25%) 40.8 / 21, 2048 x 2048 x 2048 (25%) 24 / 12.5.  Else the largest tile
+     * that FILL of are there, or 32 x 32.  us in 128 x 128, 128 x 64, 64 x 64, 32 x 64 and 32 x 32 tiles:
+     * 512 x 960 x 5120 7.3, 8.8, 8.7, 9.7, 10.8; 777 x 2500 x 2000 12.0, 11.2, 12.4, 18.5, 20.7; 512 x 2560 x 960 10.0, 7.8, 6.2, 5.4,
+     * 5.6; 333 x 960 x 960 6.7, 5.4, 4.4, 3.9, 4.0; 64 x 960 x 2560 6.9, 5.0, 4.7, 4.0, 3.6. */
     const long big = tiles(g.M, 256) * tiles(g.OC, 256), rounds = (big + CUS - 1) / CUS;
-    if (big * 100 >= rounds * CUS * 65 && g.lda <= PAIR_MAX_LD && g.ldw <= PAIR_MAX_LD) {
+    if (big * 10 >= rounds * CUS * 6 && g.lda <= PAIR_MAX_LD && g.ldw <= PAIR_MAX_LD) {
         const dim3 d = grid(256, 256);
         hipLaunchKernelGGL(k_i8_pair<BF16>, d, dim3(512), 0, s, g);
-    } else if (tiles(g.M, 128) * tiles(g.OC, 128) >= CUS) {
+    } else if (tiles(g.M, 128) * tiles(g.OC, 128) >= FILL) {
         const dim3 d = grid(128, 128);
-        hipLaunchKernelGGL((k_i8_tile<2, 2, 4, 4, 64, BF16>), d, dim3(256), 0, s, g);
-    } else if (tiles(g.M, 128) * tiles(g.OC, 64) >= CUS) {
+        /* stages of 64 columns for short sums: 2048 x 576 x 3000 11.6 us against 14.3, 4096 x 960 x 5120 40.3 / 42.8 */
+        if (g.C < 1024) hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 64, BF16>), d, dim3(512), 0, s, g);
+        else hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 128, BF16>), d, dim3(512), 0, s, g);
+    } else if (tiles(g.M, 128) * tiles(g.OC, 64) >= FILL) {
         const dim3 d = grid(128, 64);
-        hipLaunchKernelGGL((k_i8_tile<2, 2, 4, 2, 64, BF16>), d, dim3(256), 0, s, g);
-    } else if (tiles(g.M, 64) * tiles(g.OC, 64) >= CUS) {
+        hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 2, 128, BF16>), d, dim3(512), 0, s, g);
+    } else if (tiles(g.M, 64) * tiles(g.OC, 64) >= FILL) {
         const dim3 d = grid(64, 64);
         hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 128, BF16>), d, dim3(256), 0, s, g);
-    } else if (tiles(g.M, 32) * tiles(g.OC, 64) >= CUS) {
+    } else if (tiles(g.M, 32) * tiles(g.OC, 64) >= FILL) {
         const dim3 d = grid(32, 64);
         hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 2, 128, BF16>), d, dim3(256), 0, s, g);
     } else {
