@@ -7,7 +7,7 @@
  *                       pass over the row gives both the maximum and the sum
  *   swiglu_forward_i8   p = gate / (1 + exp(-gate)) * up
  *   dequantize_rows_i8  dst = code * scale
- * Sums of squares are kept in 64 bits.  A workgroup takes a row.
+ * Sums of squares are kept in 64 bits.
  */
 #include "i8_common.h"
 
@@ -15,22 +15,7 @@ namespace {
 
 using namespace bmk;
 
-constexpr int NT = 256;
-constexpr int MAX_GRID = 1 << 20; /* workgroups of a launch; each takes every MAX_GRID-th row past that */
-
-template <bool BF16>
-__device__ __forceinline__ float load1(const void* p, size_t i) {
-    return BF16 ? __uint_as_float((unsigned int)((const unsigned short*)p)[i] << 16) : ((const float*)p)[i];
-}
-
-/* fp32 -> bf16 bits, round to nearest even */
-__device__ __forceinline__ unsigned short bf16_of(float v) { return __builtin_bit_cast(unsigned short, (__bf16)v); }
-
-/* x / (1 + exp(-x)) with the exponential of -|x|, which does not overflow */
-__device__ __forceinline__ float silu(float x) {
-    const float e = expf(-fabsf(x));
-    return (x < 0.0f ? x * e : x) / (1.0f + e);
-}
+constexpr int MAX_GRID = 1 << 20; /* workgroups of a launch of the forms that take any row */
 
 enum { OP_QUANT, OP_NORM, OP_SWIGLU };
 
@@ -46,6 +31,235 @@ struct RowArgs {
     float eps;
 };
 
+template <bool BF16>
+__device__ __forceinline__ float load1(const void* p, size_t i) {
+    return BF16 ? __uint_as_float((unsigned int)((const unsigned short*)p)[i] << 16) : ((const float*)p)[i];
+}
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+/* G = 8 bf16 or 4 fp32 elements a lane: 16 bytes, on an element's boundary */
+template <bool BF16> constexpr int G = BF16 ? 8 : 4;
+
+template <bool BF16>
+__device__ __forceinline__ u32x4 load_raw(const void* p, size_t i) {
+    u32x4 v;
+    if (BF16) __builtin_memcpy(&v, __builtin_assume_aligned((const unsigned short*)p + i, 2), 16);
+    else __builtin_memcpy(&v, __builtin_assume_aligned((const float*)p + i, 4), 16);
+    return v;
+}
+/* element e of such a group, as fp32 */
+template <bool BF16>
+__device__ __forceinline__ float element(u32x4 v, int e) {
+    if (!BF16) return __uint_as_float(v[e]);
+    return __uint_as_float(e & 1 ? v[e >> 1] & 0xffff0000u : v[e >> 1] << 16);
+}
+/* G fp32 values */
+template <bool BF16> struct Wide {
+    f32x4 v[G<BF16> / 4];
+};
+template <bool BF16>
+__device__ __forceinline__ Wide<BF16> load_wide(const float* p) {
+    Wide<BF16> r;
+    __builtin_memcpy(&r, __builtin_assume_aligned(p, 4), sizeof r);
+    return r;
+}
+
+/* x / (1 + exp(-x)) with the exponential of -|x|, which does not overflow; the divisor lies in 1 .. 2, where the
+ * reciprocal instruction is good to its last place */
+__device__ __forceinline__ float silu(float x) {
+    const float e = exp2f(fabsf(x) * -1.44269504f);
+    return (x < 0.0f ? x * e : x) * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
+/* four codes of products p * inv: adding 1.5 * 2^23 rounds to a whole number, to even, which lies in the low byte */
+__device__ __forceinline__ unsigned int pack4(const float* p, float inv) {
+#pragma clang fp contract(off)
+    unsigned int u[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float t = p[i] * inv;
+        u[i] = __float_as_uint(t + 12582912.0f);
+    }
+    const unsigned int lo = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(u[3], u[2], 0x04000c0cu);
+    return lo | hi;
+}
+
+/* Maximum and sum over L = 16 or 64 neighbouring lanes (all of them get it): row rotations inside 16, then swaps. */
+template <int CTRL>
+__device__ __forceinline__ unsigned int dpp(unsigned int v) {
+    return (unsigned int)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+}
+template <int L, class F>
+__device__ __forceinline__ unsigned int lanes_fold(unsigned int v, F f) {
+    v = f(v, dpp<0x128>(v)); /* row_ror 8, 4, 2, 1 */
+    v = f(v, dpp<0x124>(v));
+    v = f(v, dpp<0x122>(v));
+    v = f(v, dpp<0x121>(v));
+    if (L >= 64) {
+        u32x2 s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = f(s[0], s[1]);
+        s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = f(s[0], s[1]);
+    }
+    return v;
+}
+template <int L>
+__device__ __forceinline__ unsigned int lanes_max(unsigned int v) {
+    return lanes_fold<L>(v, [](unsigned int a, unsigned int b) { return max(a, b); });
+}
+__device__ __forceinline__ double dbl(unsigned int lo, unsigned int hi) {
+    return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double v) {
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+    return v + dbl(dpp<CTRL>((unsigned int)b), dpp<CTRL>((unsigned int)(b >> 32)));
+}
+template <int L>
+__device__ __forceinline__ double lanes_sum(double v) {
+    v = dpp_add<0x128>(v);
+    v = dpp_add<0x124>(v);
+    v = dpp_add<0x122>(v);
+    v = dpp_add<0x121>(v);
+    if (L >= 64) {
+        unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+        u32x2 lo = __builtin_amdgcn_permlane16_swap((unsigned int)b, (unsigned int)b, false, false);
+        u32x2 hi = __builtin_amdgcn_permlane16_swap((unsigned int)(b >> 32), (unsigned int)(b >> 32), false, false);
+        v = dbl(lo[0], hi[0]) + dbl(lo[1], hi[1]);
+        b = __builtin_bit_cast(unsigned long long, v);
+        lo = __builtin_amdgcn_permlane32_swap((unsigned int)b, (unsigned int)b, false, false);
+        hi = __builtin_amdgcn_permlane32_swap((unsigned int)(b >> 32), (unsigned int)(b >> 32), false, false);
+        v = dbl(lo[0], hi[0]) + dbl(lo[1], hi[1]);
+    }
+    return v;
+}
+
+/* the norm's scale: top * rstd / 127, rounded once */
+__device__ __forceinline__ float norm_scale(unsigned int top, double ss, int C, float eps) {
+    return (float)((double)__uint_as_float(top) / (127.0 * sqrt(ss / C + (double)eps)));
+}
+
+/* Rows of up to LPR * NV * G columns: LPR lanes a row (16: four rows a wave;
+ * 64: a wave; more: a workgroup), which read it once, 16 bytes a lane and load, all
+ * loads before the first use, and keep it in registers until the codes are
+ * written.  A workgroup takes several rows in turn where there are more than
+ * the launch has workgroups, and keeps the norm's weights. */
+template <int OP, bool BF16, int LPR, int NV>
+__global__ __launch_bounds__(LPR < 64 ? 64 : LPR) void k_rows_i8(RowArgs a) {
+    constexpr int E = G<BF16>, NT = LPR < 64 ? 64 : LPR, RPW = NT / LPR, WAVES = NT / 64;
+    __shared__ unsigned int tops[2][WAVES];
+    __shared__ double sums[2][WAVES];
+    const int l = threadIdx.x % LPR, wave = threadIdx.x >> 6, C = a.C;
+    const int end = (int)i8_row_bytes(C), ragged = C % E, clamp = max(C - E, 0);
+    Wide<BF16> w[NV];
+    if (OP == OP_NORM && C >= E) {
+#pragma unroll
+        for (int v = 0; v < NV; v++) w[v] = load_wide<BF16>(a.w + min((v * LPR + l) * E, clamp));
+    }
+    int turn = 0;
+    for (size_t row = (size_t)blockIdx.x * RPW + threadIdx.x / LPR; row < (size_t)a.rows; row += (size_t)gridDim.x * RPW) {
+        float p[NV][E];
+        unsigned int top = 0;
+        double ss = 0.0;
+        const size_t at = row * a.ldx, hat = row * (size_t)C;
+        if (C >= E) {
+            u32x4 x[NV], y[NV];
+            Wide<BF16> r[NV];
+#pragma unroll
+            for (int v = 0; v < NV; v++) { /* groups past the row read its last one and count as zeros */
+                const int c = min((v * LPR + l) * E, clamp);
+                x[v] = load_raw<BF16>(a.x, at + c);
+                if (OP == OP_SWIGLU) y[v] = load_raw<BF16>(a.y, at + c);
+                if (OP == OP_NORM && a.y) r[v] = load_wide<BF16>((const float*)a.y + hat + c);
+            }
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                const int c = (v * LPR + l) * E;
+                const bool in = c + E <= C;
+                Wide<BF16> h;
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const float xe = element<BF16>(x[v], e);
+                    float pe = xe;
+                    if (OP == OP_SWIGLU) pe = silu(xe) * element<BF16>(y[v], e);
+                    if (OP == OP_NORM) {
+                        const float he = a.y ? xe + r[v].v[e >> 2][e & 3] : xe;
+                        h.v[e >> 2][e & 3] = he;
+                        pe = he * w[v].v[e >> 2][e & 3];
+                        if (in) ss += (double)he * he;
+                    }
+                    p[v][e] = in ? pe : 0.0f;
+                    top = max(top, i8_mag(p[v][e]));
+                }
+                if (OP == OP_NORM && a.y && in)
+                    __builtin_memcpy(__builtin_assume_aligned(a.h + hat + c, 4), &h, sizeof h);
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < NV; v++)
+#pragma unroll
+                for (int e = 0; e < E; e++) p[v][e] = 0.0f;
+        }
+        if (ragged) { /* the last group, element by element */
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                const int c = (v * LPR + l) * E;
+                if (c >= C || c + E <= C) continue;
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    if (c + e >= C) continue;
+                    const float xe = load1<BF16>(a.x, at + c + e);
+                    float pe = xe;
+                    if (OP == OP_SWIGLU) pe = silu(xe) * load1<BF16>(a.y, at + c + e);
+                    if (OP == OP_NORM) {
+                        const float he = a.y ? xe + ((const float*)a.y)[hat + c + e] : xe;
+                        if (a.y) a.h[hat + c + e] = he;
+                        ss += (double)he * he;
+                        pe = he * a.w[c + e];
+                    }
+                    p[v][e] = pe;
+                    top = max(top, i8_mag(pe));
+                }
+            }
+        }
+        top = lanes_max<(LPR < 64 ? LPR : 64)>(top);
+        if (OP == OP_NORM) ss = lanes_sum<(LPR < 64 ? LPR : 64)>(ss);
+        if (WAVES > 1) { /* two places in turn: one barrier a row */
+            if ((threadIdx.x & 63) == 0) {
+                tops[turn][wave] = top;
+                sums[turn][wave] = ss;
+            }
+            __syncthreads();
+            top = tops[turn][0];
+#pragma unroll
+            for (int i = 1; i < WAVES; i++) top = max(top, tops[turn][i]);
+            if (OP == OP_NORM) {
+                ss = sums[turn][0];
+#pragma unroll
+                for (int i = 1; i < WAVES; i++) ss += sums[turn][i];
+            }
+            turn ^= 1;
+        }
+        const I8Grid g = i8_grid(top);
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            const int c = (v * LPR + l) * E;
+            if (c >= end) continue;
+            unsigned int* q = (unsigned int*)(a.q + row * a.ldq + c);
+            const unsigned int q0 = g.inv == 0.0f ? 0u : pack4(p[v], g.inv);
+            if (BF16) *(u32x2*)q = u32x2{q0, g.inv == 0.0f ? 0u : pack4(p[v] + E - 4, g.inv)};
+            else *q = q0;
+        }
+        if (l == 0) a.s[row] = OP == OP_NORM && g.inv != 0.0f ? norm_scale(top, ss, C, a.eps) : g.step;
+    }
+}
+
+/* Rows of any length, read twice. */
 template <int OP, bool BF16>
 __device__ __forceinline__ float row_value(const RowArgs& a, size_t row, int c, float* h) {
     const float x = load1<BF16>(a.x, row * a.ldx + c);
@@ -58,10 +272,11 @@ __device__ __forceinline__ float row_value(const RowArgs& a, size_t row, int c, 
 }
 
 template <int OP, bool BF16>
-__global__ __launch_bounds__(NT) void k_rows_i8(RowArgs a) {
+__global__ __launch_bounds__(1024) void k_rows_i8_long(RowArgs a) {
+    constexpr int NT = 1024;
     __shared__ unsigned int tops[NT / 64];
     __shared__ double sums[NT / 64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = threadIdx.x >> 6;
     for (size_t row = blockIdx.x; row < (size_t)a.rows; row += gridDim.x) {
         unsigned int top = 0;
         double ss = 0.0;
@@ -70,27 +285,22 @@ __global__ __launch_bounds__(NT) void k_rows_i8(RowArgs a) {
             top = max(top, i8_mag(row_value<OP, BF16>(a, row, c, &h)));
             if (OP == OP_NORM) ss += (double)h * h;
         }
-        for (int off = 32; off > 0; off >>= 1) {
-            top = max(top, (unsigned int)__shfl_xor((int)top, off));
-            if (OP == OP_NORM) ss += __shfl_xor(ss, off);
-        }
+        top = lanes_max<64>(top);
+        if (OP == OP_NORM) ss = lanes_sum<64>(ss);
         __syncthreads(); /* the row before has been read */
-        if (lane == 0) {
+        if ((threadIdx.x & 63) == 0) {
             tops[wave] = top;
             sums[wave] = ss;
         }
         __syncthreads();
-        top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
-        const I8Grid g = i8_grid(top);
-        if (threadIdx.x == 0) {
-            if (OP == OP_NORM) {
-                ss = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-                const double k = 1.0 / sqrt(ss / a.C + (double)a.eps) / 127.0;
-                a.s[row] = g.inv == 0.0f ? g.step : (float)(__uint_as_float(top) * k);
-            } else {
-                a.s[row] = g.step;
-            }
+        top = 0;
+        ss = 0.0;
+        for (int i = 0; i < NT / 64; i++) {
+            top = max(top, tops[i]);
+            if (OP == OP_NORM) ss += sums[i];
         }
+        const I8Grid g = i8_grid(top);
+        if (threadIdx.x == 0) a.s[row] = OP == OP_NORM && g.inv != 0.0f ? norm_scale(top, ss, a.C, a.eps) : g.step;
         const int end = (int)i8_row_bytes(a.C);
         for (int c = threadIdx.x; c < end; c += NT) {
             float h = 0.0f;
@@ -101,26 +311,88 @@ __global__ __launch_bounds__(NT) void k_rows_i8(RowArgs a) {
     }
 }
 
-template <bool BF16>
-__global__ __launch_bounds__(NT) void k_rows_back(const unsigned char* q, const float* s, void* dst, size_t ldq,
-                                                  size_t ldd, int rows, int C) {
-    for (size_t row = blockIdx.x; row < (size_t)rows; row += gridDim.x) {
+/* code * scale: LPR lanes a row, 8 (to bf16) or 4 codes a lane and step, so that a lane stores 16 bytes */
+template <bool BF16, int LPR>
+__global__ __launch_bounds__(256) void k_rows_back(const unsigned char* q, const float* s, void* dst, size_t ldq,
+                                                   size_t ldd, int rows, int C) {
+    constexpr int E = G<BF16>, RPB = 256 / LPR;
+    const int l = threadIdx.x % LPR;
+    for (size_t row = (size_t)blockIdx.x * RPB + threadIdx.x / LPR; row < (size_t)rows; row += (size_t)gridDim.x * RPB) {
         const float sc = s[row];
-        for (int c = threadIdx.x; c < C; c += NT) {
-            const float v = (float)(signed char)q[row * ldq + c] * sc;
-            if (BF16) ((unsigned short*)dst)[row * ldd + c] = bf16_of(v);
-            else ((float*)dst)[row * ldd + c] = v;
+        const unsigned char* qr = q + row * ldq;
+        for (int c = l * E; c < C; c += LPR * E) {
+            unsigned int u[2];
+            __builtin_memcpy(u, __builtin_assume_aligned(qr + c, E), E); /* whole 16-byte groups are there */
+            float v[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) v[e] = (float)(signed char)(u[e >> 2] >> (8 * (e & 3))) * sc;
+            if (c + E <= C) {
+                u32x4 o;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    o[i] = BF16 ? __builtin_bit_cast(unsigned int, __builtin_convertvector(f32x2{v[(2 * i) % E], v[(2 * i + 1) % E]}, bf16x2))
+                                : __float_as_uint(v[i]);
+                if (BF16) __builtin_memcpy(__builtin_assume_aligned((unsigned short*)dst + row * ldd + c, 2), &o, 16);
+                else __builtin_memcpy(__builtin_assume_aligned((float*)dst + row * ldd + c, 4), &o, 16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    if (c + e >= C) continue;
+                    if (BF16) ((unsigned short*)dst)[row * ldd + c + e] = __builtin_bit_cast(unsigned short, (__bf16)v[e]);
+                    else ((float*)dst)[row * ldd + c + e] = v[e];
+                }
+            }
         }
     }
 }
 
+template <int OP, bool BF16, int LPR, int NV>
+void go(const RowArgs& r, hipStream_t s) {
+    constexpr int NT = LPR < 64 ? 64 : LPR, RPW = NT / LPR;
+    const long wgs = ((long)r.rows + RPW - 1) / RPW, most = 256 * 32 * 64 / NT;
+    hipLaunchKernelGGL((k_rows_i8<OP, BF16, LPR, NV>), dim3((unsigned)(wgs < most ? wgs : most)), dim3(NT), 0, s, r);
+}
+
+template <int OP, bool BF16>
+void launch_form(const RowArgs& r, hipStream_t s) {
+    const int groups = (int)(i8_row_bytes(r.C) / G<BF16>); /* of 16 bytes of source, the zeros behind a row's codes among them */
+    if (groups <= 16) go<OP, BF16, 16, 1>(r, s);
+    else if (groups <= 32) go<OP, BF16, 16, 2>(r, s);
+    else if (groups <= 64) go<OP, BF16, 64, 1>(r, s);
+    else if (groups <= 128) go<OP, BF16, 64, 2>(r, s);
+    else if (groups <= 256) go<OP, BF16, 64, 4>(r, s);
+    else if (groups <= 512) go<OP, BF16, 256, 2>(r, s);
+    else if (groups <= 1024) go<OP, BF16, 256, 4>(r, s);
+    else if (groups <= 2048) go<OP, BF16, 512, 4>(r, s);
+    else if (groups <= 4096) go<OP, BF16, 1024, 4>(r, s);
+    else
+        hipLaunchKernelGGL((k_rows_i8_long<OP, BF16>), dim3((unsigned)(r.rows < MAX_GRID ? r.rows : MAX_GRID)), dim3(1024),
+                           0, s, r);
+}
+
 template <int OP>
 int launch_rows(const RowArgs& r, bool bf16, hipStream_t s) {
-    const dim3 grid((unsigned)(r.rows < MAX_GRID ? r.rows : MAX_GRID));
-    if (bf16) hipLaunchKernelGGL((k_rows_i8<OP, true>), grid, dim3(NT), 0, s, r);
-    else hipLaunchKernelGGL((k_rows_i8<OP, false>), grid, dim3(NT), 0, s, r);
+    if (bf16) launch_form<OP, true>(r, s);
+    else launch_form<OP, false>(r, s);
     BMK_LAUNCH_CHECK();
     return 0;
+}
+
+template <bool BF16>
+void launch_back(const bmk_launch_t* a, int M, int C, int ldq, int ldd) {
+    const unsigned char* q = (const unsigned char*)a->dev[0];
+    const float* s = (const float*)a->dev[1];
+    const int groups = (C + G<BF16> - 1) / G<BF16>;
+    auto grid = [&](int rpb) {
+        const long n = ((long)M + rpb - 1) / rpb;
+        return dim3((unsigned)(n < MAX_GRID ? n : MAX_GRID));
+    };
+    if (groups <= 32)
+        hipLaunchKernelGGL((k_rows_back<BF16, 16>), grid(16), dim3(256), 0, a->stream, q, s, a->dev[2], (size_t)ldq, (size_t)ldd, M, C);
+    else if (groups <= 256)
+        hipLaunchKernelGGL((k_rows_back<BF16, 64>), grid(4), dim3(256), 0, a->stream, q, s, a->dev[2], (size_t)ldq, (size_t)ldd, M, C);
+    else
+        hipLaunchKernelGGL((k_rows_back<BF16, 256>), grid(1), dim3(256), 0, a->stream, q, s, a->dev[2], (size_t)ldq, (size_t)ldd, M, C);
 }
 
 /* bytes of a row-major matrix of rows ld elements apart */
@@ -223,11 +495,8 @@ int launch_dequantize_rows(const bmk_launch_t* a, bool bf16) {
     BMK_NEED_BYTES(a, 2, span(M, C, ldd, esz), "dst");
     BMK_REQUIRE(((uintptr_t)a->dev[2] & (esz - 1)) == 0 && ((uintptr_t)a->dev[1] & 3) == 0,
                 "dequantize_rows_i8: misaligned scale or dst offset");
-    const dim3 grid((unsigned)(M < MAX_GRID ? M : MAX_GRID));
-    const unsigned char* q = (const unsigned char*)a->dev[0];
-    const float* s = (const float*)a->dev[1];
-    if (bf16) hipLaunchKernelGGL(k_rows_back<true>, grid, dim3(NT), 0, a->stream, q, s, a->dev[2], (size_t)ldq, (size_t)ldd, M, C);
-    else hipLaunchKernelGGL(k_rows_back<false>, grid, dim3(NT), 0, a->stream, q, s, a->dev[2], (size_t)ldq, (size_t)ldd, M, C);
+    if (bf16) launch_back<true>(a, M, C, ldq, ldd);
+    else launch_back<false>(a, M, C, ldq, ldd);
     BMK_LAUNCH_CHECK();
     return 0;
 }
