@@ -42,37 +42,49 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
-/* G = 8 bf16 or 4 fp32 elements a lane: 16 bytes, on an element's boundary */
-template <bool BF16> constexpr int G = BF16 ? 8 : 4;
+/* Elements a lane takes at once: 16 bytes of the source, or with fp32 operands
+ * beside a bf16 source (the norm) 16 bytes of those, so that every access of a
+ * wave is one span (eight elements a lane there: 72 us for 8192 x 4096 against 68). */
+template <int OP, bool BF16> constexpr int G = BF16 && OP != OP_NORM ? 8 : 4;
 
-template <bool BF16>
-__device__ __forceinline__ u32x4 load_raw(const void* p, size_t i) {
-    u32x4 v;
-    if (BF16) __builtin_memcpy(&v, __builtin_assume_aligned((const unsigned short*)p + i, 2), 16);
-    else __builtin_memcpy(&v, __builtin_assume_aligned((const float*)p + i, 4), 16);
-    return v;
-}
-/* element e of such a group, as fp32 */
-template <bool BF16>
-__device__ __forceinline__ float element(u32x4 v, int e) {
-    if (!BF16) return __uint_as_float(v[e]);
-    return __uint_as_float(e & 1 ? v[e >> 1] & 0xffff0000u : v[e >> 1] << 16);
-}
-/* G fp32 values */
-template <bool BF16> struct Wide {
-    f32x4 v[G<BF16> / 4];
+/* Loads on an element's boundary.  Rows are read once, so past the caches
+ * (nontemporal: 8192 x 4096 fp32 quantized 31.3 -> 28.0 us, SwiGLU of 4096 x 8192 58.6 -> 51.8; the norm's
+ * sum written so too: 78.2 -> 69.9). */
+typedef u32x4 u32x4_2 __attribute__((aligned(2)));
+typedef u32x4 u32x4_4 __attribute__((aligned(4)));
+typedef u32x2 u32x2_2 __attribute__((aligned(2)));
+typedef f32x4 f32x4_4 __attribute__((aligned(4)));
+
+/* E source elements as they are, in dwords */
+template <bool BF16, int E> struct Raw {
+    unsigned int u[BF16 ? E / 2 : E];
 };
-template <bool BF16>
-__device__ __forceinline__ Wide<BF16> load_wide(const float* p) {
-    Wide<BF16> r;
-    __builtin_memcpy(&r, __builtin_assume_aligned(p, 4), sizeof r);
+template <bool BF16, int E>
+__device__ __forceinline__ Raw<BF16, E> load_raw(const void* p, size_t i) {
+    Raw<BF16, E> r;
+    if (BF16 && E == 4) {
+        const u32x2 v = __builtin_nontemporal_load((const u32x2_2*)((const unsigned short*)p + i));
+        __builtin_memcpy(&r, &v, 8);
+    } else {
+        const u32x4 v = BF16 ? __builtin_nontemporal_load((const u32x4_2*)((const unsigned short*)p + i))
+                             : __builtin_nontemporal_load((const u32x4_4*)((const float*)p + i));
+        __builtin_memcpy(&r, &v, sizeof r);
+    }
     return r;
 }
+/* element e, as fp32 */
+template <bool BF16, int E>
+__device__ __forceinline__ float element(const Raw<BF16, E>& v, int e) {
+    if (!BF16) return __uint_as_float(v.u[e]);
+    return __uint_as_float(e & 1 ? v.u[e >> 1] & 0xffff0000u : v.u[e >> 1] << 16);
+}
 
-/* x / (1 + exp(-x)) with the exponential of -|x|, which does not overflow; the divisor lies in 1 .. 2, where the
- * reciprocal instruction is good to its last place */
+/* x / (1 + exp(-x)) with the exponential of -|x|, which does not overflow; the
+ * divisor lies in 1 .. 2, where the reciprocal instruction is good to its last
+ * place.  exp(-|x|) is the square of exp(-|x| / 2): the instruction gives no
+ * subnormal numbers, the product does, and |x| up to 174 has a root above them. */
 __device__ __forceinline__ float silu(float x) {
-    const float e = exp2f(fabsf(x) * -1.44269504f);
+    const float r = __builtin_amdgcn_exp2f(fabsf(x) * -0.72134752f), e = r * r;
     return (x < 0.0f ? x * e : x) * __builtin_amdgcn_rcpf(1.0f + e);
 }
 
@@ -148,18 +160,22 @@ __device__ __forceinline__ float norm_scale(unsigned int top, double ss, int C, 
  * 64: a wave; more: a workgroup), which read it once, 16 bytes a lane and load, all
  * loads before the first use, and keep it in registers until the codes are
  * written.  A workgroup takes several rows in turn where there are more than
- * the launch has workgroups, and keeps the norm's weights. */
+ * the launch has workgroups, and keeps the norm's weights.
+ * What bounds it: HBM, with many rows (TB/s of what is read and written: 49152 x
+ * 960 6.0, 8192 x 4096 norm 6.3, 4096 x 8192 bf16 SwiGLU 5.7, where its arithmetic
+ * is close behind; a 1 GiB copy reaches 5.1); with few, the chain of load,
+ * reduction and store (one row of 576 2.5 us, 333 of 960 2.8). */
 template <int OP, bool BF16, int LPR, int NV>
 __global__ __launch_bounds__(LPR < 64 ? 64 : LPR) void k_rows_i8(RowArgs a) {
-    constexpr int E = G<BF16>, NT = LPR < 64 ? 64 : LPR, RPW = NT / LPR, WAVES = NT / 64;
+    constexpr int E = G<OP, BF16>, NT = LPR < 64 ? 64 : LPR, RPW = NT / LPR, WAVES = NT / 64;
     __shared__ unsigned int tops[2][WAVES];
     __shared__ double sums[2][WAVES];
     const int l = threadIdx.x % LPR, wave = threadIdx.x >> 6, C = a.C;
     const int end = (int)i8_row_bytes(C), ragged = C % E, clamp = max(C - E, 0);
-    Wide<BF16> w[NV];
+    f32x4 w[NV];
     if (OP == OP_NORM && C >= E) {
 #pragma unroll
-        for (int v = 0; v < NV; v++) w[v] = load_wide<BF16>(a.w + min((v * LPR + l) * E, clamp));
+        for (int v = 0; v < NV; v++) w[v] = *(const f32x4_4*)(a.w + min((v * LPR + l) * E, clamp));
     }
     int turn = 0;
     for (size_t row = (size_t)blockIdx.x * RPW + threadIdx.x / LPR; row < (size_t)a.rows; row += (size_t)gridDim.x * RPW) {
@@ -168,36 +184,35 @@ __global__ __launch_bounds__(LPR < 64 ? 64 : LPR) void k_rows_i8(RowArgs a) {
         double ss = 0.0;
         const size_t at = row * a.ldx, hat = row * (size_t)C;
         if (C >= E) {
-            u32x4 x[NV], y[NV];
-            Wide<BF16> r[NV];
+            Raw<BF16, E> x[NV], y[NV];
+            f32x4 r[NV];
 #pragma unroll
             for (int v = 0; v < NV; v++) { /* groups past the row read its last one and count as zeros */
                 const int c = min((v * LPR + l) * E, clamp);
-                x[v] = load_raw<BF16>(a.x, at + c);
-                if (OP == OP_SWIGLU) y[v] = load_raw<BF16>(a.y, at + c);
-                if (OP == OP_NORM && a.y) r[v] = load_wide<BF16>((const float*)a.y + hat + c);
+                x[v] = load_raw<BF16, E>(a.x, at + c);
+                if (OP == OP_SWIGLU) y[v] = load_raw<BF16, E>(a.y, at + c);
+                if (OP == OP_NORM && a.y) r[v] = __builtin_nontemporal_load((const f32x4_4*)((const float*)a.y + hat + c));
             }
 #pragma unroll
             for (int v = 0; v < NV; v++) {
                 const int c = (v * LPR + l) * E;
-                const bool in = c + E <= C;
-                Wide<BF16> h;
+                const bool in = v < NV - 1 || c + E <= C; /* all but the last group of a lane lie inside (launch_form) */
+                f32x4 h;
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    const float xe = element<BF16>(x[v], e);
+                    const float xe = element<BF16, E>(x[v], e);
                     float pe = xe;
-                    if (OP == OP_SWIGLU) pe = silu(xe) * element<BF16>(y[v], e);
+                    if (OP == OP_SWIGLU) pe = silu(xe) * element<BF16, E>(y[v], e);
                     if (OP == OP_NORM) {
-                        const float he = a.y ? xe + r[v].v[e >> 2][e & 3] : xe;
-                        h.v[e >> 2][e & 3] = he;
-                        pe = he * w[v].v[e >> 2][e & 3];
+                        const float he = a.y ? xe + r[v][e & 3] : xe;
+                        h[e & 3] = he;
+                        pe = he * w[v][e & 3];
                         if (in) ss += (double)he * he;
                     }
                     p[v][e] = in ? pe : 0.0f;
                     top = max(top, i8_mag(p[v][e]));
                 }
-                if (OP == OP_NORM && a.y && in)
-                    __builtin_memcpy(__builtin_assume_aligned(a.h + hat + c, 4), &h, sizeof h);
+                if (OP == OP_NORM && a.y && in) __builtin_nontemporal_store(h, (f32x4_4*)(a.h + hat + c));
             }
         } else {
 #pragma unroll
@@ -252,7 +267,7 @@ __global__ __launch_bounds__(LPR < 64 ? 64 : LPR) void k_rows_i8(RowArgs a) {
             if (c >= end) continue;
             unsigned int* q = (unsigned int*)(a.q + row * a.ldq + c);
             const unsigned int q0 = g.inv == 0.0f ? 0u : pack4(p[v], g.inv);
-            if (BF16) *(u32x2*)q = u32x2{q0, g.inv == 0.0f ? 0u : pack4(p[v] + E - 4, g.inv)};
+            if (E == 8) *(u32x2*)q = u32x2{q0, g.inv == 0.0f ? 0u : pack4(p[v] + E - 4, g.inv)};
             else *q = q0;
         }
         if (l == 0) a.s[row] = OP == OP_NORM && g.inv != 0.0f ? norm_scale(top, ss, C, a.eps) : g.step;
@@ -315,7 +330,7 @@ __global__ __launch_bounds__(1024) void k_rows_i8_long(RowArgs a) {
 template <bool BF16, int LPR>
 __global__ __launch_bounds__(256) void k_rows_back(const unsigned char* q, const float* s, void* dst, size_t ldq,
                                                    size_t ldd, int rows, int C) {
-    constexpr int E = G<BF16>, RPB = 256 / LPR;
+    constexpr int E = BF16 ? 8 : 4, RPB = 256 / LPR;
     const int l = threadIdx.x % LPR;
     for (size_t row = (size_t)blockIdx.x * RPB + threadIdx.x / LPR; row < (size_t)rows; row += (size_t)gridDim.x * RPB) {
         const float sc = s[row];
@@ -346,25 +361,36 @@ __global__ __launch_bounds__(256) void k_rows_back(const unsigned char* q, const
     }
 }
 
+/* A workgroup a row where that is one to eight waves (49152 x 960 43.5 -> 41.8 us, 4096 x 8192 SwiGLU 54.0 -> 51.8);
+ * the shortest rows and the longest take what the CUs hold, in turns (1000000 x 64 66.6 -> 58.0, 2048 x 16384 35.9 -> 33.1). */
 template <int OP, bool BF16, int LPR, int NV>
 void go(const RowArgs& r, hipStream_t s) {
     constexpr int NT = LPR < 64 ? 64 : LPR, RPW = NT / LPR;
-    const long wgs = ((long)r.rows + RPW - 1) / RPW, most = 256 * 32 * 64 / NT;
+    constexpr long most = LPR >= 64 && LPR <= 512 ? MAX_GRID : 256 * 32 * 64 / NT;
+    const long wgs = ((long)r.rows + RPW - 1) / RPW;
     hipLaunchKernelGGL((k_rows_i8<OP, BF16, LPR, NV>), dim3((unsigned)(wgs < most ? wgs : most)), dim3(NT), 0, s, r);
 }
 
+/* Lanes a row and groups a lane, the fewest lanes that hold the row (8192 x 2560
+ * bf16 SwiGLU, 320 groups: 26.7 us with two on each of 256 lanes, 19.3 with three on 128).
+ * NV is the smallest that does, so all but a lane's last group lie inside the row. */
 template <int OP, bool BF16>
 void launch_form(const RowArgs& r, hipStream_t s) {
-    const int groups = (int)(i8_row_bytes(r.C) / G<BF16>); /* of 16 bytes of source, the zeros behind a row's codes among them */
+    const int groups = (int)(i8_row_bytes(r.C) / G<OP, BF16>); /* the zeros behind a row's codes among them */
     if (groups <= 16) go<OP, BF16, 16, 1>(r, s);
     else if (groups <= 32) go<OP, BF16, 16, 2>(r, s);
     else if (groups <= 64) go<OP, BF16, 64, 1>(r, s);
     else if (groups <= 128) go<OP, BF16, 64, 2>(r, s);
+    else if (groups <= 192) go<OP, BF16, 64, 3>(r, s);
     else if (groups <= 256) go<OP, BF16, 64, 4>(r, s);
-    else if (groups <= 512) go<OP, BF16, 256, 2>(r, s);
+    else if (groups <= 384) go<OP, BF16, 128, 3>(r, s);
+    else if (groups <= 512) go<OP, BF16, 128, 4>(r, s);
+    else if (groups <= 768) go<OP, BF16, 256, 3>(r, s);
     else if (groups <= 1024) go<OP, BF16, 256, 4>(r, s);
+    else if (groups <= 1536) go<OP, BF16, 512, 3>(r, s);
     else if (groups <= 2048) go<OP, BF16, 512, 4>(r, s);
-    else if (groups <= 4096) go<OP, BF16, 1024, 4>(r, s);
+    else if (groups <= 3072 && OP != OP_NORM) go<OP, BF16, 1024, 3>(r, s);
+    else if (groups <= 4096 && OP != OP_NORM) go<OP, BF16, 1024, 4>(r, s);
     else
         hipLaunchKernelGGL((k_rows_i8_long<OP, BF16>), dim3((unsigned)(r.rows < MAX_GRID ? r.rows : MAX_GRID)), dim3(1024),
                            0, s, r);
@@ -382,7 +408,8 @@ template <bool BF16>
 void launch_back(const bmk_launch_t* a, int M, int C, int ldq, int ldd) {
     const unsigned char* q = (const unsigned char*)a->dev[0];
     const float* s = (const float*)a->dev[1];
-    const int groups = (C + G<BF16> - 1) / G<BF16>;
+    constexpr int E = BF16 ? 8 : 4;
+    const int groups = (C + E - 1) / E;
     auto grid = [&](int rpb) {
         const long n = ((long)M + rpb - 1) / rpb;
         return dim3((unsigned)(n < MAX_GRID ? n : MAX_GRID));
