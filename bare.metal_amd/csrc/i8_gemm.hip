@@ -370,19 +370,20 @@ __global__ __launch_bounds__(64 * MW * NW, 2) void k_i8_tile(GemmArgs g) {
 /* ------------------------------------------------------------------ */
 /* 256 x 256 */
 
-constexpr int PAIR_RING = 5;
 constexpr size_t PAIR_MAX_LD = (size_t)1 << 23; /* 256 rows of it stay inside 32-bit offsets */
 
 /* Eight waves of 128 x 64 (2 x 4), two on each SIMD, in two groups of four a
  * half turn apart: while one group's 16 MFMAs of a half stage run, the other
- * reads the fragments of its next, and a barrier ends each turn.  What bounds
- * it: LDS (96 KB read and 32 KB written of a stage's 64 columns) and, on every CU
- * at once, the part's power: 4096 x 4096 x 8192 takes 97 us on zeros and 125 on
- * codes of a normal distribution.  Against it: the whole workgroup
- * in step and fragments read as they are used 173 us; four waves of 128 x 128 142; turns
- * without fragments read ahead 132; a ring of four stages 129.
- * A stage of 64 columns is 32 KB; the ring of five fills the CU's LDS, and four
- * stages are under way or landed while one is multiplied. */
+ * reads the fragments of its next, and a barrier ends each turn.
+ * A stage of 64 columns is 32 KB; the ring of five fills the CU's LDS.  Stages 2t
+ * and 2t + 1 share the 128-byte lines of their rows, and a CU fetches whole lines
+ * (from L2 84 KB/us in 128-byte pieces of rows, 47 in 64-byte ones), so the two are
+ * requested line by line, in two halves.
+ * What bounds it: on every CU at once, the part's power (4096 x 4096 x 8192 takes 97 us
+ * on zeros, 115 on codes of a normal distribution), then the turns (MFMAs alone 96).
+ * Against those 115 us: each stage requested by itself 125, the two at once 123;
+ * turns without fragments read ahead 132; four waves of 128 x 128 142; the
+ * whole workgroup in step and fragments read as they are used 173. */
 template <bool BF16>
 __global__ __launch_bounds__(512, 2) void k_i8_pair(GemmArgs g) {
     constexpr int W = 8, MW = 2, TM = 8, TN = 4, HM = TM / 2, BM = 256, BN = 256, BK = 64, SB = (BM + BN) * BK;
@@ -404,12 +405,16 @@ __global__ __launch_bounds__(512, 2) void k_i8_pair(GemmArgs g) {
         ro[i] = i * W * 16 < BM ? min(row, g.M - 1 - m0) * (unsigned int)g.lda
                                 : min(row - BM, g.OC - 1 - n0) * (unsigned int)g.ldw;
     }
-    auto request = [&](int stage, unsigned char* buf) {
-        const unsigned int k = min(stage * BK + group, last16);
+    /* loads i0 .. i0 + NI / 2 - 1 of stages `stage` (even) and stage + 1 */
+    auto request = [&](int stage, unsigned char* even, unsigned char* odd, int i0) {
+        const unsigned int k0 = min(stage * BK + group, last16), k1 = min(stage * BK + BK + group, last16);
 #pragma unroll
-        for (int i = 0; i < NI; i++)
-            __builtin_amdgcn_global_load_lds((const gvoid*)((i * W * 16 < BM ? ab : wb) + (ro[i] + k)),
-                                             (lvoid*)(buf + (i * W + wave) * 1024), 16, 0, 0);
+        for (int j = 0; j < NI / 2; j++) {
+            const int i = i0 + j;
+            const unsigned char* p = i * W * 16 < BM ? ab : wb;
+            __builtin_amdgcn_global_load_lds((const gvoid*)(p + (ro[i] + k0)), (lvoid*)(even + (i * W + wave) * 1024), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((const gvoid*)(p + (ro[i] + k1)), (lvoid*)(odd + (i * W + wave) * 1024), 16, 0, 0);
+        }
     };
     i32x4 acc[TM][TN];
     clear(acc);
@@ -440,65 +445,94 @@ __global__ __launch_bounds__(512, 2) void k_i8_pair(GemmArgs g) {
                     __builtin_amdgcn_mfma_i32_16x16x64_i8(b.v[j], a.v[i], acc[i + half * HM][j], 0, 0, 0);
         __builtin_amdgcn_s_setprio(0);
     };
-    /* Turns are counted by barriers: the first group reads for a stage's second
-     * half in turn 4s and for stage s + 1 in turn 4s + 2, the other group a
-     * turn later.  So stage s + 1 has to have landed for all before turn
-     * 4s + 2 (each wave waits for its own part in its first reads of stage s),
-     * and stage s has been read by all, the reads waited for, before turn 4s + 5:
-     * its buffer is requested again in the second reads of stage s + 1, turn 4s + 6
-     * at the earliest. */
-    auto body = [&](int stage, const unsigned char* buf, const unsigned char* next, unsigned char* before, const Cols& b,
-                    Cols& bn) {
-        read_rows(buf, 1, a1);
-        wait_loads<(PAIR_RING - 3) * NI, false>();
+    auto turn = [&](const Rows& a, const Cols& b, int half) {
         barrier();
-        multiply(a0, b, 0);
-        barrier();
-        read_cols(next, bn);
-        read_rows(next, 0, a0);
-        request(stage + PAIR_RING - 1, before);
-        barrier();
-        multiply(a1, b, 1);
+        multiply(a, b, half);
         barrier();
     };
-    request(0, s0);
-    request(1, s1);
-    request(2, s2);
-    request(3, s3);
-    wait_loads<(PAIR_RING - 2) * NI, false>();
+    /* Turns are counted by barriers: the first group reads for a stage's second
+     * half in turn 4s and for the first half of stage s + 1 in turn 4s + 2, the
+     * other group a turn later.  So stage s + 1 has to have landed for all before turn
+     * 4s + 2 (each wave waits for its own part in its first reads of stage s),
+     * and stage s has been read by all, the reads waited for, before turn 4s + 5.
+     * In two(), s odd, stages s + 3 and s + 4 take the places of s - 2 and s - 1 from turn
+     * 4s + 2 on.  Its waits: stage s + 1 has landed when at most the last load, of stage s + 2, is
+     * under way; stage s + 2 when only the first half of the next request is. */
+    auto two = [&](int s, const unsigned char* x, const unsigned char* y, const unsigned char* next, unsigned char* even,
+                   unsigned char* odd) {
+        read_rows(x, 1, a1);
+        wait_loads<1, false>();
+        turn(a0, b1, 0);
+        read_cols(y, b0);
+        read_rows(y, 0, a0);
+        request(s + 3, even, odd, 0);
+        turn(a1, b1, 1);
+        read_rows(y, 1, a1);
+        wait_loads<NI, false>();
+        request(s + 3, even, odd, NI / 2);
+        turn(a0, b0, 0);
+        read_cols(next, b1);
+        read_rows(next, 0, a0);
+        turn(a1, b0, 1);
+    };
+    /* a stage without a request; the next one has landed */
+    auto one = [&](const unsigned char* x, const unsigned char* next, const Cols& b, Cols& bn) {
+        read_rows(x, 1, a1);
+        turn(a0, b, 0);
+        read_cols(next, bn);
+        read_rows(next, 0, a0);
+        turn(a1, b, 1);
+    };
+    request(0, s0, s1, 0);
+    request(0, s0, s1, NI / 2);
+    request(2, s2, s3, 0);
+    request(2, s2, s3, NI / 2);
+    wait_loads<2 * NI, false>(); /* stages 0 and 1 */
     barrier();
     read_cols(s0, b0);
     read_rows(s0, 0, a0);
     if (wave >= W / 2) barrier(); /* the half turn */
-    int stage = 0;
-    for (; stage + PAIR_RING <= last; stage += PAIR_RING) {
-        body(stage, s0, s1, s4, b0, b1);
-        body(stage + 1, s1, s2, s0, b1, b0);
-        body(stage + 2, s2, s3, s1, b0, b1);
-        body(stage + 3, s3, s4, s2, b1, b0);
-        body(stage + 4, s4, s0, s3, b0, b1);
-        b0 = b1;
-    }
     const unsigned char* end = s0;
-    if (stage < last) {
-        body(stage, s0, s1, s4, b0, b1);
-        b0 = b1;
+    if (last > 0) {
+        one(s0, s1, b0, b1);
+        int s = 1;
+        for (; s + 10 <= last; s += 10) {
+            two(s, s1, s2, s3, s4, s0);
+            two(s + 2, s3, s4, s0, s1, s2);
+            two(s + 4, s0, s1, s2, s3, s4);
+            two(s + 6, s2, s3, s4, s0, s1);
+            two(s + 8, s4, s0, s1, s2, s3);
+        }
+        const int rest = last - s;
+        const unsigned char* next = s2;
         end = s1;
-    }
-    if (stage + 1 < last) {
-        body(stage + 1, s1, s2, s0, b0, b1);
-        b0 = b1;
-        end = s2;
-    }
-    if (stage + 2 < last) {
-        body(stage + 2, s2, s3, s1, b0, b1);
-        b0 = b1;
-        end = s3;
-    }
-    if (stage + 3 < last) {
-        body(stage + 3, s3, s4, s2, b0, b1);
-        b0 = b1;
-        end = s4;
+        if (rest >= 2) {
+            two(s, s1, s2, s3, s4, s0);
+            end = s3;
+            next = s4;
+        }
+        if (rest >= 4) {
+            two(s + 2, s3, s4, s0, s1, s2);
+            end = s0;
+            next = s1;
+        }
+        if (rest >= 6) {
+            two(s + 4, s0, s1, s2, s3, s4);
+            end = s2;
+            next = s3;
+        }
+        if (rest >= 8) {
+            two(s + 6, s2, s3, s4, s0, s1);
+            end = s4;
+            next = s0;
+        }
+        if (rest & 1) {
+            wait_loads<0, false>(); /* ahead of the first reads' barrier: the next stage, for all */
+            one(end, next, b1, b0);
+            end = next;
+        } else {
+            b0 = b1;
+        }
     }
     read_rows(end, 1, a1);
     const int left = g.C - last * BK - 16 * (lane >> 4);

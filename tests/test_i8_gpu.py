@@ -325,6 +325,33 @@ def test_matmul(be, M, C, OC, bf16):
         check_product(from_bf16(got[:, :OC]) if bf16 else got[:, :OC], y, want, bf16, bias)
 
 
+# rows, outputs, and sums of every count of stages up to a full turn of the rings and past it: few outputs, tiles of
+# 32 x 32, 32 x 64, 64 x 64, 128 x 64, 128 x 128 (stages of 64 columns, of 128) and 256 x 256, ragged on both sides
+FORMS = [(9, 700), (13, 16399), (200, 600), (395, 800), (700, 1000), (1000, 1300), (1601, 1590), (3300, 3290)]
+SUMS = [1, 15, 64, 65, 100, 128, 129, 200, 257, 300, 384, 400, 450, 513, 576, 640, 700, 770, 832, 900, 1001, 1024, 1100, 1300,
+        1500]
+
+
+@pytest.mark.parametrize("M,OC", FORMS)
+def test_matmul_every_form(be, M, OC):
+    """Whole sums (scales of one), for equality: random codes' sums are whole fp32 numbers, in numpy's products too."""
+    rng = np.random.default_rng(M)
+    ld = ld16(max(SUMS))
+    a, w = rng.integers(-128, 128, (M, ld)).astype(np.int8), rng.integers(-128, 128, (OC, ld)).astype(np.int8)
+    ba, bw, one = be.upload(a), be.upload(w), be.upload(np.ones(max(M, OC), np.float32))
+    fa, fw = a.astype(np.float32), w.astype(np.float32)
+    out = marked(be, M * OC * 4)
+    for C in SUMS:
+        if M * OC > 10 ** 7 and C > 1024 and C != 1500:
+            continue
+        assert be.dispatch("matmul_forward_i8", [ba, one, bw, one, one, out, be.params(M, C, OC, 0, ld, ld, OC)], (OC, M),
+                           (256,)) == 0
+        got = out.read(np.float32).reshape(M, OC)
+        want = fa[:, :C] @ fw[:, :C].T
+        assert np.abs(want).max() < 2 ** 24
+        assert np.array_equal(got, want), (C, np.argwhere(got != want)[:4])
+
+
 @pytest.mark.parametrize("M", [1, 20, 300])
 def test_matmul_longest_sums(be, M):
     """The longest row of the lowest codes stays inside 32 bits, and its sum is exact."""
