@@ -44,7 +44,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 /* Elements a lane takes at once: 16 bytes of the source, or with fp32 operands
  * beside a bf16 source (the norm) 16 bytes of those, so that every access of a
- * wave is one span (eight elements a lane there: 72 us for 8192 x 4096 against 68). */
+ * wave is one span (eight elements a lane there: 70 us for 8192 x 4096 against 61). */
 template <int OP, bool BF16> constexpr int G = BF16 && OP != OP_NORM ? 8 : 4;
 
 /* Loads on an element's boundary.  Rows are read once, so past the caches
@@ -326,7 +326,8 @@ __global__ __launch_bounds__(1024) void k_rows_i8_long(RowArgs a) {
     }
 }
 
-/* code * scale: LPR lanes a row, 8 (to bf16) or 4 codes a lane and step, so that a lane stores 16 bytes */
+/* code * scale: LPR lanes a row, 8 (to bf16) or 4 codes a lane and step, so that a lane stores 16 bytes.  HBM-bound: 49152 x
+ * 960 to bf16 21.7 us (6.5 TB/s, the codes from the Infinity Cache), 8192 x 4096 15.4 (6.5). */
 template <bool BF16, int LPR>
 __global__ __launch_bounds__(256) void k_rows_back(const unsigned char* q, const float* s, void* dst, size_t ldq,
                                                    size_t ldd, int rows, int C) {
@@ -345,7 +346,8 @@ __global__ __launch_bounds__(256) void k_rows_back(const unsigned char* q, const
                 u32x4 o;
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    o[i] = BF16 ? __builtin_bit_cast(unsigned int, __builtin_convertvector(f32x2{v[(2 * i) % E], v[(2 * i + 1) % E]}, bf16x2))
+                    o[i] = BF16 ? __builtin_bit_cast(unsigned int, __builtin_convertvector(
+                                                                       f32x2{v[(2 * i) % E], v[(2 * i + 1) % E]}, bf16x2))
                                 : __float_as_uint(v[i]);
                 if (BF16) __builtin_memcpy(__builtin_assume_aligned((unsigned short*)dst + row * ldd + c, 2), &o, 16);
                 else __builtin_memcpy(__builtin_assume_aligned((float*)dst + row * ldd + c, 4), &o, 16);
@@ -371,6 +373,18 @@ void go(const RowArgs& r, hipStream_t s) {
     hipLaunchKernelGGL((k_rows_i8<OP, BF16, LPR, NV>), dim3((unsigned)(wgs < most ? wgs : most)), dim3(NT), 0, s, r);
 }
 
+/* Past 2048 groups: sixteen waves a row, or, for the norm, whose operands do not fit their registers, the form that reads
+ * twice. */
+template <int OP, bool BF16>
+void launch_wide(const RowArgs& r, int groups, hipStream_t s) {
+    if constexpr (OP != OP_NORM) {
+        if (groups <= 3 * 1024) return go<OP, BF16, 1024, 3>(r, s);
+        if (groups <= 4 * 1024) return go<OP, BF16, 1024, 4>(r, s);
+    }
+    hipLaunchKernelGGL((k_rows_i8_long<OP, BF16>), dim3((unsigned)(r.rows < MAX_GRID ? r.rows : MAX_GRID)), dim3(1024), 0, s,
+                       r);
+}
+
 /* Lanes a row and groups a lane, the fewest lanes that hold the row (8192 x 2560
  * bf16 SwiGLU, 320 groups: 26.7 us with two on each of 256 lanes, 19.3 with three on 128).
  * NV is the smallest that does, so all but a lane's last group lie inside the row. */
@@ -389,11 +403,7 @@ void launch_form(const RowArgs& r, hipStream_t s) {
     else if (groups <= 1024) go<OP, BF16, 256, 4>(r, s);
     else if (groups <= 1536) go<OP, BF16, 512, 3>(r, s);
     else if (groups <= 2048) go<OP, BF16, 512, 4>(r, s);
-    else if (groups <= 3072 && OP != OP_NORM) go<OP, BF16, 1024, 3>(r, s);
-    else if (groups <= 4096 && OP != OP_NORM) go<OP, BF16, 1024, 4>(r, s);
-    else
-        hipLaunchKernelGGL((k_rows_i8_long<OP, BF16>), dim3((unsigned)(r.rows < MAX_GRID ? r.rows : MAX_GRID)), dim3(1024),
-                           0, s, r);
+    else launch_wide<OP, BF16>(r, groups, s);
 }
 
 template <int OP>
@@ -414,12 +424,14 @@ void launch_back(const bmk_launch_t* a, int M, int C, int ldq, int ldd) {
         const long n = ((long)M + rpb - 1) / rpb;
         return dim3((unsigned)(n < MAX_GRID ? n : MAX_GRID));
     };
+    void* dst = a->dev[2];
+    const size_t lq = ldq, ld = ldd;
     if (groups <= 32)
-        hipLaunchKernelGGL((k_rows_back<BF16, 16>), grid(16), dim3(256), 0, a->stream, q, s, a->dev[2], (size_t)ldq, (size_t)ldd, M, C);
+        hipLaunchKernelGGL((k_rows_back<BF16, 16>), grid(16), dim3(256), 0, a->stream, q, s, dst, lq, ld, M, C);
     else if (groups <= 256)
-        hipLaunchKernelGGL((k_rows_back<BF16, 64>), grid(4), dim3(256), 0, a->stream, q, s, a->dev[2], (size_t)ldq, (size_t)ldd, M, C);
+        hipLaunchKernelGGL((k_rows_back<BF16, 64>), grid(4), dim3(256), 0, a->stream, q, s, dst, lq, ld, M, C);
     else
-        hipLaunchKernelGGL((k_rows_back<BF16, 256>), grid(1), dim3(256), 0, a->stream, q, s, a->dev[2], (size_t)ldq, (size_t)ldd, M, C);
+        hipLaunchKernelGGL((k_rows_back<BF16, 256>), grid(1), dim3(256), 0, a->stream, q, s, dst, lq, ld, M, C);
 }
 
 /* bytes of a row-major matrix of rows ld elements apart */
@@ -429,7 +441,8 @@ size_t span(int rows, int C, int ld, size_t esz) { return (((size_t)rows - 1) * 
 int launch_quantize_rows(const bmk_launch_t* a, bool bf16) {
     BMK_NEED_BYTES(a, 3, 16, "params");
     const int M = bmk_pi(a, 3, 0), C = bmk_pi(a, 3, 1), lds = bmk_pi(a, 3, 2), ldq = bmk_pi(a, 3, 3);
-    BMK_REQUIRE(M >= 0 && M <= I8_MAX_DIM && C > 0 && C <= I8_MAX_DIM && lds >= C, "quantize_rows_i8: bad shape M=%d C=%d lds=%d", M, C, lds);
+    BMK_REQUIRE(M >= 0 && M <= I8_MAX_DIM && C > 0 && C <= I8_MAX_DIM && lds >= C,
+                "quantize_rows_i8: bad shape M=%d C=%d lds=%d", M, C, lds);
     if (M == 0) return 0;
     const size_t esz = bf16 ? 2 : 4;
     BMK_NEED_BYTES(a, 0, span(M, C, lds, esz), "src");
@@ -489,7 +502,8 @@ int launch_rmsnorm_i8(const bmk_launch_t* a, bool bf16) {
 int launch_swiglu_i8(const bmk_launch_t* a, bool bf16) {
     BMK_NEED_BYTES(a, 4, 16, "params");
     const int N = bmk_pi(a, 4, 0), H = bmk_pi(a, 4, 1), ld = bmk_pi(a, 4, 2), ldq = bmk_pi(a, 4, 3);
-    BMK_REQUIRE(N >= 0 && N <= I8_MAX_DIM && H > 0 && H <= I8_MAX_DIM && ld >= H, "swiglu_forward_i8: bad shape N=%d H=%d ld=%d", N, H, ld);
+    BMK_REQUIRE(N >= 0 && N <= I8_MAX_DIM && H > 0 && H <= I8_MAX_DIM && ld >= H,
+                "swiglu_forward_i8: bad shape N=%d H=%d ld=%d", N, H, ld);
     if (N == 0) return 0;
     const size_t esz = bf16 ? 2 : 4;
     BMK_NEED_BYTES(a, 0, span(N, H, ld, esz), "gate");
@@ -514,7 +528,8 @@ int launch_swiglu_i8(const bmk_launch_t* a, bool bf16) {
 int launch_dequantize_rows(const bmk_launch_t* a, bool bf16) {
     BMK_NEED_BYTES(a, 3, 16, "params");
     const int M = bmk_pi(a, 3, 0), C = bmk_pi(a, 3, 1), ldq = bmk_pi(a, 3, 2), ldd = bmk_pi(a, 3, 3);
-    BMK_REQUIRE(M >= 0 && M <= I8_MAX_DIM && C > 0 && C <= I8_MAX_DIM && ldd >= C, "dequantize_rows_i8: bad shape M=%d C=%d ldd=%d", M, C, ldd);
+    BMK_REQUIRE(M >= 0 && M <= I8_MAX_DIM && C > 0 && C <= I8_MAX_DIM && ldd >= C,
+                "dequantize_rows_i8: bad shape M=%d C=%d ldd=%d", M, C, ldd);
     if (M == 0) return 0;
     const size_t esz = bf16 ? 2 : 4;
     BMK_NEED_CODES(a, 0, M, C, ldq, "codes");
