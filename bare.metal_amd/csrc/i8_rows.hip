@@ -386,14 +386,17 @@ void launch_wide(const RowArgs& r, int groups, hipStream_t s) {
 }
 
 /* Lanes a row and groups a lane, the fewest lanes that hold the row (8192 x 2560
- * bf16 SwiGLU, 320 groups: 26.7 us with two on each of 256 lanes, 19.3 with three on 128).
+ * bf16 SwiGLU, 320 groups: 26.7 us with two on each of 256 lanes, 19.3 with three on 128; 46427 x
+ * 192 quantized, 48 groups: 14.0 with one on each of 64, 9.0 with three on 16; 65536 x 256 19.5 / 15.1, but the
+ * norm of 32768 x 256, with three operands a group, 19.0 / 20.0).
  * NV is the smallest that does, so all but a lane's last group lie inside the row. */
 template <int OP, bool BF16>
 void launch_form(const RowArgs& r, hipStream_t s) {
     const int groups = (int)(i8_row_bytes(r.C) / G<OP, BF16>); /* the zeros behind a row's codes among them */
     if (groups <= 16) go<OP, BF16, 16, 1>(r, s);
     else if (groups <= 32) go<OP, BF16, 16, 2>(r, s);
-    else if (groups <= 64) go<OP, BF16, 64, 1>(r, s);
+    else if (groups <= 48) go<OP, BF16, 16, 3>(r, s);
+    else if (groups <= 64) go<OP, BF16, OP == OP_QUANT ? 16 : 64, OP == OP_QUANT ? 4 : 1>(r, s);
     else if (groups <= 128) go<OP, BF16, 64, 2>(r, s);
     else if (groups <= 192) go<OP, BF16, 64, 3>(r, s);
     else if (groups <= 256) go<OP, BF16, 64, 4>(r, s);

@@ -63,7 +63,7 @@ def check_codes(buf, want, ldq, C, lead=0):
     assert bad.size == 0, (bad[:8], raw[bad[:8]].view(np.int8), exp[bad[:8]].view(np.int8))
 
 
-SHAPES = [(1, 1), (2, 3), (5, 12), (3, 15), (2, 16), (5, 17), (1, 64), (7, 100), (3, 200), (4, 255), (3, 256), (3, 300), (2, 500), (2, 576), (3, 960), (9, 1001),
+SHAPES = [(1, 1), (2, 3), (5, 12), (3, 15), (2, 16), (5, 17), (1, 64), (7, 100), (5, 150), (3, 200), (4, 255), (3, 256), (3, 300), (2, 500), (2, 576), (3, 960), (9, 1001),
           (2, 1024), (2, 1028), (2, 2047), (3, 2560), (2, 4096), (3, 4100), (1, 8192), (2, 10007), (2, 13000), (2, 16384), (2, 20011), (2, 32768), (1, 49152), (3, 40001), (333, 33),
           (1025, 8)]
 
