@@ -564,14 +564,20 @@ void launch(GemmArgs g, hipStream_t s) {
         const long n = (long)g.tiles_m * g.tiles_n;
         return n <= MAX_GRID_X ? dim3((unsigned)n) : dim3(MAX_GRID_X, (unsigned)tiles((int)n, MAX_GRID_X));
     };
-    /* up to 16 rows, or few outputs in all (64 tiles of 32 x 32: 17 x 960 x 960 2.9 us against 4.2 in those, 100 x
-     * 8000 x 50 7.2 / 9.0, 64 x 2560 x 960 4.6 / 5.1; with 320 tiles, 48 x 960 x 5120, 4.5 / 4.0) */
-    if (g.M <= 16 || tiles(g.M, 32) * tiles(g.OC, 32) <= 64) {
-        /* more than 8 rows over many outputs share their rows' reads: 16 x 4096 x 16384 17.5 us / 13.9 with four
-         * tiles a wave, 16 x 960 x 49152 10.2 / 9.6; 16 x 8192 x 8192 16.9 / 20.9 */
-        if (g.M > 8 && g.M <= 16 && g.OC >= 16384) {
+    /* up to 16 rows, or few outputs in all: 64 tiles of 32 x 32 (17 x 960 x 960 2.9 us against 4.2 in those, 128 x 8000 x
+     * 512 8.8 / 14.2, 64 x 2560 x 960 4.6 / 5.1), or twice as many and a long sum (67 x 6978 x 1216 9.7 / 12.5, 64 x 8000 x 2048
+     * 10.2 / 14.2, 32 x 4096 x 4096 8.1 / 8.6; with 256 of them, 64 x 4096 x 4096, 13.0 / 8.7) */
+    const long t32 = tiles(g.M, 32) * tiles(g.OC, 32);
+    if (g.M <= 16 || t32 <= 64 || (t32 <= 128 && g.C >= 2048)) {
+        /* two or four tiles of outputs a wave share their rows' reads: two past 64 tiles (67 x 6978 x 1216 11.1 us with one);
+         * four where more than 8 rows meet many outputs (16 x 4096 x 16384 17.5 us with one, 13.9; 16 x 960 x 49152 10.2 /
+         * 9.6; but 16 x 8192 x 8192 16.9 / 20.9) */
+        if (g.M <= 16 && g.M > 8 && g.OC >= 16384) {
             const dim3 d = grid(16, 64);
             hipLaunchKernelGGL((k_i8_few<4, 4, 4, BF16>), d, dim3(256), 0, s, g);
+        } else if (g.M > 16 && t32 > 64) {
+            const dim3 d = grid(16, 32);
+            hipLaunchKernelGGL((k_i8_few<4, 2, 2, BF16>), d, dim3(256), 0, s, g);
         } else {
             const dim3 d = grid(16, 16);
             hipLaunchKernelGGL((k_i8_few<4, 1, 2, BF16>), d, dim3(256), 0, s, g);
@@ -580,9 +586,8 @@ void launch(GemmArgs g, hipStream_t s) {
     }
     /* 256 x 256 where its last round fills the CUs well enough: 4096 x 960 x 5120 (320 tiles, 62%) 38.5 us against 40.3 in
      * 128 x 128 tiles, 1024 x 4096 x 4096 (64 tiles, 25%) 40.8 / 21, 2048 x 2048 x 2048 (25%) 24 / 12.5.  Else the largest tile
-     * that FILL of are there, or 32 x 32.  us in 128 x 128, 128 x 64, 64 x 64, 32 x 64 and 32 x 32 tiles:
-     * 512 x 960 x 5120 7.3, 8.8, 8.7, 9.7, 10.8; 777 x 2500 x 2000 12.0, 11.2, 12.4, 18.5, 20.7; 512 x 2560 x 960 10.0, 7.8, 6.2, 5.4,
-     * 5.6; 333 x 960 x 960 6.7, 5.4, 4.4, 3.9, 4.0; 64 x 960 x 2560 6.9, 5.0, 4.7, 4.0, 3.6. */
+     * that FILL of are there, or 32 x 32.  us in 128 x 128, 128 x 64, 64 x 64, 32 x 64 and 32 x 32 tiles: 512 x 960 x
+     * 5120 7.3, 8.8, 8.7, 9.7, 10.8; 777 x 2500 x 2000 12.0, 11.2, 12.4, 18.5, 20.7; 512 x 2560 x 960 10.0, 7.8, 6.2, 5.4, 5.6; 333 x 960 x 960 6.7, 5.4, 4.4, 3.9, 4.0; 64 x 960 x 2560 6.9, 5.0, 4.7, 4.0, 3.6. */
     const long big = tiles(g.M, 256) * tiles(g.OC, 256), rounds = (big + CUS - 1) / CUS;
     if (big * 10 >= rounds * CUS * 6 && g.lda <= PAIR_MAX_LD && g.ldw <= PAIR_MAX_LD) {
         const dim3 d = grid(256, 256);

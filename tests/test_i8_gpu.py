@@ -63,9 +63,9 @@ def check_codes(buf, want, ldq, C, lead=0):
     assert bad.size == 0, (bad[:8], raw[bad[:8]].view(np.int8), exp[bad[:8]].view(np.int8))
 
 
-SHAPES = [(1, 1), (2, 3), (5, 12), (3, 15), (2, 16), (5, 17), (1, 64), (7, 100), (5, 150), (3, 200), (4, 255), (3, 256), (3, 300), (2, 500), (2, 576), (3, 960), (9, 1001),
-          (2, 1024), (2, 1028), (2, 2047), (3, 2560), (2, 4096), (3, 4100), (1, 8192), (2, 10007), (2, 13000), (2, 16384), (2, 20011), (2, 32768), (1, 49152), (3, 40001), (333, 33),
-          (1025, 8)]
+SHAPES = [(1, 1), (2, 3), (5, 12), (3, 15), (2, 16), (5, 17), (1, 64), (7, 100), (5, 150), (3, 200), (4, 255), (3, 256),
+          (3, 300), (2, 500), (2, 576), (3, 960), (9, 1001), (2, 1024), (2, 1028), (2, 2047), (3, 2560), (2, 4096), (3, 4100),
+          (1, 8192), (2, 10007), (2, 13000), (2, 16384), (2, 20011), (2, 32768), (1, 49152), (3, 40001), (333, 33), (1025, 8)]
 
 
 def rows(rng, M, C):
@@ -180,7 +180,8 @@ def test_rmsnorm(be, M, C, bf16):
         br, bw = (be.upload(np.concatenate([np.zeros(shift, np.float32), v.ravel()])) for v in (r, w))
         bh, bq, bs = marked(be, (M * C + shift) * 4 + 16), marked(be, M * ldq + 16), marked(be, 4 * M + 16)
         assert be.dispatch(name, [bx, br, bw, bh, bq, bs, be.params(M, C, ldq, int(res)), be.upload(np.float32([eps]))],
-                           (M,), (256,), offsets=[shift * (2 if bf16 else 4), 4 * shift, 4 * shift, 4 * shift, 0, 0, 0, 0]) == 0
+                           (M,), (256,),
+                           offsets=[shift * (2 if bf16 else 4), 4 * shift, 4 * shift, 4 * shift, 0, 0, 0, 0]) == 0
         raw = bh.read(np.uint8)
         if res:
             assert np.array_equal(raw[4 * shift:4 * (M * C + shift)].view(np.float32), h.ravel())
@@ -325,11 +326,11 @@ def test_matmul(be, M, C, OC, bf16):
         check_product(from_bf16(got[:, :OC]) if bf16 else got[:, :OC], y, want, bf16, bias)
 
 
-# rows, outputs, and sums of every count of stages up to a full turn of the rings and past it: few outputs, tiles of
+# rows, outputs, and sums of every count of stages up to a full turn of the rings and past it: few rows or outputs, tiles of
 # 32 x 32, 32 x 64, 64 x 64, 128 x 64, 128 x 128 (stages of 64 columns, of 128) and 256 x 256, ragged on both sides
-FORMS = [(9, 700), (13, 16399), (200, 600), (395, 800), (700, 1000), (1000, 1300), (1601, 1590), (3300, 3290)]
+FORMS = [(9, 700), (13, 16399), (70, 1000), (200, 600), (395, 800), (700, 1000), (1000, 1300), (1601, 1590), (3300, 3290)]
 SUMS = [1, 15, 64, 65, 100, 128, 129, 200, 257, 300, 384, 400, 450, 513, 576, 640, 700, 770, 832, 900, 1001, 1024, 1100, 1300,
-        1500]
+        1500, 2050, 3001]
 
 
 @pytest.mark.parametrize("M,OC", FORMS)
@@ -342,7 +343,7 @@ def test_matmul_every_form(be, M, OC):
     fa, fw = a.astype(np.float32), w.astype(np.float32)
     out = marked(be, M * OC * 4)
     for C in SUMS:
-        if M * OC > 10 ** 7 and C > 1024 and C != 1500:
+        if M * OC > 10 ** 7 and C > 1024 and C != 1500:  # the largest of them: a product in numpy takes half a second
             continue
         assert be.dispatch("matmul_forward_i8", [ba, one, bw, one, one, out, be.params(M, C, OC, 0, ld, ld, OC)], (OC, M),
                            (256,)) == 0
@@ -366,11 +367,10 @@ def test_matmul_longest_sums(be, M):
     assert (got[:, 0::2] == np.float32(128 * 128 * C)).all() and (got[:, 1::2] == np.float32(-128 * 127 * C)).all()
 
 
-@pytest.mark.parametrize("M", [1, 3, 40])
+@pytest.mark.parametrize("M", [1, 3])
 def test_matmul_rows_past_32_bits(be, M):
     """Rows of tokens, weights and outputs whose offsets pass 2^31 and 2^32 bytes."""
     C, OC, far = 100, 3, 1 << 30
-    M = min(M, 3)
     rng = np.random.default_rng(5)
     a, w = rng.integers(-128, 128, (M, 112)).astype(np.int8), rng.integers(-128, 128, (OC, 112)).astype(np.int8)
     one = be.upload(np.ones(4, np.float32))
@@ -390,6 +390,27 @@ def test_matmul_rows_past_32_bits(be, M):
         assert be.dispatch("copy_buffer", [out, small, be.params(12, dtype=np.int64)], (12,), (256,),
                            offsets=[4 * r * far, 12 * r, 0]) == 0
     assert np.array_equal(small.read(np.float32).reshape(M, OC), (a[:, :C].astype(np.int64) @ w[:, :C].astype(np.int64).T))
+
+
+@pytest.mark.parametrize("M,OC,far", [(20, 2100, 1 << 29), (3300, 3290, 1 << 23), (3300, 3290, (1 << 23) + 16)])
+def test_matmul_tiles_over_far_rows(be, M, OC, far):
+    """Tiles whose tokens' rows lie far apart: past 2^32 bytes from the first, at the widest stride of the largest tiles
+    and just past it."""
+    C = 100
+    rng = np.random.default_rng(far)
+    a, w = rng.integers(-128, 128, (M, 112)).astype(np.int8), rng.integers(-128, 128, (OC, 112)).astype(np.int8)
+    big, src, one = be.alloc((M - 1) * far + 112), be.upload(a), be.upload(np.ones(max(M, OC), np.float32))
+    k, p, enc = be.kernel("copy_buffer"), be.params(112, dtype=np.int64), be.encoder()
+    for r in range(M):
+        assert enc.dispatch(k, [src, big, p], (112,), (256,), [r * 112, r * far, 0]) == 0
+    enc.commit()
+    enc.wait_timed()
+    out = be.alloc(M * OC * 4)
+    assert be.dispatch("matmul_forward_i8", [big, one, be.upload(w), one, one, out, be.params(M, C, OC, 0, far, 112, OC)],
+                       (OC, M), (256,)) == 0
+    want = a[:, :C].astype(np.float32) @ w[:, :C].astype(np.float32).T
+    assert np.array_equal(out.read(np.float32).reshape(M, OC), want)
+    big.free()
 
 
 def test_quantize_rows_past_32_bits(be):
