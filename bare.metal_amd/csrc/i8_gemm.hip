@@ -98,6 +98,7 @@ __device__ __forceinline__ void store_vec(void* out, size_t at, T v) {
  * first, so that a lane stores 8 neighbours: 64 bytes a row and instruction. */
 template <int TM, int TN, bool BF16>
 __device__ __forceinline__ void store_tile(const GemmArgs& g, const i32x4 (&acc)[TM][TN], int m0, int n0) {
+#pragma clang fp contract(off) /* the bias is added to a rounded product */
     const int lane = threadIdx.x & 63, q = lane >> 4;
     f32x4 sw[TN], bv[TN];
 #pragma unroll

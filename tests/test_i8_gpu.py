@@ -353,6 +353,22 @@ def test_matmul_every_form(be, M, OC):
         assert np.array_equal(got, want), (C, np.argwhere(got != want)[:4])
 
 
+@pytest.mark.parametrize("M,OC", [(9, 700), (200, 600), (1000, 1300)])
+def test_matmul_rounds_each_step(be, M, OC):
+    """The sum, its product with the row's scale, that with the channel's, and the bias: four fp32 values, equal to
+    numpy's, whatever the form."""
+    rng = np.random.default_rng(M)
+    C = 300
+    a, w = rng.integers(-128, 128, (M, ld16(C))).astype(np.int8), rng.integers(-128, 128, (OC, ld16(C))).astype(np.int8)
+    sa, sw = np.exp(rng.uniform(-3, 1, M)).astype(np.float32), np.exp(rng.uniform(-3, 1, OC)).astype(np.float32)
+    b = (rng.standard_normal(OC) * 1e4).astype(np.float32)
+    out = marked(be, M * OC * 4)
+    assert be.dispatch("matmul_forward_i8", [be.upload(a), be.upload(sa), be.upload(w), be.upload(sw), be.upload(b), out,
+                                             be.params(M, C, OC, 1, ld16(C), ld16(C), OC)], (OC, M), (256,)) == 0
+    want = (a[:, :C].astype(np.float32) @ w[:, :C].astype(np.float32).T) * sa[:, None] * sw + b  # sums below 2^24: exact
+    assert want.dtype == np.float32 and np.array_equal(out.read(np.float32).reshape(M, OC), want)
+
+
 @pytest.mark.parametrize("M", [1, 20, 300])
 def test_matmul_longest_sums(be, M):
     """The longest row of the lowest codes stays inside 32 bits, and its sum is exact."""
