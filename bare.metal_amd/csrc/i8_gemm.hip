@@ -585,26 +585,30 @@ void launch(GemmArgs g, hipStream_t s) {
         }
         return;
     }
-    /* 256 x 256 where its last round fills the CUs well enough: 4096 x 960 x 5120 (320 tiles, 62%) 38.5 us against 40.3 in
+    /* A tile's side only where more than half of it is there (us in the largest tile that FILL of are there / here: 20 x 960
+     * x 16384 5.8 / 4.1, 64 x 960 x 49152 16.3 / 11.6, 65536 x 960 x 64 19.8 / 13.9, 16384 x 960 x 16 5.8 / 4.0).
+     * 256 x 256 where its last round fills the CUs well enough: 4096 x 960 x 5120 (320 tiles, 62%) 38.5 us against 40.3 in
      * 128 x 128 tiles, 1024 x 4096 x 4096 (64 tiles, 25%) 40.8 / 21, 2048 x 2048 x 2048 (25%) 24 / 12.5.  Else the largest tile
      * that FILL of are there, or 32 x 32.  us in 128 x 128, 128 x 64, 64 x 64, 32 x 64 and 32 x 32 tiles: 512 x 960 x
      * 5120 7.3, 8.8, 8.7, 9.7, 10.8; 777 x 2500 x 2000 12.0, 11.2, 12.4, 18.5, 20.7; 512 x 2560 x 960 10.0, 7.8, 6.2, 5.4, 5.6; 333 x 960 x 960 6.7, 5.4, 4.4, 3.9, 4.0; 64 x 960 x 2560 6.9, 5.0, 4.7, 4.0, 3.6. */
     const long big = tiles(g.M, 256) * tiles(g.OC, 256), rounds = (big + CUS - 1) / CUS;
-    if (big * 10 >= rounds * CUS * 6 && g.lda <= PAIR_MAX_LD && g.ldw <= PAIR_MAX_LD) {
+    auto suits = [&](int bm, int bn) { return g.M > bm / 2 && g.OC > bn / 2; };
+    auto fills = [&](int bm, int bn) { return suits(bm, bn) && tiles(g.M, bm) * tiles(g.OC, bn) >= FILL; };
+    if (suits(256, 256) && big * 10 >= rounds * CUS * 6 && g.lda <= PAIR_MAX_LD && g.ldw <= PAIR_MAX_LD) {
         const dim3 d = grid(256, 256);
         hipLaunchKernelGGL(k_i8_pair<BF16>, d, dim3(512), 0, s, g);
-    } else if (tiles(g.M, 128) * tiles(g.OC, 128) >= FILL) {
+    } else if (fills(128, 128)) {
         const dim3 d = grid(128, 128);
         /* stages of 64 columns for short sums: 2048 x 576 x 3000 11.6 us against 14.3, 4096 x 960 x 5120 40.3 / 42.8 */
         if (g.C < 1024) hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 64, BF16>), d, dim3(512), 0, s, g);
         else hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 128, BF16>), d, dim3(512), 0, s, g);
-    } else if (tiles(g.M, 128) * tiles(g.OC, 64) >= FILL) {
+    } else if (fills(128, 64)) {
         const dim3 d = grid(128, 64);
         hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 2, 128, BF16>), d, dim3(512), 0, s, g);
-    } else if (tiles(g.M, 64) * tiles(g.OC, 64) >= FILL) {
+    } else if (fills(64, 64)) {
         const dim3 d = grid(64, 64);
         hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 128, BF16>), d, dim3(256), 0, s, g);
-    } else if (tiles(g.M, 32) * tiles(g.OC, 64) >= FILL) {
+    } else if (fills(32, 64)) {
         const dim3 d = grid(32, 64);
         hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 2, 128, BF16>), d, dim3(256), 0, s, g);
     } else {

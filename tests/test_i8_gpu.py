@@ -369,6 +369,21 @@ def test_matmul_rounds_each_step(be, M, OC):
     assert want.dtype == np.float32 and np.array_equal(out.read(np.float32).reshape(M, OC), want)
 
 
+@pytest.mark.parametrize("M,OC", [(20, 16390), (33, 10250), (64, 16384), (65, 20010), (128, 49152), (129, 40000), (16400, 16),
+                                  (16384, 33), (33000, 64), (33000, 65), (40000, 128), (40000, 130)])
+def test_matmul_narrow_outputs(be, M, OC):
+    """Few rows by many outputs and few outputs of many rows: tiles no wider than there are, for equality."""
+    rng = np.random.default_rng(M + OC)
+    C, ld = 333, 336
+    a, w = rng.integers(-128, 128, (M, ld)).astype(np.int8), rng.integers(-128, 128, (OC, ld)).astype(np.int8)
+    one, out = be.upload(np.ones(max(M, OC), np.float32)), marked(be, M * OC * 4 + 64)
+    assert be.dispatch("matmul_forward_i8", [be.upload(a), one, be.upload(w), one, one, out,
+                                             be.params(M, C, OC, 0, ld, ld, OC)], (OC, M), (256,)) == 0
+    want = a[:, :C].astype(np.float32) @ w[:, :C].astype(np.float32).T
+    raw = out.read(np.float32)
+    assert np.array_equal(raw[:M * OC].reshape(M, OC), want) and (raw[M * OC:].view(np.uint8) == MARK).all()
+
+
 @pytest.mark.parametrize("M", [1, 20, 300])
 def test_matmul_longest_sums(be, M):
     """The longest row of the lowest codes stays inside 32 bits, and its sum is exact."""
@@ -461,6 +476,86 @@ def test_more_rows_than_workgroups(be):
     assert np.array_equal(bs.read(np.float32), s)
     assert be.dispatch("dequantize_rows_i8", [bq, bs, back, be.params(M, C, 16, C)], (M,), (256,)) == 0
     assert np.array_equal(back.read(np.float32).reshape(M, C), q.astype(np.float32) * s[:, None])
+
+
+@pytest.mark.parametrize("name,M,C", [("quantize_rows_i8", 700, 9000), ("quantize_rows_i8", 600, 13000),
+                                      ("quantize_rows_i8_bf16", 530, 17000), ("quantize_rows_i8", 40001, 150),
+                                      ("quantize_rows_i8_bf16", 33000, 500)])
+def test_quantize_rows_in_turns(be, name, M, C):
+    """More rows than the CUs hold, in the forms whose workgroups take several in turn."""
+    x = np.random.default_rng(C).standard_normal((M, C)).astype(np.float32)
+    bf16 = name.endswith("bf16")
+    if bf16:
+        x = from_bf16(to_bf16(x))
+    q, top, _ = grid(x)
+    bq, bs = marked(be, M * ld16(C) + 16), marked(be, 4 * M)
+    assert be.dispatch(name, [be.upload(to_bf16(x) if bf16 else x), bq, bs, be.params(M, C, C, ld16(C))], (M,), (256,)) == 0
+    assert np.array_equal(bs.read(np.float32), top / np.float32(127))
+    got = bq.read(np.int8)
+    assert (got[M * ld16(C):] == MARK).all()
+    got = got[:M * ld16(C)].reshape(M, ld16(C))
+    assert np.array_equal(got[:, :C], q) and not got[:, C:].any()
+
+
+@pytest.mark.parametrize("M,C", [(33333, 60), (40001, 150), (600, 8200)])
+def test_rmsnorm_in_turns(be, M, C):
+    rng = np.random.default_rng(C)
+    x, r = rng.standard_normal((M, C)).astype(np.float32), rng.standard_normal((M, C)).astype(np.float32)
+    w = rng.uniform(-1.5, 1.5, C).astype(np.float32)
+    h, q, s = norm_ref(x, r, w, float(np.float32(1e-5)))
+    bh, bq, bs = be.upload(r), marked(be, M * ld16(C)), marked(be, 4 * M)
+    assert be.dispatch("rmsnorm_forward_i8", [be.upload(x), bh, be.upload(w), bh, bq, bs, be.params(M, C, ld16(C), 1),
+                                              be.upload(np.float32([1e-5]))], (M,), (256,)) == 0
+    assert np.array_equal(bh.read(np.float32).reshape(M, C), h)
+    got = bq.read(np.int8).reshape(M, ld16(C))
+    assert np.array_equal(got[:, :C], q) and not got[:, C:].any()
+    assert (np.abs(bs.read(np.float32) - s) <= 4 * U32 * s).all()
+
+
+@pytest.mark.parametrize("name,C", [("quantize_rows_i8", 300), ("quantize_rows_i8_bf16", 2049), ("rmsnorm_forward_i8", 270),
+                                    ("rmsnorm_forward_i8_bf16", 600), ("swiglu_forward_i8_bf16", 1030)])
+def test_rows_past_the_largest_launch(be, name, C):
+    """2^20 rows are a launch's most workgroups where a wave or more takes a row: the first and last rows of more than that
+    (those between are zeros)."""
+    extra = 130
+    M, ldq, esz = (1 << 20) + extra, ld16(C), 2 if name.endswith("bf16") else 4
+    rng = np.random.default_rng(C)
+    x, w = rng.standard_normal((2 * extra, C)).astype(np.float32), rng.uniform(0.5, 1.5, C).astype(np.float32)
+    if esz == 2:
+        x = from_bf16(to_bf16(x))
+    src, few = be.alloc(M * C * esz), be.upload(to_bf16(x) if esz == 2 else x)
+    half = extra * C * esz
+    for at, to in ((0, 0), (half, (M - extra) * C * esz)):
+        assert be.dispatch("copy_buffer", [few, src, be.params(half, dtype=np.int64)], (half,), (256,), offsets=[at, to, 0]) == 0
+    codes, bs, back = be.alloc(M * ldq), be.alloc(4 * M), be.alloc(2 * extra * ldq)
+    if name.startswith("quantize"):
+        bufs, p = [src, codes, bs, be.params(M, C, C, ldq)], x
+    elif name.startswith("rmsnorm"):
+        bufs, p = [src, src, be.upload(w), src, codes, bs, be.params(M, C, ldq, 0), be.upload(np.float32([1e-5]))], x * w
+    else:
+        bufs = [src, src, codes, bs, be.params(M, C, C, ldq)]
+        x64 = x.astype(np.float64)
+        p = x64 / (1 + np.exp(-x64)) * x64
+    assert be.dispatch(name, bufs, (M,), (256,)) == 0
+    half = extra * ldq
+    for at, to in ((0, 0), ((M - extra) * ldq, half)):
+        assert be.dispatch("copy_buffer", [codes, back, be.params(half, dtype=np.int64)], (half,), (256,),
+                           offsets=[at, to, 0]) == 0
+    got, s = back.read(np.int8).reshape(2 * extra, ldq), bs.read(np.float32)
+    assert not got[:, C:].any() and not s[extra:-extra].any()
+    s = np.concatenate([s[:extra], s[-extra:]])
+    if name.startswith("swiglu"):
+        top = np.abs(p).max(axis=1)
+        assert (np.abs(got[:, :C] - p * (127 / top)[:, None]) <= 0.5 + 127 * (2 * SILU + 4 * U32)).all()
+        assert (np.abs(s - top / 127) <= (SILU + 2 * U32) * top / 127).all()
+        return
+    q, top, _ = grid(p)
+    assert np.array_equal(got[:, :C], q)
+    if name.startswith("rmsnorm"):
+        want = top / (127 * np.sqrt((x.astype(np.float64) ** 2).mean(axis=1) + float(np.float32(1e-5))))
+        assert (np.abs(s - want) <= 4 * U32 * want).all()
+    else:
+        assert np.array_equal(s, top / np.float32(127))
 
 
 def mlp_buffers(be, rng, N, D, H):
