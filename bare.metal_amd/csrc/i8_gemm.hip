@@ -24,6 +24,8 @@
  */
 #include "i8_common.h"
 
+#include <climits>
+
 namespace {
 
 using namespace bmk;
@@ -553,9 +555,7 @@ __global__ __launch_bounds__(512, 2) void k_i8_pair(GemmArgs g) {
 
 /* ------------------------------------------------------------------ */
 
-constexpr int FILL = 150; /* tiles a launch wants at least */
-
-long tiles(int n, int t) { return ((long)n + t - 1) / t; }
+long tiles(long n, int t) { return (n + t - 1) / t; }
 
 template <bool BF16>
 void launch(GemmArgs g, hipStream_t s) {
@@ -563,7 +563,7 @@ void launch(GemmArgs g, hipStream_t s) {
         g.tiles_m = (int)tiles(g.M, bm);
         g.tiles_n = (int)tiles(g.OC, bn);
         const long n = (long)g.tiles_m * g.tiles_n;
-        return n <= MAX_GRID_X ? dim3((unsigned)n) : dim3(MAX_GRID_X, (unsigned)tiles((int)n, MAX_GRID_X));
+        return n <= MAX_GRID_X ? dim3((unsigned)n) : dim3(MAX_GRID_X, (unsigned)tiles(n, MAX_GRID_X));
     };
     /* up to 16 rows, or few outputs in all: 64 tiles of 32 x 32 (17 x 960 x 960 2.9 us against 4.2 in those, 128 x 8000 x
      * 512 8.8 / 14.2, 64 x 2560 x 960 4.6 / 5.1), or twice as many and a long sum (67 x 6978 x 1216 9.7 / 12.5, 64 x 8000 x 2048
@@ -585,35 +585,37 @@ void launch(GemmArgs g, hipStream_t s) {
         }
         return;
     }
-    /* A tile's side only where more than half of it is there (us in the largest tile that FILL of are there / here: 20 x 960
-     * x 16384 5.8 / 4.1, 64 x 960 x 49152 16.3 / 11.6, 65536 x 960 x 64 19.8 / 13.9, 16384 x 960 x 16 5.8 / 4.0).
-     * 256 x 256 where its last round fills the CUs well enough: 4096 x 960 x 5120 (320 tiles, 62%) 38.5 us against 40.3 in
-     * 128 x 128 tiles, 1024 x 4096 x 4096 (64 tiles, 25%) 40.8 / 21, 2048 x 2048 x 2048 (25%) 24 / 12.5.  Else the largest tile
-     * that FILL of are there, or 32 x 32.  us in 128 x 128, 128 x 64, 64 x 64, 32 x 64 and 32 x 32 tiles: 512 x 960 x
-     * 5120 7.3, 8.8, 8.7, 9.7, 10.8; 777 x 2500 x 2000 12.0, 11.2, 12.4, 18.5, 20.7; 512 x 2560 x 960 10.0, 7.8, 6.2, 5.4, 5.6; 333 x 960 x 960 6.7, 5.4, 4.4, 3.9, 4.0; 64 x 960 x 2560 6.9, 5.0, 4.7, 4.0, 3.6. */
-    const long big = tiles(g.M, 256) * tiles(g.OC, 256), rounds = (big + CUS - 1) / CUS;
-    auto suits = [&](int bm, int bn) { return g.M > bm / 2 && g.OC > bn / 2; };
-    auto fills = [&](int bm, int bn) { return suits(bm, bn) && tiles(g.M, bm) * tiles(g.OC, bn) >= FILL; };
-    if (suits(256, 256) && big * 10 >= rounds * CUS * 6 && g.lda <= PAIR_MAX_LD && g.ldw <= PAIR_MAX_LD) {
-        const dim3 d = grid(256, 256);
-        hipLaunchKernelGGL(k_i8_pair<BF16>, d, dim3(512), 0, s, g);
-    } else if (fills(128, 128)) {
-        const dim3 d = grid(128, 128);
+    /* Else the tile for which the busiest CU has least to move: rounds of 256 tiles times a tile's operands, and four bytes an
+     * output for its stores and its start; of equals the largest.  (Over 330 shapes spread over 17 .. 16384 rows, 64 .. 8192
+     * columns and 16 .. 49152 outputs its choice is 1.1% slower than the best of these on average, 23% at most; the largest tile that
+     * 150 of are there 3.0% and 63%.)  us in 256 x 256, 128 x 128, 128 x 64, 64 x 64, 32 x 64 and 32 x 32 tiles: 4096 x 960 x
+     * 5120 36, 40, 48, 54, 73, 91; 1024 x 4096 x 4096 41, 21, 25 and more; 777 x 2500 x 2000 27, 12.0, 11.2, 12.4, 18.5, 20.7; 512 x 960 x 5120
+     * 15, 7.3, 8.8, 8.7, 9.7, 10.8; 142 x 6784 x 9011 -, 33, 32, 22, 32, 34; 64 x 960 x 49152 16, 14, 14, 12, 13, 16; 512 x
+     * 2560 x 960 26, 10.0, 7.8, 6.2, 5.4, 5.6; 20 x 960 x 16384 13, 6.7, 5.8, 4.7, 4.1, 4.1; 16384 x 960 x 16 14, 7.1, 5.8, 5.0, 4.9, 4.0. */
+    static constexpr int SIDES[6][2] = {{256, 256}, {128, 128}, {128, 64}, {64, 64}, {32, 64}, {32, 32}};
+    const bool near = g.lda <= PAIR_MAX_LD && g.ldw <= PAIR_MAX_LD;
+    int best = 0;
+    long least = LONG_MAX;
+    for (int i = near ? 0 : 1; i < 6; i++) {
+        const int bm = SIDES[i][0], bn = SIDES[i][1];
+        const long cost = tiles(tiles(g.M, bm) * tiles(g.OC, bn), CUS) * ((long)(bm + bn) * g.C + 4l * bm * bn);
+        if (cost < least) {
+            least = cost;
+            best = i;
+        }
+    }
+    const dim3 d = grid(SIDES[best][0], SIDES[best][1]);
+    switch (best) {
+    case 0: hipLaunchKernelGGL(k_i8_pair<BF16>, d, dim3(512), 0, s, g); break;
+    case 1:
         /* stages of 64 columns for short sums: 2048 x 576 x 3000 11.6 us against 14.3, 4096 x 960 x 5120 40.3 / 42.8 */
         if (g.C < 1024) hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 64, BF16>), d, dim3(512), 0, s, g);
         else hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 128, BF16>), d, dim3(512), 0, s, g);
-    } else if (fills(128, 64)) {
-        const dim3 d = grid(128, 64);
-        hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 2, 128, BF16>), d, dim3(512), 0, s, g);
-    } else if (fills(64, 64)) {
-        const dim3 d = grid(64, 64);
-        hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 128, BF16>), d, dim3(256), 0, s, g);
-    } else if (fills(32, 64)) {
-        const dim3 d = grid(32, 64);
-        hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 2, 128, BF16>), d, dim3(256), 0, s, g);
-    } else {
-        const dim3 d = grid(32, 32);
-        hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 1, 128, BF16>), d, dim3(256), 0, s, g);
+        break;
+    case 2: hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 2, 128, BF16>), d, dim3(512), 0, s, g); break;
+    case 3: hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 128, BF16>), d, dim3(256), 0, s, g); break;
+    case 4: hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 2, 128, BF16>), d, dim3(256), 0, s, g); break;
+    default: hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 1, 128, BF16>), d, dim3(256), 0, s, g);
     }
 }
 

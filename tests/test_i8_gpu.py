@@ -369,6 +369,18 @@ def test_matmul_rounds_each_step(be, M, OC):
     assert want.dtype == np.float32 and np.array_equal(out.read(np.float32).reshape(M, OC), want)
 
 
+# one round of tiles on 256 CUs, ragged on both sides, where every sum takes that form: 32 x 32, 32 x 64, 64 x 64, 128 x 64,
+# 128 x 128, 256 x 256
+@pytest.mark.parametrize("M,OC", [(500, 500), (500, 1020), (1000, 1020), (2000, 1020), (2000, 2040), (4000, 4090)])
+def test_matmul_one_round_of_tiles(be, M, OC):
+    test_matmul_every_form(be, M, OC)
+
+
+@pytest.mark.parametrize("far", [1 << 23, (1 << 23) + 16])
+def test_matmul_largest_tiles_over_far_rows(be, far):
+    test_matmul_tiles_over_far_rows(be, 3900, 3850, far)
+
+
 @pytest.mark.parametrize("M,OC", [(20, 16390), (33, 10250), (64, 16384), (65, 20010), (128, 49152), (129, 40000), (16400, 16),
                                   (16384, 33), (33000, 64), (33000, 65), (40000, 128), (40000, 130)])
 def test_matmul_narrow_outputs(be, M, OC):
