@@ -12,7 +12,7 @@
  * a lane then holds four neighbouring outputs of one row.  The 32 x 32 x 32 form
  * is slower on this part (registers only, all CUs, codes of a normal
  * distribution: 2.6 against 4.1 POP/s).
- *   k_i8_few   up to 16 rows, or few outputs: operands straight into registers, the sum split over four waves
+ *   k_i8_few   few rows or outputs: operands straight into registers, the sum split over four or eight waves
  *   k_i8_tile  tiles of 32 x 32 to 128 x 128 through LDS, four or eight waves
  *   k_i8_pair  256 x 256, eight waves in two groups that take turns at the matrix cores and at LDS
  * Operands go to LDS by global_load_lds, which writes 16 bytes a lane at
@@ -165,15 +165,14 @@ __device__ __forceinline__ void clear(i32x4 (&acc)[TM][TN]) {
 }
 
 /* ------------------------------------------------------------------ */
-/* up to 16 rows */
+/* few rows or outputs */
 
 /* 16 x 16 TN outputs a workgroup; wave p of KP takes every KP-th slice of 64
  * columns from p on, U slices' loads in flight, so that a workgroup reads 64 KP
  * neighbouring bytes of a row at once.  The partial sums meet in LDS.
- * What bounds it: reading the weights (8 x 960 -> 49152 9.2 us, 5.1 TB/s from the
- * Infinity Cache), with few outputs the reads of one CU (5 x 8192 -> 500 7.2 us on
- * 32 CUs), else the launch (1 x 960 -> 5120 2.9 us).  Four waves along the sum: one
- * took 5.2 us for 1 x 2560 -> 960, sixteen 4.2, four 3.8 (8 x 960 -> 49152 9.3 / 15 / 9.2). */
+ * What bounds it: reading the weights (1 x 960 -> 49152 11.0 us, 4.3 TB/s), with few outputs the reads of one CU (5 x 8192
+ * -> 500 7.2 us on 32 CUs), else the launch (1 x 960 -> 5120 3.4 us).  Four waves along the sum: one took 5.2 us for 1 x
+ * 2560 -> 960, sixteen 4.2, eight 4.5, four 3.8. */
 template <int KP, int TN, int U, bool BF16>
 __global__ __launch_bounds__(64 * KP) void k_i8_few(GemmArgs g) {
     __shared__ __attribute__((aligned(16))) i32x4 part[KP * TN * 64];
@@ -374,6 +373,8 @@ __global__ __launch_bounds__(64 * MW * NW, 2) void k_i8_tile(GemmArgs g) {
 /* 256 x 256 */
 
 constexpr size_t PAIR_MAX_LD = (size_t)1 << 23; /* 256 rows of it stay inside 32-bit offsets */
+constexpr int PAIR_MIN_C = 320;                 /* five stages; us there / in 128 x 128: 7439 x 113 x 43794 276 / 203, 2279 x 307
+                                                 * x 24615 71 / 63, 1356 x 364 x 24934 42 / 44, 5211 x 452 x 2415 22.5 / 26.8 */
 
 /* Eight waves of 128 x 64 (2 x 4), two on each SIMD, in two groups of four a
  * half turn apart: while one group's 16 MFMAs of a half stage run, the other
@@ -495,47 +496,43 @@ __global__ __launch_bounds__(512, 2) void k_i8_pair(GemmArgs g) {
     read_cols(s0, b0);
     read_rows(s0, 0, a0);
     if (wave >= W / 2) barrier(); /* the half turn */
-    const unsigned char* end = s0;
-    if (last > 0) {
-        one(s0, s1, b0, b1);
-        int s = 1;
-        for (; s + 10 <= last; s += 10) {
-            two(s, s1, s2, s3, s4, s0);
-            two(s + 2, s3, s4, s0, s1, s2);
-            two(s + 4, s0, s1, s2, s3, s4);
-            two(s + 6, s2, s3, s4, s0, s1);
-            two(s + 8, s4, s0, s1, s2, s3);
-        }
-        const int rest = last - s;
-        const unsigned char* next = s2;
-        end = s1;
-        if (rest >= 2) {
-            two(s, s1, s2, s3, s4, s0);
-            end = s3;
-            next = s4;
-        }
-        if (rest >= 4) {
-            two(s + 2, s3, s4, s0, s1, s2);
-            end = s0;
-            next = s1;
-        }
-        if (rest >= 6) {
-            two(s + 4, s0, s1, s2, s3, s4);
-            end = s2;
-            next = s3;
-        }
-        if (rest >= 8) {
-            two(s + 6, s2, s3, s4, s0, s1);
-            end = s4;
-            next = s0;
-        }
-        if (rest & 1) {
-            wait_loads<0, false>(); /* ahead of the first reads' barrier: the next stage, for all */
-            one(end, next, b1, b0);
-            end = next;
-        } else {
-            b0 = b1;
-        }
+    one(s0, s1, b0, b1);
+    int s = 1;
+    for (; s + 10 <= last; s += 10) {
+        two(s, s1, s2, s3, s4, s0);
+        two(s + 2, s3, s4, s0, s1, s2);
+        two(s + 4, s0, s1, s2, s3, s4);
+        two(s + 6, s2, s3, s4, s0, s1);
+        two(s + 8, s4, s0, s1, s2, s3);
+    }
+    const int rest = last - s;
+    const unsigned char *end = s1, *next = s2;
+    if (rest >= 2) {
+        two(s, s1, s2, s3, s4, s0);
+        end = s3;
+        next = s4;
+    }
+    if (rest >= 4) {
+        two(s + 2, s3, s4, s0, s1, s2);
+        end = s0;
+        next = s1;
+    }
+    if (rest >= 6) {
+        two(s + 4, s0, s1, s2, s3, s4);
+        end = s2;
+        next = s3;
+    }
+    if (rest >= 8) {
+        two(s + 6, s2, s3, s4, s0, s1);
+        end = s4;
+        next = s0;
+    }
+    if (rest & 1) {
+        wait_loads<0, false>(); /* ahead of the first reads' barrier: the next stage, for all */
+        one(end, next, b1, b0);
+        end = next;
+    } else {
+        b0 = b1;
     }
     read_rows(end, 1, a1);
     const int left = g.C - last * BK - 16 * (lane >> 4);
@@ -565,20 +562,21 @@ void launch(GemmArgs g, hipStream_t s) {
         const long n = (long)g.tiles_m * g.tiles_n;
         return n <= MAX_GRID_X ? dim3((unsigned)n) : dim3(MAX_GRID_X, (unsigned)tiles(n, MAX_GRID_X));
     };
-    /* up to 16 rows, or few outputs in all: 64 tiles of 32 x 32 (17 x 960 x 960 2.9 us against 4.2 in those, 128 x 8000 x
-     * 512 8.8 / 14.2, 64 x 2560 x 960 4.6 / 5.1), or twice as many and a long sum (67 x 6978 x 1216 9.7 / 12.5, 64 x 8000 x 2048
-     * 10.2 / 14.2, 32 x 4096 x 4096 8.1 / 8.6; with 256 of them, 64 x 4096 x 4096, 13.0 / 8.7) */
-    const long t32 = tiles(g.M, 32) * tiles(g.OC, 32);
-    if (g.M <= 16 || t32 <= 64 || (t32 <= 128 && g.C >= 2048)) {
-        /* two or four tiles of outputs a wave share their rows' reads: two past 64 tiles (67 x 6978 x 1216 11.1 us with one);
-         * four where more than 8 rows meet many outputs (16 x 4096 x 16384 17.5 us with one, 13.9; 16 x 960 x 49152 10.2 /
-         * 9.6; but 16 x 8192 x 8192 16.9 / 20.9) */
-        if (g.M <= 16 && g.M > 8 && g.OC >= 16384) {
-            const dim3 d = grid(16, 64);
-            hipLaunchKernelGGL((k_i8_few<4, 4, 4, BF16>), d, dim3(256), 0, s, g);
-        } else if (g.M > 16 && t32 > 64) {
+    /* Few outputs, straight from memory: at most 128 tiles of 32 x 32 (us there / in those tiles: 17 x 960 x 960 2.9 / 4.2, 68 x 99 x 1173
+     * 2.8 / 3.8, 31 x 1500 x 2346 4.1 / 4.8, 64 x 8000 x 2048 10.2 / 14.2; with 254 of them 58 x 6180 x 4061 15.4 / 12.1), or 192 with a
+     * short sum (42 x 1520 x 2630 4.1 / 5.2; 114 x 451 x 1951 3.6 / 3.3), or one tile row (5 x 3094 x 6130 5.8 / 7.5) up to where
+     * the weights' way into LDS counts (8 x 960 x 49152 12.5 / 11.6, 16 x 4096 x 14336 20.1 / 15.8; but 1 x 960 x 49152 11.0 / 11.2). */
+    const long t32 = tiles(g.M, 32) * tiles(g.OC, 32), t16 = tiles(g.M, 16) * tiles(g.OC, 16);
+    if (t32 <= 128 || (t32 <= 192 && g.C < 2048) || (g.M <= 16 && t32 < 448) || g.M < 4) {
+        /* Long sums: with a workgroup for each of many CUs, eight waves for four (1 x 8192 x 2048 6.9 us / 9.0, 44 x 6711 x 405
+         * 6.9 / 7.9; 7 x 5437 x 106 5.5 / 5.1, 52 x 3122 x 565 4.8 / 4.4); past that, two tiles of outputs a wave share
+         * their rows' reads (46 x 4225 x 2012 7.3 / 8.1, 38 x 2405 x 1432 5.6 / 5.2). */
+        if (g.M > 16 && t16 > CUS && g.C >= 2800) {
             const dim3 d = grid(16, 32);
             hipLaunchKernelGGL((k_i8_few<4, 2, 2, BF16>), d, dim3(256), 0, s, g);
+        } else if (t16 >= 48 && t16 <= CUS && g.C >= 3500) {
+            const dim3 d = grid(16, 16);
+            hipLaunchKernelGGL((k_i8_few<8, 1, 2, BF16>), d, dim3(512), 0, s, g);
         } else {
             const dim3 d = grid(16, 16);
             hipLaunchKernelGGL((k_i8_few<4, 1, 2, BF16>), d, dim3(256), 0, s, g);
@@ -593,10 +591,10 @@ void launch(GemmArgs g, hipStream_t s) {
      * 15, 7.3, 8.8, 8.7, 9.7, 10.8; 142 x 6784 x 9011 -, 33, 32, 22, 32, 34; 64 x 960 x 49152 16, 14, 14, 12, 13, 16; 512 x
      * 2560 x 960 26, 10.0, 7.8, 6.2, 5.4, 5.6; 20 x 960 x 16384 13, 6.7, 5.8, 4.7, 4.1, 4.1; 16384 x 960 x 16 14, 7.1, 5.8, 5.0, 4.9, 4.0. */
     static constexpr int SIDES[6][2] = {{256, 256}, {128, 128}, {128, 64}, {64, 64}, {32, 64}, {32, 32}};
-    const bool near = g.lda <= PAIR_MAX_LD && g.ldw <= PAIR_MAX_LD;
+    const bool pair = g.C >= PAIR_MIN_C && g.lda <= PAIR_MAX_LD && g.ldw <= PAIR_MAX_LD;
     int best = 0;
     long least = LONG_MAX;
-    for (int i = near ? 0 : 1; i < 6; i++) {
+    for (int i = pair ? 0 : 1; i < 6; i++) {
         const int bm = SIDES[i][0], bn = SIDES[i][1];
         const long cost = tiles(tiles(g.M, bm) * tiles(g.OC, bn), CUS) * ((long)(bm + bn) * g.C + 4l * bm * bn);
         if (cost < least) {

@@ -376,6 +376,22 @@ def test_matmul_one_round_of_tiles(be, M, OC):
     test_matmul_every_form(be, M, OC)
 
 
+@pytest.mark.parametrize("M,C,OC", [(1, 4096, 1000), (16, 8000, 2000), (33, 4660, 446), (17, 3499, 2000), (9, 3500, 770),
+                                    (67, 6978, 1216), (40, 2801, 2003), (38, 2405, 1432), (173, 1374, 704), (42, 2047, 2630),
+                                    (42, 2048, 2630), (3, 1100, 20000), (16, 300, 14300), (4, 800, 14337), (15, 2100, 16399)])
+def test_matmul_few_outputs(be, M, C, OC):
+    """Both sides of every border of the forms for few rows or outputs, for equality."""
+    rng = np.random.default_rng(M + OC)
+    ld = ld16(C) + 16
+    a, w = rng.integers(-100, 101, (M, ld)).astype(np.int8), rng.integers(-100, 101, (OC, ld)).astype(np.int8)
+    one, out = be.upload(np.ones(max(M, OC), np.float32)), marked(be, M * OC * 4 + 64)
+    assert be.dispatch("matmul_forward_i8", [be.upload(a), one, be.upload(w), one, one, out,
+                                             be.params(M, C, OC, 0, ld, ld, OC)], (OC, M), (256,)) == 0
+    want = (a[:, :C].astype(np.float64) @ w[:, :C].astype(np.float64).T).astype(np.float32)
+    raw = out.read(np.float32)
+    assert np.array_equal(raw[:M * OC].reshape(M, OC), want) and (raw[M * OC:].view(np.uint8) == MARK).all()
+
+
 @pytest.mark.parametrize("far", [1 << 23, (1 << 23) + 16])
 def test_matmul_largest_tiles_over_far_rows(be, far):
     test_matmul_tiles_over_far_rows(be, 3900, 3850, far)
