@@ -554,56 +554,71 @@ __global__ __launch_bounds__(512, 2) void k_i8_pair(GemmArgs g) {
 
 long tiles(long n, int t) { return (n + t - 1) / t; }
 
+dim3 grid_of(GemmArgs& g, int bm, int bn) {
+    g.tiles_m = (int)tiles(g.M, bm);
+    g.tiles_n = (int)tiles(g.OC, bn);
+    const long n = (long)g.tiles_m * g.tiles_n;
+    return n <= MAX_GRID_X ? dim3((unsigned)n) : dim3(MAX_GRID_X, (unsigned)tiles(n, MAX_GRID_X));
+}
+
+/* Few outputs, straight from memory: at most 128 tiles of 32 x 32 (us there / in those tiles: 17 x 960 x 960 2.9 / 4.2, 68 x 99 x 1173
+ * 2.8 / 3.8, 31 x 1500 x 2346 4.1 / 4.8, 64 x 8000 x 2048 10.2 / 14.2; with 254 of them 58 x 6180 x 4061 15.4 / 12.1), or 192 with a
+ * short sum (42 x 1520 x 2630 4.1 / 5.2; 114 x 451 x 1951 3.6 / 3.3), or one tile row (5 x 3094 x 6130 5.8 / 7.5) up to where
+ * the weights' way into LDS counts (8 x 960 x 49152 12.5 / 11.6, 16 x 4096 x 14336 20.1 / 15.8; but 1 x 960 x 49152 11.0 / 11.2). */
+bool few_outputs(const GemmArgs& g) {
+    const long t32 = tiles(g.M, 32) * tiles(g.OC, 32);
+    return t32 <= 128 || (t32 <= 192 && g.C < 2048) || (g.M <= 16 && t32 < 448) || g.M < 4;
+}
+
+/* Long sums: with a workgroup for each of many CUs, eight waves for four (1 x 8192 x 2048 6.9 us / 9.0, 44 x 6711 x 405
+ * 6.9 / 7.9; 7 x 5437 x 106 5.5 / 5.1, 52 x 3122 x 565 4.8 / 4.4); past that, two tiles of outputs a wave share
+ * their rows' reads (46 x 4225 x 2012 7.3 / 8.1, 38 x 2405 x 1432 5.6 / 5.2). */
 template <bool BF16>
-void launch(GemmArgs g, hipStream_t s) {
-    auto grid = [&](int bm, int bn) {
-        g.tiles_m = (int)tiles(g.M, bm);
-        g.tiles_n = (int)tiles(g.OC, bn);
-        const long n = (long)g.tiles_m * g.tiles_n;
-        return n <= MAX_GRID_X ? dim3((unsigned)n) : dim3(MAX_GRID_X, (unsigned)tiles(n, MAX_GRID_X));
-    };
-    /* Few outputs, straight from memory: at most 128 tiles of 32 x 32 (us there / in those tiles: 17 x 960 x 960 2.9 / 4.2, 68 x 99 x 1173
-     * 2.8 / 3.8, 31 x 1500 x 2346 4.1 / 4.8, 64 x 8000 x 2048 10.2 / 14.2; with 254 of them 58 x 6180 x 4061 15.4 / 12.1), or 192 with a
-     * short sum (42 x 1520 x 2630 4.1 / 5.2; 114 x 451 x 1951 3.6 / 3.3), or one tile row (5 x 3094 x 6130 5.8 / 7.5) up to where
-     * the weights' way into LDS counts (8 x 960 x 49152 12.5 / 11.6, 16 x 4096 x 14336 20.1 / 15.8; but 1 x 960 x 49152 11.0 / 11.2). */
-    const long t32 = tiles(g.M, 32) * tiles(g.OC, 32), t16 = tiles(g.M, 16) * tiles(g.OC, 16);
-    if (t32 <= 128 || (t32 <= 192 && g.C < 2048) || (g.M <= 16 && t32 < 448) || g.M < 4) {
-        /* Long sums: with a workgroup for each of many CUs, eight waves for four (1 x 8192 x 2048 6.9 us / 9.0, 44 x 6711 x 405
-         * 6.9 / 7.9; 7 x 5437 x 106 5.5 / 5.1, 52 x 3122 x 565 4.8 / 4.4); past that, two tiles of outputs a wave share
-         * their rows' reads (46 x 4225 x 2012 7.3 / 8.1, 38 x 2405 x 1432 5.6 / 5.2). */
-        if (g.M > 16 && t16 > CUS && g.C >= 2800) {
-            const dim3 d = grid(16, 32);
-            hipLaunchKernelGGL((k_i8_few<4, 2, 2, BF16>), d, dim3(256), 0, s, g);
-        } else if (t16 >= 48 && t16 <= CUS && g.C >= 3500) {
-            const dim3 d = grid(16, 16);
-            hipLaunchKernelGGL((k_i8_few<8, 1, 2, BF16>), d, dim3(512), 0, s, g);
-        } else {
-            const dim3 d = grid(16, 16);
-            hipLaunchKernelGGL((k_i8_few<4, 1, 2, BF16>), d, dim3(256), 0, s, g);
-        }
-        return;
+void launch_few(GemmArgs g, hipStream_t s) {
+    const long t16 = tiles(g.M, 16) * tiles(g.OC, 16);
+    if (g.M > 16 && t16 > CUS && g.C >= 2800) {
+        const dim3 d = grid_of(g, 16, 32);
+        hipLaunchKernelGGL((k_i8_few<4, 2, 2, BF16>), d, dim3(256), 0, s, g);
+    } else if (t16 >= 48 && t16 <= CUS && g.C >= 3500) {
+        const dim3 d = grid_of(g, 16, 16);
+        hipLaunchKernelGGL((k_i8_few<8, 1, 2, BF16>), d, dim3(512), 0, s, g);
+    } else {
+        const dim3 d = grid_of(g, 16, 16);
+        hipLaunchKernelGGL((k_i8_few<4, 1, 2, BF16>), d, dim3(256), 0, s, g);
     }
-    /* Else the tile for which the busiest CU has least to move: rounds of 256 tiles times a tile's operands, and four bytes an
-     * output for its stores and its start; of equals the largest.  (Over 330 shapes spread over 17 .. 16384 rows, 64 .. 8192
-     * columns and 16 .. 49152 outputs its choice is 1.1% slower than the best of these on average, 23% at most; the largest tile that
-     * 150 of are there 3.0% and 63%.)  us in 256 x 256, 128 x 128, 128 x 64, 64 x 64, 32 x 64 and 32 x 32 tiles: 4096 x 960 x
-     * 5120 36, 40, 48, 54, 73, 91; 1024 x 4096 x 4096 41, 21, 25 and more; 777 x 2500 x 2000 27, 12.0, 11.2, 12.4, 18.5, 20.7; 512 x 960 x 5120
-     * 15, 7.3, 8.8, 8.7, 9.7, 10.8; 142 x 6784 x 9011 -, 33, 32, 22, 32, 34; 64 x 960 x 49152 16, 14, 14, 12, 13, 16; 512 x
-     * 2560 x 960 26, 10.0, 7.8, 6.2, 5.4, 5.6; 20 x 960 x 16384 13, 6.7, 5.8, 4.7, 4.1, 4.1; 16384 x 960 x 16 14, 7.1, 5.8, 5.0, 4.9, 4.0. */
-    static constexpr int SIDES[6][2] = {{256, 256}, {128, 128}, {128, 64}, {64, 64}, {32, 64}, {32, 32}};
-    const bool pair = g.C >= PAIR_MIN_C && g.lda <= PAIR_MAX_LD && g.ldw <= PAIR_MAX_LD;
-    int best = 0;
-    long least = LONG_MAX;
-    for (int i = pair ? 0 : 1; i < 6; i++) {
-        const int bm = SIDES[i][0], bn = SIDES[i][1];
-        const long cost = tiles(tiles(g.M, bm) * tiles(g.OC, bn), CUS) * ((long)(bm + bn) * g.C + 4l * bm * bn);
-        if (cost < least) {
-            least = cost;
-            best = i;
-        }
+}
+
+/* The other tiles by their sides, and what the busiest CU has to move for M x OC outputs: its rounds of tiles times a tile's
+ * operands, and four bytes an output for its stores and its start. */
+constexpr int SIDES[6][2] = {{256, 256}, {128, 128}, {128, 64}, {64, 64}, {32, 64}, {32, 32}};
+long cost_of(int form, long rounds, int C) {
+    const int bm = SIDES[form][0], bn = SIDES[form][1];
+    return rounds * ((long)(bm + bn) * C + 4l * bm * bn);
+}
+
+struct Form {
+    int form;
+    long cost;
+};
+/* The form that costs least, of equals the largest.  (Over 330 shapes spread over 17 .. 16384 rows, 64 .. 8192
+ * columns and 16 .. 49152 outputs its choice is 1.1% slower than the best of these on average, 23% at most; the largest tile that
+ * 150 of are there 3.0% and 63%.)  us in 256 x 256, 128 x 128, 128 x 64, 64 x 64, 32 x 64 and 32 x 32 tiles: 4096 x 960 x
+ * 4096 23, 33, 39, 44, -, -; 1024 x 4096 x 4096 41, 21, 25 and more; 777 x 2500 x 2000 27, 12.0, 11.2, 12.4, 18.5, 20.7; 512 x 960 x 5120
+ * 15, 7.3, 8.8, 8.7, 9.7, 10.8; 142 x 6784 x 9011 -, 33, 32, 22, 32, 34; 64 x 960 x 49152 16, 14, 14, 12, 13, 16; 512 x
+ * 2560 x 960 26, 10.0, 7.8, 6.2, 5.4, 5.6; 20 x 960 x 16384 13, 6.7, 5.8, 4.7, 4.1, 4.1; 16384 x 960 x 16 14, 7.1, 5.8, 5.0, 4.9, 4.0. */
+Form form_of(const GemmArgs& g, int first) {
+    Form best = {first, LONG_MAX};
+    for (int i = first; i < 6; i++) {
+        const long cost = cost_of(i, tiles(tiles(g.M, SIDES[i][0]) * tiles(g.OC, SIDES[i][1]), CUS), g.C);
+        if (cost < best.cost) best = {i, cost};
     }
-    const dim3 d = grid(SIDES[best][0], SIDES[best][1]);
-    switch (best) {
+    return best;
+}
+
+template <bool BF16>
+void launch_form(GemmArgs g, int form, hipStream_t s) {
+    const dim3 d = grid_of(g, SIDES[form][0], SIDES[form][1]);
+    switch (form) {
     case 0: hipLaunchKernelGGL(k_i8_pair<BF16>, d, dim3(512), 0, s, g); break;
     case 1:
         /* stages of 64 columns for short sums: 2048 x 576 x 3000 11.6 us against 14.3, 4096 x 960 x 5120 40.3 / 42.8 */
@@ -615,6 +630,59 @@ void launch(GemmArgs g, hipStream_t s) {
     case 4: hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 2, 128, BF16>), d, dim3(256), 0, s, g); break;
     default: hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 1, 128, BF16>), d, dim3(256), 0, s, g);
     }
+}
+
+constexpr long LAUNCH_COST = 170000; /* a second launch, 2 us, at the 84 KB/us of a CU's loads into LDS */
+
+/* A product whose last round of 256 x 256 tiles is far from full goes in two launches, the full rounds' rows or columns
+ * and what is left in the form that suits it, where that costs less (4096 x 960 x 5120, a round and a
+ * quarter: 37.9 -> 31.4 us; 2048 x 4096 x 9000, 1.125: 105.6 -> 68.7). */
+template <bool BF16>
+void launch(const GemmArgs& g, hipStream_t s) {
+    if (few_outputs(g)) return launch_few<BF16>(g, s);
+    const bool pair = g.C >= PAIR_MIN_C && g.lda <= PAIR_MAX_LD && g.ldw <= PAIR_MAX_LD;
+    const Form one = form_of(g, pair ? 0 : 1);
+    const long tm = tiles(g.M, 256), tn = tiles(g.OC, 256), full = tm * tn / CUS;
+    if (pair && full > 0) {
+        const long m1 = full * CUS / tn, n1 = full * CUS / tm; /* rows and columns of tiles in the full rounds */
+        GemmArgs rest[2] = {g, g};
+        long least = one.cost;
+        int cut = -1;
+        Form other = one;
+        for (int i = 0; i < 2; i++) {
+            GemmArgs& r = rest[i];
+            const long n = 256 * (i ? n1 : m1);
+            if (n == 0 || n >= (i ? g.OC : g.M)) continue;
+            if (i) {
+                r.OC -= (int)n;
+                r.w += n * g.ldw;
+                r.sw += n;
+                if (r.bias) r.bias += n;
+                r.out = (char*)g.out + n * (BF16 ? 2 : 4);
+            } else {
+                r.M -= (int)n;
+                r.a += n * g.lda;
+                r.sa += n;
+                r.out = (char*)g.out + n * g.ldo * (BF16 ? 2 : 4);
+            }
+            const Form f = form_of(r, 1);
+            const long cost = cost_of(0, full, g.C) + f.cost + LAUNCH_COST;
+            if (cost < least) {
+                least = cost;
+                cut = i;
+                other = f;
+            }
+        }
+        if (cut >= 0) {
+            GemmArgs first = g;
+            if (cut) first.OC -= rest[1].OC;
+            else first.M -= rest[0].M;
+            launch_form<BF16>(first, 0, s);
+            launch_form<BF16>(rest[cut], other.form, s);
+            return;
+        }
+    }
+    launch_form<BF16>(g, one.form, s);
 }
 
 /* {codes [BT][lda], scale f32 [BT], weight codes [OC][ldw], scale f32 [OC], bias f32 [OC], out [BT][ldo],

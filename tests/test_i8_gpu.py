@@ -392,6 +392,25 @@ def test_matmul_few_outputs(be, M, C, OC):
     assert np.array_equal(raw[:M * OC].reshape(M, OC), want) and (raw[M * OC:].view(np.uint8) == MARK).all()
 
 
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("M,OC", [(4100, 5123), (5123, 4100), (2000, 9001), (4096, 4353), (257 * 256, 300)])
+def test_matmul_in_two_parts(be, M, OC, bf16):
+    """More 256 x 256 tiles than CUs and the rest beside them or below: scales, bias and outputs are each part's own."""
+    rng = np.random.default_rng(M)
+    C, ldo = 330, OC + 3
+    a, w = rng.integers(-128, 128, (M, ld16(C))).astype(np.int8), rng.integers(-128, 128, (OC, ld16(C))).astype(np.int8)
+    sa, sw = np.exp(rng.uniform(-3, 1, M)).astype(np.float32), np.exp(rng.uniform(-3, 1, OC)).astype(np.float32)
+    b = (rng.standard_normal(OC) * 1e4).astype(np.float32)
+    out = marked(be, M * ldo * (2 if bf16 else 4))
+    assert be.dispatch("matmul_forward_i8" + ("_bf16" if bf16 else ""), [
+        be.upload(a), be.upload(sa), be.upload(w), be.upload(sw), be.upload(b), out,
+        be.params(M, C, OC, 1, ld16(C), ld16(C), ldo)], (OC, M), (256,)) == 0
+    want = (a[:, :C].astype(np.float32) @ w[:, :C].astype(np.float32).T) * sa[:, None] * sw + b  # sums below 2^24: exact
+    got = out.read(np.uint16 if bf16 else np.float32)[:M * ldo].reshape(M, ldo)
+    assert np.array_equal(got[:, :OC], to_bf16(want) if bf16 else want)
+    assert (np.ascontiguousarray(got[:, OC:]).view(np.uint8) == MARK).all()
+
+
 @pytest.mark.parametrize("far", [1 << 23, (1 << 23) + 16])
 def test_matmul_largest_tiles_over_far_rows(be, far):
     test_matmul_tiles_over_far_rows(be, 3900, 3850, far)
