@@ -8,7 +8,7 @@
  * p * inv is at most 127 * (1 + 2^-22), so q needs no clamp.  Two kinds of row
  * have no such grid: one that holds a NaN or an infinity gets zero codes and
  * the scale NaN (so that what is computed from it shows it), one whose top is
- * so small (under 3.8e-37, or all zero) that inv overflows gets zero codes
+ * so small (under 3.73e-37, or all zero) that inv overflows gets zero codes
  * and the scale 0.
  */
 #ifndef BMK_I8_COMMON_H

@@ -51,7 +51,7 @@
  * C-th, up to that group's end, and nothing past it.  Row p of C values has
  * top = max |p|, inv = 127 / top, codes round-to-even(p * inv) in -127 .. 127
  * and scale top / 127, each step in fp32.  A row of zeros, or whose top is
- * under 3.8e-37, has zero codes and the scale 0; a row that holds a NaN or an
+ * under 3.73e-37, has zero codes and the scale 0; a row that holds a NaN or an
  * infinity has zero codes and the scale NaN.  Row counts may be 0 (nothing is
  * done); rows past them are left as they are.  Inputs and outputs may not
  * overlap but where stated.  A _bf16 name takes or gives bf16 where "T" stands,
