@@ -167,53 +167,47 @@ __device__ __forceinline__ void clear(i32x4 (&acc)[TM][TN]) {
 /* ------------------------------------------------------------------ */
 /* few rows or outputs */
 
-/* 16 x 16 TN outputs a workgroup; wave p of KP takes every KP-th slice of 64
- * columns from p on, U slices' loads in flight, so that a workgroup reads 64 KP
+/* 16 x 16 outputs a workgroup; wave p of KP takes every KP-th slice of 64
+ * columns from p on, two slices' loads in flight, so that a workgroup reads 64 KP
  * neighbouring bytes of a row at once.  The partial sums meet in LDS.
  * What bounds it: reading the weights (1 x 960 -> 49152 11.0 us, 4.3 TB/s), with few outputs the reads of one CU (5 x 8192
  * -> 500 7.2 us on 32 CUs), else the launch (1 x 960 -> 5120 3.4 us).  Four waves along the sum: one took 5.2 us for 1 x
- * 2560 -> 960, sixteen 4.2, eight 4.5, four 3.8. */
-template <int KP, int TN, int U, bool BF16>
+ * 2560 -> 960, sixteen 4.2, eight 4.5, four 3.8.  Two and four tiles of outputs a wave, and four slices in flight: slower
+ * wherever this form is the best (1 x 2560 -> 960 5.3, 7.8 and 4.5 us). */
+template <int KP, bool BF16>
 __global__ __launch_bounds__(64 * KP) void k_i8_few(GemmArgs g) {
-    __shared__ __attribute__((aligned(16))) i32x4 part[KP * TN * 64];
+    constexpr int U = 2;
+    __shared__ __attribute__((aligned(16))) i32x4 part[KP * 64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     int tm, tn;
     if (!tile_of(g, tm, tn)) return;
-    const int m0 = tm * 16, n0 = tn * 16 * TN;
+    const int m0 = tm * 16, n0 = tn * 16;
     const int c = 16 * (lane >> 4), last = 16 * ((g.C - 1) >> 4), slices = (g.C + 63) >> 6;
     const unsigned char* ap = g.a + (size_t)min(m0 + (lane & 15), g.M - 1) * g.lda;
-    const unsigned char* wp[TN];
-#pragma unroll
-    for (int j = 0; j < TN; j++) wp[j] = g.w + (size_t)min(n0 + 16 * j + (lane & 15), g.OC - 1) * g.ldw;
-    i32x4 acc[1][TN];
+    const unsigned char* wp = g.w + (size_t)min(n0 + (lane & 15), g.OC - 1) * g.ldw;
+    i32x4 acc[1][1];
     clear(acc);
     for (int s = wave; s < slices; s += KP * U) {
-        i32x4 a[U], w[U][TN];
+        i32x4 a[U], w[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int k = min(64 * (s + KP * u) + c, last);
-#pragma unroll
-            for (int j = 0; j < TN; j++) w[u][j] = *(const i32x4*)(wp[j] + k);
+            w[u] = *(const i32x4*)(wp + k);
             a[u] = *(const i32x4*)(ap + k);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int left = g.C - 64 * (s + KP * u) - c;
             if (left < 16) a[u] = head_bytes(a[u], left);
-#pragma unroll
-            for (int j = 0; j < TN; j++)
-                acc[0][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][j], a[u], acc[0][j], 0, 0, 0);
+            acc[0][0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u], a[u], acc[0][0], 0, 0, 0);
         }
     }
-#pragma unroll
-    for (int j = 0; j < TN; j++) part[(wave * TN + j) * 64 + lane] = acc[0][j];
+    part[wave * 64 + lane] = acc[0][0];
     __syncthreads();
     if (wave) return;
 #pragma unroll
-    for (int j = 0; j < TN; j++)
-#pragma unroll
-        for (int p = 1; p < KP; p++) acc[0][j] += part[(p * TN + j) * 64 + lane];
-    store_tile<1, TN, BF16>(g, acc, m0, n0);
+    for (int p = 1; p < KP; p++) acc[0][0] += part[p * 64 + lane];
+    store_tile<1, 1, BF16>(g, acc, m0, n0);
 }
 
 /* ------------------------------------------------------------------ */
@@ -225,8 +219,8 @@ __global__ __launch_bounds__(64 * KP) void k_i8_few(GemmArgs g) {
  * put these 16 groups in 16 different places of 256 bytes (64 banks). */
 template <int BK>
 __device__ __forceinline__ int group_key(int row) {
-    static_assert(BK == 64 || BK == 128, "");
-    return BK == 64 ? (0x78 >> (2 * ((row >> 2) & 3))) & 3 : (row >> 1) & 7;
+    static_assert(BK == 64 || BK == 128 || BK == 256, "");
+    return BK == 64 ? (0x78 >> (2 * ((row >> 2) & 3))) & 3 : BK == 128 ? (row >> 1) & 7 : row & 15;
 }
 
 /* keeps memory accesses on their side; no instruction */
@@ -561,31 +555,25 @@ dim3 grid_of(GemmArgs& g, int bm, int bn) {
     return n <= MAX_GRID_X ? dim3((unsigned)n) : dim3(MAX_GRID_X, (unsigned)tiles(n, MAX_GRID_X));
 }
 
-/* Few outputs, straight from memory: at most 128 tiles of 32 x 32 (us there / in those tiles: 17 x 960 x 960 2.9 / 4.2, 68 x 99 x 1173
- * 2.8 / 3.8, 31 x 1500 x 2346 4.1 / 4.8, 64 x 8000 x 2048 10.2 / 14.2; with 254 of them 58 x 6180 x 4061 15.4 / 12.1), or 192 with a
- * short sum (42 x 1520 x 2630 4.1 / 5.2; 114 x 451 x 1951 3.6 / 3.3), or one tile row (5 x 3094 x 6130 5.8 / 7.5) up to where
- * the weights' way into LDS counts (8 x 960 x 49152 12.5 / 11.6, 16 x 4096 x 14336 20.1 / 15.8; but 1 x 960 x 49152 11.0 / 11.2). */
+/* Few outputs, straight from memory (us there / in tiles): a tile of 16 x 16 for each CU at most (17 x 960 x 960 2.9 / 4.2, 40 x 5420 x 761
+ * 6.0 / 7.9; 344 x 1792 x 189, 264 of them, 6.0 / 4.5), or three times as many and a short sum (68 x 99 x 1173 2.8 / 3.8, 37 x 198
+ * x 2539 3.0 / 3.8; 114 x 451 x 1951 3.6 / 3.3), or few rows (16 x 960 x 5120 3.7 / 4.1, 8 x 1536 x 8192 4.7 / 5.2; 8 x 4096 x 6000
+ * 8.3 / 6.6, 16 x 1536 x 6000 5.2 / 4.5) up to where the weights' way into LDS counts (8 x 960 x 49152 12.5 / 11.6; but 1 x 960
+ * x 49152 11.0 / 11.2). */
 bool few_outputs(const GemmArgs& g) {
-    const long t32 = tiles(g.M, 32) * tiles(g.OC, 32);
-    return t32 <= 128 || (t32 <= 192 && g.C < 2048) || (g.M <= 16 && t32 < 448) || g.M < 4;
+    const long t32 = tiles(g.M, 32) * tiles(g.OC, 32), t16 = tiles(g.M, 16) * tiles(g.OC, 16);
+    if (g.M < 4 || t16 <= CUS) return true;
+    return (g.C < 1280 && t32 <= 192) || (g.M <= 16 && t32 < 448 && g.C < (g.M > 8 ? 1280 : 2048));
 }
 
-/* Long sums: with a workgroup for each of many CUs, eight waves for four (1 x 8192 x 2048 6.9 us / 9.0, 44 x 6711 x 405
- * 6.9 / 7.9; 7 x 5437 x 106 5.5 / 5.1, 52 x 3122 x 565 4.8 / 4.4); past that, two tiles of outputs a wave share
- * their rows' reads (46 x 4225 x 2012 7.3 / 8.1, 38 x 2405 x 1432 5.6 / 5.2). */
+/* Eight waves where the sums are long and many CUs have a workgroup, but no more than one (us in eight / four: 1 x 8192 x 2048 6.9 /
+ * 9.0, 44 x 6711 x 405 6.9 / 7.9; 7 x 5437 x 106 5.5 / 5.1, 52 x 3122 x 565 4.8 / 4.4, 8 x 8192 x 6000 16.5 / 15.4). */
 template <bool BF16>
 void launch_few(GemmArgs g, hipStream_t s) {
-    const long t16 = tiles(g.M, 16) * tiles(g.OC, 16);
-    if (g.M > 16 && t16 > CUS && g.C >= 2800) {
-        const dim3 d = grid_of(g, 16, 32);
-        hipLaunchKernelGGL((k_i8_few<4, 2, 2, BF16>), d, dim3(256), 0, s, g);
-    } else if (t16 >= 48 && t16 <= CUS && g.C >= 3500) {
-        const dim3 d = grid_of(g, 16, 16);
-        hipLaunchKernelGGL((k_i8_few<8, 1, 2, BF16>), d, dim3(512), 0, s, g);
-    } else {
-        const dim3 d = grid_of(g, 16, 16);
-        hipLaunchKernelGGL((k_i8_few<4, 1, 2, BF16>), d, dim3(256), 0, s, g);
-    }
+    const dim3 d = grid_of(g, 16, 16);
+    const long t16 = (long)g.tiles_m * g.tiles_n;
+    if (t16 >= 48 && t16 <= CUS && g.C >= 3500) hipLaunchKernelGGL((k_i8_few<8, BF16>), d, dim3(512), 0, s, g);
+    else hipLaunchKernelGGL((k_i8_few<4, BF16>), d, dim3(256), 0, s, g);
 }
 
 /* The other tiles by their sides, and what the busiest CU has to move for M x OC outputs: its rounds of tiles times a tile's
@@ -618,6 +606,7 @@ Form form_of(const GemmArgs& g, int first) {
 template <bool BF16>
 void launch_form(GemmArgs g, int form, hipStream_t s) {
     const dim3 d = grid_of(g, SIDES[form][0], SIDES[form][1]);
+    const bool one = (long)g.tiles_m * g.tiles_n <= CUS;
     switch (form) {
     case 0: hipLaunchKernelGGL(k_i8_pair<BF16>, d, dim3(512), 0, s, g); break;
     case 1:
@@ -626,9 +615,20 @@ void launch_form(GemmArgs g, int form, hipStream_t s) {
         else hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 128, BF16>), d, dim3(512), 0, s, g);
         break;
     case 2: hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 2, 128, BF16>), d, dim3(512), 0, s, g); break;
-    case 3: hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 128, BF16>), d, dim3(256), 0, s, g); break;
-    case 4: hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 2, 128, BF16>), d, dim3(256), 0, s, g); break;
-    default: hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 1, 128, BF16>), d, dim3(256), 0, s, g);
+    /* stages of 256 columns for long sums and one tile a CU at most: 512 x 2560 x 960 7.0 us against 6.2, 64 x 4096 x 4096 8.7 /
+     * 6.8, 1000 x 8192 x 960 18.3 / 16.0; with two tiles a CU 1000 x 2560 x 960 9.1 / 9.1, 1024 x 2048 x 1500 8.7 / 11.9; 128 x
+     * 64 tiles gain from 4096 columns on, 2 to 5% */
+    case 3:
+        if (one && g.C >= 2048) hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 256, BF16>), d, dim3(256), 0, s, g);
+        else hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 128, BF16>), d, dim3(256), 0, s, g);
+        break;
+    case 4:
+        if (one && g.C >= 1280) hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 2, 256, BF16>), d, dim3(256), 0, s, g);
+        else hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 2, 128, BF16>), d, dim3(256), 0, s, g);
+        break;
+    default:
+        if (one && g.C >= 1280) hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 1, 256, BF16>), d, dim3(256), 0, s, g);
+        else hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 1, 128, BF16>), d, dim3(256), 0, s, g);
     }
 }
 

@@ -392,6 +392,24 @@ def test_matmul_few_outputs(be, M, C, OC):
     assert np.array_equal(raw[:M * OC].reshape(M, OC), want) and (raw[M * OC:].view(np.uint8) == MARK).all()
 
 
+@pytest.mark.parametrize("M,OC", [(500, 500), (500, 1020), (1000, 1020)])
+def test_matmul_wide_stages(be, M, OC):
+    """Long sums of one tile a CU, stages of 256 columns: 5 to 13 of them, whole and ragged."""
+    rng = np.random.default_rng(OC)
+    sums = [1280, 1281, 1536, 1599, 1792, 1793, 2047, 2048, 2049, 2305, 2560, 2561, 2830, 3080]
+    ld = ld16(max(sums)) + 48
+    a, w = rng.integers(-100, 101, (M, ld)).astype(np.int8), rng.integers(-100, 101, (OC, ld)).astype(np.int8)
+    ba, bw, one, out = be.upload(a), be.upload(w), be.upload(np.ones(max(M, OC), np.float32)), marked(be, M * OC * 4)
+    fa, fw = a.astype(np.float32), w.astype(np.float32)
+    for C in sums:
+        assert be.dispatch("matmul_forward_i8", [ba, one, bw, one, one, out, be.params(M, C, OC, 0, ld, ld, OC)], (OC, M),
+                           (256,)) == 0
+        want = fa[:, :C] @ fw[:, :C].T  # magnitudes of at most 100: sums of 3080 products below 2^25, these below 2^24
+        assert np.abs(want).max() < 2 ** 24
+        got = out.read(np.float32).reshape(M, OC)
+        assert np.array_equal(got, want), (C, np.argwhere(got != want)[:4])
+
+
 @pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
 @pytest.mark.parametrize("M,OC", [(4100, 5123), (5123, 4100), (2000, 9001), (4096, 4353), (257 * 256, 300)])
 def test_matmul_in_two_parts(be, M, OC, bf16):
