@@ -13,7 +13,7 @@
  * is slower on this part (registers only, all CUs, codes of a normal
  * distribution: 2.6 against 4.1 POP/s).
  *   k_i8_few   few rows or outputs: operands straight into registers, the sum split over four or eight waves
- *   k_i8_tile  tiles of 32 x 32 to 128 x 128 through LDS, four or eight waves
+ *   k_i8_tile  tiles of 32 x 32 to 192 x 192 through LDS, four or eight waves
  *   k_i8_pair  256 x 256, eight waves in two groups that take turns at the matrix cores and at LDS
  * Operands go to LDS by global_load_lds, which writes 16 bytes a lane at
  * consecutive addresses, so a row's 16-byte groups are permuted on the source
@@ -578,7 +578,11 @@ void launch_few(GemmArgs g, hipStream_t s) {
 
 /* The other tiles by their sides, and what the busiest CU has to move for M x OC outputs: its rounds of tiles times a tile's
  * operands, and four bytes an output for its stores and its start. */
-constexpr int SIDES[6][2] = {{256, 256}, {128, 128}, {128, 64}, {64, 64}, {32, 64}, {32, 32}};
+enum { PAIR, T192, T256X128, T128X192, T128, T128X64, T64, T32X64, T32, FORMS };
+constexpr int SIDES[FORMS][2] = {{256, 256}, {192, 192}, {256, 128}, {128, 192}, {128, 128}, {128, 64}, {64, 64}, {32, 64}, {32, 32}};
+constexpr int WIDE_MIN_C = 512; /* the three below 256 x 256: their first loads take long (us in 128 x 192 / the best of the others: 944 x
+                                 * 192 x 9055 18.8 / 16.3, 3125 x 403 x 3131 21.0 / 20.0, 2267 x 602 x 2553 13.2 / 15.1) */
+
 long cost_of(int form, long rounds, int C) {
     const int bm = SIDES[form][0], bn = SIDES[form][1];
     return rounds * ((long)(bm + bn) * C + 4l * bm * bn);
@@ -588,15 +592,18 @@ struct Form {
     int form;
     long cost;
 };
-/* The form that costs least, of equals the largest.  (Over 330 shapes spread over 17 .. 16384 rows, 64 .. 8192
- * columns and 16 .. 49152 outputs its choice is 1.1% slower than the best of these on average, 23% at most; the largest tile that
- * 150 of are there 3.0% and 63%.)  us in 256 x 256, 128 x 128, 128 x 64, 64 x 64, 32 x 64 and 32 x 32 tiles: 4096 x 960 x
+/* The form that costs least, of equals the largest.  (Over 170 shapes with 1.5 million outputs or more, 200 .. 8192 columns, its choice is
+ * 2.0% slower than the best of these on average, 20% at most, and over 200 shapes of all sizes 1.3% and 22%; the largest tile that
+ * 150 of are there 3.0% and 63% behind.)  us in 256 x 256, 128 x 128, 128 x 64, 64 x 64, 32 x 64 and 32 x 32 tiles: 4096 x 960 x
  * 4096 23, 33, 39, 44, -, -; 1024 x 4096 x 4096 41, 21, 25 and more; 777 x 2500 x 2000 27, 12.0, 11.2, 12.4, 18.5, 20.7; 512 x 960 x 5120
  * 15, 7.3, 8.8, 8.7, 9.7, 10.8; 142 x 6784 x 9011 -, 33, 32, 22, 32, 34; 64 x 960 x 49152 16, 14, 14, 12, 13, 16; 512 x
- * 2560 x 960 26, 10.0, 7.8, 6.2, 5.4, 5.6; 20 x 960 x 16384 13, 6.7, 5.8, 4.7, 4.1, 4.1; 16384 x 960 x 16 14, 7.1, 5.8, 5.0, 4.9, 4.0. */
-Form form_of(const GemmArgs& g, int first) {
-    Form best = {first, LONG_MAX};
-    for (int i = first; i < 6; i++) {
+ * 2560 x 960 26, 10.0, 7.8, 6.2, 5.4, 5.6; 20 x 960 x 16384 13, 6.7, 5.8, 4.7, 4.1, 4.1; 16384 x 960 x 16 14, 7.1, 5.8, 5.0, 4.9, 4.0.
+ * One round of 128 x 192 for two of 128 x 128: 1024 x 960 x 5120 14.5 -> 12.0, 927 x 1774 x 4628 23.7 -> 16.3; of 256 x 128: 1400 x
+ * 2560 x 5000 27.8 -> 24.0; of 192 x 192 for one of 256 x 256: 1300 x 960 x 6000 19.7 -> 15.3. */
+Form form_of(const GemmArgs& g, bool pair) {
+    Form best = {T32, LONG_MAX};
+    for (int i = pair ? PAIR : T192; i < FORMS; i++) {
+        if (i >= T192 && i <= T128X192 && g.C < WIDE_MIN_C) continue;
         const long cost = cost_of(i, tiles(tiles(g.M, SIDES[i][0]) * tiles(g.OC, SIDES[i][1]), CUS), g.C);
         if (cost < best.cost) best = {i, cost};
     }
@@ -608,21 +615,24 @@ void launch_form(GemmArgs g, int form, hipStream_t s) {
     const dim3 d = grid_of(g, SIDES[form][0], SIDES[form][1]);
     const bool one = (long)g.tiles_m * g.tiles_n <= CUS;
     switch (form) {
-    case 0: hipLaunchKernelGGL(k_i8_pair<BF16>, d, dim3(512), 0, s, g); break;
-    case 1:
+    case PAIR: hipLaunchKernelGGL(k_i8_pair<BF16>, d, dim3(512), 0, s, g); break;
+    case T192: hipLaunchKernelGGL((k_i8_tile<2, 4, 6, 3, 128, BF16>), d, dim3(512), 0, s, g); break;
+    case T256X128: hipLaunchKernelGGL((k_i8_tile<4, 2, 4, 4, 128, BF16>), d, dim3(512), 0, s, g); break;
+    case T128X192: hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 6, 128, BF16>), d, dim3(512), 0, s, g); break;
+    case T128:
         /* stages of 64 columns for short sums: 2048 x 576 x 3000 11.6 us against 14.3, 4096 x 960 x 5120 40.3 / 42.8 */
         if (g.C < 1024) hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 64, BF16>), d, dim3(512), 0, s, g);
         else hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 128, BF16>), d, dim3(512), 0, s, g);
         break;
-    case 2: hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 2, 128, BF16>), d, dim3(512), 0, s, g); break;
+    case T128X64: hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 2, 128, BF16>), d, dim3(512), 0, s, g); break;
     /* stages of 256 columns for long sums and one tile a CU at most: 512 x 2560 x 960 7.0 us against 6.2, 64 x 4096 x 4096 8.7 /
      * 6.8, 1000 x 8192 x 960 18.3 / 16.0; with two tiles a CU 1000 x 2560 x 960 9.1 / 9.1, 1024 x 2048 x 1500 8.7 / 11.9; 128 x
      * 64 tiles gain from 4096 columns on, 2 to 5% */
-    case 3:
+    case T64:
         if (one && g.C >= 2048) hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 256, BF16>), d, dim3(256), 0, s, g);
         else hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 128, BF16>), d, dim3(256), 0, s, g);
         break;
-    case 4:
+    case T32X64:
         if (one && g.C >= 1280) hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 2, 256, BF16>), d, dim3(256), 0, s, g);
         else hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 2, 128, BF16>), d, dim3(256), 0, s, g);
         break;
@@ -641,7 +651,7 @@ template <bool BF16>
 void launch(const GemmArgs& g, hipStream_t s) {
     if (few_outputs(g)) return launch_few<BF16>(g, s);
     const bool pair = g.C >= PAIR_MIN_C && g.lda <= PAIR_MAX_LD && g.ldw <= PAIR_MAX_LD;
-    const Form one = form_of(g, pair ? 0 : 1);
+    const Form one = form_of(g, pair);
     const long tm = tiles(g.M, 256), tn = tiles(g.OC, 256), full = tm * tn / CUS;
     if (pair && full > 0) {
         const long m1 = full * CUS / tn, n1 = full * CUS / tm; /* rows and columns of tiles in the full rounds */
@@ -665,8 +675,8 @@ void launch(const GemmArgs& g, hipStream_t s) {
                 r.sa += n;
                 r.out = (char*)g.out + n * g.ldo * (BF16 ? 2 : 4);
             }
-            const Form f = form_of(r, 1);
-            const long cost = cost_of(0, full, g.C) + f.cost + LAUNCH_COST;
+            const Form f = form_of(r, false);
+            const long cost = cost_of(PAIR, full, g.C) + f.cost + LAUNCH_COST;
             if (cost < least) {
                 least = cost;
                 cut = i;
@@ -677,7 +687,7 @@ void launch(const GemmArgs& g, hipStream_t s) {
             GemmArgs first = g;
             if (cut) first.OC -= rest[1].OC;
             else first.M -= rest[0].M;
-            launch_form<BF16>(first, 0, s);
+            launch_form<BF16>(first, PAIR, s);
             launch_form<BF16>(rest[cut], other.form, s);
             return;
         }

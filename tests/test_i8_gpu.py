@@ -392,6 +392,12 @@ def test_matmul_few_outputs(be, M, C, OC):
     assert np.array_equal(raw[:M * OC].reshape(M, OC), want) and (raw[M * OC:].view(np.uint8) == MARK).all()
 
 
+@pytest.mark.parametrize("M,OC", [(1000, 5100), (2000, 4000), (2000, 4400), (193, 48003), (33001, 250)])
+def test_matmul_one_round_of_wide_tiles(be, M, OC):
+    """The same for 128 x 192, 256 x 128 and 192 x 192, which take sums from 512 on."""
+    test_matmul_every_form(be, M, OC)
+
+
 @pytest.mark.parametrize("M,OC", [(500, 500), (500, 1020), (1000, 1020)])
 def test_matmul_wide_stages(be, M, OC):
     """Long sums of one tile a CU, stages of 256 columns: 5 to 13 of them, whole and ragged."""
