@@ -620,8 +620,9 @@ void launch_form(GemmArgs g, int form, hipStream_t s) {
     case T256X128: hipLaunchKernelGGL((k_i8_tile<4, 2, 4, 4, 128, BF16>), d, dim3(512), 0, s, g); break;
     case T128X192: hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 6, 128, BF16>), d, dim3(512), 0, s, g); break;
     case T128:
-        /* stages of 64 columns for short sums: 2048 x 576 x 3000 11.6 us against 14.3, 4096 x 960 x 5120 40.3 / 42.8 */
-        if (g.C < 1024) hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 64, BF16>), d, dim3(512), 0, s, g);
+        /* stages of 64 columns for short sums, which leave a CU room for two tiles (us in 64 / 128: 2048 x 576 x 3000 11.6 / 14.3, 539 x 448
+         * x 10861 13.5 / 15.4; one tile a CU 1586 x 640 x 1292 7.0 / 6.5, 512 x 960 x 5120 8.9 / 8.6, 1272 x 448 x 2594 7.1 / 7.5) */
+        if (g.C < (one ? 512 : 1024)) hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 64, BF16>), d, dim3(512), 0, s, g);
         else hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 128, BF16>), d, dim3(512), 0, s, g);
         break;
     case T128X64: hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 2, 128, BF16>), d, dim3(512), 0, s, g); break;
