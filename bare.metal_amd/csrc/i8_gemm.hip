@@ -247,8 +247,9 @@ constexpr int RING = 3; /* stages of a tile's ring */
  * three: while a stage is multiplied, the first fragments of the next are read
  * and two more are on their way.  A stage's buffer is requested again at the
  * one barrier behind which every wave has read it.
- * What bounds it: a workgroup's chain of load, barrier and fragment reads (a CU
- * moves 40 KB/us into LDS this way; its matrix cores would take twice that).  us at
+ * What bounds it: a CU's loads into LDS (84 KB/us in 128-byte pieces of rows on
+ * 128-byte boundaries, a fifth less off them; 128 x 128 tiles reach 60), with small tiles a
+ * stage's chain of load, barrier and fragment reads (0.17 us).  us at
  * 2048 x 2048 x 2048 / 4096 x 2560 x 960 / 1024 x 4096 x 4096, tiles of 128 x 128: eight
  * waves over 128 columns a stage 12.5 / 14.1 / 21; over 64 13.4 / 16.3 / 24; four waves
  * 13.7 / 16 / 24; a ring of two 13.2 / 17.2 / 28, of four over 64 14.3 / 18 / 26. */
@@ -367,8 +368,9 @@ __global__ __launch_bounds__(64 * MW * NW, 2) void k_i8_tile(GemmArgs g) {
 /* 256 x 256 */
 
 constexpr size_t PAIR_MAX_LD = (size_t)1 << 23; /* 256 rows of it stay inside 32-bit offsets */
-constexpr int PAIR_MIN_C = 320;                 /* five stages; us there / in 128 x 128: 7439 x 113 x 43794 276 / 203, 2279 x 307
-                                                 * x 24615 71 / 63, 1356 x 364 x 24934 42 / 44, 5211 x 452 x 2415 22.5 / 26.8 */
+/* Five stages (us there / in 128 x 128 tiles: 7439 x 113 x 43794 276 / 203, 2279 x 307 x 24615 71 / 63, 1356 x 364 x 24934
+ * 42 / 44, 5211 x 452 x 2415 22.5 / 26.8). */
+constexpr int PAIR_MIN_C = 320;
 
 /* Eight waves of 128 x 64 (2 x 4), two on each SIMD, in two groups of four a
  * half turn apart: while one group's 16 MFMAs of a half stage run, the other
@@ -555,19 +557,20 @@ dim3 grid_of(GemmArgs& g, int bm, int bn) {
     return n <= MAX_GRID_X ? dim3((unsigned)n) : dim3(MAX_GRID_X, (unsigned)tiles(n, MAX_GRID_X));
 }
 
-/* Few outputs, straight from memory (us there / in tiles): a tile of 16 x 16 for each CU at most (17 x 960 x 960 2.9 / 4.2, 40 x 5420 x 761
- * 6.0 / 7.9; 344 x 1792 x 189, 264 of them, 6.0 / 4.5), or three times as many and a short sum (68 x 99 x 1173 2.8 / 3.8, 37 x 198
- * x 2539 3.0 / 3.8; 114 x 451 x 1951 3.6 / 3.3), or few rows (16 x 960 x 5120 3.7 / 4.1, 8 x 1536 x 8192 4.7 / 5.2; 8 x 4096 x 6000
- * 8.3 / 6.6, 16 x 1536 x 6000 5.2 / 4.5) up to where the weights' way into LDS counts (8 x 960 x 49152 12.5 / 11.6; but 1 x 960
- * x 49152 11.0 / 11.2). */
+/* Few outputs, straight from memory (us there / in tiles): a tile of 16 x 16 for each CU at most (17 x 960 x 960 2.9 / 4.2,
+ * 40 x 5420 x 761 6.0 / 7.9; 344 x 1792 x 189, 264 of them, 6.0 / 4.5), or three times as many and a short sum (68 x 99 x
+ * 1173 2.8 / 3.8, 37 x 198 x 2539 3.0 / 3.8; 114 x 451 x 1951 3.6 / 3.3), or few rows (16 x 960 x 5120 3.7 / 4.1, 8 x 1536 x
+ * 8192 4.7 / 5.2; 8 x 4096 x 6000 8.3 / 6.6, 16 x 1536 x 6000 5.2 / 4.5) up to where the weights' way into LDS counts (8 x
+ * 960 x 49152 12.5 / 11.6; but 1 x 960 x 49152 11.0 / 11.2). */
 bool few_outputs(const GemmArgs& g) {
     const long t32 = tiles(g.M, 32) * tiles(g.OC, 32), t16 = tiles(g.M, 16) * tiles(g.OC, 16);
     if (g.M < 4 || t16 <= CUS) return true;
     return (g.C < 1280 && t32 <= 192) || (g.M <= 16 && t32 < 448 && g.C < (g.M > 8 ? 1280 : 2048));
 }
 
-/* Eight waves where the sums are long and many CUs have a workgroup, but no more than one (us in eight / four: 1 x 8192 x 2048 6.9 /
- * 9.0, 44 x 6711 x 405 6.9 / 7.9; 7 x 5437 x 106 5.5 / 5.1, 52 x 3122 x 565 4.8 / 4.4, 8 x 8192 x 6000 16.5 / 15.4). */
+/* Eight waves where the sums are long and many CUs have a workgroup, but no more than one (us in eight / four: 1 x 8192 x
+ * 2048 6.9 / 9.0, 44 x 6711 x 405 6.9 / 7.9; 7 x 5437 x 106 5.5 / 5.1, 52 x 3122 x 565 4.8 / 4.4, 8 x 8192 x 6000 16.5 /
+ * 15.4). */
 template <bool BF16>
 void launch_few(GemmArgs g, hipStream_t s) {
     const dim3 d = grid_of(g, 16, 16);
@@ -576,12 +579,14 @@ void launch_few(GemmArgs g, hipStream_t s) {
     else hipLaunchKernelGGL((k_i8_few<4, BF16>), d, dim3(256), 0, s, g);
 }
 
-/* The other tiles by their sides, and what the busiest CU has to move for M x OC outputs: its rounds of tiles times a tile's
- * operands, and four bytes an output for its stores and its start. */
+/* The other tiles by their sides, and what the busiest CU has to move: its rounds of tiles times a tile's operands, and
+ * four bytes an output for its stores and its start. */
 enum { PAIR, T192, T256X128, T128X192, T128, T128X64, T64, T32X64, T32, FORMS };
-constexpr int SIDES[FORMS][2] = {{256, 256}, {192, 192}, {256, 128}, {128, 192}, {128, 128}, {128, 64}, {64, 64}, {32, 64}, {32, 32}};
-constexpr int WIDE_MIN_C = 512; /* the three below 256 x 256: their first loads take long (us in 128 x 192 / the best of the others: 944 x
-                                 * 192 x 9055 18.8 / 16.3, 3125 x 403 x 3131 21.0 / 20.0, 2267 x 602 x 2553 13.2 / 15.1) */
+constexpr int SIDES[FORMS][2] = {{256, 256}, {192, 192}, {256, 128}, {128, 192}, {128, 128},
+                                 {128, 64},  {64, 64},   {32, 64},   {32, 32}};
+/* The three below 256 x 256 take sums from here on, as their first loads take long (us in 128 x 192 / the best of the
+ * others: 944 x 192 x 9055 18.8 / 16.3, 3125 x 403 x 3131 21.0 / 20.0, 2267 x 602 x 2553 13.2 / 15.1). */
+constexpr int WIDE_MIN_C = 512;
 
 long cost_of(int form, long rounds, int C) {
     const int bm = SIDES[form][0], bn = SIDES[form][1];
@@ -592,14 +597,20 @@ struct Form {
     int form;
     long cost;
 };
-/* The form that costs least, of equals the largest.  (Over 170 shapes with 1.5 million outputs or more, 200 .. 8192 columns, its choice is
- * 2.0% slower than the best of these on average, 20% at most, and over 200 shapes of all sizes 1.3% and 22%; the largest tile that
- * 150 of are there 3.0% and 63% behind.)  us in 256 x 256, 128 x 128, 128 x 64, 64 x 64, 32 x 64 and 32 x 32 tiles: 4096 x 960 x
- * 4096 23, 33, 39, 44, -, -; 1024 x 4096 x 4096 41, 21, 25 and more; 777 x 2500 x 2000 27, 12.0, 11.2, 12.4, 18.5, 20.7; 512 x 960 x 5120
- * 15, 7.3, 8.8, 8.7, 9.7, 10.8; 142 x 6784 x 9011 -, 33, 32, 22, 32, 34; 64 x 960 x 49152 16, 14, 14, 12, 13, 16; 512 x
- * 2560 x 960 26, 10.0, 7.8, 6.2, 5.4, 5.6; 20 x 960 x 16384 13, 6.7, 5.8, 4.7, 4.1, 4.1; 16384 x 960 x 16 14, 7.1, 5.8, 5.0, 4.9, 4.0.
- * One round of 128 x 192 for two of 128 x 128: 1024 x 960 x 5120 14.5 -> 12.0, 927 x 1774 x 4628 23.7 -> 16.3; of 256 x 128: 1400 x
- * 2560 x 5000 27.8 -> 24.0; of 192 x 192 for one of 256 x 256: 1300 x 960 x 6000 19.7 -> 15.3. */
+/* The form that costs least, of equals the largest.  Over 170 shapes with 1.5 million outputs or more and 200 .. 8192
+ * columns, its choice is 2.0% slower than the best of these on average, 20% at most, and over 200 shapes of all sizes 1.3%
+ * and 22%; the largest tile that 150 of are there 4.2% and 63%.  us (eight sets of inputs in turn; the choice marked):
+ *                     256x256  192x192  256x128  128x192  128x128  128x64   64x64   32x64   32x32
+ *   4096 x 960 x 4096   24.2*    31.6     30.0     34.5     35.5     39.3    44.9    58.4    73.2
+ *   1300 x 960 x 6000   20.4     15.7*    26.4     20.2     22.5     22.0    22.1    29.4    35.0
+ *   2048 x 2560 x 4000  33.6     26.7     25.9*    33.4     28.9     32.8    39.8    55.4    68.3
+ *   1024 x 960 x 5120   18.0     15.6     13.2     12.1*    15.5     14.6    15.1    19.8    23.9
+ *   1024 x 4096 x 4096  40.7     29.0     25.8     22.9     20.3*    24.8    30.0    40.9    49.9
+ *   512 x 960 x 5120    17.2     14.1     12.0     10.5      8.5*     9.5    10.0    11.2    12.9
+ *   777 x 2500 x 1999   41.1     26.1     25.4     20.7     16.9     12.8*   15.2    19.8    21.5
+ *   64 x 960 x 49152    21.4     17.9     25.0     15.2     19.2     18.8    16.2*   19.8    23.4
+ *   512 x 2560 x 960    31.4     18.7     17.9     15.0     12.1      9.5     7.3     6.1*    6.7
+ *   16384 x 960 x 16    15.7     11.3     11.1      8.8      7.5      6.7     6.1     5.9     5.1* */
 Form form_of(const GemmArgs& g, bool pair) {
     Form best = {T32, LONG_MAX};
     for (int i = pair ? PAIR : T192; i < FORMS; i++) {
@@ -620,15 +631,15 @@ void launch_form(GemmArgs g, int form, hipStream_t s) {
     case T256X128: hipLaunchKernelGGL((k_i8_tile<4, 2, 4, 4, 128, BF16>), d, dim3(512), 0, s, g); break;
     case T128X192: hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 6, 128, BF16>), d, dim3(512), 0, s, g); break;
     case T128:
-        /* stages of 64 columns for short sums, which leave a CU room for two tiles (us in 64 / 128: 2048 x 576 x 3000 11.6 / 14.3, 539 x 448
-         * x 10861 13.5 / 15.4; one tile a CU 1586 x 640 x 1292 7.0 / 6.5, 512 x 960 x 5120 8.9 / 8.6, 1272 x 448 x 2594 7.1 / 7.5) */
+        /* stages of 64 columns for short sums, which leave a CU room for two tiles (us in 64 / 128: 2048 x 576 x 3000 11.6 /
+         * 14.3, 539 x 448 x 10861 13.5 / 15.4; one tile a CU 1586 x 640 x 1292 7.0 / 6.5, 1272 x 448 x 2594 7.1 / 7.5) */
         if (g.C < (one ? 512 : 1024)) hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 64, BF16>), d, dim3(512), 0, s, g);
         else hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 128, BF16>), d, dim3(512), 0, s, g);
         break;
     case T128X64: hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 2, 128, BF16>), d, dim3(512), 0, s, g); break;
-    /* stages of 256 columns for long sums and one tile a CU at most: 512 x 2560 x 960 7.0 us against 6.2, 64 x 4096 x 4096 8.7 /
-     * 6.8, 1000 x 8192 x 960 18.3 / 16.0; with two tiles a CU 1000 x 2560 x 960 9.1 / 9.1, 1024 x 2048 x 1500 8.7 / 11.9; 128 x
-     * 64 tiles gain from 4096 columns on, 2 to 5% */
+    /* stages of 256 columns for long sums and one tile a CU at most (us in 128 / 256: 512 x 2560 x 960 7.0 / 6.2, 64 x 4096 x
+     * 4096 8.7 / 6.8, 1000 x 8192 x 960 18.3 / 16.0; two tiles a CU 1024 x 2048 x 1500 8.7 / 11.9; 128 x 64 tiles gain from
+     * 4096 columns on, 2 to 5%) */
     case T64:
         if (one && g.C >= 2048) hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 256, BF16>), d, dim3(256), 0, s, g);
         else hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 128, BF16>), d, dim3(256), 0, s, g);
