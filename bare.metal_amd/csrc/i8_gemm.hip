@@ -636,10 +636,15 @@ void launch_form(GemmArgs g, int form, hipStream_t s) {
         if (g.C < (one ? 512 : 1024)) hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 64, BF16>), d, dim3(512), 0, s, g);
         else hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 128, BF16>), d, dim3(512), 0, s, g);
         break;
-    case T128X64: hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 2, 128, BF16>), d, dim3(512), 0, s, g); break;
     /* stages of 256 columns for long sums and one tile a CU at most (us in 128 / 256: 512 x 2560 x 960 7.0 / 6.2, 64 x 4096 x
-     * 4096 8.7 / 6.8, 1000 x 8192 x 960 18.3 / 16.0; two tiles a CU 1024 x 2048 x 1500 8.7 / 11.9; 128 x 64 tiles gain from
-     * 4096 columns on, 2 to 5%) */
+     * 4096 8.7 / 6.8, 1000 x 8192 x 960 18.3 / 16.0; two tiles a CU 1024 x 2048 x 1500 8.7 / 11.9), 128 x 64 earlier where rows
+     * straddle lines (777 x 2500 x 1999 13.1 / 12.3, 2048 x 5000 x 960 23.9 / 20.2; 777 x 1536 x 1984 7.4 / 7.9) */
+    case T128X64:
+        if (one && g.C >= (g.lda % 128 || g.ldw % 128 ? 1500 : 4096))
+            hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 2, 256, BF16>), d, dim3(512), 0, s, g);
+        else
+            hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 2, 128, BF16>), d, dim3(512), 0, s, g);
+        break;
     case T64:
         if (one && g.C >= 2048) hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 256, BF16>), d, dim3(256), 0, s, g);
         else hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 128, BF16>), d, dim3(256), 0, s, g);

@@ -398,7 +398,7 @@ def test_matmul_one_round_of_wide_tiles(be, M, OC):
     test_matmul_every_form(be, M, OC)
 
 
-@pytest.mark.parametrize("M,OC", [(500, 500), (500, 1020), (1000, 1020)])
+@pytest.mark.parametrize("M,OC", [(500, 500), (500, 1020), (1000, 1020), (2000, 1020)])
 def test_matmul_wide_stages(be, M, OC):
     """Long sums of one tile a CU, stages of 256 columns: 5 to 13 of them, whole and ragged."""
     rng = np.random.default_rng(OC)
