@@ -266,6 +266,23 @@ def test_swiglu(be, M, C, bf16):
         assert (bs.read(np.uint8)[4 * M:] == MARK).all()
 
 
+def test_swiglu_accuracy(be):
+    """Rows of one value: their scale is silu(g) / 127.  The exponential is good to a unit (two half steps), its
+    correction, the sum, the quotient and the scale round once each: six half steps, from g of -64 on."""
+    rng = np.random.default_rng(8)
+    g = np.concatenate([rng.uniform(-64, 90, 200000), rng.standard_normal(200000) * 3, 10.0 ** rng.uniform(-6, 30, 1000),
+                        -(10.0 ** rng.uniform(-6, 1.8, 1000))]).astype(np.float32)
+    n = g.size
+    bq, bs = be.alloc(n * 16), be.alloc(n * 4)
+    assert be.dispatch("swiglu_forward_i8", [be.upload(g), be.upload(np.ones(n, np.float32)), bq, bs,
+                                             be.params(n, 1, 1, 16)], (n,), (256,)) == 0
+    g64 = g.astype(np.float64)
+    want = np.abs(g64 / (1 + np.exp(-g64))) / 127
+    err = np.abs(bs.read(np.float32) - want) / want
+    print("largest error in half steps: %.2f at %g" % (err.max() / U32, g[err.argmax()]))
+    assert err.max() <= 6 * U32
+
+
 def test_swiglu_limits(be):
     """Gates far out on both sides, and NaN and infinities."""
     g = np.array([[-200, -1e30, 1e30, 90], [np.nan, 1, 1, 1], [-np.inf, 1, 1, 1], [1, 1, 1, 1], [-104, -104, -90, -88]],
