@@ -4,7 +4,8 @@
  * scale and its codes, and the checks of a matrix of codes.
  *
  * A row p of C values becomes codes q and one scale s (values q * s):
- *   top = max |p|, inv = 127 / top (IEEE division), q = round-to-even(p * inv), s = top / 127.
+ *   top = max |p|, inv = 127 * (1 / top), q = round-to-even(p * inv), s = top / 127,
+ * each step rounded to fp32 (a tensor program's 127 / top is this product, so the codes are the same bits as its).
  * p * inv is at most 127 * (1 + 2^-22), so q needs no clamp.  Two kinds of row
  * have no such grid: one that holds a NaN or an infinity gets zero codes and
  * the scale NaN (so that what is computed from it shows it), one whose top is
@@ -28,7 +29,7 @@ struct I8Grid {
 __device__ __forceinline__ I8Grid i8_grid(unsigned int top_bits) {
     I8Grid g;
     const float top = __uint_as_float(top_bits);
-    g.inv = 127.0f / top;
+    g.inv = 127.0f * (1.0f / top);
     g.step = top / 127.0f;
     if (top_bits >= 0x7f800000u) {
         g.inv = 0.0f;

@@ -49,7 +49,7 @@
  * the offset too), each row, the last one included, C codes rounded up to
  * whole 16-byte groups; the kernels that make codes write zeros behind the
  * C-th, up to that group's end, and nothing past it.  Row p of C values has
- * top = max |p|, inv = 127 / top, codes round-to-even(p * inv) in -127 .. 127
+ * top = max |p|, inv = 127 * (1 / top), codes round-to-even(p * inv) in -127 .. 127
  * and scale top / 127, each step in fp32.  A row of zeros, or whose top is
  * under 3.73e-37, has zero codes and the scale 0; a row that holds a NaN or an
  * infinity has zero codes and the scale NaN.  Row counts may be 0 (nothing is

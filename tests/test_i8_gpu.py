@@ -35,7 +35,7 @@ def grid(p):
     """Codes and the largest magnitude of fp32 rows, each step in fp32 (see include/bm_q8.h); rows without a grid: 0."""
     with np.errstate(all="ignore"):
         top = np.abs(p).max(axis=1)
-        inv = np.float32(127) / top
+        inv = np.float32(127) * (np.float32(1) / top)
         fine = np.isfinite(inv) & np.isfinite(top)
         q = np.where(fine[:, None], np.rint(p * np.where(fine, inv, 0).astype(np.float32)[:, None]), 0)
     return q.astype(np.int8), top, fine
