@@ -80,21 +80,24 @@ __device__ __forceinline__ float element(const Raw<BF16, E>& v, int e) {
 }
 
 /* x / (1 + exp(-x)), within 1.6 units in the last place, so that few codes differ from those of other sound fp32 forms
- * (4096 x 8192 bf16: 28.6 us; with one product for the exponent and the reciprocal for the quotient, within about 3 units, 29.2).
+ * (us, with one product for the exponent and the reciprocal for the quotient, within about 3 units, first: 4096 x 8192 bf16
+ * 29.2 / 28.6, 8192 x 2560 19.2 / 20.7).
  * -x log2(e) is a product t and what its rounding and that of the constant left out, w: exp(-x) = 2^t (1 + w ln 2).  The quotient
- * is corrected by its remainder.  Under -64, where exp(-x) nears the end of fp32's range and 1 + exp(x) is 1: x exp(x), as the
- * square of a root that is above the subnormal numbers, which the instruction does not give. */
+ * is corrected by its remainder.  Under -64, where exp(-x) nears the end of fp32's range and 1 + exp(x) is 1: x exp(x), as
+ * (x 2^-64) (2^(64 - t) (1 - w ln 2)), whose last product alone may be a subnormal number, which the instruction does not
+ * give; 64 - t is exact. */
 __device__ __forceinline__ float silu(float x) {
 #pragma clang fp contract(off)
-    const float c = -1.44269502f, c_rest = -1.92596299e-8f;
+    const float c = -1.44269502f, c_rest = -1.92596299e-8f, ln2 = 0.693147182f;
     const float xe = fminf(x, 128.0f), t = xe * c, w = __builtin_fmaf(xe, c_rest, __builtin_fmaf(xe, c, -t));
-    const float p = __builtin_amdgcn_exp2f(t), d = 1.0f + __builtin_fmaf(p, w * 0.693147182f, p);
+    const float p = __builtin_amdgcn_exp2f(t), d = 1.0f + __builtin_fmaf(p, w * ln2, p);
     const float r = __builtin_amdgcn_rcpf(d), q = x * r;
     float y = __builtin_fmaf(__builtin_fmaf(-q, d, x), r, q);
     if (__builtin_expect(__any(x < -64.0f), 0)) { /* a branch of the wave: choosing a lane's value cost 4 us of those 28.6 */
         asm volatile("");
-        const float h = __builtin_amdgcn_exp2f(x * 0.72134752f);
-        y = x < -64.0f ? x * (h * h) : y;
+        const float xl = fmaxf(x, -256.0f), tl = xl * c, wl = __builtin_fmaf(xl, c_rest, __builtin_fmaf(xl, c, -tl));
+        const float e = __builtin_amdgcn_exp2f(64.0f - tl);
+        y = x < -64.0f ? x * 0x1p-64f * __builtin_fmaf(e, -wl * ln2, e) : y;
     }
     return y;
 }

@@ -737,3 +737,43 @@ def test_runs_kept_in_flight_and_two_contexts(be):
         del calls2, prod2, y2
     finally:
         other.close()
+
+
+@pytest.mark.parametrize("lo,hi", [(64, 80), (80, 87), (87, 92), (92, 112)])
+def test_swiglu_accuracy_of_far_gates(be, lo, hi):
+    """silu under -64, down to where it is nothing, in rows of one value times 2^40 (exact), which keeps their scales off the
+    border of rows without a grid.  The exponential is good to a unit (two half steps), its correction, the product with g and
+    the scale round once each: five, and one for what the correction leaves out.  Under fp32's normal range silu is rounded to
+    a multiple of 2^-149."""
+    n = 100000
+    g = -np.random.default_rng(lo).uniform(lo, hi, n).astype(np.float32)
+    bq, bs = be.alloc(n * 16), be.alloc(n * 4)
+    assert be.dispatch("swiglu_forward_i8", [be.upload(g), be.upload(np.full(n, 2.0 ** 40, np.float32)), bq, bs,
+                                             be.params(n, 1, 1, 16)], (n,), (256,)) == 0
+    g64 = g.astype(np.float64)
+    want = np.abs(g64 / (1 + np.exp(-g64))) * 2.0 ** 40 / 127
+    err = np.abs(bs.read(np.float32) - want)
+    print("largest error in half steps: %.2f" % (err / (U32 * want + 2.0 ** (40 - 150) / 127)).max())
+    assert (err <= 6 * U32 * want + 2.0 ** (40 - 150) / 127).all()
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_swiglu_codes_of_far_gates(be, bf16):
+    """Rows of far gates alone: codes off the nearest by the errors of the value and of the row's largest, of 127 at most."""
+    rng = np.random.default_rng(5)
+    M, C = 300, 500
+    g, u = -rng.uniform(64, 80, (M, C)).astype(np.float32), rng.uniform(-1e3, 1e3, (M, C)).astype(np.float32)
+    g[:, 7] = g.max(axis=1)  # neighbours of the largest gate, so that a row has more than one code but 0
+    for k in range(1, C, 3):
+        g[:, k] = g[:, 7] - rng.uniform(0, 1, M).astype(np.float32)
+    if bf16:
+        g, u = from_bf16(to_bf16(g)), from_bf16(to_bf16(u))
+    p = g.astype(np.float64) / (1 + np.exp(-g.astype(np.float64))) * u
+    top = np.abs(p).max(axis=1)
+    cast = to_bf16 if bf16 else np.copy
+    bq, bs = be.alloc(M * ld16(C)), be.alloc(M * 4)
+    assert be.dispatch("swiglu_forward_i8" + ("_bf16" if bf16 else ""), [be.upload(cast(g)), be.upload(cast(u)), bq, bs,
+                                                                         be.params(M, C, C, ld16(C))], (M,), (256,)) == 0
+    q = bq.read(np.int8).reshape(M, ld16(C))[:, :C]
+    # silu 5 half steps, its product with up 1; twice (value, largest); the grid's factor 2, its product 1
+    assert (np.abs(q - p * (127 / top)[:, None]) <= 0.5 + 127 * 16 * U32).all()
