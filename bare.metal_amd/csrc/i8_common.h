@@ -5,8 +5,10 @@
  *
  * A row p of C values becomes codes q and one scale s (values q * s):
  *   top = max |p|, inv = 127 * (1 / top), q = round-to-even(p * inv), s = top / 127,
- * each step rounded to fp32 (a tensor program's 127 / top is this product, so the codes are the same bits as its).
- * p * inv is at most 127 * (1 + 2^-22), so q needs no clamp.  Two kinds of row
+ * each step rounded to fp32.  127 / top would be one rounding for inv's two, as numpy and C compute it; torch computes a
+ * number over a tensor as this product, and weights quantized there have the same codes here.
+ * p * inv is at most 127 * (1 + 2^-21), so q needs no clamp: 1 / top is off by 2^-24, or by 2^-22 where it is subnormal (top
+ * over 2^126), and the two products by 2^-24 each.  Two kinds of row
  * have no such grid: one that holds a NaN or an infinity gets zero codes and
  * the scale NaN (so that what is computed from it shows it), one whose top is
  * so small (under 3.73e-37, or all zero) that inv overflows gets zero codes

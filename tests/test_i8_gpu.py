@@ -777,3 +777,22 @@ def test_swiglu_codes_of_far_gates(be, bf16):
     q = bq.read(np.int8).reshape(M, ld16(C))[:, :C]
     # silu 5 half steps, its product with up 1; twice (value, largest); the grid's factor 2, its product 1
     assert (np.abs(q - p * (127 / top)[:, None]) <= 0.5 + 127 * 16 * U32).all()
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("C", [5, 300, 20011, 40001])
+def test_quantize_rows_up_to_the_largest_number(be, C, bf16):
+    """Rows whose largest value lies over 2^126, so that its reciprocal is subnormal, up to the type's largest."""
+    rng = np.random.default_rng(C)
+    tops = np.array([2.0 ** 126, 2.0 ** 126 * 1.01, 1e38, 1.7e38, 2.0 ** 127, 3e38, 3.3895314e38, 3.4028235e38], np.float32)
+    x = (rng.uniform(-1, 1, (8, C)).astype(np.float32) * tops[:, None]).astype(np.float32)
+    x[:, C // 2] = -tops
+    if bf16:
+        x[7, C // 2] = 3.3895314e38  # bf16's largest
+        x = from_bf16(to_bf16(np.clip(x, -3.3895314e38, 3.3895314e38)))
+    q, top, fine = grid(x)
+    assert fine.all() and (np.abs(q).max(axis=1) == 127).all()
+    bq, bs = marked(be, 8 * ld16(C)), marked(be, 32)
+    assert be.dispatch("quantize_rows_i8" + ("_bf16" if bf16 else ""), [be.upload(to_bf16(x) if bf16 else x), bq, bs,
+                                                                        be.params(8, C, C, ld16(C))], (8,), (256,)) == 0
+    check_codes(bq, q, ld16(C), C)
+    assert np.array_equal(bs.read(np.float32), top / np.float32(127))
