@@ -243,6 +243,9 @@ __device__ __forceinline__ void barrier() {
 
 constexpr int RING = 3; /* stages of a tile's ring */
 
+/* waves on each SIMD: two, of one workgroup, or of two where a CU's 160 KB hold their rings */
+constexpr int tile_waves(int waves, int stage_bytes) { return waves >= 8 || RING * stage_bytes <= 80 * 1024 ? 2 : 1; }
+
 /* MW x NW waves of TM x TN 16 x 16 tiles, stages of BK columns, a ring of
  * three: while a stage is multiplied, the first fragments of the next are read
  * and two more are on their way.  A stage's buffer is requested again at the
@@ -254,7 +257,7 @@ constexpr int RING = 3; /* stages of a tile's ring */
  * waves over 128 columns a stage 12.5 / 14.1 / 21; over 64 13.4 / 16.3 / 24; four waves
  * 13.7 / 16 / 24; a ring of two 13.2 / 17.2 / 28, of four over 64 14.3 / 18 / 26. */
 template <int MW, int NW, int TM, int TN, int BK, bool BF16>
-__global__ __launch_bounds__(64 * MW * NW, 2) void k_i8_tile(GemmArgs g) {
+__global__ __launch_bounds__(64 * MW * NW, tile_waves(MW * NW, 16 * (TM * MW + TN * NW) * BK)) void k_i8_tile(GemmArgs g) {
     constexpr int W = MW * NW, BM = 16 * TM * MW, BN = 16 * TN * NW, SB = (BM + BN) * BK;
     constexpr int CPR = BK / 16, RPI = 1024 / BK, NI = SB / 1024 / W, S = BK / 64;
     static_assert(SB % (1024 * W) == 0 && BM % (RPI * W) == 0, "whole loads, each of one operand");
