@@ -571,15 +571,28 @@ bool few_outputs(const GemmArgs& g) {
     return (g.C < 1280 && t32 <= 192) || (g.M <= 16 && t32 < 448 && g.C < (g.M > 8 ? 1280 : 2048));
 }
 
+/* The kernels by the outputs of a workgroup and, where there are more than one over them, the waves or the columns of a
+ * stage. */
+enum Kernel {
+    K_FEW_4, K_FEW_8, K_PAIR, K_192, K_256X128, K_128X192, K_128_S64, K_128_S128, K_128X64_S128, K_128X64_S256, K_64_S128,
+    K_64_S256, K_32X64_S128, K_32X64_S256, K_32_S128, K_32_S256
+};
+struct KernelInfo {
+    const char* name;
+    int bm, bn;
+};
+constexpr KernelInfo KERNELS[] = {
+    {"few 4", 16, 16}, {"few 8", 16, 16}, {"256x256", 256, 256}, {"192x192", 192, 192}, {"256x128", 256, 128},
+    {"128x192", 128, 192}, {"128x128 64", 128, 128}, {"128x128 128", 128, 128}, {"128x64 128", 128, 64},
+    {"128x64 256", 128, 64}, {"64x64 128", 64, 64}, {"64x64 256", 64, 64}, {"32x64 128", 32, 64}, {"32x64 256", 32, 64},
+    {"32x32 128", 32, 32}, {"32x32 256", 32, 32}};
+
 /* Eight waves where the sums are long and many CUs have a workgroup, but no more than one (us in eight / four: 1 x 8192 x
  * 2048 6.9 / 9.0, 44 x 6711 x 405 6.9 / 7.9; 7 x 5437 x 106 5.5 / 5.1, 52 x 3122 x 565 4.8 / 4.4, 8 x 8192 x 6000 16.5 /
  * 15.4). */
-template <bool BF16>
-void launch_few(GemmArgs g, hipStream_t s) {
-    const dim3 d = grid_of(g, 16, 16);
-    const long t16 = (long)g.tiles_m * g.tiles_n;
-    if (t16 >= 48 && t16 <= CUS && g.C >= 3500) hipLaunchKernelGGL((k_i8_few<8, BF16>), d, dim3(512), 0, s, g);
-    else hipLaunchKernelGGL((k_i8_few<4, BF16>), d, dim3(256), 0, s, g);
+Kernel few_kernel(const GemmArgs& g) {
+    const long t16 = tiles(g.M, 16) * tiles(g.OC, 16);
+    return t16 >= 48 && t16 <= CUS && g.C >= 3500 ? K_FEW_8 : K_FEW_4;
 }
 
 /* The other tiles by their sides, and what the busiest CU has to move: its rounds of tiles times a tile's operands, and
@@ -624,95 +637,99 @@ Form form_of(const GemmArgs& g, bool pair) {
     return best;
 }
 
-template <bool BF16>
-void launch_form(GemmArgs g, int form, hipStream_t s) {
-    const dim3 d = grid_of(g, SIDES[form][0], SIDES[form][1]);
-    const bool one = (long)g.tiles_m * g.tiles_n <= CUS;
+Kernel kernel_of(const GemmArgs& g, int form) {
+    const bool one = tiles(g.M, SIDES[form][0]) * tiles(g.OC, SIDES[form][1]) <= CUS;
     switch (form) {
-    case PAIR: hipLaunchKernelGGL(k_i8_pair<BF16>, d, dim3(512), 0, s, g); break;
-    case T192: hipLaunchKernelGGL((k_i8_tile<2, 4, 6, 3, 128, BF16>), d, dim3(512), 0, s, g); break;
-    case T256X128: hipLaunchKernelGGL((k_i8_tile<4, 2, 4, 4, 128, BF16>), d, dim3(512), 0, s, g); break;
-    case T128X192: hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 6, 128, BF16>), d, dim3(512), 0, s, g); break;
-    case T128:
-        /* stages of 64 columns for short sums, which leave a CU room for two tiles (us in 64 / 128: 2048 x 576 x 3000 11.6 /
-         * 14.3, 539 x 448 x 10861 13.5 / 15.4; one tile a CU 1586 x 640 x 1292 7.0 / 6.5, 1272 x 448 x 2594 7.1 / 7.5) */
-        if (g.C < (one ? 512 : 1024)) hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 64, BF16>), d, dim3(512), 0, s, g);
-        else hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 128, BF16>), d, dim3(512), 0, s, g);
-        break;
+    case PAIR: return K_PAIR;
+    case T192: return K_192;
+    case T256X128: return K_256X128;
+    case T128X192: return K_128X192;
+    /* stages of 64 columns for short sums, which leave a CU room for two tiles (us in 64 / 128: 2048 x 576 x 3000 11.6 /
+     * 14.3, 539 x 448 x 10861 13.5 / 15.4; one tile a CU 1586 x 640 x 1292 7.0 / 6.5, 1272 x 448 x 2594 7.1 / 7.5) */
+    case T128: return g.C < (one ? 512 : 1024) ? K_128_S64 : K_128_S128;
     /* stages of 256 columns for long sums and one tile a CU at most (us in 128 / 256: 512 x 2560 x 960 7.0 / 6.2, 64 x 4096 x
      * 4096 8.7 / 6.8, 1000 x 8192 x 960 18.3 / 16.0; two tiles a CU 1024 x 2048 x 1500 8.7 / 11.9), 128 x 64 earlier where rows
      * straddle lines (777 x 2500 x 1999 13.1 / 12.3, 2048 x 5000 x 960 23.9 / 20.2; 777 x 1536 x 1984 7.4 / 7.9) */
-    case T128X64:
-        if (one && g.C >= (g.lda % 128 || g.ldw % 128 ? 1500 : 4096))
-            hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 2, 256, BF16>), d, dim3(512), 0, s, g);
-        else
-            hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 2, 128, BF16>), d, dim3(512), 0, s, g);
-        break;
-    case T64:
-        if (one && g.C >= 2048) hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 256, BF16>), d, dim3(256), 0, s, g);
-        else hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 128, BF16>), d, dim3(256), 0, s, g);
-        break;
-    case T32X64:
-        if (one && g.C >= 1280) hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 2, 256, BF16>), d, dim3(256), 0, s, g);
-        else hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 2, 128, BF16>), d, dim3(256), 0, s, g);
-        break;
-    default:
-        if (one && g.C >= 1280) hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 1, 256, BF16>), d, dim3(256), 0, s, g);
-        else hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 1, 128, BF16>), d, dim3(256), 0, s, g);
+    case T128X64: return one && g.C >= (g.lda % 128 || g.ldw % 128 ? 1500 : 4096) ? K_128X64_S256 : K_128X64_S128;
+    case T64: return one && g.C >= 2048 ? K_64_S256 : K_64_S128;
+    case T32X64: return one && g.C >= 1280 ? K_32X64_S256 : K_32X64_S128;
+    default: return one && g.C >= 1280 ? K_32_S256 : K_32_S128;
+    }
+}
+
+template <bool BF16>
+void launch_kernel(GemmArgs g, Kernel k, hipStream_t s) {
+    const dim3 d = grid_of(g, KERNELS[k].bm, KERNELS[k].bn);
+    switch (k) {
+    case K_FEW_4: hipLaunchKernelGGL((k_i8_few<4, BF16>), d, dim3(256), 0, s, g); break;
+    case K_FEW_8: hipLaunchKernelGGL((k_i8_few<8, BF16>), d, dim3(512), 0, s, g); break;
+    case K_PAIR: hipLaunchKernelGGL(k_i8_pair<BF16>, d, dim3(512), 0, s, g); break;
+    case K_192: hipLaunchKernelGGL((k_i8_tile<2, 4, 6, 3, 128, BF16>), d, dim3(512), 0, s, g); break;
+    case K_256X128: hipLaunchKernelGGL((k_i8_tile<4, 2, 4, 4, 128, BF16>), d, dim3(512), 0, s, g); break;
+    case K_128X192: hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 6, 128, BF16>), d, dim3(512), 0, s, g); break;
+    case K_128_S64: hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 64, BF16>), d, dim3(512), 0, s, g); break;
+    case K_128_S128: hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 4, 128, BF16>), d, dim3(512), 0, s, g); break;
+    case K_128X64_S128: hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 2, 128, BF16>), d, dim3(512), 0, s, g); break;
+    case K_128X64_S256: hipLaunchKernelGGL((k_i8_tile<4, 2, 2, 2, 256, BF16>), d, dim3(512), 0, s, g); break;
+    case K_64_S128: hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 128, BF16>), d, dim3(256), 0, s, g); break;
+    case K_64_S256: hipLaunchKernelGGL((k_i8_tile<2, 2, 2, 2, 256, BF16>), d, dim3(256), 0, s, g); break;
+    case K_32X64_S128: hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 2, 128, BF16>), d, dim3(256), 0, s, g); break;
+    case K_32X64_S256: hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 2, 256, BF16>), d, dim3(256), 0, s, g); break;
+    case K_32_S128: hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 1, 128, BF16>), d, dim3(256), 0, s, g); break;
+    case K_32_S256: hipLaunchKernelGGL((k_i8_tile<2, 2, 1, 1, 256, BF16>), d, dim3(256), 0, s, g); break;
     }
 }
 
 constexpr long LAUNCH_COST = 170000; /* a second launch, 2 us, at the 84 KB/us of a CU's loads into LDS */
 
-/* A product whose last round of 256 x 256 tiles is far from full goes in two launches, the full rounds' rows or columns
- * and what is left in the form that suits it, where that costs less (4096 x 960 x 5120, a round and a
+struct Part {
+    GemmArgs g;
+    Kernel kernel;
+};
+/* The launches of a product.  One whose last round of 256 x 256 tiles is far from full goes in two, the full rounds' rows or
+ * columns and what is left in the form that suits it, where that costs less (4096 x 960 x 5120, a round and a
  * quarter: 37.9 -> 31.4 us; 2048 x 4096 x 9000, 1.125: 105.6 -> 68.7). */
-template <bool BF16>
-void launch(const GemmArgs& g, hipStream_t s) {
-    if (few_outputs(g)) return launch_few<BF16>(g, s);
+int parts_of(const GemmArgs& g, size_t out_size, Part (&parts)[2]) {
+    parts[0].g = parts[1].g = g;
+    if (few_outputs(g)) {
+        parts[0].kernel = few_kernel(g);
+        return 1;
+    }
     const bool pair = g.C >= PAIR_MIN_C && g.lda <= PAIR_MAX_LD && g.ldw <= PAIR_MAX_LD;
     const Form one = form_of(g, pair);
+    parts[0].kernel = kernel_of(g, one.form);
     const long tm = tiles(g.M, 256), tn = tiles(g.OC, 256), full = tm * tn / CUS;
-    if (pair && full > 0) {
-        const long m1 = full * CUS / tn, n1 = full * CUS / tm; /* rows and columns of tiles in the full rounds */
-        GemmArgs rest[2] = {g, g};
-        long least = one.cost;
-        int cut = -1;
-        Form other = one;
-        for (int i = 0; i < 2; i++) {
-            GemmArgs& r = rest[i];
-            const long n = 256 * (i ? n1 : m1);
-            if (n == 0 || n >= (i ? g.OC : g.M)) continue;
-            if (i) {
-                r.OC -= (int)n;
-                r.w += n * g.ldw;
-                r.sw += n;
-                if (r.bias) r.bias += n;
-                r.out = (char*)g.out + n * (BF16 ? 2 : 4);
-            } else {
-                r.M -= (int)n;
-                r.a += n * g.lda;
-                r.sa += n;
-                r.out = (char*)g.out + n * g.ldo * (BF16 ? 2 : 4);
-            }
-            const Form f = form_of(r, false);
-            const long cost = cost_of(PAIR, full, g.C) + f.cost + LAUNCH_COST;
-            if (cost < least) {
-                least = cost;
-                cut = i;
-                other = f;
-            }
+    if (!pair || full == 0) return 1;
+    long least = one.cost;
+    int n_parts = 1;
+    for (int columns = 0; columns < 2; columns++) {
+        const long n = 256 * (full * CUS / (columns ? tm : tn)); /* rows or columns in the full rounds */
+        if (n == 0 || n >= (columns ? g.OC : g.M)) continue;
+        GemmArgs first = g, rest = g;
+        if (columns) {
+            first.OC = (int)n;
+            rest.OC -= (int)n;
+            rest.w += n * g.ldw;
+            rest.sw += n;
+            if (rest.bias) rest.bias += n;
+            rest.out = (char*)g.out + n * out_size;
+        } else {
+            first.M = (int)n;
+            rest.M -= (int)n;
+            rest.a += n * g.lda;
+            rest.sa += n;
+            rest.out = (char*)g.out + n * g.ldo * out_size;
         }
-        if (cut >= 0) {
-            GemmArgs first = g;
-            if (cut) first.OC -= rest[1].OC;
-            else first.M -= rest[0].M;
-            launch_form<BF16>(first, PAIR, s);
-            launch_form<BF16>(rest[cut], other.form, s);
-            return;
+        const Form f = form_of(rest, false);
+        const long cost = cost_of(PAIR, full, g.C) + f.cost + LAUNCH_COST;
+        if (cost < least) {
+            least = cost;
+            parts[0] = {first, K_PAIR};
+            parts[1] = {rest, kernel_of(rest, f.form)};
+            n_parts = 2;
         }
     }
-    launch_form<BF16>(g, one.form, s);
+    return n_parts;
 }
 
 /* {codes [BT][lda], scale f32 [BT], weight codes [OC][ldw], scale f32 [OC], bias f32 [OC], out [BT][ldo],
@@ -748,8 +765,12 @@ int launch_matmul_i8(const bmk_launch_t* a, bool bf16) {
     g.M = BT;
     g.C = C;
     g.OC = OC;
-    if (bf16) launch<true>(g, a->stream);
-    else launch<false>(g, a->stream);
+    Part parts[2];
+    const int n = parts_of(g, esz, parts);
+    for (int i = 0; i < n; i++) {
+        if (bf16) launch_kernel<true>(parts[i].g, parts[i].kernel, a->stream);
+        else launch_kernel<false>(parts[i].g, parts[i].kernel, a->stream);
+    }
     BMK_LAUNCH_CHECK();
     return 0;
 }
@@ -758,3 +779,19 @@ int launch_matmul_i8(const bmk_launch_t* a, bool bf16) {
 
 extern "C" int bmk_launch_matmul_i8(const bmk_launch_t* a) { return launch_matmul_i8(a, false); }
 extern "C" int bmk_launch_matmul_i8_bf16(const bmk_launch_t* a) { return launch_matmul_i8(a, true); }
+
+/* The kernel of a product's launch `part` (from 0) and its rows and columns, or NULL past the last: for tests, so that each
+ * can say which kernel it runs. */
+extern "C" const char* bmk_matmul_i8_kernel(int BT, int C, int OC, int lda, int ldw, int part, int* rows, int* cols) {
+    GemmArgs g = {};
+    g.lda = lda;
+    g.ldw = ldw;
+    g.M = BT;
+    g.C = C;
+    g.OC = OC;
+    Part parts[2];
+    if (part < 0 || part >= parts_of(g, 4, parts)) return nullptr;
+    *rows = parts[part].g.M;
+    *cols = parts[part].g.OC;
+    return KERNELS[parts[part].kernel].name;
+}
