@@ -170,10 +170,12 @@ __device__ __forceinline__ void clear(i32x4 (&acc)[TM][TN]) {
 /* 16 x 16 outputs a workgroup; wave p of KP takes every KP-th slice of 64
  * columns from p on, two slices' loads in flight, so that a workgroup reads 64 KP
  * neighbouring bytes of a row at once.  The partial sums meet in LDS.
- * What bounds it: reading the weights (1 x 960 -> 49152 11.0 us, 4.3 TB/s), with few outputs the reads of one CU (5 x 8192
- * -> 500 7.2 us on 32 CUs), else the launch (1 x 960 -> 5120 3.4 us).  Four waves along the sum: one took 5.2 us for 1 x
- * 2560 -> 960, sixteen 4.2, eight 4.5, four 3.8.  Two and four tiles of outputs a wave, and four slices in flight: slower
- * wherever this form is the best (1 x 2560 -> 960 5.3, 7.8 and 4.5 us). */
+ * What bounds it: with many outputs reading the weights (1 x 960 -> 49152 11.0 us, 4.3 TB/s); with few, one workgroup's chain
+ * of loads, the join, the scales and the store (us with the weights in the Infinity Cache / from memory: 1 x 960 -> 5120 3.5 /
+ * 4.0, 1 x 2560 -> 960 on 60 CUs 3.9 / 5.9, 5 x 8192 -> 500 on 32 8.7 / 12.3; reading back one row of 576 codes, a load and
+ * a store, takes 1.5).  Four waves along the sum: one took 5.2 us for 1 x 2560 -> 960, sixteen 4.2, eight 4.5, four 3.8 (in the
+ * cache).  Two and four tiles of outputs a wave, and four slices in flight: slower wherever this form is the best (1 x
+ * 2560 -> 960 5.3, 7.8 and 4.5 us). */
 template <int KP, bool BF16>
 __global__ __launch_bounds__(64 * KP) void k_i8_few(GemmArgs g) {
     constexpr int U = 2;
@@ -371,8 +373,8 @@ __global__ __launch_bounds__(64 * MW * NW, tile_waves(MW * NW, 16 * (TM * MW + T
 /* 256 x 256 */
 
 constexpr size_t PAIR_MAX_LD = (size_t)1 << 23; /* 256 rows of it stay inside 32-bit offsets */
-/* Five stages (us there / in 128 x 128 tiles: 7439 x 113 x 43794 276 / 203, 2279 x 307 x 24615 71 / 63, 1356 x 364 x 24934
- * 42 / 44, 5211 x 452 x 2415 22.5 / 26.8). */
+/* Five stages (us there / in 128 x 128 tiles: 1356 x 364 x 24934 47.4 / 47.3, 5211 x 452 x 2415 21.7 / 25.4; when it took fewer,
+ * 7439 x 113 x 43794 276 / 203, 2279 x 307 x 24615 71 / 63). */
 constexpr int PAIR_MIN_C = 320;
 
 /* Eight waves of 128 x 64 (2 x 4), two on each SIMD, in two groups of four a
@@ -560,11 +562,14 @@ dim3 grid_of(GemmArgs& g, int bm, int bn) {
     return n <= MAX_GRID_X ? dim3((unsigned)n) : dim3(MAX_GRID_X, (unsigned)tiles(n, MAX_GRID_X));
 }
 
-/* Few outputs, straight from memory (us there / in tiles): a tile of 16 x 16 for each CU at most (17 x 960 x 960 2.9 / 4.2,
- * 40 x 5420 x 761 6.0 / 7.9; 344 x 1792 x 189, 264 of them, 6.0 / 4.5), or three times as many and a short sum (68 x 99 x
- * 1173 2.8 / 3.8, 37 x 198 x 2539 3.0 / 3.8; 114 x 451 x 1951 3.6 / 3.3), or few rows (16 x 960 x 5120 3.7 / 4.1, 8 x 1536 x
- * 8192 4.7 / 5.2; 8 x 4096 x 6000 8.3 / 6.6, 16 x 1536 x 6000 5.2 / 4.5) up to where the weights' way into LDS counts (8 x
- * 960 x 49152 12.5 / 11.6; but 1 x 960 x 49152 11.0 / 11.2). */
+/* Few outputs, straight from memory (us there / in tiles, eight sets of inputs in turn, which the Infinity Cache holds but for
+ * the last two's; then both over enough sets to pass it): a tile
+ * of 16 x 16 for each CU at most (17 x 960 x 960 3.0 / 3.4, 4.0 / 4.2; 40 x 5420 x 761 6.0 / 7.9, 7.0 / 10.3; 344 x 1792 x
+ * 189, 264 of them, 6.0 / 4.2, 6.6 / 5.4), or three times as many and a short sum (68 x 99 x 1173 2.7 / 2.8, 3.6 / 3.8; 37 x
+ * 198 x 2539 2.9 / 2.9, 3.7 / 3.6; 114 x 451 x 1951 3.5 / 3.3, 4.2 / 4.0), or few rows (16 x 960 x 5120 3.7 / 3.9, 4.3 /
+ * 4.4; 8 x 1536 x 8192 4.7 / 4.8, 5.6 / 5.6; 8 x 4096 x 6000 8.1 / 6.6, 9.3 / 9.2; 16 x 1536 x 6000 5.1 / 4.5, 5.9 / 5.4) up
+ * to where the weights' way into LDS counts (8 x 960 x 49152 12.7 / 12.0, 12.7 / 12.2; but 1 x 960 x 49152 10.9 / 11.2,
+ * 11.0 / 11.4). */
 bool few_outputs(const GemmArgs& g) {
     const long t32 = tiles(g.M, 32) * tiles(g.OC, 32), t16 = tiles(g.M, 16) * tiles(g.OC, 16);
     if (g.M < 4 || t16 <= CUS) return true;
@@ -587,9 +592,10 @@ constexpr KernelInfo KERNELS[] = {
     {"128x64 256", 128, 64}, {"64x64 128", 64, 64}, {"64x64 256", 64, 64}, {"32x64 128", 32, 64}, {"32x64 256", 32, 64},
     {"32x32 128", 32, 32}, {"32x32 256", 32, 32}};
 
-/* Eight waves where the sums are long and many CUs have a workgroup, but no more than one (us in eight / four: 1 x 8192 x
- * 2048 6.9 / 9.0, 44 x 6711 x 405 6.9 / 7.9; 7 x 5437 x 106 5.5 / 5.1, 52 x 3122 x 565 4.8 / 4.4, 8 x 8192 x 6000 16.5 /
- * 15.4). */
+/* Eight waves where the sums are long and many CUs have a workgroup, but no more than one (us in eight / four, inputs in the
+ * Infinity Cache: 1 x 8192 x 2048 6.8 / 8.9, 44 x 6711 x 405 6.8 / 7.9; 7 x 5437 x 106 5.2 / 5.1, 52 x 3122 x 565 4.3 / 4.4,
+ * 8 x 8192 x 6000 16.5 / 15.3).  With weights from HBM eight are ahead before that (8.3 / 12.4, 8.2 / 10.8; 6.5 / 9.1, 5.3 /
+ * 6.7; 1 x 2560 x 960 5.0 / 5.9): the border is the cache's. */
 Kernel few_kernel(const GemmArgs& g) {
     const long t16 = tiles(g.M, 16) * tiles(g.OC, 16);
     return t16 >= 48 && t16 <= CUS && g.C >= 3500 ? K_FEW_8 : K_FEW_4;
@@ -601,7 +607,8 @@ enum { PAIR, T192, T256X128, T128X192, T128, T128X64, T64, T32X64, T32, FORMS };
 constexpr int SIDES[FORMS][2] = {{256, 256}, {192, 192}, {256, 128}, {128, 192}, {128, 128},
                                  {128, 64},  {64, 64},   {32, 64},   {32, 32}};
 /* The three below 256 x 256 take sums from here on, as their first loads take long (us in 128 x 192 / the best of the
- * others: 944 x 192 x 9055 18.8 / 16.3, 3125 x 403 x 3131 21.0 / 20.0, 2267 x 602 x 2553 13.2 / 15.1). */
+ * others: 944 x 192 x 9055 18.5 / 15.4, though 192 x 192 takes 13.7, 3125 x 403 x 3131 20.2 / 19.1, 2267 x 602 x 2553 13.1 /
+ * 14.3). */
 constexpr int WIDE_MIN_C = 512;
 
 long cost_of(int form, long rounds, int C) {
@@ -614,19 +621,20 @@ struct Form {
     long cost;
 };
 /* The form that costs least, of equals the largest.  Over 170 shapes with 1.5 million outputs or more and 200 .. 8192
- * columns, its choice is 2.0% slower than the best of these on average, 20% at most, and over 200 shapes of all sizes 1.3%
- * and 22%; the largest tile that 150 of are there 4.2% and 63%.  us (eight sets of inputs in turn; the choice marked):
- *                     256x256  192x192  256x128  128x192  128x128  128x64   64x64   32x64   32x32
- *   4096 x 960 x 4096   24.2*    31.6     30.0     34.5     35.5     39.3    44.9    58.4    73.2
- *   1300 x 960 x 6000   20.4     15.7*    26.4     20.2     22.5     22.0    22.1    29.4    35.0
- *   2048 x 2560 x 4000  33.6     26.7     25.9*    33.4     28.9     32.8    39.8    55.4    68.3
- *   1024 x 960 x 5120   18.0     15.6     13.2     12.1*    15.5     14.6    15.1    19.8    23.9
- *   1024 x 4096 x 4096  40.7     29.0     25.8     22.9     20.3*    24.8    30.0    40.9    49.9
- *   512 x 960 x 5120    17.2     14.1     12.0     10.5      8.5*     9.5    10.0    11.2    12.9
- *   777 x 2500 x 1999   41.1     26.1     25.4     20.7     16.9     12.8*   15.2    19.8    21.5
- *   64 x 960 x 49152    21.4     17.9     25.0     15.2     19.2     18.8    16.2*   19.8    23.4
- *   512 x 2560 x 960    31.4     18.7     17.9     15.0     12.1      9.5     7.3     6.1*    6.7
- *   16384 x 960 x 16    15.7     11.3     11.1      8.8      7.5      6.7     6.1     5.9     5.1* */
+ * columns, what is chosen is 2.3% slower than the best kernel on average, 44% at most (1134 x 338 x 7412 16.7 us, 11.6 in 192 x
+ * 192, which starts at WIDE_MIN_C); over 200 shapes of all sizes 2.7%, 47% at most (455 x 894 x 289 5.1 straight from memory,
+ * 3.5 in 32 x 32); the largest tile that 150 of are there, over other shapes, 4.2% and 63%.  us (eight sets of inputs in turn; the choice marked):
+ *                      256x256  192x192  256x128  128x192  128x128   128x64    64x64    32x64    32x32
+ *   4096 x 960 x 4096     22.0*    32.7     30.4     34.8     31.5     35.8     41.9     57.6     71.2
+ *   1300 x 960 x 6000     19.3     15.3*    26.4     20.5     21.9     21.7     21.8     28.1     33.7
+ *   2048 x 2560 x 4000    31.5     25.2     25.1*    34.4     28.2     31.7     39.1     55.2     68.2
+ *   1024 x 960 x 5120     17.7     14.8     12.7     12.4*    14.4     14.3     15.1     19.5     23.2
+ *   1024 x 4096 x 4096    40.0     27.3     24.7     23.1     21.6*    24.0     29.5     41.0     50.1
+ *   512 x 960 x 5120      17.1     13.7     11.9     10.4      8.4*     9.4      9.6     11.2     12.6
+ *   777 x 2500 x 1999     41.0     26.0     25.3     20.6     16.8     11.8*    15.1     19.7     21.3
+ *   64 x 960 x 49152      20.6     19.3     26.0     16.1*    19.6     20.8     17.1     20.1     23.6
+ *   512 x 2560 x 960      31.3     18.7     17.9     14.9     12.1      9.5      7.3      6.1*     6.7
+ *   16384 x 960 x 16      15.4     11.2     11.2      8.7      7.4      6.7      6.1      5.8      5.1* */
 Form form_of(const GemmArgs& g, bool pair) {
     Form best = {T32, LONG_MAX};
     for (int i = pair ? PAIR : T192; i < FORMS; i++) {
@@ -644,12 +652,13 @@ Kernel kernel_of(const GemmArgs& g, int form) {
     case T192: return K_192;
     case T256X128: return K_256X128;
     case T128X192: return K_128X192;
-    /* stages of 64 columns for short sums, which leave a CU room for two tiles (us in 64 / 128: 2048 x 576 x 3000 11.6 /
-     * 14.3, 539 x 448 x 10861 13.5 / 15.4; one tile a CU 1586 x 640 x 1292 7.0 / 6.5, 1272 x 448 x 2594 7.1 / 7.5) */
+    /* stages of 64 columns for short sums, which leave a CU room for two tiles (us in 64 / 128: 2048 x 576 x 3000 11.8 /
+     * 14.5, 539 x 448 x 10861 13.3 / 15.0; one tile a CU 1586 x 640 x 1292 7.0 / 6.4, 1272 x 448 x 2594 7.1 / 7.4) */
     case T128: return g.C < (one ? 512 : 1024) ? K_128_S64 : K_128_S128;
-    /* stages of 256 columns for long sums and one tile a CU at most (us in 128 / 256: 512 x 2560 x 960 7.0 / 6.2, 64 x 4096 x
-     * 4096 8.7 / 6.8, 1000 x 8192 x 960 18.3 / 16.0; two tiles a CU 1024 x 2048 x 1500 8.7 / 11.9), 128 x 64 earlier where rows
-     * straddle lines (777 x 2500 x 1999 13.1 / 12.3, 2048 x 5000 x 960 23.9 / 20.2; 777 x 1536 x 1984 7.4 / 7.9) */
+    /* stages of 256 columns for long sums and one tile a CU at most (us in 128 / 256: 32 x 64 512 x 2560 x 960 7.0 / 6.1, 32 x
+     * 32 64 x 4096 x 4096 8.6 / 6.6, 64 x 64 1000 x 8192 x 960 18.2 / 16.4; two tiles a CU 1024 x 2048 x 1500 8.7 / 11.7), 128 x
+     * 64 earlier where rows straddle lines (777 x 2500 x 1999 12.7 / 11.8, 2048 x 5000 x 960 21.5 / 19.6; 777 x 1536 x 1984
+     * 7.3 / 7.7) */
     case T128X64: return one && g.C >= (g.lda % 128 || g.ldw % 128 ? 1500 : 4096) ? K_128X64_S256 : K_128X64_S128;
     case T64: return one && g.C >= 2048 ? K_64_S256 : K_64_S128;
     case T32X64: return one && g.C >= 1280 ? K_32X64_S256 : K_32X64_S128;
@@ -688,7 +697,7 @@ struct Part {
 };
 /* The launches of a product.  One whose last round of 256 x 256 tiles is far from full goes in two, the full rounds' rows or
  * columns and what is left in the form that suits it, where that costs less (4096 x 960 x 5120, a round and a
- * quarter: 37.9 -> 31.4 us; 2048 x 4096 x 9000, 1.125: 105.6 -> 68.7). */
+ * quarter: 41.7 -> 35.1 us; 2048 x 4096 x 9000, 1.125: 108 -> 82). */
 int parts_of(const GemmArgs& g, size_t out_size, Part (&parts)[2]) {
     parts[0].g = parts[1].g = g;
     if (few_outputs(g)) {

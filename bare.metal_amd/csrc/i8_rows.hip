@@ -81,7 +81,7 @@ __device__ __forceinline__ float element(const Raw<BF16, E>& v, int e) {
 
 /* x / (1 + exp(-x)), within 1.6 units in the last place, so that few codes differ from those of other sound fp32 forms
  * (us, with one product for the exponent and the reciprocal for the quotient, within about 3 units, first: 4096 x 8192 bf16
- * 29.2 / 28.6, 8192 x 2560 19.2 / 20.7).
+ * 30.0 / 30.0, 8192 x 2560 20.7 / 22.9).  Under -64 within 1.8.
  * -x log2(e) is a product t and what its rounding and that of the constant left out, w: exp(-x) = 2^t (1 + w ln 2).  The quotient
  * is corrected by its remainder.  Under -64, where exp(-x) nears the end of fp32's range and 1 + exp(x) is 1: x exp(x), as
  * (x 2^-64) (2^(64 - t) (1 - w ln 2)), whose last product alone may be a subnormal number, which the instruction does not
@@ -93,7 +93,7 @@ __device__ __forceinline__ float silu(float x) {
     const float p = __builtin_amdgcn_exp2f(t), d = 1.0f + __builtin_fmaf(p, w * ln2, p);
     const float r = __builtin_amdgcn_rcpf(d), q = x * r;
     float y = __builtin_fmaf(__builtin_fmaf(-q, d, x), r, q);
-    if (__builtin_expect(__any(x < -64.0f), 0)) { /* a branch of the wave: choosing a lane's value cost 4 us of those 28.6 */
+    if (__builtin_expect(__any(x < -64.0f), 0)) { /* a branch of the wave: choosing a lane's value cost 4 us of those 30.0 */
         asm volatile("");
         const float xl = fmaxf(x, -256.0f), tl = xl * c, wl = __builtin_fmaf(xl, c_rest, __builtin_fmaf(xl, c, -tl));
         const float e = __builtin_amdgcn_exp2f(64.0f - tl);
@@ -176,9 +176,9 @@ __device__ __forceinline__ float norm_scale(unsigned int top, double ss, int C, 
  * written.  A workgroup takes several rows in turn where there are more than
  * the launch has workgroups, and keeps the norm's weights.
  * What bounds it: HBM, with many rows (TB/s of what is read and written: 49152 x
- * 960 6.0, 8192 x 4096 norm 6.3, 4096 x 8192 bf16 SwiGLU 5.7, where its arithmetic
- * is close behind; a 1 GiB copy reaches 5.1); with few, the chain of load,
- * reduction and store (one row of 576 2.5 us, 333 of 960 2.8). */
+ * 960 6.0, and 5.4 with its codes' reading back between, 8192 x 4096 norm 6.3, 4096 x 8192 bf16 SwiGLU 5.6, where its
+ * arithmetic is close behind; a 1 GiB copy reaches 5.1); with few, the chain of load,
+ * reduction and store (the norm of one row of 576 2.3 us, 333 of 960 bf16 4.2). */
 template <int OP, bool BF16, int LPR, int NV>
 __global__ __launch_bounds__(LPR < 64 ? 64 : LPR) void k_rows_i8(RowArgs a) {
     constexpr int E = G<OP, BF16>, NT = LPR < 64 ? 64 : LPR, RPW = NT / LPR, WAVES = NT / 64;
@@ -288,7 +288,8 @@ __global__ __launch_bounds__(LPR < 64 ? 64 : LPR) void k_rows_i8(RowArgs a) {
     }
 }
 
-/* Rows of any length, read twice. */
+/* Rows of any length, read twice, an element a lane and load.  TB/s of what has to be read and written: norm of 2048 x 16384
+ * 3.0 (144 us), fp32 SwiGLU of 2048 x 28672 2.3 (233), 2048 x 40000 quantized 2.5 (165). */
 template <int OP, bool BF16>
 __device__ __forceinline__ float row_value(const RowArgs& a, size_t row, int c, float* h) {
     const float x = load1<BF16>(a.x, row * a.ldx + c);
@@ -341,7 +342,8 @@ __global__ __launch_bounds__(1024) void k_rows_i8_long(RowArgs a) {
 }
 
 /* code * scale: LPR lanes a row, 8 (to bf16) or 4 codes a lane and step, so that a lane stores 16 bytes.  HBM-bound: 49152 x
- * 960 to bf16 21.7 us (6.5 TB/s, the codes from the Infinity Cache), 8192 x 4096 15.4 (6.5). */
+ * 960 to bf16 21.7 us (6.5 TB/s) with the codes from the Infinity Cache, where they were just written, 28.0 (5.1) with them
+ * from memory, to fp32 48.6 (4.9); 8192 x 4096 15.4, 20.1 and 33.5. */
 template <bool BF16, int LPR>
 __global__ __launch_bounds__(256) void k_rows_back(const unsigned char* q, const float* s, void* dst, size_t ldq,
                                                    size_t ldd, int rows, int C) {
@@ -400,7 +402,7 @@ void launch_wide(const RowArgs& r, int groups, hipStream_t s) {
 }
 
 /* Lanes a row and groups a lane, the fewest lanes that hold the row (8192 x 2560
- * bf16 SwiGLU, 320 groups: 26.7 us with two on each of 256 lanes, 19.3 with three on 128; 46427 x
+ * bf16 SwiGLU, 320 groups: 27.2 us with two on each of 256 lanes, 22.9 with three on 128; 46427 x
  * 192 quantized, 48 groups: 14.0 with one on each of 64, 9.0 with three on 16; 65536 x 256 19.5 / 15.1, but the
  * norm of 32768 x 256, with three operands a group, 19.0 / 20.0).
  * NV is the smallest that does, so all but a lane's last group lie inside the row. */

@@ -65,7 +65,8 @@
  *   "rmsnorm_forward_i8", "rmsnorm_forward_i8_bf16"
  *                        {x T [N][C], residual f32 [N][C], weight f32 [C], sum f32 [N][C],
  *                         codes [N][ldq], scale f32 [N], params int{N, C, ldq, has_residual},
- *                         eps f32}: sum = x + residual, p = sum * weight (fp32 products), the codes
+ *                         eps f32}: sum = x + residual, p = sum * weight (fp32 products: one past fp32's
+ *                         range is an infinity of its row, whatever the norm), the codes
  *                         and scale of p / sqrt(mean sum^2 + eps); sum may be the residual's (or an
  *                         f32 x's) own buffer.  With has_residual 0, x takes the sum's place and
  *                         buffers 1 and 3 are not touched (bind any)
