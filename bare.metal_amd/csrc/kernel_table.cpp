@@ -3,7 +3,8 @@
  * kernel_table.cpp — the named gfx950 kernels the HIP backend resolves in
  * backend_kernel_create.  Names and buffer orders follow the reference's
  * Metal kernels where one exists (cited per entry); the rest are MI355X
- * additions whose buffer orders are documented in include/bm_q8.h.
+ * additions whose buffer orders are documented in include/bm_q8.h and
+ * include/bm_paged.h.
  *
  * Columns: name, buffers bound, by-value buffer mask, written buffer mask.
  */
@@ -51,6 +52,14 @@ int bmk_launch_swiglu_i8(const bmk_launch_t* a);
 int bmk_launch_swiglu_i8_bf16(const bmk_launch_t* a);
 int bmk_launch_matmul_i8(const bmk_launch_t* a);
 int bmk_launch_matmul_i8_bf16(const bmk_launch_t* a);
+int bmk_launch_rope_rows(const bmk_launch_t* a);
+int bmk_launch_rope_rows_bf16(const bmk_launch_t* a);
+int bmk_launch_qk_norm_rope(const bmk_launch_t* a);
+int bmk_launch_qk_norm_rope_bf16(const bmk_launch_t* a);
+int bmk_launch_kv_append(const bmk_launch_t* a);
+int bmk_launch_kv_append_bf16(const bmk_launch_t* a);
+int bmk_launch_attn_paged(const bmk_launch_t* a);
+int bmk_launch_attn_paged_bf16(const bmk_launch_t* a);
 }
 
 #define B(i) (1u << (i))
@@ -165,5 +174,19 @@ extern "C" const bmk_desc_t bmk_table[] = {
     /* {codes, scale, weight codes, weight scale, bias, out, params{BT,C,OC,has_bias,lda,ldw,ldo}} */
     {"matmul_forward_i8", 7, B(6), B(5), bmk_launch_matmul_i8, 0},
     {"matmul_forward_i8_bf16", 7, B(6), B(5), bmk_launch_matmul_i8_bf16, 0},
+    /* new: several sequences over a paged cache (include/bm_paged.h); _bf16: bf16 rows and cache */
+    /* {x, out, pos, turns, params{N,NH,HD,rot,layout,ldx,ldo}, mscale} */
+    {"rope_forward_rows", 6, B(4) | B(5), B(1), bmk_launch_rope_rows, 0},
+    {"rope_forward_rows_bf16", 6, B(4) | B(5), B(1), bmk_launch_rope_rows_bf16, 0},
+    /* {q, k, q out, k out, pos, turns, gain, params{N,NH,NKV,HD,rot,layout,ldq,ldk,ldqo,ldko}, {mscale,eps}} */
+    {"qk_norm_rope_forward", 9, B(7) | B(8), B(2) | B(3), bmk_launch_qk_norm_rope, 0},
+    {"qk_norm_rope_forward_bf16", 9, B(7) | B(8), B(2) | B(3), bmk_launch_qk_norm_rope_bf16, 0},
+    /* {q, k, v, q out, cache, start, len, pages, turns, gain,
+     *  params{N,S,NH,NKV,HD,rot,layout,ldq,ldk,ldv,ldqo,page,n_pages,max_pages,norm}, {mscale,eps}} */
+    {"kv_append_paged", 12, B(10) | B(11), B(3) | B(4), bmk_launch_kv_append, 0},
+    {"kv_append_paged_bf16", 12, B(10) | B(11), B(3) | B(4), bmk_launch_kv_append_bf16, 0},
+    /* {q, cache, out, start, len, pages, params{N,S,NH,NKV,HD,ldq,ldo,page,n_pages,max_pages,causal,window}, scale} */
+    {"attention_forward_paged", 8, B(6) | B(7), B(2), bmk_launch_attn_paged, 0},
+    {"attention_forward_paged_bf16", 8, B(6) | B(7), B(2), bmk_launch_attn_paged_bf16, 0},
     {nullptr, 0, 0, 0, nullptr, 0},
 };

@@ -4,7 +4,7 @@
 The library's C ABI is declared in include/backend.h (the reference's
 backend interface, src/backend/backend.h:12-67), include/baremetal.h (the
 engine API, reference include/baremetal.h:120-206) and include/bm_q8.h /
-include/bm_synth.h (MI355X additions).  This module only marshals numpy
+include/bm_paged.h / include/bm_synth.h (MI355X additions).  This module only marshals numpy
 arrays across that ABI; it never computes anything itself, and it raises if
 the built library is missing instead of falling back to any other path.
 """
@@ -111,6 +111,7 @@ def lib() -> C.CDLL:
         "dec_persist_nch": (i, [i, i]),
         "dec_persist_hw_ok": (i, [C.c_char_p, i]),
         "bm_profile_phases": (C.c_long, [vp, vp]),
+        "bm_rope_turns": (i, [i, i, d, d, d, d, d, vp, vp]),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)
@@ -151,6 +152,21 @@ def synth_uniform_int(seed: int, lo: int, hi: int, n: int) -> np.ndarray:
     out = np.empty(n, dtype=np.int32)
     lib().bm_synth_uniform_int(seed, lo, hi, _ptr(out), n)
     return out
+
+
+# ---------------------------------------------------------------- rotary table (include/bm_paged.h)
+
+TURNS_SCALING = {"none": 0, "llama3": 1, "linear": 2, "yarn": 3}
+
+
+def rope_turns(rot: int, theta: float, scaling: str = "none", factor: float = 1.0, low: float = 0.0, high: float = 0.0,
+               original: float = 0.0):
+    """The table of turns a position (u64 [rot / 2]) and the factor of the rotated part, of bm_rope_turns."""
+    table, mscale = np.zeros(max(rot // 2, 1), np.uint64), C.c_float()
+    if lib().bm_rope_turns(rot, TURNS_SCALING[scaling], theta, factor, low, high, original, _ptr(table),
+                           C.byref(mscale)) != 0:
+        raise ValueError("bm_rope_turns rejected the rotation")
+    return table, mscale.value
 
 
 # ---------------------------------------------------------------- Q8 multi-matvec plan

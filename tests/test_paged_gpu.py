@@ -1,0 +1,831 @@
+# SPDX-License-Identifier: MPL-2.0
+"""Serving from a paged cache (include/bm_paged.h) through the backend's C ABI against the formulas in 64 bits.
+
+Tolerances count roundings: U32 = 2^-24 and UB16 = 2^-8, half a step relative to the value."""
+import numpy as np
+import pytest
+
+import bmhip
+
+pytestmark = pytest.mark.gpu
+U32, UB16 = 2.0 ** -24, 2.0 ** -8
+MARK = 0x5A  # what lies in buffers where nothing may be written
+THETA = 500000.0
+SCALED = dict(factor=8.0, low=1.0, high=4.0, original=8192.0)
+
+
+def to_bf16(x):
+    """fp32 -> bf16 bits, round to nearest even; NaN stays one."""
+    u = np.ascontiguousarray(x, np.float32).view(np.uint32).astype(np.uint64)
+    r = ((u + 0x7FFF + ((u >> 16) & 1)) >> 16).astype(np.uint16)
+    return np.where(np.isnan(x), np.uint16(0x7FC0), r)
+
+
+def from_bf16(b):
+    return (np.asarray(b, np.uint16).astype(np.uint32) << 16).view(np.float32)
+
+
+class Kind:
+    """f32 or bf16 values: how they lie in memory, and half a step of theirs."""
+
+    def __init__(self, bf16):
+        self.bf16, self.suffix, self.size = bf16, "_bf16" if bf16 else "", 2 if bf16 else 4
+        self.memory, self.step = (np.uint16, UB16) if bf16 else (np.float32, 0.0)
+
+    def held(self, x):
+        """The values that memory holds of x."""
+        return from_bf16(to_bf16(x)) if self.bf16 else np.ascontiguousarray(x, np.float32)
+
+    def raw(self, x):
+        return to_bf16(x) if self.bf16 else np.ascontiguousarray(x, np.float32)
+
+    def values(self, raw):
+        return from_bf16(raw) if self.bf16 else raw
+
+
+KINDS = [Kind(False), Kind(True)]
+both = pytest.mark.parametrize("kind", KINDS, ids=["f32", "bf16"])
+
+
+def strided(kind, x, ld, lead):
+    """Rows of x, ld elements apart, behind `lead` elements, the mark between and behind them."""
+    out = np.zeros(lead + len(x) * ld + 3, kind.memory)
+    out.view(np.uint8)[:] = MARK
+    for r in range(len(x)):
+        out[lead + r * ld:lead + r * ld + x.shape[1]] = kind.raw(x[r])
+    return out
+
+
+def rows_of(kind, buf, n, width, ld, lead, written=None):
+    """The rows' values; everything outside them (and the rows that are not written) still holds the mark."""
+    raw = buf.read(kind.memory).copy()
+    out = np.stack([raw[lead + r * ld:lead + r * ld + width] for r in range(n)]) if n else np.zeros((0, width), kind.memory)
+    for r in range(n):
+        if written is None or written[r]:
+            raw[lead + r * ld:lead + r * ld + width].view(np.uint8)[:] = MARK
+    assert (raw.view(np.uint8) == MARK).all()
+    return kind.values(out)
+
+
+def marked(be, nbytes):
+    return be.upload(np.full((nbytes + 3) // 4 * 4, MARK, np.uint8))
+
+
+def floats(be, *v):
+    return be.upload(np.float32(v))
+
+
+# ---------------------------------------------------------------- the rotation
+
+def turn_table(rot, scaling):
+    return bmhip.rope_turns(rot, THETA, scaling, **SCALED)
+
+
+def turned(x, pos, rot, layout, table, mscale):
+    """x [n][heads][HD] in 64 bits, turned, and what the fp32 steps may be off: the angle of the table's turns is exact
+    in integers.  cos and sin are off by 3 units of 2^-24 (the angle's two roundings at up to pi/4, their own one, the
+    series' end), mscale, product and sum round once each: 6 (|x0| + |x1|) mscale."""
+    x = x.astype(np.float64)
+    y, off = x.copy(), np.zeros_like(x)
+    h = rot // 2
+    a = np.array([[(int(p) * int(t) % (1 << 64)) / 2.0 ** 64 for t in table[:h]] for p in pos]).reshape(len(pos), 1, h) * 2 * np.pi
+    c, s = np.cos(a) * mscale, np.sin(a) * mscale
+    i0, i1 = (np.arange(h), np.arange(h) + h) if layout == 0 else (2 * np.arange(h), 2 * np.arange(h) + 1)
+    x0, x1 = x[..., i0], x[..., i1]
+    y[..., i0], y[..., i1] = x0 * c - x1 * s, x0 * s + x1 * c
+    off[..., i0] = off[..., i1] = 6 * U32 * (np.abs(x0) + np.abs(x1)) * abs(mscale)
+    return y, off
+
+
+def normed(x, gain, eps):
+    """RMSNorm of heads in 64 bits: two roundings of fp32, and the sums' and root's far smaller ones."""
+    x = x.astype(np.float64)
+    return x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * gain.astype(np.float64)
+
+
+def check(kind, got, want, off):
+    """Within off (of the fp32 steps) and the result's rounding."""
+    bad = ~(np.abs(got - want) <= off * 1.001 + kind.step * (np.abs(want) + off) + 1e-37)
+    assert not bad.any(), (np.argwhere(bad)[:5], got[bad][:5], want[bad][:5])
+
+
+def positions(rng, n, far):
+    p = rng.integers(-far, far, n).astype(np.int32)
+    p[:1] = 0
+    p[1:3] = [(1 << 31) - 1, -(1 << 31)][:max(0, n - 1)]
+    return p
+
+
+ROPE = [  # rows, heads, head size, rot
+    (1, 1, 2, 2), (2, 3, 6, 4), (1, 12, 64, 64), (5, 2, 64, 0), (3, 5, 64, 32), (7, 3, 80, 40), (4, 2, 96, 96), (9, 4, 80, 20),
+    (6, 3, 128, 64), (2, 40, 128, 128), (33, 2, 256, 256), (5, 1, 256, 64), (3, 2, 254, 252), (130, 9, 16, 8), (1, 1, 256, 2),
+    (4, 3, 72, 24), (4, 3, 88, 88)]
+
+
+@both
+@pytest.mark.parametrize("layout", [0, 1], ids=["halves", "pairs"])
+@pytest.mark.parametrize("N,NH,HD,rot", ROPE)
+def test_rope_rows(be, N, NH, HD, rot, layout, kind):
+    rng = np.random.default_rng(N * 1009 + NH * 101 + HD + rot)
+    W = NH * HD
+    x = kind.held(rng.standard_normal((N, W)) * np.exp(rng.uniform(-3, 3, (N, 1))))
+    pos = positions(rng, N, 1 << 20)
+    for scaling, ldx, ldo, lead in (("none", W, W, 0), ("yarn", W + 1, W + 3, 1), ("llama3", W + 8, W + 16, 8),
+                                    ("linear", W + 4, W + 2, 4)):
+        table, m = turn_table(rot, scaling)
+        want, off = turned(x.reshape(N, NH, HD), pos, rot, layout, table, m)
+        src, out = be.upload(strided(kind, x, ldx, lead)), marked(be, (lead + N * ldo + 3) * kind.size)
+        shift = [lead * kind.size, lead * kind.size, 0, 0, 0, 0]
+        assert be.dispatch("rope_forward_rows" + kind.suffix, [
+            src, out, be.upload(pos), be.upload(table), be.params(N, NH, HD, rot, layout, ldx, ldo), floats(be, m)], (N,),
+            (256,), offsets=shift) == 0
+        got = rows_of(kind, out, N, W, ldo, lead)
+        check(kind, got, want.reshape(N, W), off.reshape(N, W))
+        # in place: the same bits
+        assert be.dispatch("rope_forward_rows" + kind.suffix, [
+            src, src, be.upload(pos), be.upload(table), be.params(N, NH, HD, rot, layout, ldx, ldx), floats(be, m)], (N,),
+            (256,), offsets=shift) == 0
+        assert np.array_equal(rows_of(kind, src, N, W, ldx, lead).view(np.uint32), got.view(np.uint32))
+
+
+@both
+def test_rope_leaves_the_rest_of_a_head(be, kind):
+    """Elements from rot on come through bit for bit, infinities and NaN too, and do not touch the turned ones."""
+    N, NH, HD, rot = 3, 4, 64, 32
+    rng = np.random.default_rng(1)
+    x = kind.held(rng.standard_normal((N, NH, HD)))
+    x[..., rot:] = np.float32([np.inf, np.nan, -np.inf, -0.0])[rng.integers(0, 4, (N, NH, HD - rot))]
+    table, m = turn_table(rot, "none")
+    for layout in (0, 1):
+        out = marked(be, N * NH * HD * kind.size)
+        assert be.dispatch("rope_forward_rows" + kind.suffix, [
+            be.upload(kind.raw(x)), out, be.upload(np.int32([0, 5, 1 << 20])), be.upload(table),
+            be.params(N, NH, HD, rot, layout, NH * HD, NH * HD), floats(be, m)], (N,), (256,)) == 0
+        got = kind.values(out.read(kind.memory, N * NH * HD)).reshape(N, NH, HD)
+        assert np.array_equal(got[..., rot:], x[..., rot:], equal_nan=True) and np.isfinite(got[..., :rot]).all()
+        assert np.array_equal(got[0], x[0], equal_nan=True)  # position 0: no turn
+
+
+def test_rope_keeps_lengths_and_distances(be):
+    """Closed forms: a turn keeps a pair's length, and a dot product depends on the positions' difference alone."""
+    NH, HD = 2, 64
+    rng = np.random.default_rng(2)
+    x = rng.standard_normal((1, NH * HD)).astype(np.float32)
+    pos = np.int32([0, 7, 1000, 1007, 1 << 20, (1 << 20) + 7, (1 << 30), (1 << 30) + 7])
+    rows = np.repeat(x, len(pos), 0)
+    table, m = turn_table(HD, "none")
+    out = marked(be, rows.nbytes)
+    assert be.dispatch("rope_forward_rows", [be.upload(rows), out, be.upload(pos), be.upload(table),
+                                             be.params(len(pos), NH, HD, HD, 0, NH * HD, NH * HD), floats(be, m)],
+                       (8,), (256,)) == 0
+    y = out.read(np.float32).reshape(len(pos), NH, HD).astype(np.float64)
+    length = np.hypot(y[..., :HD // 2], y[..., HD // 2:])
+    x = x.reshape(NH, HD).astype(np.float64)
+    assert np.abs(length - np.hypot(x[:, :HD // 2], x[:, HD // 2:])).max() <= 12 * U32 * np.abs(x).max() * 2
+    dots = np.einsum("phd,phd->ph", y[0::2], y[1::2])
+    # each product of two elements is off by 12 U32 of the pair's magnitudes
+    assert np.abs(dots - dots[0]).max() <= 2 * 12 * U32 * 2 * (x * x).sum(-1).max() * 2
+
+
+@both
+@pytest.mark.parametrize("layout", [0, 1], ids=["halves", "pairs"])
+@pytest.mark.parametrize("N,NH,NKV,HD,rot", [(1, 1, 1, 2, 2), (1, 9, 3, 64, 64), (5, 4, 1, 64, 32), (3, 15, 5, 64, 64),
+                                             (7, 3, 3, 80, 40), (2, 32, 8, 128, 128), (4, 2, 1, 256, 128), (66, 2, 1, 96, 0),
+                                             (3, 2, 2, 254, 250), (2, 2, 5, 72, 72)])
+def test_qk_norm_rope(be, N, NH, NKV, HD, rot, layout, kind):
+    rng = np.random.default_rng(N * 1009 + NH * 101 + HD + rot)
+    Q, K, eps = NH * HD, NKV * HD, 1e-5
+    q, k = (kind.held(rng.standard_normal((N, w)) * np.exp(rng.uniform(-3, 3, (N, 1)))) for w in (Q, K))
+    gain = (1 + 0.3 * rng.standard_normal((2, HD))).astype(np.float32)
+    pos = positions(rng, N, 1 << 17)
+    table, m = turn_table(rot, "yarn")
+    for ldq, ldk, ldqo, ldko, lead in ((Q, K, Q, K, 0), (Q + 1, K + 2, Q + 3, K + 1, 1), (Q + K, Q + K, Q + 8, K + 8, 8)):
+        bq, bk = be.upload(strided(kind, q, ldq, lead)), be.upload(strided(kind, k, ldk, lead))
+        oq, ok = marked(be, (lead + N * ldqo + 3) * kind.size), marked(be, (lead + N * ldko + 3) * kind.size)
+        sh = lead * kind.size
+
+        def call(a, b, c, d, lc, ld):
+            return be.dispatch("qk_norm_rope_forward" + kind.suffix, [
+                a, b, c, d, be.upload(pos), be.upload(table), be.upload(gain),
+                be.params(N, NH, NKV, HD, rot, layout, ldq, ldk, lc, ld), floats(be, m, eps)], (N,), (256,),
+                offsets=[sh] * 4 + [0] * 5)
+
+        assert call(bq, bk, oq, ok, ldqo, ldko) == 0
+        first = []
+        for x, buf, ld, g in ((q, oq, ldqo, gain[0]), (k, ok, ldko, gain[1])):
+            y = normed(x.reshape(N, -1, HD), g, np.float64(np.float32(eps)))
+            want, off = turned(y, pos, rot, layout, table, m)
+            # the norm's two roundings of each element, carried through the turn
+            carried = turned_sum(np.abs(y), rot, layout, abs(m)) * 2 * U32
+            got = rows_of(kind, buf, N, x.shape[1], ld, lead)
+            check(kind, got, want.reshape(got.shape), (off + carried).reshape(got.shape))
+            first.append(got)
+        assert call(bq, bk, bq, bk, ldq, ldk) == 0  # in place: the same bits
+        for x, buf, ld, got in ((q, bq, ldq, first[0]), (k, bk, ldk, first[1])):
+            assert np.array_equal(rows_of(kind, buf, N, x.shape[1], ld, lead).view(np.uint32), got.view(np.uint32))
+
+
+def turned_sum(y, rot, layout, m):
+    """|x0| + |x1| of each element's pair, times m; the element itself where nothing turns."""
+    out, h = y.copy(), rot // 2
+    i0, i1 = (np.arange(h), np.arange(h) + h) if layout == 0 else (2 * np.arange(h), 2 * np.arange(h) + 1)
+    out[..., i0] = out[..., i1] = (y[..., i0] + y[..., i1]) * m
+    return out
+
+
+def test_qk_norm_of_extreme_heads(be):
+    """Heads of zeros, of values whose squares leave fp32 on either side, and NaN or infinities in one head alone."""
+    HD, NH = 64, 6
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((NH, HD)).astype(np.float32)
+    x[0] = 0
+    x[1] *= np.float32(1e30)
+    x[2] *= np.float32(1e-30)
+    x[3, 5], x[4, 60] = np.nan, np.inf
+    gain, one = np.ones((2, HD), np.float32), be.upload(np.int32([0]))
+    for eps in (1e-5, 0.0):
+        oq, ok = marked(be, x.nbytes), marked(be, x.nbytes)
+        assert be.dispatch("qk_norm_rope_forward", [
+            be.upload(x), be.upload(x), oq, ok, one, one, be.upload(gain),
+            be.params(1, NH, NH, HD, 0, 0, NH * HD, NH * HD, NH * HD, NH * HD), floats(be, 1.0, eps)], (1,), (256,)) == 0
+        got = oq.read(np.float32).reshape(NH, HD)
+        assert np.array_equal(got, ok.read(np.float32).reshape(NH, HD), equal_nan=True)
+        rows = [1, 5] + ([2] if eps == 0 else [])
+        want = normed(x[rows], gain[0], np.float64(np.float32(eps)))
+        assert (np.abs(got[rows] - want) <= 3 * U32 * np.abs(want)).all()
+        assert (got[0] == 0).all() if eps else np.isnan(got[0]).all()  # 0 / sqrt(0)
+        assert np.isnan(got[3]).all() and np.isnan(got[4, 60]) and (got[4, :60] == 0).all()
+
+
+# ---------------------------------------------------------------- the cache
+
+class Batch:
+    """Sequences of `new` tokens behind cached ones, total keys each, in pages dealt out at random; `lead` rows before
+    the first sequence and `tail` behind the last are no one's."""
+
+    def __init__(self, be, rng, kind, new, total, page, NKV, HD, lead=0, tail=0, spare=2, fill=np.nan):
+        self.new, self.total, self.page, self.NKV, self.HD, self.kind = list(new), list(total), page, NKV, HD, kind
+        self.S = len(new)
+        need = [(t + page - 1) // page for t in total]
+        self.width, self.count = max(max(need), 1) + 1, sum(need) + spare
+        order = rng.permutation(self.count).astype(np.int32)
+        self.pages = rng.choice(np.int32([-1, self.count, 1 << 30, -(1 << 31)]), (self.S, self.width)).astype(np.int32)
+        at = 0
+        for s in range(self.S):  # entries past a sequence's keys are never read: they hold anything
+            self.pages[s, :need[s]] = order[at:at + need[s]]
+            at += need[s]
+        self.start = np.int32([lead + sum(self.new[:s]) for s in range(self.S + 1)])
+        self.len = np.int32(total)
+        self.N = int(self.start[-1]) + tail
+        self.seq = np.full(self.N, -1)
+        self.pos = np.zeros(self.N, np.int64)
+        for s in range(self.S):
+            for i in range(self.new[s]):
+                self.seq[self.start[s] + i], self.pos[self.start[s] + i] = s, total[s] - self.new[s] + i
+        self.cache = np.full((self.count, 2, NKV, page, HD), fill, np.float32)
+
+    def place(self, s, j):
+        return self.pages[s, j // self.page], j % self.page
+
+    def fill(self, rng, sharp=1.0):
+        """Keys and values of every sequence; returned as [S] lists of [NKV][total][HD]."""
+        self.K, self.V = [], []
+        for s in range(self.S):
+            k, v = (self.kind.held(rng.standard_normal((self.NKV, self.total[s], self.HD)) * g) for g in (sharp, 1.0))
+            self.set(s, k, v)
+            self.K.append(k)
+            self.V.append(v)
+
+    def set(self, s, k, v):
+        for j in range(k.shape[1]):
+            pg, at = self.place(s, j)
+            self.cache[pg, 0, :, at], self.cache[pg, 1, :, at] = k[:, j], v[:, j]
+
+    def tables(self, be):
+        return [be.upload(self.start), be.upload(self.len), be.upload(self.pages)]
+
+
+BATCHES = [  # new tokens, total keys, page, lead, tail
+    ([1], [1], 16, 0, 0),
+    ([1], [17], 16, 0, 1),
+    ([3], [3], 1, 0, 0),
+    ([1, 1, 1], [5, 16, 33], 16, 0, 0),
+    ([5, 0, 1, 9], [5, 7, 40, 20], 8, 2, 3),
+    ([0, 0, 4, 0], [0, 3, 4, 0], 4, 1, 0),
+    ([40, 1], [70, 1], 32, 0, 5),
+]
+
+
+@both
+@pytest.mark.parametrize("norm", [0, 1], ids=["plain", "norm"])
+@pytest.mark.parametrize("NH,NKV,HD,rot,layout", [(3, 1, 64, 64, 0), (15, 5, 64, 64, 0), (4, 2, 128, 64, 1), (2, 2, 80, 40, 0),
+                                                  (0, 3, 64, 64, 0), (6, 3, 8, 0, 0), (2, 1, 256, 256, 1), (4, 4, 72, 24, 0)])
+@pytest.mark.parametrize("new,total,page,lead,tail", BATCHES)
+def test_kv_append(be, new, total, page, lead, tail, NH, NKV, HD, rot, layout, norm, kind):
+    rng = np.random.default_rng(sum(total) * 31 + HD + NH)
+    b = Batch(be, rng, kind, new, total, page, NKV, HD, lead, tail)
+    Q, K, N = NH * HD, NKV * HD, b.N
+    q, k, v = (kind.held(rng.standard_normal((N, w))) for w in (max(Q, 1), K, K))
+    v.reshape(-1)[:4] = [np.inf, np.nan, -0.0, -np.inf]  # values go in as they are
+    gain = (1 + 0.3 * rng.standard_normal((2, HD))).astype(np.float32)
+    table, m = turn_table(rot, "llama3")
+    eps = np.float64(np.float32(1e-5))
+    cache0 = rng.integers(0, 1 << 16, (b.count, 2, NKV, page, HD * kind.size // 2)).astype(np.uint16)
+    at = b.seq >= 0
+    for ldq, ldk, ldv, ldqo, off0 in ((Q, K, K, Q, 0), (Q + 2 * K, Q + 2 * K, Q + 2 * K, Q, 0), (Q + 1, K + 3, K + 1, Q + 5, 3)):
+        ldq, ldqo = max(ldq, 1), max(ldqo, 1)
+        cache = be.upload(cache0)
+        out = marked(be, (off0 + N * ldqo + 3) * kind.size)
+        bufs = [be.upload(strided(kind, x, ld, off0)) for x, ld in ((q, ldq), (k, ldk), (v, ldv))]
+        sh = off0 * kind.size
+        assert be.dispatch("kv_append_paged" + kind.suffix, bufs + [out, cache] + b.tables(be) + [
+            be.upload(table), be.upload(gain),
+            be.params(N, b.S, NH, NKV, HD, rot, layout, ldq, ldk, ldv, ldqo, page, b.count, b.width, norm),
+            floats(be, m, 1e-5)], (N,), (256,), offsets=[sh, sh, sh, sh] + [0] * 8) == 0
+        if NH:
+            y = q.reshape(N, NH, HD).astype(np.float64)
+            y = normed(y, gain[0], eps) if norm else y
+            want, off = turned(y, b.pos, rot, layout, table, m)
+            off = off + turned_sum(np.abs(y), rot, layout, abs(m)) * 2 * U32 * norm
+            got = rows_of(kind, out, N, Q, ldqo, off0, at)
+            check(kind, got[at], want.reshape(N, Q)[at], off.reshape(N, Q)[at])
+        else:
+            assert (out.read(np.uint8) == MARK).all()
+        y = k.reshape(N, NKV, HD).astype(np.float64)
+        y = normed(y, gain[1], eps) if norm else y
+        want, off = turned(y, b.pos, rot, layout, table, m)
+        off = off + turned_sum(np.abs(y), rot, layout, abs(m)) * 2 * U32 * norm
+        raw = cache.read(np.uint16)[:cache0.size].reshape(cache0.shape)
+        held = kind.values(raw.view(kind.memory)).reshape(b.count, 2, NKV, page, HD)
+        rest = raw.copy()
+        for n in np.flatnonzero(at):
+            pg, j = b.place(b.seq[n], int(b.pos[n]))
+            check(kind, held[pg, 0, :, j], want[n], off[n])
+            assert np.array_equal(held[pg, 1, :, j].reshape(-1), v[n], equal_nan=True)
+            rest[pg, :, :, j] = cache0[pg, :, :, j]
+        assert np.array_equal(rest, cache0)  # nothing else was written
+
+
+@both
+def test_kv_append_skips_what_has_no_place(be, kind):
+    """Rows before position 0, on pages that are none and past the table: the cache keeps its bits there, q is turned all
+    the same."""
+    NH, NKV, HD, page = 2, 1, 64, 4
+    # sequence 0: five rows over three keys (positions -2 .. 2); 1: pages 9 (none) and 0; 2: past the table; 3: page -1
+    start, length = np.int32([0, 5, 11, 13, 14]), np.int32([3, 6, 13, 1])
+    pages = np.int32([[2, -1, -1], [9, 0, -1], [3, 1, 4], [-1, -1, -1]])
+    N, count = 14, 6
+    pos = np.concatenate([np.arange(length[s] - (start[s + 1] - start[s]), length[s]) for s in range(4)])
+    rng = np.random.default_rng(9)
+    q, k, v = (kind.held(rng.standard_normal((N, w * HD))) for w in (NH, NKV, NKV))
+    table, m = turn_table(HD, "none")
+    cache = marked(be, count * 2 * NKV * page * HD * kind.size)
+    out = marked(be, N * NH * HD * kind.size)
+    assert be.dispatch("kv_append_paged" + kind.suffix, [be.upload(kind.raw(x)) for x in (q, k, v)] + [
+        out, cache, be.upload(start), be.upload(length), be.upload(pages), be.upload(table), be.upload(table),
+        be.params(N, 4, NH, NKV, HD, HD, 0, NH * HD, HD, HD, NH * HD, page, count, 3, 0), floats(be, m, 0.0)], (N,),
+        (256,)) == 0
+    want, off = turned(q.reshape(N, NH, HD), pos, HD, 0, table, m)
+    check(kind, kind.values(out.read(kind.memory)).reshape(N, NH, HD), want, off)
+    raw = cache.read(kind.memory).reshape(count, 2, page, HD)
+    written = {(2, j): 2 + j for j in range(3)}  # sequence 0's positions 0 .. 2
+    written.update({(0, j): 9 + j for j in range(2)})  # sequence 1's positions 4 and 5
+    # sequence 2's positions 11 and 12: the first is in page 4, the second past the table's 12
+    written[(4, 3)] = 11
+    for pg in range(count):
+        for j in range(page):
+            if (pg, j) in written:
+                assert np.array_equal(kind.values(raw[pg, 1, j]), v[written[pg, j]])
+            else:
+                assert (raw[pg, :, j].copy().view(np.uint8) == MARK).all(), (pg, j)
+
+
+# ---------------------------------------------------------------- attention
+
+def attend(b, q, NH, scale, causal=1, window=0):
+    """The formula in 64 bits, and per element how far fp32 steps (and bf16's weights) may be off.
+
+    A score: HD products and sums in any order, the scale and the exponent's argument: (HD + 12) U32 of scale * sum |q| |k|
+    (the fp32 form's split operands leave three products of 2^-24 out: 4 more), and its own few roundings.  A weight: e^that, the exponential's 2 units, and for
+    bf16 the rounding of the weights (not of their sum).  The sums over the keys: one rounding a key at most, and 64 for
+    the partial sums that are joined.  The quotient: numerator and denominator."""
+    out = np.zeros((b.N, NH, b.HD))
+    off = np.zeros_like(out)
+    R = NH // b.NKV
+    for n in range(b.N):
+        s = b.seq[n]
+        if s < 0:
+            continue
+        last = b.pos[n] if causal else b.total[s] - 1
+        first = max(0, last - window + 1) if window else 0
+        if last < first:
+            continue
+        for h in range(NH):
+            k, v = (x[s][h // R, first:last + 1].astype(np.float64) for x in (b.K, b.V))
+            x = q[n, h].astype(np.float64)
+            sc = k @ x * scale
+            p = np.exp(sc - sc.max())
+            p /= p.sum()
+            out[n, h] = p @ v
+            span = (np.abs(k) @ np.abs(x)).max() * abs(scale)
+            e = (b.HD + 16) * U32 * span + 6 * U32 * np.abs(sc).max() + 4 * U32 + (len(p) + 64) * U32
+            e = np.expm1(e)
+            off[n, h] = (2 * e + b.kind.step) * (p @ np.abs(v))
+    return out, off
+
+
+def attention(be, b, q, NH, scale, causal=1, window=0, ldq=None, ldo=None, lead=0, cache=None, tables=None, out=None):
+    """One call; the rows of out, checked to hold the mark wherever no sequence has a row."""
+    kind, W = b.kind, NH * b.HD
+    ldq, ldo = ldq or W, ldo or W
+    out = out or marked(be, (lead + b.N * ldo + 3) * kind.size)
+    cache = cache or be.upload(kind.raw(b.cache))
+    assert be.dispatch("attention_forward_paged" + kind.suffix, [
+        be.upload(strided(kind, q.reshape(b.N, W), ldq, lead)), cache, out] + (tables or b.tables(be)) + [
+        be.params(b.N, b.S, NH, b.NKV, b.HD, ldq, ldo, b.page, b.count, b.width, causal, window), floats(be, scale)],
+        (b.N,), (256,), offsets=[lead * kind.size, 0, lead * kind.size] + [0] * 5) == 0
+    return rows_of(kind, out, b.N, W, ldo, lead, b.seq >= 0).reshape(b.N, NH, b.HD)
+
+
+def compare(b, got, want, off):
+    at = b.seq >= 0
+    check(b.kind, got[at], want[at], off[at])
+
+
+HEADS = [(1, 1, 64), (3, 1, 64), (15, 5, 64), (9, 3, 64), (8, 1, 128), (4, 4, 128), (16, 2, 80), (6, 2, 96), (7, 1, 8),
+         (2, 1, 256), (20, 1, 64), (33, 1, 64), (12, 2, 40), (5, 5, 192), (40, 1, 128)]
+ATTEND = BATCHES + [
+    ([1, 1, 1, 1], [300, 64, 65, 129], 16, 0, 0),
+    ([17], [60], 16, 0, 0),
+    ([1, 130, 2], [200, 131, 2], 64, 0, 2),
+    ([64, 33], [64, 97], 128, 0, 0),
+    ([1], [1100], 16, 0, 0),
+    ([2, 1], [515, 1030], 8, 1, 0),
+    ([200], [333], 32, 0, 0),
+]
+
+
+@both
+@pytest.mark.parametrize("NH,NKV,HD", HEADS)
+@pytest.mark.parametrize("new,total,page,lead,tail", ATTEND)
+def test_attention(be, new, total, page, lead, tail, NH, NKV, HD, kind):
+    """Every batch by every head layout; pages' ends and pages of no one hold NaN."""
+    rng = np.random.default_rng(sum(total) * 31 + sum(new) + HD + NH)
+    b = Batch(be, rng, kind, new, total, page, NKV, HD, lead, tail)
+    b.fill(rng)
+    q = kind.held(rng.standard_normal((b.N, NH, HD)) * rng.uniform(0.5, 3, (NH, 1)))
+    scale = float(np.float32(HD ** -0.5))
+    want, off = attend(b, q, NH, scale)
+    compare(b, attention(be, b, q, NH, scale), want, off)
+
+
+@both
+@pytest.mark.parametrize("window", [1, 2, 16, 31, 64, 100, 1000])
+@pytest.mark.parametrize("new,total,page", [([1, 1], [300, 90], 16), ([70], [150], 32), ([130, 1, 5], [130, 400, 64], 64)])
+def test_attention_window(be, new, total, page, window, kind):
+    rng = np.random.default_rng(window + sum(total))
+    b = Batch(be, rng, kind, new, total, page, 2, 64)
+    b.fill(rng)
+    q = kind.held(rng.standard_normal((b.N, 6, 64)))
+    want, off = attend(b, q, 6, 0.125, 1, window)
+    compare(b, attention(be, b, q, 6, 0.125, 1, window), want, off)
+
+
+@both
+@pytest.mark.parametrize("NH,NKV,HD", [(4, 2, 64), (3, 1, 128)])
+@pytest.mark.parametrize("new,total,page", [([1, 3], [40, 7], 16), ([70, 1, 0, 9], [50, 200, 8, 0], 32)])
+def test_attention_without_order(be, new, total, page, NH, NKV, HD, kind):
+    """causal 0: every row sees all of its sequence's keys (more new tokens than keys among them, and none)."""
+    rng = np.random.default_rng(HD + sum(total))
+    b = Batch(be, rng, kind, new, total, page, NKV, HD)
+    b.fill(rng)
+    q = kind.held(rng.standard_normal((b.N, NH, HD)))
+    want, off = attend(b, q, NH, HD ** -0.5, 0)
+    got = attention(be, b, q, NH, HD ** -0.5, 0)
+    compare(b, got, want, off)
+    assert (got[b.seq == 3] == 0).all()
+
+
+@both
+@pytest.mark.parametrize("new", [1, 3, 40, 140])
+def test_attention_rows_that_see_nothing(be, new, kind):
+    """More new tokens than keys: the rows before position 0 get zeros, whatever q holds there."""
+    rng = np.random.default_rng(new)
+    b = Batch(be, rng, kind, [new, new + 2], [0, new], 16, 2, 64)
+    b.fill(rng)
+    q = kind.held(rng.standard_normal((b.N, 4, 64)))
+    q[:new] = np.nan
+    q[new:new + 2] = np.inf
+    got = attention(be, b, q, 4, 0.125)
+    assert (got[:new + 2] == 0).all()
+    want, off = attend(b, np.where(np.isfinite(q), q, 0), 4, 0.125)
+    check(kind, got[new + 2:], want[new + 2:], off[new + 2:])
+
+
+@both
+@pytest.mark.parametrize("HD", [64, 128, 256])
+@pytest.mark.parametrize("new,total,window", [([1, 1], [64, 40], 0), ([64], [64], 0), ([50, 3], [61, 64], 0), ([64], [64], 7),
+                                              ([33, 1], [64, 64], 20)])
+def test_attention_weights(be, new, total, window, HD, kind):
+    """V as the identity shows the weights: zeros exactly where a key is masked, and the softmax where it is not."""
+    rng = np.random.default_rng(HD + sum(total))
+    b = Batch(be, rng, kind, new, total, 16, 1, HD, fill=0.0)
+    b.fill(rng)
+    for s in range(b.S):
+        b.V[s] = np.eye(total[s], HD, dtype=np.float32)[None]
+        b.set(s, b.K[s], b.V[s])
+    q = kind.held(rng.standard_normal((b.N, 3, HD)))
+    want, off = attend(b, q, 3, HD ** -0.5, 1, window)
+    got = attention(be, b, q, 3, HD ** -0.5, 1, window)
+    assert np.array_equal(got == 0, want == 0)
+    compare(b, got, want, off)
+    assert (got[want > 0] > 0).all()
+
+
+@both
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf], ids=["nan", "inf", "-inf"])
+@pytest.mark.parametrize("NH,NKV,HD", [(3, 1, 64), (4, 2, 128), (2, 1, 96)])
+@pytest.mark.parametrize("new,total,window", [([64], [100], 0), ([5, 1], [33, 70], 0), ([40], [90], 16), ([150], [150], 50)])
+def test_attention_masked_keys_hold_anything(be, new, total, window, NH, NKV, HD, what, kind):
+    """A key or a value that is no number, at a place that only later rows (or with a window only earlier ones) see: the
+    rows that do not see it are as ever, bit for bit; of those that do, a value's element, and for a key the row, is no
+    finite number (a key's weight may also be 0, where its score is -infinity)."""
+    rng = np.random.default_rng(HD + sum(total) + window)
+    b = Batch(be, rng, kind, new, total, 16, NKV, HD)
+    b.fill(rng)
+    q = kind.held(np.abs(rng.standard_normal((b.N, NH, HD))) + 0.1)
+    scale = HD ** -0.5
+    want, off = attend(b, q, NH, scale, 1, window)
+    clean = attention(be, b, q, NH, scale, 1, window)
+    compare(b, clean, want, off)
+    for part in (0, 1):
+        for s in range(b.S):
+            for j in sorted({total[s] - 1, max(0, total[s] - new[s]), total[s] - (new[s] + 1) // 2, max(0, total[s] - new[s] - 1)}):
+                pg, at = b.place(s, j)
+                kept = b.cache[pg, part, :, at].copy()
+                b.cache[pg, part, 0, at, 5] = what
+                got = attention(be, b, q, NH, scale, 1, window)
+                b.cache[pg, part, :, at] = kept
+                sees = (b.seq == s) & (b.pos >= j) & ((b.pos < j + window) if window else True)
+                R = NH // NKV
+                assert np.array_equal(got[~sees], clean[~sees]), (part, s, j)
+                assert np.array_equal(got[:, R:], clean[:, R:])
+                if part:
+                    assert not np.isfinite(got[sees][:, :R, 5]).any()
+                    rest = np.arange(HD) != 5
+                    assert np.array_equal(got[:, :, rest], clean[:, :, rest])
+                elif what != -np.inf:
+                    assert not np.isfinite(got[sees][:, :R]).any()
+
+
+@both
+def test_attention_missing_pages(be, kind):
+    """Rows that see a key whose page is none, or lies past the table, get NaN; the others are as ever."""
+    rng = np.random.default_rng(4)
+    b = Batch(be, rng, kind, [40, 1, 2], [60, 70, 33], 16, 2, 64)
+    b.fill(rng)
+    q = kind.held(rng.standard_normal((b.N, 4, 64)))
+    want, off = attend(b, q, 4, 0.125)
+    for bad in (-1, b.count, -(1 << 31), (1 << 31) - 1):
+        t = b.tables(be)
+        pages = b.pages.copy()
+        pages[0, 2] = bad  # keys 32 .. 47 of sequence 0
+        pages[2, 2] = bad  # key 32 of sequence 2, which its second row alone sees
+        got = attention(be, b, q, 4, 0.125, tables=t[:2] + [be.upload(pages)])
+        gone = ((b.seq == 0) & (b.pos >= 32)) | ((b.seq == 2) & (b.pos >= 32))
+        assert np.isnan(got[gone]).all()
+        check(kind, got[~gone], want[~gone], off[~gone])
+        # a window that has passed them
+        got = attention(be, b, q, 4, 0.125, 1, 4, tables=t[:2] + [be.upload(pages)])
+        gone = ((b.seq == 0) & (b.pos >= 32) & (b.pos < 51)) | ((b.seq == 2) & (b.pos >= 32))
+        assert np.isnan(got[gone]).all() and np.isfinite(got[~gone]).all()
+    # keys past the table's room
+    length = b.len.copy()
+    length[1] = b.width * 16 + 1
+    pages = np.where(b.pages < 0, 0, b.pages % b.count).astype(np.int32)
+    t = b.tables(be)
+    got = attention(be, b, q, 4, 0.125, tables=[t[0], be.upload(length), be.upload(pages)])
+    assert np.isnan(got[b.seq == 1]).all()
+    check(kind, got[b.seq == 0], want[b.seq == 0], off[b.seq == 0])
+
+
+@both
+@pytest.mark.parametrize("new,total", [([1, 1], [200, 3]), ([90], [120])])
+def test_attention_strides(be, new, total, kind):
+    rng = np.random.default_rng(8)
+    b = Batch(be, rng, kind, new, total, 32, 2, 64, 1, 2)
+    b.fill(rng)
+    q = kind.held(rng.standard_normal((b.N, 6, 64)))
+    want, off = attend(b, q, 6, 0.125)
+    W = 6 * 64
+    for ldq, ldo, lead in ((W + 1, W + 3, 1), (W + 2, W + 2, 2), (W + 8, W + 24, 8), (3 * W, 2 * W, 4)):
+        compare(b, attention(be, b, q, 6, 0.125, 1, 0, ldq, ldo, lead), want, off)
+
+
+@both
+def test_attention_scores_far_apart(be, kind):
+    """Scores of +-1000s: the largest takes all; equal ones give the mean; a scale of 0 and a negative one."""
+    rng = np.random.default_rng(11)
+    for new, total in (([1], [500]), ([100], [130])):
+        b = Batch(be, rng, kind, new, total, 16, 1, 64)
+        b.fill(rng, 8.0)
+        q = kind.held(rng.standard_normal((b.N, 4, 64)) * 8)
+        for scale in (1.0, -1.0, 0.0):
+            want, off = attend(b, q, 4, scale)
+            compare(b, attention(be, b, q, 4, scale), want, off)
+
+
+@both
+def test_attention_many_sequences(be, kind):
+    """More sequences than lanes, some without tokens, some without keys."""
+    rng = np.random.default_rng(12)
+    S = 300
+    new = [int(x) for x in rng.choice([0, 1, 1, 1, 2, 5], S)]
+    total = [n + int(rng.integers(0, 60)) if n else int(rng.integers(0, 5)) for n in new]
+    b = Batch(be, rng, kind, new, total, 16, 1, 64, 0, 3)
+    b.fill(rng)
+    q = kind.held(rng.standard_normal((b.N, 2, 64)))
+    want, off = attend(b, q, 2, 0.125)
+    compare(b, attention(be, b, q, 2, 0.125), want, off)
+
+
+@both
+def test_attention_long_context_beside_short_ones(be, kind):
+    """One long sequence (joined from parts where the work is split) among short ones; the same bits every time."""
+    rng = np.random.default_rng(13)
+    b = Batch(be, rng, kind, [1, 1, 3, 1], [5000, 3, 700, 90], 16, 2, 64)
+    b.fill(rng)
+    q = kind.held(rng.standard_normal((b.N, 6, 64)))
+    want, off = attend(b, q, 6, 0.125)
+    cache = be.upload(kind.raw(b.cache))
+    first = attention(be, b, q, 6, 0.125, cache=cache)
+    compare(b, first, want, off)
+    for _ in range(5):
+        assert np.array_equal(attention(be, b, q, 6, 0.125, cache=cache), first)
+
+
+@both
+def test_attention_a_cache_past_32_bits(be, kind):
+    """Pages whose elements lie past 2^32 bytes and past 2^31 elements of the cache's start."""
+    NKV, HD, page = 1, 64, 65536
+    count = (1 << 31) // (2 * NKV * page * HD) + 1  # the last page begins at element 2^31
+    cache = be.alloc(count * 2 * NKV * page * HD * kind.size)
+    table, m = turn_table(0, "none")
+    rng = np.random.default_rng(14)
+    n, start, length, pages = 70, np.int32([0, 70]), np.int32([70]), np.int32([[count - 1]])
+    k, v, q = (kind.held(rng.standard_normal((n, HD))) for _ in range(3))
+    tables = [be.upload(start), be.upload(length), be.upload(pages)]
+    out = marked(be, n * HD * kind.size)
+    assert be.dispatch("kv_append_paged" + kind.suffix, [
+        out, be.upload(kind.raw(k)), be.upload(kind.raw(v)), out, cache] + tables + [be.upload(table), be.upload(table), be.params(
+            n, 1, 0, NKV, HD, 0, 0, HD, HD, HD, HD, page, count, 1, 0), floats(be, 1.0, 0.0)], (n,), (256,)) == 0
+    assert be.dispatch("attention_forward_paged" + kind.suffix, [be.upload(kind.raw(q)), cache, out] + tables + [be.params(
+        n, 1, 1, NKV, HD, HD, HD, page, count, 1, 1, 0), floats(be, 0.125)], (n,), (256,)) == 0
+    b = Batch.__new__(Batch)
+    b.N, b.NKV, b.HD, b.kind, b.total = n, 1, HD, kind, [n]
+    b.seq, b.pos, b.K, b.V = np.zeros(n, int), np.arange(n), [k[None]], [v[None]]
+    want, off = attend(b, q[:, None], 1, 0.125)
+    got = kind.values(out.read(kind.memory)).reshape(n, 1, HD)
+    cache.free()
+    check(kind, got, want, off)
+
+
+# ---------------------------------------------------------------- the operators together
+
+@both
+@pytest.mark.parametrize("norm", [0, 1], ids=["plain", "norm"])
+def test_prompts_in_chunks_then_tokens(be, norm, kind):
+    """Three sequences served as a program would: prompts in chunks of different sizes beside the others' single tokens,
+    positions and pages growing, every step append and attention in one encoder over the same cache.  Each row against
+    the formula over all that its sequence holds by then."""
+    NH, NKV, HD, page, S = 6, 2, 64, 16, 3
+    rng = np.random.default_rng(20 + norm)
+    table, m = turn_table(HD, "none")
+    gain = (1 + 0.3 * rng.standard_normal((2, HD))).astype(np.float32)
+    steps = [[37, 5, 0], [40, 1, 1], [1, 1, 30], [0, 70, 1], [1, 1, 1], [1, 1, 1]]
+    count, width, eps = 40, 12, np.float64(np.float32(1e-5))
+    pages = rng.permutation(count)[:S * width].astype(np.int32).reshape(S, width)
+    cache = be.alloc(count * 2 * NKV * page * HD * kind.size)
+    held = [0] * S
+    K, V, Koff = ([np.zeros((NKV, 0, HD)) for _ in range(S)] for _ in range(3))
+    kern = [be.kernel(n + kind.suffix) for n in ("kv_append_paged", "attention_forward_paged")]
+    for new in steps:
+        N = sum(new)
+        held = [a + n for a, n in zip(held, new)]
+        start, length = np.int32([sum(new[:s]) for s in range(S + 1)]), np.int32(held)
+        W = (NH + 2 * NKV) * HD
+        qkv = kind.held(rng.standard_normal((N, W)))  # one stacked product's rows
+        src, qo, out = be.upload(kind.raw(qkv)), marked(be, N * NH * HD * kind.size), marked(be, N * NH * HD * kind.size)
+        tables = [be.upload(start), be.upload(length), be.upload(pages)]
+        e = be.encoder()
+        assert e.dispatch(kern[0], [src, src, src, qo, cache] + tables + [be.upload(table), be.upload(gain), be.params(
+            N, S, NH, NKV, HD, HD, 0, W, W, W, NH * HD, page, count, width, norm), floats(be, m, 1e-5)], (N,), (256,),
+            offsets=[0, NH * HD * kind.size, (NH + NKV) * HD * kind.size] + [0] * 9) == 0
+        assert e.dispatch(kern[1], [qo, cache, out] + tables + [be.params(
+            N, S, NH, NKV, HD, NH * HD, NH * HD, page, count, width, 1, 0), floats(be, 0.125)], (N,), (256,)) == 0
+        e.commit()
+        e.wait_timed()
+        b = Batch.__new__(Batch)
+        b.N, b.NKV, b.HD, b.kind, b.total = N, NKV, HD, kind, held
+        b.seq = np.repeat(np.arange(S), new)
+        b.pos = np.concatenate([np.arange(h - n, h) for h, n in zip(held, new)])
+        q, k, v = (qkv[:, a:c].reshape(N, -1, HD).astype(np.float64) for a, c in (
+            (0, NH * HD), (NH * HD, (NH + NKV) * HD), ((NH + NKV) * HD, W)))
+        if norm:
+            q, k = normed(q, gain[0], eps), normed(k, gain[1], eps)
+        qt, _ = turned(q, b.pos, HD, 0, table, m)
+        kt, _ = turned(k, b.pos, HD, 0, table, m)
+        got_q = kind.values(qo.read(kind.memory)).reshape(N, NH, HD)
+        raw = kind.values(cache.read(kind.memory)).reshape(count, 2, NKV, page, HD)
+        # the operators are checked alone above: here each works on what the one before gave, and the whole stays near the formula
+        assert np.abs(got_q - qt).max() <= (1e-5 if not kind.bf16 else 2 * UB16) * np.abs(qt).max()
+        for s in range(S):
+            at = b.seq == s
+            K[s] = np.concatenate([K[s], kt[at].transpose(1, 0, 2)], 1)
+            V[s] = np.concatenate([V[s], v[at].transpose(1, 0, 2)], 1)
+        b.K = [np.stack([raw[pages[s, j // page], 0, :, j % page] for j in range(held[s])], 1) if held[s] else K[s] for s in range(S)]
+        b.V = V
+        for s in range(S):
+            assert held[s] == 0 or np.abs(b.K[s] - K[s]).max() <= (1e-5 if not kind.bf16 else 2 * UB16) * np.abs(K[s]).max()
+        want, off = attend(b, got_q, NH, 0.125)
+        check(kind, kind.values(out.read(kind.memory)).reshape(N, NH, HD), want, off)
+
+
+def test_agrees_with_the_one_sequence_kernels(be):
+    """One sequence, fp32, a page for the whole context: kv_store and attention_forward over the same keys."""
+    NH, NKV, HD, S = 15, 5, 64, 200
+    rng = np.random.default_rng(30)
+    k, v = (rng.standard_normal((S, NKV * HD)).astype(np.float32) for _ in range(2))
+    q = rng.standard_normal((1, NH * HD)).astype(np.float32)
+    flat, out1 = be.upload(np.stack([k, v])), marked(be, q.nbytes)
+    assert be.dispatch("attention_forward", [be.upload(q), flat, out1, be.params(NH, HD, NKV, NKV * HD, S, 3, 0, S),
+                                             floats(be, 0.125)], (NH,), (64,)) == 0
+    b = Batch(be, rng, KINDS[0], [1], [S], 256, NKV, HD)
+    b.K, b.V = ([x.reshape(S, NKV, HD).transpose(1, 0, 2)] for x in (k, v))
+    b.set(0, b.K[0], b.V[0])
+    got = attention(be, b, q.reshape(1, NH, HD), NH, 0.125)
+    want, off = attend(b, q.reshape(1, NH, HD), NH, 0.125)
+    check(KINDS[0], got, want, off)
+    check(KINDS[0], out1.read(np.float32).reshape(1, NH, HD), want, off)
+
+
+def test_two_contexts_at_once(be):
+    """Passes of two contexts, each on its own stream and scratch memory, in flight together."""
+    kind = KINDS[1]
+    other = bmhip.Backend()
+    try:
+        rng = np.random.default_rng(31)
+        jobs = []
+        for c in (be, other):
+            b = Batch(c, rng, kind, [1, 1], [3000, 2500], 16, 1, 64)
+            b.fill(rng)
+            q = kind.held(rng.standard_normal((b.N, 4, 64)))
+            want, off = attend(b, q, 4, 0.125)
+            out = marked(c, q.size * 2)
+            bufs = [c.upload(kind.raw(q)), c.upload(kind.raw(b.cache)), out] + b.tables(c) + [c.params(
+                2, 2, 4, 1, 64, 256, 256, 16, b.count, b.width, 1, 0), floats(c, 0.125)]
+            c.synchronize()
+            jobs.append((c, b, bufs, out, want, off))
+        flying = []
+        for _ in range(8):
+            for c, b, bufs, out, want, off in jobs:
+                e = c.encoder()
+                for _ in range(4):
+                    assert e.dispatch(c.kernel("attention_forward_paged_bf16"), bufs, (2,), (256,)) == 0
+                e.commit()
+                flying.append(e)
+        for e in flying:
+            e.wait_timed()
+        for c, b, bufs, out, want, off in jobs:
+            check(kind, kind.values(out.read(np.uint16)).reshape(want.shape), want, off)
+        del jobs, bufs, out, flying
+    finally:
+        other.close()
+
+
+def test_scratch_is_left_for_the_next_kernel(be):
+    """Kernels that split their work share a context's scratch memory in stream order: attention_forward between passes
+    over pages, both the same every time."""
+    rng = np.random.default_rng(32)
+    NH, NKV, HD, S = 15, 5, 64, 2048
+    kv = rng.standard_normal((2, S, NKV * HD)).astype(np.float32)
+    q = rng.standard_normal((1, NH * HD)).astype(np.float32)
+    flat = [be.upload(q), be.upload(kv), marked(be, q.nbytes), be.params(NH, HD, NKV, NKV * HD, S, 3, 0, S), floats(be, 0.125)]
+    b = Batch(be, rng, KINDS[0], [1, 1], [2048, 700], 16, NKV, HD)
+    b.fill(rng)
+    q2 = rng.standard_normal((2, NH, HD)).astype(np.float32)
+    paged = [be.upload(q2), be.upload(b.cache), marked(be, q2.nbytes)] + b.tables(be) + [be.params(
+        2, 2, NH, NKV, HD, NH * HD, NH * HD, 16, b.count, b.width, 1, 0), floats(be, 0.125)]
+    seen = []
+    for _ in range(4):
+        e = be.encoder()
+        for _ in range(3):
+            assert e.dispatch(be.kernel("attention_forward"), flat, (NH,), (64,)) == 0
+            assert e.dispatch(be.kernel("attention_forward_paged"), paged, (2,), (256,)) == 0
+        e.commit()
+        e.wait_timed()
+        seen.append((flat[2].read(np.float32), paged[2].read(np.float32)))
+    for x, y in seen[1:]:
+        assert np.array_equal(x, seen[0][0]) and np.array_equal(y, seen[0][1])
+    want, off = attend(b, q2, NH, 0.125)
+    check(KINDS[0], seen[0][1].reshape(2, NH, HD), want, off)
