@@ -41,6 +41,7 @@ constexpr int AT_MAX_SPLIT = 64; /* records the merge holds weights for in LDS *
  * the counters stay zero between launches of any shape. */
 constexpr int AT_DONE_STRIDE = 32, AT_MAX_GROUPS = 1024;
 constexpr size_t AT_DONE_BYTES = (size_t)AT_DONE_STRIDE * AT_MAX_GROUPS * 4;
+constexpr size_t AT_SCRATCH_BYTES = (size_t)8 << 20; /* as much of it as the splits are cut for */
 
 /* Keys a wave takes per tile: each load instruction covers 256 / HD keys (16
  * bytes a lane), AT_UN of them in flight for K and for V. */
@@ -286,6 +287,7 @@ template <int HD>
 int at_split(int S, int groups, int qh, size_t scratch_bytes, int* keys) {
     const int tile = AtTile<HD>::KEYS, tiles = (S + tile - 1) / tile;
     size_t most = 1;
+    scratch_bytes = std::min(scratch_bytes, AT_SCRATCH_BYTES);
     if (tiles > AT_ONE_TILES && groups <= AT_MAX_GROUPS && scratch_bytes > AT_DONE_BYTES)
         most = (scratch_bytes - AT_DONE_BYTES) / ((size_t)groups * qh * (HD + 2) * 4);
     most = std::min<size_t>(std::max<size_t>(most, 1), AT_MAX_SPLIT);

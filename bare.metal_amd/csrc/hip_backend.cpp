@@ -62,7 +62,7 @@ static bool hip_ok(hipError_t e, const char* what, const char* file, int line) {
     return false;
 }
 
-#define BMK_SCRATCH_BYTES ((size_t)8 << 20)
+#define BMK_SCRATCH_BYTES ((size_t)64 << 20)
 
 static inline hipStream_t ctx_stream(backend_ctx_t* ctx) { return (hipStream_t)ctx->queue; }
 

@@ -305,7 +305,7 @@ int launch_kv_append(const bmk_launch_t* l, bool bf16) {
     const int N = bmk_pi(l, 10, 0), S = bmk_pi(l, 10, 1), NH = bmk_pi(l, 10, 2), NKV = bmk_pi(l, 10, 3), HD = bmk_pi(l, 10, 4);
     const int ldq = bmk_pi(l, 10, 7), ldk = bmk_pi(l, 10, 8), ldv = bmk_pi(l, 10, 9), ldqo = bmk_pi(l, 10, 10);
     const int norm = bmk_pi(l, 10, 14);
-    BMK_REQUIRE(N >= 0 && N <= PG_MAX_DIM && S >= 0 && S <= PG_MAX_DIM && NH >= 0 && NH <= PG_MAX_DIM / 2 && NKV > 0 &&
+    BMK_REQUIRE(N >= 0 && N <= PG_MAX_DIM && S >= 0 && S <= PG_MAX_SEQS && NH >= 0 && NH <= PG_MAX_DIM / 2 && NKV > 0 &&
                     NKV <= PG_MAX_DIM / 4 && HD > 0 && HD <= PG_MAX_HD && (norm == 0 || norm == 1),
                 "kv_append_paged: bad shape N=%d S=%d NH=%d NKV=%d HD=%d norm=%d", N, S, NH, NKV, HD, norm);
     BMK_REQUIRE(!norm || bmk_pf(l, 11, 1) >= 0, "kv_append_paged: bad eps %g", (double)bmk_pf(l, 11, 1));
