@@ -54,6 +54,18 @@ constexpr int WANTED = 1024;     /* workgroups that the splits aim at */
 constexpr int DONE_STRIDE = 32, MAX_UNITS = 1024;
 constexpr size_t DONE_BYTES = (size_t)DONE_STRIDE * MAX_UNITS * 4;
 
+/* x / d for x below 2^31 by one product */
+struct Div {
+    unsigned int d, mul, shift;
+    __device__ __forceinline__ int of(int x) const { return (int)((__umulhi((unsigned int)x, mul) + (unsigned int)x) >> shift); }
+};
+Div div_by(int d) {
+    Div v = {(unsigned int)d, 0, 0};
+    while ((1ull << v.shift) < (unsigned int)d) v.shift++;
+    v.mul = (unsigned int)(((1ull << 32) * ((1ull << v.shift) - d)) / d + 1);
+    return v;
+}
+
 struct PaArgs {
     const void* q;
     const void* cache;
@@ -61,7 +73,9 @@ struct PaArgs {
     unsigned int* done;
     float* rec;
     PgBatch b;
-    int NH, R; /* R: query heads a KV head */
+    int R; /* query heads a KV head */
+    Div by_r, by_kv;
+    int q_wide; /* q's heads begin on 16-byte boundaries */
     int causal, window;
     size_t ldq, ldo;
     float scale2; /* |scale| * log2(e) */
@@ -72,7 +86,7 @@ struct PaArgs {
 /* How a tile lies: HDP is the head size rounded up, with zeros behind it. */
 template <bool BF16, int HDP> struct Tile {
     static constexpr int TERMS = BF16 ? 1 : 3;
-    static constexpr int KT = BF16 ? (HDP == 256 ? 32 : 64) : (HDP == 64 ? 64 : 32);
+    static constexpr int KT = !BF16 && HDP == 64 ? 64 : 32;
     static constexpr int KB = KT / 32;
     static constexpr int ROWB = HDP * 2, CPR = HDP / 8; /* bytes and 16-byte chunks of a row's term */
     static constexpr int PLANE = KT * ROWB;
@@ -85,7 +99,17 @@ template <bool BF16, int HDP> struct Tile {
 __device__ __forceinline__ int k_place(int r, int c) { return c ^ (r & 7); }
 __device__ __forceinline__ int v_place(int r, int c) { return c ^ (2 * (r & 3)); }
 
-__device__ const u32x4 pg_zeros = {0, 0, 0, 0}, pg_nans = {0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+/* a load's worth of a missing page's keys: NaN in bf16 */
+#define N4 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u
+#define N64 N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4
+__device__ __attribute__((aligned(16))) const unsigned int pg_nans[256] = {N64, N64, N64, N64};
+#undef N64
+#undef N4
+
+/* bits 15 and 31: the half below is an infinity or NaN (an exponent of ones carries) */
+__device__ __forceinline__ unsigned int no_numbers(unsigned int two) {
+    return ((two & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+}
 
 __device__ __forceinline__ void agent_store2(float* p, float x, float y) {
     const unsigned long long u = ((unsigned long long)__float_as_uint(y) << 32) | __float_as_uint(x);
@@ -118,6 +142,15 @@ __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
+/* all waves of the workgroup; memory accesses stay on their side of it */
+__device__ __forceinline__ void barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
+
 __device__ __forceinline__ float other_half(float v) {
     const u32x2 s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float((threadIdx.x & 32) ? s[0] : s[1]);
@@ -126,12 +159,48 @@ __device__ __forceinline__ float other_half(float v) {
 /* ---------------------------------------------------------------- the work */
 
 struct Seq {
-    int n, len, T; /* new tokens, keys, tiles of keys that a unit sees at most */
+    int start, n, len, T; /* first row, new tokens, keys, tiles of keys that a unit sees at most */
     unsigned int units; /* per KV head */
 };
 
-/* What is to be done, from the tables alone: every wave finds it for itself, 64 sequences at a time, the first of them
- * kept in registers. */
+/* Sums over the lanes up to each, and the largest of all lanes, by row shifts and broadcasts (a shuffle through LDS takes
+ * ten times as long, and some forty of them stood before a small launch's first load). */
+template <class V>
+__device__ __forceinline__ V dpp_sums(V v) {
+    unsigned int u;
+#define STEP(ctrl, rows) \
+    u = (unsigned int)__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, rows, 0xF, false); \
+    v += __builtin_bit_cast(V, u);
+    STEP(0x111, 0xF) /* row_shr 1, 2, 4, 8 */
+    STEP(0x112, 0xF)
+    STEP(0x114, 0xF)
+    STEP(0x118, 0xF)
+    STEP(0x142, 0xA) /* lane 15 of rows 0 and 2 to the next row */
+    STEP(0x143, 0xC) /* lane 31 to rows 2 and 3 */
+#undef STEP
+    return v;
+}
+template <class V>
+__device__ __forceinline__ V lane_of(V v, int l) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+}
+__device__ __forceinline__ int dpp_most(int v) { /* of values from 0 on */
+    int u;
+#define STEP(ctrl, rows) \
+    u = __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xF, false); \
+    v = max(v, u);
+    STEP(0x111, 0xF)
+    STEP(0x112, 0xF)
+    STEP(0x114, 0xF)
+    STEP(0x118, 0xF)
+    STEP(0x142, 0xA)
+    STEP(0x143, 0xC)
+#undef STEP
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
+/* What is to be done, from the tables alone: every wave finds it for itself, 64 sequences at a time; up to 64 stay in
+ * registers. */
 template <int KT>
 struct Plan {
     const PaArgs& a;
@@ -139,22 +208,31 @@ struct Plan {
     Seq first;
     int per;            /* tiles a part */
     unsigned int total; /* pieces of work; 0 where the tables are none */
+    struct Sums { /* of pieces, records and units in parts, over a chunk's sequences up to the lane's */
+        unsigned int w, recs, units;
+    } sums;
 
     __device__ __forceinline__ Seq seq(int s) const {
-        Seq q = {0, 0, 0, 0};
+        Seq q = {};
         if (s < a.b.S) {
             const int at = a.b.start[s], end = a.b.start[s + 1];
             q.len = max(a.b.len[s], 0);
+            q.start = at;
             if (at >= 0 && at < end && end <= a.b.N) q.n = end - at;
             q.units = ((unsigned int)q.n * (unsigned int)a.R + ROWS - 1) / ROWS;
             int span = min(q.len, a.b.room());
-            if (a.window) span = min(span, a.window + ROWS / a.R + 1 + KT);
+            if (a.window) span = min(span, a.window + a.by_r.of(ROWS) + 1 + KT);
             q.T = (span + KT - 1) / KT;
         }
         return q;
     }
     __device__ __forceinline__ Seq chunk(int c) const { return c ? seq(c + lane) : first; }
     __device__ __forceinline__ unsigned int parts(const Seq& q) const { return max(1, (q.T + per - 1) / per); }
+    __device__ __forceinline__ Sums own(const Seq& q) const {
+        const unsigned int p = parts(q);
+        return Sums{q.units * p * a.b.NKV, p > 1 ? (unsigned int)q.n * a.R * p * a.b.NKV : 0, p > 1 ? q.units * a.b.NKV : 0};
+    }
+    __device__ __forceinline__ Sums up_to(const Sums& m) const { return Sums{dpp_sums(m.w), dpp_sums(m.recs), dpp_sums(m.units)}; }
 
     __device__ __forceinline__ Plan(const PaArgs& args) : a(args), lane(threadIdx.x & 63) {
         first = seq(lane);
@@ -166,9 +244,9 @@ struct Plan {
             rows += (float)q.n;
             longest = max(longest, q.T);
         }
-        tiles = wave_sum(tiles) * a.b.NKV;
-        rows = wave_sum(rows);
-        for (int o = 1; o < 64; o <<= 1) longest = max(longest, __shfl_xor(longest, o));
+        tiles = lane_of(dpp_sums(tiles), 63) * a.b.NKV;
+        rows = lane_of(dpp_sums(rows), 63);
+        longest = dpp_most(longest);
         per = max((int)(tiles / WANTED) + 1, (longest + MAX_SPLIT - 1) / MAX_SPLIT);
         if (!a.most) per = max(longest, 1);
         per = __builtin_amdgcn_readfirstlane(per);
@@ -176,32 +254,27 @@ struct Plan {
         if (rows > (float)a.b.N * 1.0001f) return; /* sequences that overlap: no batch */
         for (;;) { /* parts as long as their records and counters need; ends at one part a unit */
             float recs = 0, units = 0;
-            unsigned int w = 0;
             for (int c = 0; c < a.b.S; c += 64) {
-                const Seq q = chunk(c);
-                const unsigned int p = parts(q);
-                w += q.units * p * a.b.NKV;
-                if (p > 1) {
-                    recs += (float)q.n * a.R * p * a.b.NKV;
-                    units += (float)q.units * a.b.NKV;
+                const Sums m = own(chunk(c));
+                recs += (float)m.recs;
+                units += (float)m.units;
+                if (c == 0) {
+                    sums = up_to(m);
+                    total = 0;
                 }
+                total += c == 0 ? lane_of(sums.w, 63) : lane_of(dpp_sums(m.w), 63);
             }
-            recs = wave_sum(recs);
-            units = wave_sum(units);
-            if (per >= longest || (recs * 1.0001f < (float)a.most && units <= (float)MAX_UNITS)) {
-                for (int o = 1; o < 64; o <<= 1) w += __shfl_xor(w, o);
-                total = __builtin_amdgcn_readfirstlane(w);
-                return;
-            }
-            per = per > longest / 2 ? longest : 2 * per;
-            per = __builtin_amdgcn_readfirstlane(per);
+            recs = lane_of(dpp_sums(recs), 63);
+            units = lane_of(dpp_sums(units), 63);
+            if (per >= longest || (recs * 1.0001f < (float)a.most && units <= (float)MAX_UNITS)) return;
+            per = __builtin_amdgcn_readfirstlane(per > longest / 2 ? longest : 2 * per);
         }
     }
 
     struct Item {
         int s, kh, unit, part, parts;
-        int n, len;
-        unsigned int rec, done; /* first of the unit's records, its counter */
+        int start, n, len;
+        unsigned int rec, done; /* first of the sequence's records, the unit's counter */
     };
     /* piece w < total of the work: within a sequence the KV heads side by side, the last units, which see the most keys, first */
     __device__ __forceinline__ Item item(unsigned int w) const {
@@ -209,37 +282,28 @@ struct Plan {
         unsigned int recs = 0, units = 0;
         for (int c = 0; c < a.b.S; c += 64) {
             const Seq q = chunk(c);
-            const unsigned int p = parts(q), mine = q.units * p * a.b.NKV;
-            const unsigned int r = p > 1 ? (unsigned int)q.n * a.R * p * a.b.NKV : 0, u = p > 1 ? q.units * a.b.NKV : 0;
-            unsigned int iw = mine, ir = r, iu = u; /* sums up to this lane */
-            for (int o = 1; o < 64; o <<= 1) {
-                const unsigned int x = __shfl_up(iw, o), y = __shfl_up(ir, o), z = __shfl_up(iu, o);
-                if (lane >= o) {
-                    iw += x;
-                    ir += y;
-                    iu += z;
-                }
-            }
-            const unsigned long long past = __ballot(iw > w);
+            const Sums m = own(q), up = c ? up_to(m) : sums;
+            const unsigned long long past = __ballot(up.w > w);
             if (past) {
                 const int l = __builtin_ctzll(past);
                 it.s = c + l;
-                it.n = __builtin_amdgcn_readlane(q.n, l);
-                it.len = __builtin_amdgcn_readlane(q.len, l);
-                it.parts = __builtin_amdgcn_readlane((int)p, l);
-                const unsigned int local = w - (unsigned int)__builtin_amdgcn_readlane((int)(iw - mine), l);
-                const unsigned int nu = (unsigned int)__builtin_amdgcn_readlane((int)q.units, l);
-                it.kh = local % a.b.NKV;
-                const unsigned int rest = local / a.b.NKV;
-                it.part = rest % it.parts;
-                it.unit = (int)(nu - 1 - rest / it.parts);
-                it.rec = recs + (unsigned int)__builtin_amdgcn_readlane((int)(ir - r), l);
-                it.done = units + (unsigned int)__builtin_amdgcn_readlane((int)(iu - u), l) + it.unit * a.b.NKV + it.kh;
+                it.start = lane_of(q.start, l);
+                it.n = lane_of(q.n, l);
+                it.len = lane_of(q.len, l);
+                it.parts = (int)lane_of(parts(q), l);
+                const unsigned int local = w - lane_of(up.w - m.w, l), nu = lane_of(q.units, l);
+                const int rest = a.by_kv.of(local);
+                it.kh = (int)local - rest * a.b.NKV;
+                const int back = it.parts == 1 ? rest : rest / it.parts;
+                it.part = rest - back * it.parts;
+                it.unit = (int)nu - 1 - back;
+                it.rec = recs + lane_of(up.recs - m.recs, l);
+                it.done = units + lane_of(up.units - m.units, l) + it.unit * a.b.NKV + it.kh;
                 return it;
             }
-            w -= __builtin_amdgcn_readlane((int)iw, 63);
-            recs += (unsigned int)__builtin_amdgcn_readlane((int)ir, 63);
-            units += (unsigned int)__builtin_amdgcn_readlane((int)iu, 63);
+            w -= lane_of(up.w, 63);
+            recs += lane_of(up.recs, 63);
+            units += lane_of(up.units, 63);
         }
         it.s = -1;
         return it;
@@ -288,71 +352,83 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
     constexpr int TERMS = T::TERMS, KT = T::KT, KB = T::KB, CPR = T::CPR, PLANE = T::PLANE;
     constexpr int STEPS = HDP / 16, DT = HDP / 32; /* of the first product's sum; tiles of the output's dimensions */
     constexpr int RPI = 1024 / T::ROWB, NI = PLANE / 1024 / NW; /* rows of a wave's load into LDS, loads of keys a wave */
-    /* two arrays, not one: reads of the one then wait for no load into the other */
-    __shared__ __attribute__((aligned(16))) unsigned char lds0[T::BYTES], lds1[BF16 ? T::BYTES : 16];
-    __shared__ float row_m[ROWS], row_l[ROWS];
+    /* a ring of four arrays, not one array: reads of one then wait for no load into another */
+    constexpr int RING = BF16 ? T::BYTES : 16;
+    __shared__ __attribute__((aligned(16))) unsigned char lds0[T::BYTES], lds1[RING], lds2[RING], lds3[RING];
+    __shared__ float part_m[3][64], part_l[3][64];
     __shared__ int last_one;
     const PgBatch& b = a.b;
     const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
     const int col = lane & 31, half = lane >> 5;
-    const int HD = b.HD;
+    const int HD = b.HD, R = a.R;
     const Plan<KT> plan(a);
 
-    for (unsigned int w = blockIdx.x; w < plan.total; w += gridDim.x) {
-        const auto it = plan.item(w);
+    if (blockIdx.x >= plan.total) return;
+    {
+        const auto it = plan.item(blockIdx.x);
         if (it.s < 0) return;
-        const int rows_all = it.n * a.R, r0 = it.unit * ROWS, nrows = min(ROWS, rows_all - r0);
+        const int rows_all = it.n * R, r0 = it.unit * ROWS, nrows = min(ROWS, rows_all - r0);
         const int p0 = (int)((unsigned)it.len - (unsigned)it.n); /* position of the sequence's first new token */
-        const int n0 = b.start[it.s];
-        const int tok0 = r0 / a.R, tok1 = (r0 + nrows - 1) / a.R;
+        const int n0 = it.start;
+        const int tok0 = a.by_r.of(r0), tok1 = a.by_r.of(r0 + nrows - 1);
         const int room = b.room();
         /* tiles of keys that some row of the unit sees, and this part's */
         const int lo = seen(a, p0 + tok0, it.len).first, hi = min(seen(a, p0 + tok1, it.len).last + 1, room);
         const int t0 = lo / KT, t1 = hi > lo ? (hi + KT - 1) / KT : t0;
-        const int parts = max(1, (t1 - t0 + plan.per - 1) / plan.per);
-        if (it.part >= parts) continue;
         const int kt0 = t0 + it.part * plan.per, kt1 = min(kt0 + plan.per, t1);
-        /* waves side by side on rows, the rest on parts of the tile's keys */
-        const int groups = nrows <= 32 ? 1 : nrows <= 64 ? 2 : 4, kparts = min(NW / groups, KB);
+        if (it.part && kt0 >= t1) return;
+        const bool whole = t1 - t0 <= plan.per; /* this part is all of them */
+        /* waves side by side on rows, the rest in turns on the keys, 32 at a time */
+        const int groups = nrows <= 32 ? 1 : nrows <= 64 ? 2 : 4, kparts = NW / groups;
         const int group = wave & (groups - 1), kpart = wave / groups;
-        const bool active = kpart < kparts && 32 * group < nrows;
-        const int r = r0 + 32 * group + col, tok = r / a.R, head = it.kh * a.R + (r - tok * a.R);
+        const bool active = 32 * group < nrows;
+        const int r = r0 + 32 * group + col, tok = a.by_r.of(r), head = it.kh * R + (r - tok * R);
         const bool mine = r < r0 + nrows;
         const Seen sn = mine ? seen(a, p0 + tok, it.len) : Seen{0, -1};
         /* of the wave's rows: keys from all_first to all_last are seen by all, outside any_first .. any_last by none */
-        const int gtok0 = min(r0 + 32 * group, r0 + nrows - 1) / a.R, gtok1 = min(r0 + 32 * group + 31, r0 + nrows - 1) / a.R;
+        const int gtok0 = a.by_r.of(min(r0 + 32 * group, r0 + nrows - 1)), gtok1 = a.by_r.of(min(r0 + 32 * group + 31, r0 + nrows - 1));
         const Seen sa = seen(a, p0 + gtok0, it.len), sz = seen(a, p0 + gtok1, it.len);
         const int any_first = sa.first, any_last = sz.last, all_first = sz.first, all_last = sa.last;
 
+        const size_t kv = (size_t)HD << b.shift; /* elements of one head's keys or values in a page */
+        const int mask = (1 << b.shift) - 1;
+        const int* table = b.pages + (size_t)it.s * b.max_pages;
+
         bf16x8 qf[TERMS][STEPS]; /* step s: dimensions 16 s + 8 half .. + 7 of the lane's row */
-        {
-            const size_t at = (size_t)(n0 + min(tok, tok1)) * a.ldq + (size_t)(mine ? head : it.kh * a.R) * HD;
+        u32x4 qr[STEPS][BF16 ? 1 : 2];
+        auto q_request = [&]() {
+            const size_t at = (size_t)(n0 + min(tok, tok1)) * a.ldq + (size_t)(mine ? head : it.kh * R) * HD;
 #pragma unroll
             for (int s = 0; s < STEPS; s++) {
                 const int d = 16 * s + 8 * half;
-                unsigned int u[TERMS][4];
-                if (!mine || d >= HD) {
 #pragma unroll
-                    for (int x = 0; x < TERMS; x++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) u[x][e] = 0;
-                } else if constexpr (BF16) {
-                    const unsigned short* p = (const unsigned short*)a.q + at + d;
-                    if (((uintptr_t)p & 15) == 0) {
-                        __builtin_memcpy(u[0], __builtin_assume_aligned(p, 16), 16);
+                for (int i = 0; i < (BF16 ? 1 : 2); i++) {
+                    qr[s][i] = u32x4{0, 0, 0, 0};
+                    if (!mine || d >= HD) continue;
+                    const char* p = (const char*)a.q + (at + d + 4 * i) * (BF16 ? 2 : 4);
+                    if (a.q_wide) {
+                        qr[s][i] = *(const u32x4*)p;
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) u[0][e] = p[2 * e] | (unsigned int)p[2 * e + 1] << 16;
+                        for (int e = 0; e < 4; e++)
+                            qr[s][i][e] = BF16 ? ((const unsigned short*)p)[2 * e] | (unsigned int)((const unsigned short*)p)[2 * e + 1] << 16
+                                               : ((const unsigned int*)p)[e];
                     }
+                }
+            }
+        };
+        auto q_take = [&]() {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) u[0][e] ^= a.flip >> 16 | a.flip;
-                } else {
-                    const float* p = (const float*)a.q + at + d;
+            for (int s = 0; s < STEPS; s++) {
+                unsigned int u[TERMS][4];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
+                for (int e = 0; e < 4; e++) {
+                    if constexpr (BF16) {
+                        u[0][e] = qr[s][0][e] ^ (a.flip >> 16 | a.flip);
+                    } else {
                         unsigned int y[3];
-                        split2(__uint_as_float(__float_as_uint(p[2 * e]) ^ a.flip),
-                               __uint_as_float(__float_as_uint(p[2 * e + 1]) ^ a.flip), y);
+                        split2(__uint_as_float(qr[s][e >> 1][2 * (e & 1)] ^ a.flip),
+                               __uint_as_float(qr[s][e >> 1][2 * (e & 1) + 1] ^ a.flip), y);
 #pragma unroll
                         for (int x = 0; x < TERMS; x++) u[x][e] = y[x];
                     }
@@ -360,7 +436,7 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
 #pragma unroll
                 for (int x = 0; x < TERMS; x++) __builtin_memcpy(&qf[x][s], u[x], 16);
             }
-        }
+        };
 
         f32x16 acc[DT];
 #pragma unroll
@@ -369,34 +445,61 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
             for (int e = 0; e < 16; e++) acc[d][e] = 0.0f;
         float m = -INFINITY, l = 0.0f; /* in powers of two, of the row; this lane's keys' sum */
 
-        const size_t kv = (size_t)HD << b.shift; /* elements of one head's keys or values in a page */
-        const int mask = (1 << b.shift) - 1;
-        const int* table = b.pages + (size_t)it.s * b.max_pages;
-        auto page_at = [&](int key) { /* page of a key before hi, or none */
-            const int pg = table[key >> b.shift];
-            return pg >= 0 && pg < b.n_pages ? pg : -1;
-        };
-
-        /* 32 keys at k0, block kb of the tile in LDS at `buf` */
+        /* 32 keys at k0, block kb of the tile in LDS at `buf`.  Reads are issued in groups ahead of the products that take
+         * them, the first of V's ahead of the softmax. */
+        constexpr int KG = BF16 ? 4 : 2, VG = BF16 ? 2 : 1;
         auto block = [&](const unsigned char* buf, int kb, int k0) {
             f32x16 sc;
 #pragma unroll
             for (int e = 0; e < 16; e++) sc[e] = 0.0f;
-            const int row = 32 * kb + col;
+            bf16x8 kf[2][KG][TERMS];
+            auto read_k = [&](int g) {
 #pragma unroll
-            for (int s = 0; s < STEPS; s++) {
-                bf16x8 kf[TERMS];
+                for (int s = 0; s < KG; s++)
 #pragma unroll
-                for (int x = 0; x < TERMS; x++)
-                    kf[x] = *(const bf16x8*)(buf + x * PLANE + row * T::ROWB + 16 * k_place(row, 2 * s + half));
-                if constexpr (!BF16) { /* the small terms first */
-                    sc = mfma(kf[2], qf[0][s], sc);
-                    sc = mfma(kf[0], qf[2][s], sc);
-                    sc = mfma(kf[1], qf[1][s], sc);
-                    sc = mfma(kf[1], qf[0][s], sc);
-                    sc = mfma(kf[0], qf[1][s], sc);
+                    for (int x = 0; x < TERMS; x++) {
+                        const int row = 32 * kb + col;
+                        kf[g & 1][s][x] = *(const bf16x8*)(buf + x * PLANE + row * T::ROWB + 16 * k_place(row, 2 * (g * KG + s) + half));
+                    }
+            };
+            /* dimension 32 d + col, keys 16 s + 4 half + 0 .. 3 and 8 more, of V's term x */
+            u32x4 vf[2][VG][TERMS][2];
+            auto read_v = [&](int g) {
+#pragma unroll
+                for (int d = 0; d < VG; d++)
+#pragma unroll
+                    for (int x = 0; x < TERMS; x++)
+#pragma unroll
+                        for (int s = 0; s < 2; s++) {
+                            const int vr = 32 * kb + 16 * s + 4 * half + ((lane & 15) >> 2);
+                            const int dim = 32 * (g * VG + d) + (lane & 16) + 4 * (lane & 3);
+                            const unsigned char* at = buf + (TERMS + x) * PLANE + vr * T::ROWB + 16 * v_place(vr, dim >> 3) + 2 * (dim & 4);
+                            s16x4 y[2]; /* the second set lies 8 rows on, in the same place of its row */
+                            y[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lvoid*)at);
+                            y[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lvoid*)(at + 8 * T::ROWB));
+                            vf[g & 1][d][x][s] = __builtin_bit_cast(u32x4, y);
+                        }
+            };
+            read_k(0);
+#pragma unroll
+            for (int g = 0; g < STEPS / KG; g++) {
+                if (g + 1 < STEPS / KG) read_k(g + 1);
+                else read_v(0);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int s = 0; s < KG; s++) {
+                    const bf16x8* k = kf[g & 1][s];
+                    const int at = g * KG + s;
+                    if constexpr (!BF16) { /* the small terms first */
+                        sc = mfma(k[2], qf[0][at], sc);
+                        sc = mfma(k[0], qf[2][at], sc);
+                        sc = mfma(k[1], qf[1][at], sc);
+                        sc = mfma(k[1], qf[0][at], sc);
+                        sc = mfma(k[0], qf[1][at], sc);
+                    }
+                    sc = mfma(k[0], qf[0][at], sc);
                 }
-                sc = mfma(kf[0], qf[0][s], sc);
+                __builtin_amdgcn_sched_barrier(0);
             }
             /* lane's score e: key k0 + 8 (e / 4) + 4 half + e % 4 */
             const bool masked = k0 < all_first || k0 + 31 > all_last;
@@ -454,132 +557,147 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
 #pragma unroll
                 for (int x = 0; x < TERMS; x++) __builtin_memcpy(&pf[x][s], u[x], 16);
             }
-            /* dimension 32 d + col, keys 16 s + 4 half + 0 .. 3 and 8 more, of V's term x */
-            auto values = [&](int x, int d, int s) {
-                const int vr = 32 * kb + 16 * s + 4 * half + ((lane & 15) >> 2), dim = 32 * d + (lane & 16) + 4 * (lane & 3);
-                const unsigned char* at = buf + (TERMS + x) * PLANE + vr * T::ROWB + 16 * v_place(vr, dim >> 3) + 2 * (dim & 4);
-                /* the second set lies 8 rows on, in the same place of its row */
-                s16x4 y[2];
-                y[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lvoid*)at);
-                y[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lvoid*)(at + 8 * T::ROWB));
-                return __builtin_bit_cast(u32x4, y);
-            };
-            /* A value that is no number times a masked key's weight 0 would be NaN.  Where some row of the wave does not see
-             * one of the keys, such values are taken out, and the rows that do see one get NaN by a product of their own. */
-            unsigned int vis[2][4];
-            if (masked) {
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int s = 0; s < 2; s++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const unsigned int two = sees >> (8 * s + 2 * e);
-                        vis[s][e] = (two & 1 ? 0x3f80u : 0u) | (two & 2 ? 0x3f800000u : 0u); /* 1 in bf16 */
-                    }
-            }
-#pragma unroll
-            for (int d = 0; d < DT; d++) {
-                u32x4 v[TERMS][2];
-#pragma unroll
-                for (int x = 0; x < TERMS; x++)
-#pragma unroll
-                    for (int s = 0; s < 2; s++) v[x][s] = values(x, d, s);
+            for (int g = 0; g < DT / VG; g++) {
+                if (g + 1 < DT / VG) read_v(g + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                /* A value that is no number times a masked key's weight 0 would be NaN.  Where some row of the wave does not
+                 * see one of the keys, such values are taken out, and the rows that do see one get NaN by a product of
+                 * their own. */
                 if (masked) {
                     unsigned int odd = 0;
 #pragma unroll
-                    for (int s = 0; s < 2; s++)
+                    for (int d = 0; d < VG; d++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) /* an exponent of ones carries into bit 15 or 31 */
-                            odd |= (((v[0][s][e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u);
+                        for (int s = 0; s < 2; s++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) odd |= no_numbers(vf[g & 1][d][0][s][e]);
                     if (__builtin_expect(__any(odd != 0), 0)) {
-                        f32x16 hit;
+                        u32x4 vis[2];
 #pragma unroll
-                        for (int e = 0; e < 16; e++) hit[e] = 0.0f;
-#pragma unroll
-                        for (int s = 0; s < 2; s++) {
-                            u32x4 flag, one;
+                        for (int s = 0; s < 2; s++)
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
-                                const unsigned int o = ((v[0][s][e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-                                const unsigned int all = (o >> 15) * 0xffffu; /* both halves' bits */
-                                flag[e] = all & 0x3f803f80u;
-                                one[e] = vis[s][e];
-#pragma unroll
-                                for (int x = 0; x < TERMS; x++) v[x][s][e] &= ~all;
+                                const unsigned int two = sees >> (8 * s + 2 * e);
+                                vis[s][e] = (two & 1 ? 0x3f80u : 0u) | (two & 2 ? 0x3f800000u : 0u); /* 1 in bf16 */
                             }
-                            hit = mfma(__builtin_bit_cast(bf16x8, flag), __builtin_bit_cast(bf16x8, one), hit);
+#pragma unroll
+                        for (int d = 0; d < VG; d++) {
+                            f32x16 hit;
+#pragma unroll
+                            for (int e = 0; e < 16; e++) hit[e] = 0.0f;
+#pragma unroll
+                            for (int s = 0; s < 2; s++) {
+                                u32x4 flag;
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    const unsigned int all = (no_numbers(vf[g & 1][d][0][s][e]) >> 15) * 0xffffu; /* the halves' bits */
+                                    flag[e] = all & 0x3f803f80u;
+#pragma unroll
+                                    for (int x = 0; x < TERMS; x++) vf[g & 1][d][x][s][e] &= ~all;
+                                }
+                                hit = mfma(__builtin_bit_cast(bf16x8, flag), __builtin_bit_cast(bf16x8, vis[s]), hit);
+                            }
+#pragma unroll
+                            for (int e = 0; e < 16; e++) acc[g * VG + d][e] = hit[e] > 0.0f ? NAN : acc[g * VG + d][e];
                         }
-#pragma unroll
-                        for (int e = 0; e < 16; e++) acc[d][e] = hit[e] > 0.0f ? NAN : acc[d][e];
                     }
                 }
 #pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    bf16x8 vf[TERMS];
+                for (int s = 0; s < 2; s++)
 #pragma unroll
-                    for (int x = 0; x < TERMS; x++) vf[x] = __builtin_bit_cast(bf16x8, v[x][s]);
-                    if constexpr (!BF16) {
-                        acc[d] = mfma(vf[2], pf[0][s], acc[d]);
-                        acc[d] = mfma(vf[0], pf[2][s], acc[d]);
-                        acc[d] = mfma(vf[1], pf[1][s], acc[d]);
-                        acc[d] = mfma(vf[1], pf[0][s], acc[d]);
-                        acc[d] = mfma(vf[0], pf[1][s], acc[d]);
+                    for (int d = 0; d < VG; d++) {
+                        f32x16& o = acc[g * VG + d];
+                        bf16x8 v[TERMS];
+#pragma unroll
+                        for (int x = 0; x < TERMS; x++) v[x] = __builtin_bit_cast(bf16x8, vf[g & 1][d][x][s]);
+                        if constexpr (!BF16) {
+                            o = mfma(v[2], pf[0][s], o);
+                            o = mfma(v[0], pf[2][s], o);
+                            o = mfma(v[1], pf[1][s], o);
+                            o = mfma(v[1], pf[0][s], o);
+                            o = mfma(v[0], pf[1][s], o);
+                        }
+                        o = mfma(v[0], pf[0][s], o);
                     }
-                    acc[d] = mfma(vf[0], pf[0][s], acc[d]);
-                }
+                __builtin_amdgcn_sched_barrier(0);
             }
         };
         auto compute = [&](const unsigned char* buf, int kt) {
             if (!active) return;
-            for (int kb = kpart; kb < KB; kb += kparts) {
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) {
                 const int k0 = kt * KT + 32 * kb;
-                if (k0 <= any_last && k0 + 31 >= any_first && k0 < hi) block(buf, kb, k0);
+                if (((kt * KB + kb) & (kparts - 1)) == kpart && k0 <= any_last && k0 + 31 >= any_first && k0 < hi) block(buf, kb, k0);
             }
         };
 
         if constexpr (BF16) {
-            /* straight into LDS, 16 bytes a lane: load i of a wave fills rows (i NW + wave) RPI .. + RPI - 1 */
+            /* Straight into LDS, 16 bytes a lane: load i of a wave fills rows (i NW + wave) RPI .. + RPI - 1, eight at most,
+             * which lie in one page.  Its number is read into a scalar register, apart from the loads' count, so that nothing
+             * waits for the tiles that are under way; what lies behind the load's rows or a head's end comes as zeros by the
+             * buffer's bounds, a missing page's keys from a row of NaN. */
             int pg[NI];
             auto pages = [&](int kt) {
 #pragma unroll
                 for (int i = 0; i < NI; i++) {
-                    const int key = kt * KT + (i * NW + wave) * RPI + lane / CPR;
-                    pg[i] = kt < kt1 && key < hi ? page_at(key) : -2; /* -2: behind the keys */
+                    const int key = min(kt * KT + (i * NW + wave) * RPI, hi - 1);
+                    pg[i] = ((const __attribute__((address_space(4))) int*)table)[max(key, 0) >> b.shift];
                 }
             };
+            int kv_off[2]; /* the lane's place in a load's rows of keys and of values */
+            static_assert(NW * RPI % 8 == 0, "the same for all of a wave's loads");
+            {
+                const int row = wave * RPI + lane / CPR, place = lane % CPR;
+                const int kc = k_place(row, place), vc = v_place(row, place); /* their own inverses */
+                kv_off[0] = 8 * kc < HD ? (lane / CPR) * HD * 2 + 16 * kc : 1 << 30;
+                kv_off[1] = 8 * vc < HD ? (lane / CPR) * HD * 2 + 16 * vc : 1 << 30;
+            }
+            const int end = min(hi, kt1 * KT);
+            const size_t page_bytes = (size_t)b.NKV * kv * 4, kh_bytes = (size_t)it.kh * kv * 2;
             auto request = [&](int kt, unsigned char* buf) {
 #pragma unroll
                 for (int i = 0; i < NI; i++) {
-                    const int row = (i * NW + wave) * RPI + lane / CPR, place = lane % CPR;
-                    const int kc = k_place(row, place), vc = v_place(row, place); /* their own inverses */
-                    const size_t at = b.base(max(pg[i], 0), 0, it.kh) + (size_t)((kt * KT + row) & mask) * HD;
-                    const unsigned short* k = (const unsigned short*)a.cache + at;
-                    const unsigned short* v = k + (size_t)b.NKV * kv;
-                    const void* ks = 8 * kc >= HD || pg[i] == -2 ? (const void*)&pg_zeros : pg[i] < 0 ? (const void*)&pg_nans : (const void*)(k + 8 * kc);
-                    const void* vs = 8 * vc >= HD || pg[i] < 0 ? (const void*)&pg_zeros : (const void*)(v + 8 * vc);
+                    const int key = kt * KT + (i * NW + wave) * RPI;
+                    const bool there = (unsigned int)pg[i] < (unsigned int)b.n_pages;
+                    const int bytes = min(max(end - key, 0), RPI) * HD * 2;
+                    const char* k = (const char*)a.cache + (there ? pg[i] : 0) * page_bytes + kh_bytes + (unsigned int)((key & mask) * HD * 2);
+                    const auto ks = __builtin_amdgcn_make_buffer_rsrc((void*)(there ? k : (const char*)pg_nans), 0, bytes, 0x00027000);
+                    const auto vs = __builtin_amdgcn_make_buffer_rsrc((void*)(k + page_bytes / 2), 0, there ? bytes : 0, 0x00027000);
                     unsigned char* to = buf + (i * NW + wave) * 1024;
-                    __builtin_amdgcn_global_load_lds((const gvoid*)ks, (lvoid*)to, 16, 0, 0);
-                    __builtin_amdgcn_global_load_lds((const gvoid*)vs, (lvoid*)(to + PLANE), 16, 0, 0);
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(ks, (lvoid*)to, 16, kv_off[0], 0, 0, 0);
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(vs, (lvoid*)(to + PLANE), 16, kv_off[1], 0, 0, 0);
                 }
             };
-            __syncthreads(); /* an item before this one is through with LDS */
-            if (kt0 < kt1) {
-                pages(kt0);
-                request(kt0, lds0);
-                pages(kt0 + 1);
-            }
-            auto step = [&](int kt, unsigned char* buf, unsigned char* next) {
-                __builtin_amdgcn_s_waitcnt(0xF70); /* vmcnt(0): the tile has landed (and the next one's pages) */
-                __syncthreads();
-                if (kt + 1 < kt1) {
-                    request(kt + 1, next);
-                    pages(kt + 2);
-                }
+            pages(kt0);
+            q_request();
+            __builtin_amdgcn_sched_barrier(0);
+            request(kt0, lds0);
+            pages(kt0 + 1);
+            request(kt0 + 1, lds1);
+            pages(kt0 + 2);
+            request(kt0 + 2, lds2);
+            pages(kt0 + 3);
+            __builtin_amdgcn_sched_barrier(0);
+            q_take();
+            /* Three tiles are under way while one is read; a tile's array is requested again behind the barrier that all
+             * waves reach when they have read it.  Tiles behind the last are zeros. */
+            constexpr int AHEAD = 4 * NI; /* loads of the two tiles after the one to be read */
+            auto step = [&](int kt, unsigned char* buf, unsigned char* before) {
+                __builtin_amdgcn_s_waitcnt(0x0F70 | (AHEAD & 15) | ((AHEAD >> 4) << 14));
+                barrier();
+                request(kt + 3, before);
+                pages(kt + 4);
                 compute(buf, kt);
             };
-            for (int kt = kt0; kt < kt1; kt += 2) {
-                step(kt, lds0, lds1);
+            for (int kt = kt0; kt < kt1; kt += 4) {
+                step(kt, lds0, lds3);
                 if (kt + 1 < kt1) step(kt + 1, lds1, lds0);
+                if (kt + 2 < kt1) step(kt + 2, lds2, lds1);
+                if (kt + 3 < kt1) step(kt + 3, lds3, lds2);
             }
+            __builtin_amdgcn_s_waitcnt(0x0F70); /* none under way */
         } else {
             /* through registers: thread's part i of a tile is chunk c = x % CPR of row x / CPR, x = i NT + t: eight values
              * of keys and of values, split into their terms on the way into LDS */
@@ -590,8 +708,12 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
 #pragma unroll
                 for (int i = 0; i < PER; i++) {
                     const int x = i * NT + t, row = x / CPR, c = x % CPR, key = kt * KT + row;
-                    const int pg = key < hi ? page_at(key) : -2;
-                    const size_t at = b.base(max(pg, 0), 0, it.kh) + (size_t)(key & mask) * HD + 8 * c;
+                    int pg = -2;
+                    if (key < hi) {
+                        pg = table[key >> b.shift];
+                        if (pg < 0 || pg >= b.n_pages) pg = -1;
+                    }
+                    const size_t at = b.base(max(pg, 0), 0, it.kh) + (size_t)((key & mask) * HD + 8 * c);
                     const bool there = pg >= 0 && 8 * c < HD;
                     const float fill = pg == -1 && 8 * c < HD ? NAN : 0.0f;
                     const f32x4* k = (const f32x4*)((const float*)a.cache + at);
@@ -619,7 +741,9 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
                     }
                 }
             };
+            q_request();
             if (kt0 < kt1) fetch(kt0);
+            q_take();
             for (int kt = kt0; kt < kt1; kt++) {
                 __syncthreads(); /* the tile before has been read */
                 put(lds0);
@@ -630,38 +754,41 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
         }
         l += other_half(l);
 
-        /* the waves' parts of the tiles' keys, joined in the first one's registers */
-        if constexpr (KB > 1) {
-            constexpr int REGS = HDP / 2 + 2;
-            static_assert(KB == 2 && REGS * 64 * 4 <= sizeof lds0, "two parts, one group at a time");
-            float* mem = (float*)lds0 + lane;
-            for (int g = 0; kparts > 1 && g < groups; g++) {
-                __syncthreads();
-                if (active && group == g && kpart == 1) {
-                    mem[0] = m;
-                    mem[64] = l;
+        /* the waves' parts of the keys, joined in the first one's registers */
+        if (kparts > 1) {
+            const int at = (kpart - 1) * groups + group; /* 0 .. 2 */
+            auto place = [&](int i) { return (float*)(BF16 ? i == 0 ? lds0 : i == 1 ? lds1 : lds2 : lds0 + i * (HDP * 128)) + lane; };
+            static_assert(BF16 ? HDP * 128 <= T::BYTES : 3 * HDP * 128 <= T::BYTES, "a wave's sums in an array");
+            __syncthreads();
+            if (active && kpart) {
+                float* mem = place(at);
+                part_m[at][lane] = m;
+                part_l[at][lane] = l;
 #pragma unroll
-                    for (int d = 0; d < DT; d++)
+                for (int d = 0; d < DT; d++)
 #pragma unroll
-                        for (int e = 0; e < 16; e++) mem[(2 + 16 * d + e) * 64] = acc[d][e];
-                }
-                __syncthreads();
-                if (active && group == g && kpart == 0) {
+                    for (int e = 0; e < 16; e++) mem[(16 * d + e) * 64] = acc[d][e];
+            }
+            __syncthreads();
+            if (active && !kpart) {
+                for (int k = 1; k < kparts; k++) {
                     /* a part without a finite score has what its scores left there: 0, or NaN */
-                    const float m1 = mem[0], mx = fmaxf(m, m1);
+                    const int i = (k - 1) * groups + group;
+                    const float* mem = place(i);
+                    const float m1 = part_m[i][lane], mx = fmaxf(m, m1);
                     const float f0 = m > -INFINITY ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
                     const float f1 = m1 > -INFINITY ? __builtin_amdgcn_exp2f(m1 - mx) : 1.0f;
-                    l = l * f0 + mem[64] * f1;
+                    l = l * f0 + part_l[i][lane] * f1;
 #pragma unroll
                     for (int d = 0; d < DT; d++)
 #pragma unroll
-                        for (int e = 0; e < 16; e++) acc[d][e] = acc[d][e] * f0 + mem[(2 + 16 * d + e) * 64] * f1;
+                        for (int e = 0; e < 16; e++) acc[d][e] = acc[d][e] * f0 + mem[(16 * d + e) * 64] * f1;
                     m = mx;
                 }
             }
         }
         const bool writes = active && kpart == 0 && mine;
-        if (parts == 1) {
+        if (whole) {
             if (writes) {
                 const size_t row = (size_t)(n0 + tok) * a.ldo + (size_t)head * HD;
                 const bool none = sn.last < sn.first, gone = sn.last >= room;
@@ -676,12 +803,13 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
                         if (dim < HD) store4<BF16>(a, row, dim, o);
                     }
             }
-            continue;
+            return;
         }
         /* Records cross XCDs: they are written and read with agent-scope accesses, past the XCDs' own L2s, and each wave
          * waits for its stores before the barrier, so a part is counted only after its record has arrived.  A unit's
          * records: [part][row]{HDP values, maximum, sum}, from the unit's rows and KV heads before it. */
         constexpr int REC = HDP + 2;
+        const int parts = (t1 - t0 + plan.per - 1) / plan.per; /* with keys */
         float* recs = a.rec + ((size_t)it.rec + (size_t)it.parts * ((size_t)rows_all * it.kh + r0)) * REC;
         if (writes) {
             float* rec = recs + ((size_t)it.part * nrows + (r - r0)) * REC;
@@ -705,62 +833,46 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
             if (last_one) __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
         __syncthreads();
-        if (!last_one) continue;
-        /* the rows' maxima and sums over the parts: as many threads a row as there are */
-        {
-            int tpr = 64;
-            while (tpr * nrows > NT) tpr >>= 1;
-            const int row = t / tpr, sub = t % tpr;
-            float mx = -INFINITY, sum = 0.0f;
-            if (row < nrows)
-                for (int i = sub; i < parts; i += tpr) {
-                    const f32x2 ml = agent_load2(recs + ((size_t)i * nrows + row) * REC + HDP);
-                    const float mn = fmaxf(mx, ml[0]);
-                    sum = sum * (mx > -INFINITY ? __builtin_amdgcn_exp2f(mx - mn) : 1.0f) +
-                          ml[1] * (ml[0] > -INFINITY ? __builtin_amdgcn_exp2f(ml[0] - mn) : 1.0f);
-                    mx = mn;
-                }
-            for (int o = 1; o < tpr; o <<= 1) {
-                const float m1 = __shfl_xor(mx, o), s1 = __shfl_xor(sum, o), mn = fmaxf(mx, m1);
-                sum = sum * (mx > -INFINITY ? __builtin_amdgcn_exp2f(mx - mn) : 1.0f) +
-                      s1 * (m1 > -INFINITY ? __builtin_amdgcn_exp2f(m1 - mn) : 1.0f);
-                mx = mn;
-            }
-            if (row < nrows && sub == 0) {
-                row_m[row] = mx;
-                row_l[row] = sum;
-            }
-        }
-        __syncthreads();
+        if (!last_one) return;
+        /* each output from its records, 8 of them read at once */
         for (int x = t; x < nrows * (HD / 4); x += NT) {
             const int row = x / (HD / 4), dim = 4 * (x - row * (HD / 4));
-            const float mx = row_m[row];
-            float o[4] = {0, 0, 0, 0};
+            float o[4] = {0, 0, 0, 0}, mx = -INFINITY, sum = 0.0f;
             for (int i = 0; i < parts; i += 8) {
                 f32x2 y[8][3];
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const float* rec = recs + ((size_t)min(i + e, parts - 1) * nrows + row) * REC;
+                    const float* rec = recs + ((size_t)(i + e) * nrows + row) * REC;
+                    y[e][0] = y[e][1] = f32x2{0, 0};
+                    y[e][2] = f32x2{-INFINITY, 0};
+                    if (i + e >= parts) continue;
+                    y[e][2] = agent_load2(rec + HDP);
                     y[e][0] = agent_load2(rec + dim);
                     y[e][1] = agent_load2(rec + dim + 2);
-                    y[e][2] = agent_load2(rec + HDP);
                 }
+                float mn = mx;
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    if (i + e >= parts) continue;
-                    const float f = y[e][2][0] > -INFINITY ? __builtin_amdgcn_exp2f(y[e][2][0] - mx) : 1.0f;
+                for (int e = 0; e < 8; e++) mn = fmaxf(mn, y[e][2][0]);
+                const float f = mx > -INFINITY ? __builtin_amdgcn_exp2f(mx - mn) : 1.0f;
+                sum *= f;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) o[j] = fmaf(f, y[e][j >> 1][j & 1], o[j]);
+                for (int j = 0; j < 4; j++) o[j] *= f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) { /* a part without a finite score has 0 or NaN */
+                    const float g = y[e][2][0] > -INFINITY ? __builtin_amdgcn_exp2f(y[e][2][0] - mn) : 1.0f;
+                    sum = fmaf(g, y[e][2][1], sum);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) o[j] = fmaf(g, y[e][j >> 1][j & 1], o[j]);
                 }
+                mx = mn;
             }
-            const int rr = r0 + row, rtok = rr / a.R;
+            const int rr = r0 + row, rtok = a.by_r.of(rr);
             const Seen s = seen(a, p0 + rtok, it.len);
             const bool none = s.last < s.first, gone = s.last >= room;
 #pragma unroll
-            for (int j = 0; j < 4; j++) o[j] = none ? 0.0f : gone ? NAN : o[j] / row_l[row];
-            store4<BF16>(a, (size_t)(n0 + rtok) * a.ldo + (size_t)(it.kh * a.R + rr - rtok * a.R) * HD, dim, o);
+            for (int j = 0; j < 4; j++) o[j] = none ? 0.0f : gone ? NAN : o[j] / sum;
+            store4<BF16>(a, (size_t)(n0 + rtok) * a.ldo + (size_t)(it.kh * R + rr - rtok * R) * HD, dim, o);
         }
-        __syncthreads(); /* before another item's rows lie there */
     }
 }
 
@@ -772,10 +884,11 @@ int start(PaArgs& a, const bmk_launch_t* l) {
         a.most = (unsigned int)std::min<size_t>((l->scratch_bytes - DONE_BYTES) / ((HDP + 2) * 4), 1u << 30);
     a.done = (unsigned int*)l->scratch;
     a.rec = (float*)((char*)l->scratch + DONE_BYTES);
-    /* pieces of work: a unit for every new token or ROWS rows, in parts of a tile at least, WANTED more at most */
-    const int64_t units = a.b.NKV * std::min<int64_t>(a.b.N, a.b.S + (int64_t)a.b.N * a.R / ROWS);
+    /* A workgroup a piece: no more than a unit for every sequence with new tokens and every ROWS rows, and WANTED (the 8:
+     * sums rounded in fp32). */
+    const int64_t units = a.b.NKV * (std::min<int64_t>(a.b.N, a.b.S) + (int64_t)a.b.N * a.R / ROWS);
     const int64_t tiles = std::min<int64_t>((a.b.room() + KT - 1) / KT, MAX_SPLIT);
-    const int64_t grid = std::min<int64_t>(std::min(units * tiles, units + WANTED), 1 << 20);
+    const int64_t grid = std::min(units * tiles, units + WANTED + 8);
     hipLaunchKernelGGL((k_attn_paged<BF16, HDP>), dim3((unsigned)grid), dim3(NT), 0, l->stream, a);
     BMK_LAUNCH_CHECK();
     return 0;
@@ -793,7 +906,7 @@ int launch_attn_paged(const bmk_launch_t* l, bool bf16) {
                 "attention_forward_paged: bad shape N=%d S=%d NH=%d NKV=%d HD=%d", N, S, NH, NKV, HD);
     BMK_REQUIRE((causal == 1 && window >= 0) || (causal == 0 && window == 0),
                 "attention_forward_paged: bad mask causal=%d window=%d", causal, window);
-    BMK_REQUIRE((int64_t)N * NH < (1LL << 31), "attention_forward_paged: %d rows of %d heads are over 2^31 heads", N, NH);
+    BMK_REQUIRE((int64_t)N * NH < (1LL << 30), "attention_forward_paged: %d rows of %d heads are over 2^30 heads", N, NH);
     if (N == 0 || S == 0) return 0;
     const size_t esz = bf16 ? 2 : 4;
     PaArgs a = {};
@@ -809,8 +922,10 @@ int launch_attn_paged(const bmk_launch_t* l, bool bf16) {
     a.q = l->dev[0];
     a.cache = l->dev[1];
     a.out = l->dev[2];
-    a.NH = NH;
     a.R = NH / NKV;
+    a.by_r = div_by(a.R);
+    a.by_kv = div_by(NKV);
+    a.q_wide = (uintptr_t)l->dev[0] % 16 == 0 && ldq * esz % 16 == 0;
     a.causal = causal;
     a.window = std::min(window, PG_MAX_DIM); /* keys lie below that */
     a.ldq = ldq;

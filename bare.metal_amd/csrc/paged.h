@@ -77,7 +77,7 @@ inline int pg_log2(int v) { /* of a power of two, else -1 */
 /* The tables in buffers i, i + 1, i + 2 and the cache in buffer c, for a batch whose numbers are set. */
 #define BMK_NEED_BATCH(a, b, page, i, c, esz) do { \
     (b).shift = bmk::pg_log2(page); \
-    BMK_REQUIRE((b).shift >= 0 && (page) <= 65536 && (b).n_pages > 0 && (b).max_pages > 0 && \
+    BMK_REQUIRE((b).shift >= 3 && (page) <= 65536 && (b).n_pages > 0 && (b).max_pages > 0 && \
                     (int64_t)(b).max_pages * (page) <= bmk::PG_MAX_DIM && (int64_t)(b).n_pages * (page) <= (1LL << 38), \
                 "%s: bad cache: page %d, n_pages %d, max_pages %d", __func__, (int)(page), (b).n_pages, (b).max_pages); \
     BMK_REQUIRE((b).HD % 8 == 0 && (b).NKV <= 4096, "%s: cache of %d heads of %d", __func__, (b).NKV, (b).HD); \

@@ -15,7 +15,7 @@
  * where stated.
  *
  * The cache: T [n_pages][2][NKV][page][HD], keys then values, on a 16-byte
- * boundary; page a power of two up to 65536, max_pages * page at most 2^30,
+ * boundary; page a power of two from 8 to 65536, max_pages * page at most 2^30,
  * n_pages * page at most 2^38, NKV at most 4096.
  * A layer's cache goes in by its buffer's offset.
  * The batch: S sequences, at most 2^20; start int32 [S + 1], not falling: the new tokens

@@ -50,7 +50,7 @@ def refused(capfd, *args, **kw):
 
 
 # each operator: launcher, buffer sizes of one call, its params, its floats
-N, S, NH, NKV, HD, ROT, PAGE, COUNT, WIDTH = 5, 2, 6, 3, 16, 8, 4, 7, 3
+N, S, NH, NKV, HD, ROT, PAGE, COUNT, WIDTH = 5, 2, 6, 3, 16, 8, 8, 7, 3
 Q, K = NH * HD, NKV * HD
 
 
@@ -104,7 +104,7 @@ NAMES = {
 }
 BAD = {
     "N": [-1, (1 << 30) + 1], "S": [-1, (1 << 30) + 1], "NH": [-1, (1 << 30) + 1], "NKV": [0, -1, 4097],
-    "HD": [0, -8, 258, 264, 7], "rot": [-2, 3, 18], "layout": [-1, 2], "page": [0, -4, 3, 12, 131072],
+    "HD": [0, -8, 258, 264, 7], "rot": [-2, 3, 18], "layout": [-1, 2], "page": [0, -8, 1, 4, 12, 131072],
     "n_pages": [0, -1, (1 << 31) - 1], "max_pages": [0, -1, (1 << 30)], "norm": [-1, 2], "causal": [-1, 2], "window": [-1],
 }
 

@@ -308,10 +308,10 @@ class Batch:
 BATCHES = [  # new tokens, total keys, page, lead, tail
     ([1], [1], 16, 0, 0),
     ([1], [17], 16, 0, 1),
-    ([3], [3], 1, 0, 0),
+    ([3], [3], 8, 0, 0),
     ([1, 1, 1], [5, 16, 33], 16, 0, 0),
     ([5, 0, 1, 9], [5, 7, 40, 20], 8, 2, 3),
-    ([0, 0, 4, 0], [0, 3, 4, 0], 4, 1, 0),
+    ([0, 0, 4, 0], [0, 3, 4, 0], 8, 1, 0),
     ([40, 1], [70, 1], 32, 0, 5),
 ]
 
@@ -370,9 +370,9 @@ def test_kv_append(be, new, total, page, lead, tail, NH, NKV, HD, rot, layout, n
 def test_kv_append_skips_what_has_no_place(be, kind):
     """Rows before position 0, on pages that are none and past the table: the cache keeps its bits there, q is turned all
     the same."""
-    NH, NKV, HD, page = 2, 1, 64, 4
+    NH, NKV, HD, page = 2, 1, 64, 8
     # sequence 0: five rows over three keys (positions -2 .. 2); 1: pages 9 (none) and 0; 2: past the table; 3: page -1
-    start, length = np.int32([0, 5, 11, 13, 14]), np.int32([3, 6, 13, 1])
+    start, length = np.int32([0, 5, 11, 13, 14]), np.int32([3, 10, 25, 1])
     pages = np.int32([[2, -1, -1], [9, 0, -1], [3, 1, 4], [-1, -1, -1]])
     N, count = 14, 6
     pos = np.concatenate([np.arange(length[s] - (start[s + 1] - start[s]), length[s]) for s in range(4)])
@@ -389,9 +389,9 @@ def test_kv_append_skips_what_has_no_place(be, kind):
     check(kind, kind.values(out.read(kind.memory)).reshape(N, NH, HD), want, off)
     raw = cache.read(kind.memory).reshape(count, 2, page, HD)
     written = {(2, j): 2 + j for j in range(3)}  # sequence 0's positions 0 .. 2
-    written.update({(0, j): 9 + j for j in range(2)})  # sequence 1's positions 4 and 5
-    # sequence 2's positions 11 and 12: the first is in page 4, the second past the table's 12
-    written[(4, 3)] = 11
+    written.update({(0, j): 9 + j for j in range(2)})  # sequence 1's positions 8 and 9
+    # sequence 2's positions 23 and 24: the first is in page 4, the second past the table's 24
+    written[(4, 7)] = 11
     for pg in range(count):
         for j in range(page):
             if (pg, j) in written:
