@@ -27,6 +27,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -43,11 +44,11 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(1))) void gvoid;
 typedef __attribute__((address_space(3))) void lvoid;
 
-constexpr int NT = 256, NW = 4;
-constexpr int ROWS = 32 * NW;    /* of a unit */
+constexpr int KT = 32;           /* keys of a tile */
 constexpr float SLACK = 8.0f;    /* in powers of two: how far a score may pass the running maximum before that moves */
-constexpr int MAX_SPLIT = 64;    /* parts of a unit's keys */
-constexpr int WANTED = 1024;     /* workgroups that the splits aim at */
+constexpr int MAX_SPLIT = 128;   /* parts of a unit's keys */
+constexpr int LEAST = 4;         /* tiles a part, at least: one a wave */
+constexpr int CUS = 256, ROUNDS = 4, ROUND_TILES = 32;
 
 /* The scratch memory begins with arrival counters, each on a line of its own, that are zero between launches of any
  * kernel; the units' partial results lie behind them. */
@@ -81,28 +82,49 @@ struct PaArgs {
     float scale2; /* |scale| * log2(e) */
     unsigned int flip; /* scale's sign, for q's */
     unsigned int most; /* rows' records that fit behind the counters */
+    int slots; /* workgroups that run at once */
 };
 
-/* How a tile lies: HDP is the head size rounded up, with zeros behind it. */
-template <bool BF16, int HDP> struct Tile {
-    static constexpr int TERMS = BF16 ? 1 : 3;
-    static constexpr int KT = !BF16 && HDP == 64 ? 64 : 32;
-    static constexpr int KB = KT / 32;
-    static constexpr int ROWB = HDP * 2, CPR = HDP / 8; /* bytes and 16-byte chunks of a row's term */
+/* How a tile lies in LDS: keys, then values, a row behind the other, HDP elements each (the head size rounded up, with zeros
+ * behind it).
+ *   AS_BF16  bf16 as it is
+ *   AS_F32   fp32 as it is; the wave that reads it takes it apart
+ *   TERMS3   fp32's three terms, one plane each, taken apart once for the waves that read them */
+enum { AS_BF16, AS_F32, TERMS3 };
+template <int FORM, int HDP> struct Tile {
+    static constexpr int TERMS = FORM == AS_BF16 ? 1 : 3, PLANES = FORM == TERMS3 ? 3 : 1;
+    static constexpr int ESZ = FORM == AS_F32 ? 4 : 2;
+    static constexpr int ROWB = HDP * ESZ, CPR = ROWB / 16; /* bytes and 16-byte chunks of a row */
+    static constexpr int RPI = 1024 / ROWB;                  /* rows of a wave's load into LDS */
     static constexpr int PLANE = KT * ROWB;
-    static constexpr int BYTES = 2 * TERMS * PLANE; /* keys' terms, then values' */
-    static constexpr int WAVES = HDP <= (BF16 ? 128 : 64) ? 2 : 1; /* a SIMD */
+    static constexpr int BYTES = 2 * PLANES * PLANE;
 };
 
-/* Chunk c of row r lies at c ^ key: K is read 8 rows of one chunk at a time, V 4 rows of two neighbouring ones, each
- * set on all banks. */
+/* Chunk c of row r lies at c ^ key: K is read 8 rows of one chunk at a time, V 4 rows of two neighbouring chunks (fp32: two
+ * rows 4 apart of eight), each set on all banks. */
 __device__ __forceinline__ int k_place(int r, int c) { return c ^ (r & 7); }
-__device__ __forceinline__ int v_place(int r, int c) { return c ^ (2 * (r & 3)); }
+template <int FORM>
+__device__ __forceinline__ int v_place(int r, int c) { return FORM == AS_F32 ? c ^ (2 * (r & 4)) : c ^ (2 * (r & 3)); }
 
-/* a load's worth of a missing page's keys: NaN in bf16 */
+/* A workgroup's waves and LDS: every wave has a tile of its own while it goes alone, and where rows fill the waves all have
+ * a ring of four (bf16) or two (fp32, in terms; heads over 128 have no such form: their registers spill). */
+template <bool BF16, int HDP> struct Shape {
+    static constexpr int NW = !BF16 && HDP == 256 ? 2 : 4, NT = 64 * NW, ROWS = 32 * NW;
+    static constexpr int ALONE = BF16 ? AS_BF16 : AS_F32;
+    static constexpr bool SHARED = BF16 || HDP <= 128;
+    static constexpr int ALONE_BYTES = Tile<ALONE, HDP>::BYTES, ARRAYS = BF16 ? 4 : 1;
+    static constexpr int BYTES = NW / ARRAYS * ALONE_BYTES; /* of an array */
+    /* waves a SIMD, as registers (512 a lane) and LDS allow */
+    static constexpr int WAVES = BF16 ? (HDP == 64 ? 3 : HDP == 128 ? 2 : 1) : HDP == 64 ? 2 : 1;
+    static constexpr int SLOTS = CUS * WAVES; /* workgroups that run at once */
+};
+
+/* eight rows of a missing page's keys: NaN in either type */
 #define N4 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u
 #define N64 N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4
-__device__ __attribute__((aligned(16))) const unsigned int pg_nans[256] = {N64, N64, N64, N64};
+#define N512 N64, N64, N64, N64, N64, N64, N64, N64
+__device__ __attribute__((aligned(16))) const unsigned int pg_nans[8 * PG_MAX_HD] = {N512, N512, N512, N512};
+#undef N512
 #undef N64
 #undef N4
 
@@ -201,7 +223,7 @@ __device__ __forceinline__ int dpp_most(int v) { /* of values from 0 on */
 
 /* What is to be done, from the tables alone: every wave finds it for itself, 64 sequences at a time; up to 64 stay in
  * registers. */
-template <int KT>
+template <int ROWS>
 struct Plan {
     const PaArgs& a;
     const int lane;
@@ -236,24 +258,28 @@ struct Plan {
 
     __device__ __forceinline__ Plan(const PaArgs& args) : a(args), lane(threadIdx.x & 63) {
         first = seq(lane);
-        float tiles = 0, rows = 0;
+        float tiles = 0, units = 0, rows = 0;
         int longest = 0;
         for (int c = 0; c < a.b.S; c += 64) {
             const Seq q = chunk(c);
             tiles += (float)q.units * (float)q.T;
+            units += (float)q.units;
             rows += (float)q.n;
             longest = max(longest, q.T);
         }
         tiles = lane_of(dpp_sums(tiles), 63) * a.b.NKV;
+        units = lane_of(dpp_sums(units), 63) * a.b.NKV;
         rows = lane_of(dpp_sums(rows), 63);
         longest = dpp_most(longest);
-        per = max((int)(tiles / WANTED) + 1, (longest + MAX_SPLIT - 1) / MAX_SPLIT);
+        const float want = a.slots * fminf(fmaxf(tiles / (a.slots * ROUND_TILES), 1.0f), ROUNDS);
+        per = max(max((int)(tiles / fmaxf(want - 0.5f * units, 0.25f * want)) + 1, LEAST), (longest + MAX_SPLIT - 1) / MAX_SPLIT);
         if (!a.most) per = max(longest, 1);
         per = __builtin_amdgcn_readfirstlane(per);
         total = 0;
         if (rows > (float)a.b.N * 1.0001f) return; /* sequences that overlap: no batch */
         for (;;) { /* parts as long as their records and counters need; ends at one part a unit */
-            float recs = 0, units = 0;
+            float recs = 0;
+            units = 0;
             for (int c = 0; c < a.b.S; c += 64) {
                 const Sums m = own(chunk(c));
                 recs += (float)m.recs;
@@ -347,21 +373,21 @@ __device__ __forceinline__ void store4(const PaArgs& a, size_t row, int d, const
 /* ---------------------------------------------------------------- the kernel */
 
 template <bool BF16, int HDP>
-__global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaArgs a) {
-    typedef Tile<BF16, HDP> T;
-    constexpr int TERMS = T::TERMS, KT = T::KT, KB = T::KB, CPR = T::CPR, PLANE = T::PLANE;
+__global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) void k_attn_paged(PaArgs a) {
+#ifdef __HIP_DEVICE_COMPILE__ /* buffer descriptors are no type of the host's, which then leaves the kernel's entry out */
+    typedef Shape<BF16, HDP> W;
+    constexpr int NT = W::NT, NW = W::NW, ROWS = W::ROWS, TERMS = BF16 ? 1 : 3;
     constexpr int STEPS = HDP / 16, DT = HDP / 32; /* of the first product's sum; tiles of the output's dimensions */
-    constexpr int RPI = 1024 / T::ROWB, NI = PLANE / 1024 / NW; /* rows of a wave's load into LDS, loads of keys a wave */
     /* a ring of four arrays, not one array: reads of one then wait for no load into another */
-    constexpr int RING = BF16 ? T::BYTES : 16;
-    __shared__ __attribute__((aligned(16))) unsigned char lds0[T::BYTES], lds1[RING], lds2[RING], lds3[RING];
+    constexpr int REST = W::ARRAYS == 4 ? W::BYTES : 16;
+    __shared__ __attribute__((aligned(16))) unsigned char lds0[W::BYTES], lds1[REST], lds2[REST], lds3[REST];
     __shared__ float part_m[3][64], part_l[3][64];
     __shared__ int last_one;
     const PgBatch& b = a.b;
     const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
     const int col = lane & 31, half = lane >> 5;
     const int HD = b.HD, R = a.R;
-    const Plan<KT> plan(a);
+    const Plan<ROWS> plan(a);
 
     if (blockIdx.x >= plan.total) return;
     {
@@ -375,11 +401,11 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
         /* tiles of keys that some row of the unit sees, and this part's */
         const int lo = seen(a, p0 + tok0, it.len).first, hi = min(seen(a, p0 + tok1, it.len).last + 1, room);
         const int t0 = lo / KT, t1 = hi > lo ? (hi + KT - 1) / KT : t0;
-        const int kt0 = t0 + it.part * plan.per, kt1 = min(kt0 + plan.per, t1);
-        if (it.part && kt0 >= t1) return;
-        const bool whole = t1 - t0 <= plan.per; /* this part is all of them */
+        const int parts = max(1, (t1 - t0 + plan.per - 1) / plan.per), per = (t1 - t0 + parts - 1) / parts; /* as even as they go */
+        if (it.part >= parts) return;
+        const int kt0 = t0 + it.part * per, kt1 = min(kt0 + per, t1);
         /* waves side by side on rows, the rest in turns on the keys, 32 at a time */
-        const int groups = nrows <= 32 ? 1 : nrows <= 64 ? 2 : 4, kparts = NW / groups;
+        const int groups = nrows <= 32 ? 1 : nrows <= 64 ? 2 : NW, kparts = NW / groups;
         const int group = wave & (groups - 1), kpart = wave / groups;
         const bool active = 32 * group < nrows;
         const int r = r0 + 32 * group + col, tok = a.by_r.of(r), head = it.kh * R + (r - tok * R);
@@ -445,40 +471,69 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
             for (int e = 0; e < 16; e++) acc[d][e] = 0.0f;
         float m = -INFINITY, l = 0.0f; /* in powers of two, of the row; this lane's keys' sum */
 
-        /* 32 keys at k0, block kb of the tile in LDS at `buf`.  Reads are issued in groups ahead of the products that take
+        /* The tile of keys k0 .. k0 + 31, in LDS at `buf`.  Reads are issued in groups ahead of the products that take
          * them, the first of V's ahead of the softmax. */
-        constexpr int KG = BF16 ? 4 : 2, VG = BF16 ? 2 : 1;
-        auto block = [&](const unsigned char* buf, int kb, int k0) {
+        constexpr int KG = BF16 ? (HDP == 64 ? 2 : 4) : HDP == 256 ? 1 : 2, VG = BF16 && HDP != 64 ? 2 : 1;
+        auto block = [&](auto form, const unsigned char* buf, int k0) __attribute__((always_inline)) {
+            constexpr int FORM = decltype(form)::value, PLANES = Tile<FORM, HDP>::PLANES, PLANE = Tile<FORM, HDP>::PLANE;
+            constexpr int ROWB = Tile<FORM, HDP>::ROWB;
             f32x16 sc;
 #pragma unroll
             for (int e = 0; e < 16; e++) sc[e] = 0.0f;
-            bf16x8 kf[2][KG][TERMS];
+            typedef __attribute__((address_space(3))) s16x4 lds4;
+            bf16x8 kf[2][KG][PLANES];
+            f32x4 kw[2][KG][FORM == AS_F32 ? 2 : 1];
             auto read_k = [&](int g) {
+                const int row = col;
 #pragma unroll
-                for (int s = 0; s < KG; s++)
+                for (int s = 0; s < KG; s++) {
+                    const int at = g * KG + s;
+                    if constexpr (FORM == AS_F32) {
 #pragma unroll
-                    for (int x = 0; x < TERMS; x++) {
-                        const int row = 32 * kb + col;
-                        kf[g & 1][s][x] = *(const bf16x8*)(buf + x * PLANE + row * T::ROWB + 16 * k_place(row, 2 * (g * KG + s) + half));
+                        for (int i = 0; i < 2; i++)
+                            kw[g & 1][s][i] = *(const f32x4*)(buf + row * ROWB + 16 * k_place(row, 4 * at + 2 * half + i));
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < PLANES; x++)
+                            kf[g & 1][s][x] = *(const bf16x8*)(buf + x * PLANE + row * ROWB + 16 * k_place(row, 2 * at + half));
                     }
+                }
             };
-            /* dimension 32 d + col, keys 16 s + 4 half + 0 .. 3 and 8 more, of V's term x */
-            u32x4 vf[2][VG][TERMS][2];
+            /* dimension 32 d + col, keys 16 s + 4 half + 0 .. 3 and 8 more, of V */
+            u32x4 vf[2][VG][PLANES][2];
+            float vw[2][VG][2][FORM == AS_F32 ? 8 : 1];
             auto read_v = [&](int g) {
 #pragma unroll
                 for (int d = 0; d < VG; d++)
 #pragma unroll
-                    for (int x = 0; x < TERMS; x++)
+                    for (int s = 0; s < 2; s++) {
+                        if constexpr (FORM == AS_F32) {
+                            const int vr = 16 * s + 4 * half, dim = 32 * (g * VG + d) + col;
+                            const unsigned char* at = buf + PLANE + vr * ROWB + 16 * v_place<FORM>(vr, dim >> 2) + 4 * (dim & 3);
 #pragma unroll
-                        for (int s = 0; s < 2; s++) {
-                            const int vr = 32 * kb + 16 * s + 4 * half + ((lane & 15) >> 2);
+                            for (int e = 0; e < 8; e++) vw[g & 1][d][s][e] = *(const float*)(at + ((e & 3) + 2 * (e & 4)) * ROWB);
+                        } else {
+                            const int vr = 16 * s + 4 * half + ((lane & 15) >> 2);
                             const int dim = 32 * (g * VG + d) + (lane & 16) + 4 * (lane & 3);
-                            const unsigned char* at = buf + (TERMS + x) * PLANE + vr * T::ROWB + 16 * v_place(vr, dim >> 3) + 2 * (dim & 4);
-                            s16x4 y[2]; /* the second set lies 8 rows on, in the same place of its row */
-                            y[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lvoid*)at);
-                            y[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lvoid*)(at + 8 * T::ROWB));
-                            vf[g & 1][d][x][s] = __builtin_bit_cast(u32x4, y);
+#pragma unroll
+                            for (int x = 0; x < PLANES; x++) {
+                                const unsigned char* at = buf + (PLANES + x) * PLANE + vr * ROWB + 16 * v_place<FORM>(vr, dim >> 3) + 2 * (dim & 4);
+                                s16x4 y[2]; /* the second set lies 8 rows on, in the same place of its row */
+                                y[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(lvoid*)at);
+                                y[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(lvoid*)(at + 8 * ROWB));
+                                vf[g & 1][d][x][s] = __builtin_bit_cast(u32x4, y);
+                            }
                         }
+                    }
+            };
+            auto terms_of = [&](const float* w, u32x4* t) { /* eight values' three terms */
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    unsigned int z[3];
+                    split2(w[2 * e], w[2 * e + 1], z);
+#pragma unroll
+                    for (int x = 0; x < 3; x++) t[x][e] = z[x];
+                }
             };
             read_k(0);
 #pragma unroll
@@ -488,8 +543,19 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int s = 0; s < KG; s++) {
-                    const bf16x8* k = kf[g & 1][s];
                     const int at = g * KG + s;
+                    bf16x8 k[TERMS];
+                    if constexpr (FORM == AS_F32) {
+                        float w[8];
+                        u32x4 z[TERMS];
+                        __builtin_memcpy(w, kw[g & 1][s], 32);
+                        terms_of(w, z);
+#pragma unroll
+                        for (int x = 0; x < TERMS; x++) k[x] = __builtin_bit_cast(bf16x8, z[x]);
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < TERMS; x++) k[x] = kf[g & 1][s][x];
+                    }
                     if constexpr (!BF16) { /* the small terms first */
                         sc = mfma(k[2], qf[0][at], sc);
                         sc = mfma(k[0], qf[2][at], sc);
@@ -520,7 +586,8 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
             cm *= a.scale2; /* -infinity times 0 is NaN, which moves nothing */
             if (__any(cm > m + SLACK)) {
                 cm = fmaxf(cm, other_half(cm));
-                const float mn = fmaxf(m, cm), f = mn > -INFINITY ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+                /* of its own scores alone: what another row of the wave sees does not touch a row's roundings */
+                const float mn = cm > m + SLACK ? cm : m, f = mn > -INFINITY ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
                 l *= f;
 #pragma unroll
                 for (int d = 0; d < DT; d++) acc[d] *= f;
@@ -562,6 +629,21 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
             for (int g = 0; g < DT / VG; g++) {
                 if (g + 1 < DT / VG) read_v(g + 1);
                 __builtin_amdgcn_sched_barrier(0);
+                u32x4 v[VG][TERMS][2];
+#pragma unroll
+                for (int d = 0; d < VG; d++)
+#pragma unroll
+                    for (int s = 0; s < 2; s++) {
+                        u32x4 z[TERMS];
+                        if constexpr (FORM == AS_F32) {
+                            terms_of(vw[g & 1][d][s], z);
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < TERMS; x++) z[x] = vf[g & 1][d][x][s];
+                        }
+#pragma unroll
+                        for (int x = 0; x < TERMS; x++) v[d][x][s] = z[x];
+                    }
                 /* A value that is no number times a masked key's weight 0 would be NaN.  Where some row of the wave does not
                  * see one of the keys, such values are taken out, and the rows that do see one get NaN by a product of
                  * their own. */
@@ -572,7 +654,7 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
 #pragma unroll
                         for (int s = 0; s < 2; s++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++) odd |= no_numbers(vf[g & 1][d][0][s][e]);
+                            for (int e = 0; e < 4; e++) odd |= no_numbers(v[d][0][s][e]);
                     if (__builtin_expect(__any(odd != 0), 0)) {
                         u32x4 vis[2];
 #pragma unroll
@@ -592,10 +674,10 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
                                 u32x4 flag;
 #pragma unroll
                                 for (int e = 0; e < 4; e++) {
-                                    const unsigned int all = (no_numbers(vf[g & 1][d][0][s][e]) >> 15) * 0xffffu; /* the halves' bits */
+                                    const unsigned int all = (no_numbers(v[d][0][s][e]) >> 15) * 0xffffu; /* the halves' bits */
                                     flag[e] = all & 0x3f803f80u;
 #pragma unroll
-                                    for (int x = 0; x < TERMS; x++) vf[g & 1][d][x][s][e] &= ~all;
+                                    for (int x = 0; x < TERMS; x++) v[d][x][s][e] &= ~all;
                                 }
                                 hit = mfma(__builtin_bit_cast(bf16x8, flag), __builtin_bit_cast(bf16x8, vis[s]), hit);
                             }
@@ -609,66 +691,113 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
 #pragma unroll
                     for (int d = 0; d < VG; d++) {
                         f32x16& o = acc[g * VG + d];
-                        bf16x8 v[TERMS];
+                        bf16x8 y[TERMS];
 #pragma unroll
-                        for (int x = 0; x < TERMS; x++) v[x] = __builtin_bit_cast(bf16x8, vf[g & 1][d][x][s]);
+                        for (int x = 0; x < TERMS; x++) y[x] = __builtin_bit_cast(bf16x8, v[d][x][s]);
                         if constexpr (!BF16) {
-                            o = mfma(v[2], pf[0][s], o);
-                            o = mfma(v[0], pf[2][s], o);
-                            o = mfma(v[1], pf[1][s], o);
-                            o = mfma(v[1], pf[0][s], o);
-                            o = mfma(v[0], pf[1][s], o);
+                            o = mfma(y[2], pf[0][s], o);
+                            o = mfma(y[0], pf[2][s], o);
+                            o = mfma(y[1], pf[1][s], o);
+                            o = mfma(y[1], pf[0][s], o);
+                            o = mfma(y[0], pf[1][s], o);
                         }
-                        o = mfma(v[0], pf[0][s], o);
+                        o = mfma(y[0], pf[0][s], o);
                     }
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        auto compute = [&](const unsigned char* buf, int kt) {
-            if (!active) return;
-#pragma unroll
-            for (int kb = 0; kb < KB; kb++) {
-                const int k0 = kt * KT + 32 * kb;
-                if (((kt * KB + kb) & (kparts - 1)) == kpart && k0 <= any_last && k0 + 31 >= any_first && k0 < hi) block(buf, kb, k0);
-            }
+        auto compute = [&](auto form, const unsigned char* buf, int kt) __attribute__((always_inline)) {
+            const int k0 = kt * KT;
+            if (active && (kt & (kparts - 1)) == kpart && k0 <= any_last && k0 + 31 >= any_first && k0 < hi) block(form, buf, k0);
         };
 
-        if constexpr (BF16) {
-            /* Straight into LDS, 16 bytes a lane: load i of a wave fills rows (i NW + wave) RPI .. + RPI - 1, eight at most,
-             * which lie in one page.  Its number is read into a scalar register, apart from the loads' count, so that nothing
-             * waits for the tiles that are under way; what lies behind the load's rows or a head's end comes as zeros by the
-             * buffer's bounds, a missing page's keys from a row of NaN. */
-            int pg[NI];
+        /* Straight into LDS, 16 bytes a lane, a wave's load RPI rows, eight at most, which lie in one page.  Its number is read
+         * into a scalar register, apart from the loads' count, so that nothing waits for the tiles that are under way; what lies
+         * behind this part's keys or a head's end comes as zeros by the buffer's bounds, a missing page's keys from rows of
+         * NaN. */
+        constexpr int ESZ = BF16 ? 2 : 4;
+        typedef Tile<W::ALONE, HDP> T;
+        constexpr int RPI = T::RPI, CPR = T::CPR, PLANE = T::PLANE, KINDS = 8 / RPI;
+        const int end = min(hi, kt1 * KT), rowb = HD * ESZ;
+        const size_t page_bytes = (size_t)b.NKV * kv * (2 * ESZ), kh_bytes = (size_t)it.kh * kv * ESZ;
+        auto page_of = [&](int key) { /* key: a multiple of 8, or within them; wave-uniform */
+            return ((const __attribute__((address_space(4))) int*)table)[__builtin_amdgcn_readfirstlane(max(min(key, hi - 1), 0) >> b.shift)];
+        };
+        /* a lane's place in the rows of a load whose first row is `first` mod 8, of keys and of values */
+        auto lane_place = [&](int first, int& k, int& v) {
+            const int row = lane / CPR, place = lane % CPR;
+            const int kc = k_place(first + row, place), vc = v_place<W::ALONE>(first + row, place); /* their own inverses */
+            k = 16 * kc < rowb ? row * rowb + 16 * kc : 1 << 30;
+            v = 16 * vc < rowb ? row * rowb + 16 * vc : 1 << 30;
+        };
+        auto load = [&](int pg, int key, unsigned char* to, int k_off, int v_off) {
+            const bool there = (unsigned int)pg < (unsigned int)b.n_pages;
+            const int bytes = min(max(end - key, 0), RPI) * rowb;
+            const char* k = (const char*)a.cache + (there ? pg : 0) * page_bytes + kh_bytes + (unsigned int)((key & mask) * rowb);
+            const auto ks = __builtin_amdgcn_make_buffer_rsrc((void*)(there ? k : (const char*)pg_nans), 0, bytes, 0x00027000);
+            const auto vs = __builtin_amdgcn_make_buffer_rsrc((void*)(k + page_bytes / 2), 0, there ? bytes : 0, 0x00027000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ks, (lvoid*)to, 16, k_off, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(vs, (lvoid*)(to + PLANE), 16, v_off, 0, 0, 0);
+        };
+
+        if (!W::SHARED || groups == 1) {
+            /* Few rows: each wave goes over tiles of its own, one at a time, with no barrier; the other waves' loads are under
+             * way while it computes. */
+            unsigned char* buf;
+            if constexpr (W::ARRAYS == 4) buf = wave == 0 ? lds0 : wave == 1 ? lds1 : wave == 2 ? lds2 : lds3;
+            else buf = lds0 + wave * T::BYTES;
+            int k_off[KINDS], v_off[KINDS];
+#pragma unroll
+            for (int i = 0; i < KINDS; i++) lane_place(i * RPI, k_off[i], v_off[i]);
+            int pg[4]; /* of eight rows each */
             auto pages = [&](int kt) {
 #pragma unroll
-                for (int i = 0; i < NI; i++) {
-                    const int key = min(kt * KT + (i * NW + wave) * RPI, hi - 1);
-                    pg[i] = ((const __attribute__((address_space(4))) int*)table)[max(key, 0) >> b.shift];
-                }
+                for (int i = 0; i < 4; i++) pg[i] = page_of(kt * KT + 8 * i);
             };
-            int kv_off[2]; /* the lane's place in a load's rows of keys and of values */
-            static_assert(NW * RPI % 8 == 0, "the same for all of a wave's loads");
-            {
-                const int row = wave * RPI + lane / CPR, place = lane % CPR;
-                const int kc = k_place(row, place), vc = v_place(row, place); /* their own inverses */
-                kv_off[0] = 8 * kc < HD ? (lane / CPR) * HD * 2 + 16 * kc : 1 << 30;
-                kv_off[1] = 8 * vc < HD ? (lane / CPR) * HD * 2 + 16 * vc : 1 << 30;
+            auto request = [&](int kt) {
+                if constexpr (RPI == 1) { /* 32 descriptors at once spill scalar registers */
+#pragma unroll 1
+                    for (int g = 0; g < 4; g++) {
+                        const int key = kt * KT + 8 * g, p = page_of(key);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) load(p, key + i, buf + (8 * g + i) * 1024, k_off[i], v_off[i]);
+                    }
+                    return;
+                }
+#pragma unroll
+                for (int i = 0; i < KT / RPI; i++) load(pg[i * RPI / 8], kt * KT + i * RPI, buf + i * 1024, k_off[i % KINDS], v_off[i % KINDS]);
+            };
+            int kt = kt0 + ((kpart - kt0) & (kparts - 1)); /* tiles kpart mod kparts, as compute takes them */
+            pages(kt);
+            q_request();
+            if constexpr (!BF16 && HDP == 256) q_take(); /* no registers for both */
+            __builtin_amdgcn_sched_barrier(0);
+            request(kt);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (BF16 || HDP < 256) q_take();
+            for (; kt < kt1; kt += kparts) {
+                pages(kt + kparts);
+                __builtin_amdgcn_s_waitcnt(0x0F70); /* vmcnt(0) */
+                asm volatile("" ::: "memory");
+                compute(std::integral_constant<int, W::ALONE>{}, buf, kt);
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_sched_barrier(0);
+                if (kt + kparts < kt1) request(kt + kparts);
             }
-            const int end = min(hi, kt1 * KT);
-            const size_t page_bytes = (size_t)b.NKV * kv * 4, kh_bytes = (size_t)it.kh * kv * 2;
+            __builtin_amdgcn_s_waitcnt(0x0F70); /* none under way */
+        } else if constexpr (BF16) {
+            /* Load i of a wave fills rows (i NW + wave) RPI .. + RPI - 1. */
+            constexpr int NI = PLANE / 1024 / NW;
+            static_assert(NW % KINDS == 0, "a wave's loads begin at the same row of eight");
+            int k_off, v_off, pg[NI];
+            lane_place(wave * RPI & 7, k_off, v_off);
+            auto pages = [&](int kt) {
+#pragma unroll
+                for (int i = 0; i < NI; i++) pg[i] = page_of(kt * KT + (i * NW + wave) * RPI);
+            };
             auto request = [&](int kt, unsigned char* buf) {
 #pragma unroll
-                for (int i = 0; i < NI; i++) {
-                    const int key = kt * KT + (i * NW + wave) * RPI;
-                    const bool there = (unsigned int)pg[i] < (unsigned int)b.n_pages;
-                    const int bytes = min(max(end - key, 0), RPI) * HD * 2;
-                    const char* k = (const char*)a.cache + (there ? pg[i] : 0) * page_bytes + kh_bytes + (unsigned int)((key & mask) * HD * 2);
-                    const auto ks = __builtin_amdgcn_make_buffer_rsrc((void*)(there ? k : (const char*)pg_nans), 0, bytes, 0x00027000);
-                    const auto vs = __builtin_amdgcn_make_buffer_rsrc((void*)(k + page_bytes / 2), 0, there ? bytes : 0, 0x00027000);
-                    unsigned char* to = buf + (i * NW + wave) * 1024;
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(ks, (lvoid*)to, 16, kv_off[0], 0, 0, 0);
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(vs, (lvoid*)(to + PLANE), 16, kv_off[1], 0, 0, 0);
-                }
+                for (int i = 0; i < NI; i++) load(pg[i], kt * KT + (i * NW + wave) * RPI, buf + (i * NW + wave) * 1024, k_off, v_off);
             };
             pages(kt0);
             q_request();
@@ -684,12 +813,12 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
             /* Three tiles are under way while one is read; a tile's array is requested again behind the barrier that all
              * waves reach when they have read it.  Tiles behind the last are zeros. */
             constexpr int AHEAD = 4 * NI; /* loads of the two tiles after the one to be read */
-            auto step = [&](int kt, unsigned char* buf, unsigned char* before) {
+            auto step = [&](int kt, unsigned char* buf, unsigned char* before) __attribute__((always_inline)) {
                 __builtin_amdgcn_s_waitcnt(0x0F70 | (AHEAD & 15) | ((AHEAD >> 4) << 14));
                 barrier();
                 request(kt + 3, before);
                 pages(kt + 4);
-                compute(buf, kt);
+                compute(std::integral_constant<int, AS_BF16>{}, buf, kt);
             };
             for (int kt = kt0; kt < kt1; kt += 4) {
                 step(kt, lds0, lds3);
@@ -698,16 +827,17 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
                 if (kt + 3 < kt1) step(kt + 3, lds3, lds2);
             }
             __builtin_amdgcn_s_waitcnt(0x0F70); /* none under way */
-        } else {
-            /* through registers: thread's part i of a tile is chunk c = x % CPR of row x / CPR, x = i NT + t: eight values
-             * of keys and of values, split into their terms on the way into LDS */
-            constexpr int PER = KT * CPR / NT;
-            static_assert(KT * CPR % NT == 0, "whole parts");
+        } else if constexpr (W::SHARED) {
+            /* Through registers: thread's part i of a tile is eight values, chunk c = x % C3 of row x / C3, x = i NT + t, of keys
+             * and of values, split into their terms on the way into LDS, two tiles in turn. */
+            typedef Tile<TERMS3, HDP> T3;
+            constexpr int C3 = T3::CPR, PER = KT * C3 / NT;
+            static_assert(KT * C3 % NT == 0 && 2 * T3::BYTES <= W::BYTES, "whole parts, two tiles");
             f32x4 kr[PER][2], vr[PER][2];
             auto fetch = [&](int kt) {
 #pragma unroll
                 for (int i = 0; i < PER; i++) {
-                    const int x = i * NT + t, row = x / CPR, c = x % CPR, key = kt * KT + row;
+                    const int x = i * NT + t, row = x / C3, c = x % C3, key = kt * KT + row;
                     int pg = -2;
                     if (key < hi) {
                         pg = table[key >> b.shift];
@@ -728,16 +858,16 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
             auto put = [&](unsigned char* buf) {
 #pragma unroll
                 for (int i = 0; i < PER; i++) {
-                    const int x = i * NT + t, row = x / CPR, c = x % CPR;
+                    const int x = i * NT + t, row = x / C3, c = x % C3;
 #pragma unroll
                     for (int part = 0; part < 2; part++) {
                         const f32x4* src = part ? vr[i] : kr[i];
                         unsigned int z[4][3];
 #pragma unroll
                         for (int e = 0; e < 4; e++) split2(src[e >> 1][2 * (e & 1)], src[e >> 1][2 * (e & 1) + 1], z[e]);
-                        unsigned char* to = buf + part * TERMS * PLANE + row * T::ROWB + 16 * (part ? v_place(row, c) : k_place(row, c));
+                        unsigned char* to = buf + part * 3 * T3::PLANE + row * T3::ROWB + 16 * (part ? v_place<TERMS3>(row, c) : k_place(row, c));
 #pragma unroll
-                        for (int y = 0; y < TERMS; y++) *(u32x4*)(to + y * PLANE) = u32x4{z[0][y], z[1][y], z[2][y], z[3][y]};
+                        for (int y = 0; y < 3; y++) *(u32x4*)(to + y * T3::PLANE) = u32x4{z[0][y], z[1][y], z[2][y], z[3][y]};
                     }
                 }
             };
@@ -745,11 +875,11 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
             if (kt0 < kt1) fetch(kt0);
             q_take();
             for (int kt = kt0; kt < kt1; kt++) {
-                __syncthreads(); /* the tile before has been read */
-                put(lds0);
-                __syncthreads();
+                unsigned char* buf = lds0 + ((kt - kt0) & 1) * T3::BYTES;
+                put(buf);
+                __syncthreads(); /* the tile is there, and the one before has been read */
                 if (kt + 1 < kt1) fetch(kt + 1);
-                compute(lds0, kt);
+                compute(std::integral_constant<int, TERMS3>{}, buf, kt);
             }
         }
         l += other_half(l);
@@ -757,24 +887,28 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
         /* the waves' parts of the keys, joined in the first one's registers */
         if (kparts > 1) {
             const int at = (kpart - 1) * groups + group; /* 0 .. 2 */
-            auto place = [&](int i) { return (float*)(BF16 ? i == 0 ? lds0 : i == 1 ? lds1 : lds2 : lds0 + i * (HDP * 128)) + lane; };
-            static_assert(BF16 ? HDP * 128 <= T::BYTES : 3 * HDP * 128 <= T::BYTES, "a wave's sums in an array");
+            /* up to three waves' sums at 16-byte places of the lanes */
+            constexpr int SUMS = HDP * 128;
+            static_assert(W::ARRAYS == 4 ? SUMS <= W::BYTES : (NW - 1) * SUMS <= W::BYTES, "");
+            auto place = [&](int i) {
+                return (f32x4*)(W::ARRAYS == 1 ? lds0 + i * SUMS : i == 0 ? lds0 : i == 1 ? lds1 : lds2) + lane;
+            };
             __syncthreads();
             if (active && kpart) {
-                float* mem = place(at);
+                f32x4* mem = place(at);
                 part_m[at][lane] = m;
                 part_l[at][lane] = l;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) mem[(16 * d + e) * 64] = acc[d][e];
+                    for (int e = 0; e < 4; e++) mem[(4 * d + e) * 64] = f32x4{acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2], acc[d][4 * e + 3]};
             }
             __syncthreads();
             if (active && !kpart) {
                 for (int k = 1; k < kparts; k++) {
                     /* a part without a finite score has what its scores left there: 0, or NaN */
                     const int i = (k - 1) * groups + group;
-                    const float* mem = place(i);
+                    const f32x4* mem = place(i);
                     const float m1 = part_m[i][lane], mx = fmaxf(m, m1);
                     const float f0 = m > -INFINITY ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
                     const float f1 = m1 > -INFINITY ? __builtin_amdgcn_exp2f(m1 - mx) : 1.0f;
@@ -782,13 +916,17 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
 #pragma unroll
                     for (int d = 0; d < DT; d++)
 #pragma unroll
-                        for (int e = 0; e < 16; e++) acc[d][e] = acc[d][e] * f0 + mem[(16 * d + e) * 64] * f1;
+                        for (int e = 0; e < 4; e++) {
+                            const f32x4 x = mem[(4 * d + e) * 64];
+#pragma unroll
+                            for (int j = 0; j < 4; j++) acc[d][4 * e + j] = acc[d][4 * e + j] * f0 + x[j] * f1;
+                        }
                     m = mx;
                 }
             }
         }
         const bool writes = active && kpart == 0 && mine;
-        if (whole) {
+        if (parts == 1) {
             if (writes) {
                 const size_t row = (size_t)(n0 + tok) * a.ldo + (size_t)head * HD;
                 const bool none = sn.last < sn.first, gone = sn.last >= room;
@@ -809,7 +947,6 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
          * waits for its stores before the barrier, so a part is counted only after its record has arrived.  A unit's
          * records: [part][row]{HDP values, maximum, sum}, from the unit's rows and KV heads before it. */
         constexpr int REC = HDP + 2;
-        const int parts = (t1 - t0 + plan.per - 1) / plan.per; /* with keys */
         float* recs = a.rec + ((size_t)it.rec + (size_t)it.parts * ((size_t)rows_all * it.kh + r0)) * REC;
         if (writes) {
             float* rec = recs + ((size_t)it.part * nrows + (r - r0)) * REC;
@@ -834,18 +971,23 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
         }
         __syncthreads();
         if (!last_one) return;
-        /* each output from its records, 8 of them read at once */
-        for (int x = t; x < nrows * (HD / 4); x += NT) {
-            const int row = x / (HD / 4), dim = 4 * (x - row * (HD / 4));
+        /* Each four outputs from their records, by as many lanes as there are for them (up to 64, side by side), each lane
+         * reading 8 records at once. */
+        const int outs = nrows * (HD / 4);
+        int by_log = 0;
+        while (by_log < 6 && outs << (by_log + 1) <= NT && 4 << by_log < parts) by_log++;
+        for (int x0 = 0; x0 < outs; x0 += NT >> by_log) {
+            const int x = x0 + (t >> by_log), row = min(x, outs - 1) / (HD / 4), dim = 4 * (min(x, outs - 1) - row * (HD / 4));
             float o[4] = {0, 0, 0, 0}, mx = -INFINITY, sum = 0.0f;
-            for (int i = 0; i < parts; i += 8) {
+            for (int i = t & ((1 << by_log) - 1); i < parts; i += 8 << by_log) {
                 f32x2 y[8][3];
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const float* rec = recs + ((size_t)(i + e) * nrows + row) * REC;
+                    const int part = i + (e << by_log);
+                    const float* rec = recs + ((size_t)part * nrows + row) * REC;
                     y[e][0] = y[e][1] = f32x2{0, 0};
                     y[e][2] = f32x2{-INFINITY, 0};
-                    if (i + e >= parts) continue;
+                    if (part >= parts) continue;
                     y[e][2] = agent_load2(rec + HDP);
                     y[e][0] = agent_load2(rec + dim);
                     y[e][1] = agent_load2(rec + dim + 2);
@@ -866,6 +1008,16 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
                 }
                 mx = mn;
             }
+            for (int k = 0; k < by_log; k++) {
+                const float m1 = __shfl_xor(mx, 1 << k), mn = fmaxf(mx, m1);
+                const float f = mx > -INFINITY ? __builtin_amdgcn_exp2f(mx - mn) : 1.0f;
+                const float g = m1 > -INFINITY ? __builtin_amdgcn_exp2f(m1 - mn) : 1.0f;
+                sum = sum * f + __shfl_xor(sum, 1 << k) * g;
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[j] = o[j] * f + __shfl_xor(o[j], 1 << k) * g;
+                mx = mn;
+            }
+            if (x >= outs || (t & ((1 << by_log) - 1))) continue;
             const int rr = r0 + row, rtok = a.by_r.of(rr);
             const Seen s = seen(a, p0 + rtok, it.len);
             const bool none = s.last < s.first, gone = s.last >= room;
@@ -874,22 +1026,24 @@ __global__ __launch_bounds__(NT, (Tile<BF16, HDP>::WAVES)) void k_attn_paged(PaA
             store4<BF16>(a, (size_t)(n0 + rtok) * a.ldo + (size_t)(it.kh * R + rr - rtok * R) * HD, dim, o);
         }
     }
+#endif
 }
 
 template <bool BF16, int HDP>
 int start(PaArgs& a, const bmk_launch_t* l) {
-    constexpr int KT = Tile<BF16, HDP>::KT;
+    typedef Shape<BF16, HDP> W;
     a.most = 0;
     if (l->scratch_bytes > DONE_BYTES)
         a.most = (unsigned int)std::min<size_t>((l->scratch_bytes - DONE_BYTES) / ((HDP + 2) * 4), 1u << 30);
     a.done = (unsigned int*)l->scratch;
     a.rec = (float*)((char*)l->scratch + DONE_BYTES);
-    /* A workgroup a piece: no more than a unit for every sequence with new tokens and every ROWS rows, and WANTED (the 8:
-     * sums rounded in fp32). */
-    const int64_t units = a.b.NKV * (std::min<int64_t>(a.b.N, a.b.S) + (int64_t)a.b.N * a.R / ROWS);
+    a.slots = W::SLOTS;
+    /* A workgroup a piece: no more than a unit for every sequence with new tokens and every ROWS rows, each in one part more
+     * than the tiles' share (units / 2 taken off that: the plan's want; the 8: sums rounded in fp32). */
+    const int64_t units = a.b.NKV * (std::min<int64_t>(a.b.N, a.b.S) + (int64_t)a.b.N * a.R / W::ROWS);
     const int64_t tiles = std::min<int64_t>((a.b.room() + KT - 1) / KT, MAX_SPLIT);
-    const int64_t grid = std::min(units * tiles, units + WANTED + 8);
-    hipLaunchKernelGGL((k_attn_paged<BF16, HDP>), dim3((unsigned)grid), dim3(NT), 0, l->stream, a);
+    const int64_t grid = std::min(units * tiles, units + a.slots * ROUNDS + 8);
+    hipLaunchKernelGGL((k_attn_paged<BF16, HDP>), dim3((unsigned)grid), dim3(W::NT), 0, l->stream, a);
     BMK_LAUNCH_CHECK();
     return 0;
 }
