@@ -164,6 +164,13 @@ __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
+/* of all lanes alike: in scalar registers, where a descriptor has to be (the compiler loops over the lanes' descriptors otherwise) */
+__device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ const char* scalar(const char* p) {
+    const unsigned long long u = (unsigned long long)p;
+    return (const char*)((unsigned long long)(unsigned int)scalar((int)(u >> 32)) << 32 | (unsigned int)scalar((int)u));
+}
+
 /* all waves of the workgroup; memory accesses stay on their side of it */
 __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
@@ -473,7 +480,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
 
         /* The tile of keys k0 .. k0 + 31, in LDS at `buf`.  Reads are issued in groups ahead of the products that take
          * them, the first of V's ahead of the softmax. */
-        constexpr int KG = BF16 ? (HDP == 64 ? 2 : 4) : HDP == 256 ? 1 : 2, VG = BF16 && HDP != 64 ? 2 : 1;
+        constexpr int KG = !BF16 && HDP == 256 ? 1 : 2, VG = BF16 && HDP != 64 ? 2 : 1;
         auto block = [&](auto form, const unsigned char* buf, int k0) __attribute__((always_inline)) {
             constexpr int FORM = decltype(form)::value, PLANES = Tile<FORM, HDP>::PLANES, PLANE = Tile<FORM, HDP>::PLANE;
             constexpr int ROWB = Tile<FORM, HDP>::ROWB;
@@ -734,8 +741,8 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
             const bool there = (unsigned int)pg < (unsigned int)b.n_pages;
             const int bytes = min(max(end - key, 0), RPI) * rowb;
             const char* k = (const char*)a.cache + (there ? pg : 0) * page_bytes + kh_bytes + (unsigned int)((key & mask) * rowb);
-            const auto ks = __builtin_amdgcn_make_buffer_rsrc((void*)(there ? k : (const char*)pg_nans), 0, bytes, 0x00027000);
-            const auto vs = __builtin_amdgcn_make_buffer_rsrc((void*)(k + page_bytes / 2), 0, there ? bytes : 0, 0x00027000);
+            const auto ks = __builtin_amdgcn_make_buffer_rsrc((void*)scalar(there ? k : (const char*)pg_nans), 0, scalar(bytes), 0x00027000);
+            const auto vs = __builtin_amdgcn_make_buffer_rsrc((void*)scalar(k + page_bytes / 2), 0, scalar(there ? bytes : 0), 0x00027000);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(ks, (lvoid*)to, 16, k_off, 0, 0, 0);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(vs, (lvoid*)(to + PLANE), 16, v_off, 0, 0, 0);
         };
@@ -1039,10 +1046,11 @@ int start(PaArgs& a, const bmk_launch_t* l) {
     a.rec = (float*)((char*)l->scratch + DONE_BYTES);
     a.slots = W::SLOTS;
     /* A workgroup a piece: no more than a unit for every sequence with new tokens and every ROWS rows, each in one part more
-     * than the tiles' share (units / 2 taken off that: the plan's want; the 8: sums rounded in fp32). */
+     * than the tiles' share of the plan's want (the 8: sums rounded in fp32). */
     const int64_t units = a.b.NKV * (std::min<int64_t>(a.b.N, a.b.S) + (int64_t)a.b.N * a.R / W::ROWS);
-    const int64_t tiles = std::min<int64_t>((a.b.room() + KT - 1) / KT, MAX_SPLIT);
-    const int64_t grid = std::min(units * tiles, units + a.slots * ROUNDS + 8);
+    const int64_t tiles = (a.b.room() + KT - 1) / KT;
+    const double rounds = std::min(std::max((double)units * tiles / ((double)a.slots * ROUND_TILES), 1.0), (double)ROUNDS);
+    const int64_t grid = std::min(units * std::min<int64_t>(tiles, MAX_SPLIT), units + (int64_t)(a.slots * rounds) + 8);
     hipLaunchKernelGGL((k_attn_paged<BF16, HDP>), dim3((unsigned)grid), dim3(W::NT), 0, l->stream, a);
     BMK_LAUNCH_CHECK();
     return 0;
