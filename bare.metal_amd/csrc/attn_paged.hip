@@ -55,18 +55,6 @@ constexpr int CUS = 256, ROUNDS = 4, ROUND_TILES = 32;
 constexpr int DONE_STRIDE = 32, MAX_UNITS = 1024;
 constexpr size_t DONE_BYTES = (size_t)DONE_STRIDE * MAX_UNITS * 4;
 
-/* x / d for x below 2^31 by one product */
-struct Div {
-    unsigned int d, mul, shift;
-    __device__ __forceinline__ int of(int x) const { return (int)((__umulhi((unsigned int)x, mul) + (unsigned int)x) >> shift); }
-};
-Div div_by(int d) {
-    Div v = {(unsigned int)d, 0, 0};
-    while ((1ull << v.shift) < (unsigned int)d) v.shift++;
-    v.mul = (unsigned int)(((1ull << 32) * ((1ull << v.shift) - d)) / d + 1);
-    return v;
-}
-
 struct PaArgs {
     const void* q;
     const void* cache;

@@ -14,6 +14,18 @@ namespace bmk {
 constexpr int PG_MAX_DIM = 1 << 30;
 constexpr int PG_MAX_HD = 256, PG_MAX_SEQS = 1 << 20;
 
+/* x / d for x below 2^31 by one product */
+struct Div {
+    unsigned int d, mul, shift;
+    __device__ __forceinline__ int of(int x) const { return (int)((__umulhi((unsigned int)x, mul) + (unsigned int)x) >> shift); }
+};
+inline Div div_by(int d) {
+    Div v = {(unsigned int)d, 0, 0};
+    while ((1ull << v.shift) < (unsigned int)d) v.shift++;
+    v.mul = (unsigned int)(((1ull << 32) * ((1ull << v.shift) - d)) / d + 1);
+    return v;
+}
+
 /* The batch's tables and the cache's shape. */
 struct PgBatch {
     const int* start; /* [S + 1] */

@@ -5,18 +5,21 @@
  *   rope_forward_rows     out = turn(x, pos)
  *   qk_norm_rope_forward  out = turn(x / sqrt(mean x^2 + eps) * gain, pos)
  *   kv_append_paged       q out = turn([norm] q), cache = turn([norm] k), v
- * One kernel: a group of LP lanes takes one head of one row (an item), a lane
+ * One kernel: a group of lanes takes one head of one row (an item), a lane
  * two chunks of E elements, which hold whole rotation pairs, so nothing but
  * the norm's sum passes between lanes, and a lane stores what it loaded (an
  * output may be its input's buffer).
  */
 #include "paged.h"
 
+#include <algorithm>
+
 namespace {
 
 using namespace bmk;
 
 constexpr int NT = 256;
+constexpr int MAX_TURNS = 2048, MAX_ROWS = 256; /* pairs and rows of a workgroup */
 
 struct RopeArgs {
     const void *q, *k, *v;
@@ -30,7 +33,9 @@ struct RopeArgs {
     int rot, pairs;
     int units, lp_log; /* lanes with work in a group, log2 of its lanes */
     size_t ldq, ldk, ldv, ldqo, ldko;
-    unsigned int items;
+    int per; /* rows of a workgroup */
+    Div by_heads, by_half;
+    double by_hd; /* 1 / HD */
     float mscale, eps;
 };
 
@@ -43,15 +48,15 @@ template <bool BF16, int E> struct alignas(E * (BF16 ? 2 : 4)) Chunk {
 };
 
 template <bool BF16, int E>
-__device__ __forceinline__ void load(const void* p, size_t i, float* x) {
-    const Chunk<BF16, E> c = *(const Chunk<BF16, E>*)((const char*)p + i * (BF16 ? 2 : 4));
+__device__ __forceinline__ float value(const Chunk<BF16, E>& c, int e) {
     if constexpr (BF16) {
         unsigned short u[E];
         __builtin_memcpy(u, &c, sizeof c);
-#pragma unroll
-        for (int e = 0; e < E; e++) x[e] = __uint_as_float((unsigned int)u[e] << 16);
+        return __uint_as_float((unsigned int)u[e] << 16);
     } else {
+        float x[E];
         __builtin_memcpy(x, &c, sizeof c);
+        return x[e];
     }
 }
 
@@ -88,114 +93,175 @@ __device__ __forceinline__ void cos_sin(unsigned int t, float* c, float* s) {
     *s = quarter >= 2 ? -b : b;
 }
 
-/* UN: units a lane takes at most */
-template <bool BF16, int E, int UN>
+/* Sum over 2^k neighbouring lanes, which all get it: up to 16 by moves inside a row of lanes. */
+template <int CTRL>
+__device__ __forceinline__ double lanes_add(double v) {
+    const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+    const unsigned int lo = (unsigned int)__builtin_amdgcn_update_dpp(0, (int)(unsigned int)u, CTRL, 0xF, 0xF, false);
+    const unsigned int hi = (unsigned int)__builtin_amdgcn_update_dpp(0, (int)(unsigned int)(u >> 32), CTRL, 0xF, 0xF, false);
+    return v + __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ double group_sum(double v, int lanes) {
+    if (lanes > 1) v = lanes_add<0xB1>(v);  /* lane ^ 1 */
+    if (lanes > 2) v = lanes_add<0x4E>(v);  /* lane ^ 2 */
+    if (lanes > 4) v = lanes_add<0x141>(v); /* the other four of eight */
+    if (lanes > 8) v = lanes_add<0x140>(v); /* the other eight of sixteen */
+    if (lanes > 16) v += __shfl_xor(v, 16);
+    if (lanes > 32) v += __shfl_xor(v, 32);
+    return v;
+}
+/* 1 / sqrt(m), of the instruction's 23 bits by one Newton step; 0 of infinity */
+__device__ __forceinline__ double root_inverse(double m) {
+    const double r = __builtin_amdgcn_rsq(m);
+    return m == INFINITY ? 0.0 : fma(r * 0.5, fma(-m * r, r, 1.0), r);
+}
+
+/* A workgroup takes `per` rows: their positions, places and (cos, sin) go to LDS once, the heads to groups of 1 << lp_log
+ * lanes in turn, AHEAD of them loaded at once.  UN: units a lane takes at most. */
+template <bool BF16, int E, int UN, bool PAIRS>
 __global__ __launch_bounds__(NT) void k_rope_rows(RopeArgs a) {
-    const unsigned int lane = threadIdx.x & ((1u << a.lp_log) - 1);
-    const unsigned int item = (blockIdx.x * (unsigned int)NT + threadIdx.x) >> a.lp_log;
-    if (item >= a.items) return; /* whole groups */
-    const int n = (int)(item / (unsigned int)a.heads);
-    int h = (int)(item - (unsigned int)n * (unsigned int)a.heads);
-    int p;
-    size_t place = 0; /* of the row in the cache, KV head 0's keys */
-    bool kept = false;
-    if (a.pos) {
-        p = a.pos[n];
-    } else {
-        const int s = a.b.seq_of(n);
-        if (s < 0) return;
-        p = a.b.pos_of(s, n);
-        const int pg = a.b.page_of(s, p);
-        kept = pg >= 0;
-        if (kept) place = a.b.base(pg, 0, 0) + (size_t)(p & ((1 << a.b.shift) - 1)) * a.b.HD;
-    }
-    const int HD = a.b.HD;
+    constexpr int AHEAD = UN == 1 ? 4 : 2;
+    __shared__ __attribute__((aligned(16))) float tc[MAX_TURNS], ts[MAX_TURNS];
+    __shared__ size_t places[MAX_ROWS];
+    __shared__ int where[MAX_ROWS]; /* bit 0: a row of the batch, bit 1: with a place in the cache */
+    const int t = threadIdx.x, lanes = 1 << a.lp_log, lane = t & (lanes - 1), slot = t >> a.lp_log, slots = NT >> a.lp_log;
+    const int HD = a.b.HD, half = a.rot / 2;
+    const int n0 = (int)blockIdx.x * a.per, rows = min(a.per, a.b.N - n0), items = rows * a.heads;
     const size_t plane = (size_t)HD << a.b.shift; /* of one KV head's part of a page */
-    const void* src;
-    void* dst;
-    size_t from, to;
-    bool turned = true;
-    const float* gain = a.gain;
-    if (h < a.NH) {
-        src = a.q;
-        dst = a.qo;
-        from = (size_t)n * a.ldq + (size_t)h * HD;
-        to = (size_t)n * a.ldqo + (size_t)h * HD;
-    } else if (h < a.NH + a.NK) {
-        h -= a.NH;
-        if (gain) gain += HD;
-        src = a.k;
-        from = (size_t)n * a.ldk + (size_t)h * HD;
-        dst = a.ko ? a.ko : a.cache;
-        to = a.ko ? (size_t)n * a.ldko + (size_t)h * HD : place + h * plane;
-        if (!a.ko && !kept) return;
-    } else {
-        h -= a.NH + a.NK;
-        gain = nullptr;
-        turned = false;
-        src = a.v;
-        from = (size_t)n * a.ldv + (size_t)h * HD;
-        dst = a.cache;
-        to = place + (a.b.NKV + h) * plane;
-        if (!kept) return;
-    }
-    /* unit u's chunks: in the turned part by halves E u and rot/2 + E u, else 2 E u and the next */
-    const int halves = a.pairs ? 0 : a.rot / (2 * E); /* units that lie so */
-    float x[UN][2][E];
-    int at[UN][2];
-#pragma unroll
-    for (int i = 0; i < UN; i++) {
-        const int u = (int)lane + (i << a.lp_log);
-        at[i][0] = u < halves ? E * u : 2 * E * u;
-        at[i][1] = u < halves ? a.rot / 2 + E * u : 2 * E * u + E;
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            if (u < a.units) load<BF16, E>(src, from + at[i][j], x[i][j]);
-            else
-#pragma unroll
-                for (int e = 0; e < E; e++) x[i][j][e] = 0.0f;
+    const int halves = PAIRS ? 0 : a.rot / (2 * E); /* units whose chunks lie half of the turned part apart */
+
+    struct Item {
+        int row, kind, h; /* kind: 0 q, 1 k, 2 v; -1: none */
+    };
+    auto item = [&](int x) {
+        Item it = {0, -1, 0};
+        if (x < items) {
+            it.row = a.by_heads.of(x);
+            it.h = x - it.row * a.heads;
+            it.kind = it.h < a.NH ? 0 : it.h < a.NH + a.NK ? 1 : 2;
+            it.h -= it.kind == 0 ? 0 : it.kind == 1 ? a.NH : a.NH + a.NK;
         }
-    }
-    if (gain) { /* squares and their sum in 64 bits: heads past 2^64 or under 2^-64 need no care */
-        double sum = 0;
+        return it;
+    };
+    auto at = [&](int i, int j) { /* of the lane's unit i, chunk j: its place in a head */
+        const int u = lane + (i << a.lp_log);
+        return u < halves ? E * u + (j ? half : 0) : 2 * E * u + (j ? E : 0);
+    };
+    Chunk<BF16, E> raw[AHEAD][UN][2];
+    auto fetch = [&](int k, const Item& it) {
+        if (it.kind < 0) return;
+        const void* src = it.kind == 0 ? a.q : it.kind == 1 ? a.k : a.v;
+        const size_t from = (size_t)(n0 + it.row) * (it.kind == 0 ? a.ldq : it.kind == 1 ? a.ldk : a.ldv) + (size_t)it.h * HD;
 #pragma unroll
         for (int i = 0; i < UN; i++)
 #pragma unroll
             for (int j = 0; j < 2; j++)
+                if (lane + (i << a.lp_log) < a.units) raw[k][i][j] = *(const Chunk<BF16, E>*)((const char*)src + (from + at(i, j)) * (BF16 ? 2 : 4));
+    };
+    Item its[AHEAD];
 #pragma unroll
-                for (int e = 0; e < E; e++) sum = fma((double)x[i][j][e], (double)x[i][j][e], sum);
-        for (int o = 1; o < 1 << a.lp_log; o <<= 1) sum += __shfl_xor(sum, o);
-        const double inv = 1.0 / sqrt(sum / HD + (double)a.eps);
-#pragma unroll
-        for (int i = 0; i < UN; i++)
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int e = 0; e < E; e++)
-                    if ((int)lane + (i << a.lp_log) < a.units)
-                        x[i][j][e] = (float)((double)x[i][j][e] * inv) * gain[at[i][j] + e];
+    for (int k = 0; k < AHEAD; k++) {
+        its[k] = item(slot + k * slots);
+        fetch(k, its[k]);
     }
-#pragma unroll
-    for (int i = 0; i < UN; i++) {
-        const int u = (int)lane + (i << a.lp_log);
-        if (u >= a.units) continue;
-        if (turned && 2 * E * u < a.rot) {
-#pragma unroll
-            for (int e = 0; e < E; e++) { /* pair E u + e: element e of both chunks, or neighbours along them */
-                const unsigned long long t = (unsigned long long)(long long)p * a.turns[E * u + e];
-                float c, s;
-                cos_sin((unsigned int)(t >> 32), &c, &s);
-                c *= a.mscale;
-                s *= a.mscale;
-                float &x0 = a.pairs ? x[i][2 * e / E][2 * e % E] : x[i][0][e];
-                float &x1 = a.pairs ? x[i][(2 * e + 1) / E][(2 * e + 1) % E] : x[i][1][e];
-                const float y0 = x0 * c - x1 * s, y1 = x0 * s + x1 * c;
-                x0 = y0;
-                x1 = y1;
+
+    /* position of each row for its pairs, and (once) its place */
+    for (int x = t; x < rows * max(half, 1); x += NT) {
+        const int row = half ? a.by_half.of(x) : x, pair = x - row * half, n = n0 + row;
+        int p, in = 1;
+        if (a.pos) {
+            p = a.pos[n];
+        } else {
+            const int s = a.b.seq_of(n);
+            in = s >= 0;
+            p = in ? a.b.pos_of(s, n) : 0;
+            if (half == 0 || pair == 0) {
+                const int pg = in ? a.b.page_of(s, p) : -1;
+                places[row] = pg >= 0 ? a.b.base(pg, 0, 0) + (size_t)(p & ((1 << a.b.shift) - 1)) * HD : 0;
+                in |= pg >= 0 ? 2 : 0;
             }
         }
+        if (half == 0 || pair == 0) where[row] = in;
+        if (half) {
+            const unsigned long long turn = (unsigned long long)(long long)p * a.turns[pair];
+            float c, s;
+            cos_sin((unsigned int)(turn >> 32), &c, &s);
+            tc[x] = c * a.mscale;
+            ts[x] = s * a.mscale;
+        }
+    }
+    __syncthreads();
+
+    for (int x0 = slot; x0 < items; x0 += AHEAD * slots) {
 #pragma unroll
-        for (int j = 0; j < 2; j++) store<BF16, E>(dst, to + at[i][j], x[i][j]);
+        for (int k = 0; k < AHEAD; k++) {
+            const Item it = its[k];
+            if (it.kind < 0) continue;
+            const int flags = where[it.row];
+            const bool cached = it.kind == 2 || (it.kind == 1 && !a.ko);
+            if (!(flags & 1) || (cached && !(flags & 2))) continue;
+            void* dst = it.kind == 0 ? a.qo : cached ? a.cache : a.ko;
+            const size_t to = it.kind == 0 ? (size_t)(n0 + it.row) * a.ldqo + (size_t)it.h * HD
+                              : !cached    ? (size_t)(n0 + it.row) * a.ldko + (size_t)it.h * HD
+                                           : places[it.row] + (size_t)(it.h + (it.kind == 2 ? a.b.NKV : 0)) * plane;
+            float y[UN][2][E];
+#pragma unroll
+            for (int i = 0; i < UN; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int e = 0; e < E; e++) y[i][j][e] = lane + (i << a.lp_log) < a.units ? value<BF16, E>(raw[k][i][j], e) : 0.0f;
+            if (a.gain && it.kind < 2) { /* squares and their sum in 64 bits: heads past 2^64 or under 2^-64 need no care */
+                const float* gain = a.gain + (it.kind == 1 ? HD : 0);
+                double sum = 0;
+#pragma unroll
+                for (int i = 0; i < UN; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+#pragma unroll
+                        for (int e = 0; e < E; e++) sum = fma((double)y[i][j][e], (double)y[i][j][e], sum);
+                const double inv = root_inverse(group_sum(sum, lanes) * a.by_hd + (double)a.eps);
+                const float f = (float)inv;
+                const bool tiny = f < 0x1p-100f; /* the last bits of a factor under 2^-126 are not fp32's */
+#pragma unroll
+                for (int i = 0; i < UN; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+#pragma unroll
+                        for (int e = 0; e < E; e++)
+                            if (lane + (i << a.lp_log) < a.units)
+                                y[i][j][e] = (tiny ? (float)((double)y[i][j][e] * inv) : y[i][j][e] * f) * gain[at(i, j) + e];
+            }
+#pragma unroll
+            for (int i = 0; i < UN; i++) {
+                const int u = lane + (i << a.lp_log);
+                if (u >= a.units) continue;
+                if (it.kind < 2 && 2 * E * u < a.rot) {
+                    const float *c = tc + it.row * half + E * u, *s = ts + it.row * half + E * u;
+                    float cs[E], sn[E];
+                    __builtin_memcpy(cs, __builtin_assume_aligned(c, E * 4 < 16 ? E * 4 : 16), sizeof cs);
+                    __builtin_memcpy(sn, __builtin_assume_aligned(s, E * 4 < 16 ? E * 4 : 16), sizeof sn);
+#pragma unroll
+                    for (int e = 0; e < E; e++) { /* pair E u + e: element e of both chunks, or neighbours along them */
+                        float &x0 = PAIRS ? y[i][2 * e / E][2 * e % E] : y[i][0][e];
+                        float &x1 = PAIRS ? y[i][(2 * e + 1) / E][(2 * e + 1) % E] : y[i][1][e];
+                        /* spelt out, so that every form gives the same bits */
+                        const float y0 = fmaf(x0, cs[e], -(x1 * sn[e])), y1 = fmaf(x0, sn[e], x1 * cs[e]);
+                        x0 = y0;
+                        x1 = y1;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 2; j++) store<BF16, E>(dst, to + at(i, j), y[i][j]);
+            }
+        }
+        if (x0 + AHEAD * slots < items) {
+#pragma unroll
+            for (int k = 0; k < AHEAD; k++) {
+                its[k] = item(x0 + (AHEAD + k) * slots);
+                fetch(k, its[k]);
+            }
+        }
     }
 }
 
@@ -204,8 +270,18 @@ int launch(RopeArgs& a, hipStream_t stream) {
     a.units = a.b.HD / (2 * E);
     a.lp_log = 0;
     while ((UN << a.lp_log) < a.units) a.lp_log++;
-    const unsigned int per = NT >> a.lp_log;
-    hipLaunchKernelGGL((k_rope_rows<BF16, E, UN>), dim3((a.items + per - 1) / per), dim3(NT), 0, stream, a);
+    /* rows of a workgroup: as many as give its lanes one head each, or up to four where there are more workgroups than the
+     * chip holds (a row's cos and sin serve all its heads whatever that is) */
+    const int slots = NT >> a.lp_log, half = a.rot / 2;
+    const int least = std::max(1, slots / a.heads), most = std::max(1, 4 * slots / a.heads);
+    a.per = std::min(std::max(a.b.N / 1024, least), most);
+    a.per = std::min({a.per, MAX_ROWS, MAX_TURNS / std::max(half, 1)});
+    a.by_heads = div_by(a.heads);
+    a.by_half = div_by(std::max(half, 1));
+    a.by_hd = 1.0 / a.b.HD;
+    const dim3 grid((a.b.N + a.per - 1) / a.per);
+    if (a.pairs) hipLaunchKernelGGL((k_rope_rows<BF16, E, UN, true>), grid, dim3(NT), 0, stream, a);
+    else hipLaunchKernelGGL((k_rope_rows<BF16, E, UN, false>), grid, dim3(NT), 0, stream, a);
     BMK_LAUNCH_CHECK();
     return 0;
 }
@@ -223,8 +299,17 @@ int run(const bmk_launch_t* l, RopeArgs& a, bool bf16, int layout, int turns_at,
     BMK_REQUIRE((int64_t)a.b.N * a.heads < (1LL << 31), "%s: %d rows of %d heads are over 2^31 heads", what, a.b.N, a.heads);
     a.turns = (const unsigned long long*)l->dev[turns_at];
     a.pairs = layout;
-    a.items = (unsigned int)a.b.N * (unsigned int)a.heads;
-    return bf16 ? launch<true, 1, 2>(a, l->stream) : launch<false, 1, 2>(a, l->stream);
+    /* Chunks of up to 16 bytes: as many elements as divide every stride and address, the turned part's halves and the rest
+     * of a head. */
+    const size_t esz = bf16 ? 2 : 4;
+    size_t all = a.ldq | a.ldk | a.ldv | a.ldqo | a.ldko | (size_t)a.rot / 2 | (size_t)HD / 2 | 16 / esz;
+    for (const void* p : {a.q, a.k, a.v, (const void*)a.qo, (const void*)a.ko}) all |= (uintptr_t)p / esz;
+    switch ((all & -all) * (bf16 ? 1 : 2)) { /* of bf16's 8 */
+    case 8: return bf16 ? launch<true, 8, 1>(a, l->stream) : launch<false, 4, 1>(a, l->stream);
+    case 4: return bf16 ? launch<true, 4, 1>(a, l->stream) : launch<false, 2, 1>(a, l->stream);
+    case 2: return bf16 ? launch<true, 2, 1>(a, l->stream) : launch<false, 1, 2>(a, l->stream);
+    default: return launch<true, 1, 2>(a, l->stream);
+    }
 }
 
 /* {x T [N][ldx], out T [N][ldo], pos int32 [N], turns, params int{N, NH, HD, rot, layout, ldx, ldo}, f32{mscale}} */

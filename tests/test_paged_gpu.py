@@ -98,7 +98,8 @@ def turned(x, pos, rot, layout, table, mscale):
 
 
 def normed(x, gain, eps):
-    """RMSNorm of heads in 64 bits: two roundings of fp32, and the sums' and root's far smaller ones."""
+    """RMSNorm of heads in 64 bits.  The kernels round the factor 1 / sqrt, its product with the element and that with the gain
+    to fp32: three roundings, beside the sum's and the root's far smaller ones (64 bits)."""
     x = x.astype(np.float64)
     return x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * gain.astype(np.float64)
 
@@ -215,8 +216,8 @@ def test_qk_norm_rope(be, N, NH, NKV, HD, rot, layout, kind):
         for x, buf, ld, g in ((q, oq, ldqo, gain[0]), (k, ok, ldko, gain[1])):
             y = normed(x.reshape(N, -1, HD), g, np.float64(np.float32(eps)))
             want, off = turned(y, pos, rot, layout, table, m)
-            # the norm's two roundings of each element, carried through the turn
-            carried = turned_sum(np.abs(y), rot, layout, abs(m)) * 2 * U32
+            # the norm's three roundings of each element, carried through the turn
+            carried = turned_sum(np.abs(y), rot, layout, abs(m)) * 3 * U32
             got = rows_of(kind, buf, N, x.shape[1], ld, lead)
             check(kind, got, want.reshape(got.shape), (off + carried).reshape(got.shape))
             first.append(got)
@@ -242,6 +243,7 @@ def test_qk_norm_of_extreme_heads(be):
     x[1] *= np.float32(1e30)
     x[2] *= np.float32(1e-30)
     x[3, 5], x[4, 60] = np.nan, np.inf
+    x[5] *= np.float32(1e38 / np.abs(x[5]).max())  # a factor below fp32's normal numbers
     gain, one = np.ones((2, HD), np.float32), be.upload(np.int32([0]))
     for eps in (1e-5, 0.0):
         oq, ok = marked(be, x.nbytes), marked(be, x.nbytes)
@@ -252,7 +254,7 @@ def test_qk_norm_of_extreme_heads(be):
         assert np.array_equal(got, ok.read(np.float32).reshape(NH, HD), equal_nan=True)
         rows = [1, 5] + ([2] if eps == 0 else [])
         want = normed(x[rows], gain[0], np.float64(np.float32(eps)))
-        assert (np.abs(got[rows] - want) <= 3 * U32 * np.abs(want)).all()
+        assert (np.abs(got[rows] - want) <= 3.01 * U32 * np.abs(want)).all()
         assert (got[0] == 0).all() if eps else np.isnan(got[0]).all()  # 0 / sqrt(0)
         assert np.isnan(got[3]).all() and np.isnan(got[4, 60]) and (got[4, :60] == 0).all()
 
@@ -346,7 +348,7 @@ def test_kv_append(be, new, total, page, lead, tail, NH, NKV, HD, rot, layout, n
             y = q.reshape(N, NH, HD).astype(np.float64)
             y = normed(y, gain[0], eps) if norm else y
             want, off = turned(y, b.pos, rot, layout, table, m)
-            off = off + turned_sum(np.abs(y), rot, layout, abs(m)) * 2 * U32 * norm
+            off = off + turned_sum(np.abs(y), rot, layout, abs(m)) * 3 * U32 * norm
             got = rows_of(kind, out, N, Q, ldqo, off0, at)
             check(kind, got[at], want.reshape(N, Q)[at], off.reshape(N, Q)[at])
         else:
@@ -354,7 +356,7 @@ def test_kv_append(be, new, total, page, lead, tail, NH, NKV, HD, rot, layout, n
         y = k.reshape(N, NKV, HD).astype(np.float64)
         y = normed(y, gain[1], eps) if norm else y
         want, off = turned(y, b.pos, rot, layout, table, m)
-        off = off + turned_sum(np.abs(y), rot, layout, abs(m)) * 2 * U32 * norm
+        off = off + turned_sum(np.abs(y), rot, layout, abs(m)) * 3 * U32 * norm
         raw = cache.read(np.uint16)[:cache0.size].reshape(cache0.shape)
         held = kind.values(raw.view(kind.memory)).reshape(b.count, 2, NKV, page, HD)
         rest = raw.copy()
