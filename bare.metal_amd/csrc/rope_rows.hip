@@ -19,7 +19,7 @@ namespace {
 using namespace bmk;
 
 constexpr int NT = 256;
-constexpr int MAX_TURNS = 2048, MAX_ROWS = 256; /* pairs and rows of a workgroup */
+constexpr int MAX_ROWS = 264; /* that a workgroup touches */
 
 struct RopeArgs {
     const void *q, *k, *v;
@@ -33,7 +33,8 @@ struct RopeArgs {
     int rot, pairs;
     int units, lp_log; /* lanes with work in a group, log2 of its lanes */
     size_t ldq, ldk, ldv, ldqo, ldko;
-    int per; /* rows of a workgroup */
+    int items; /* heads of all rows */
+    int turns_held;
     Div by_heads, by_half;
     double by_hd; /* 1 / HD */
     float mscale, eps;
@@ -116,66 +117,52 @@ __device__ __forceinline__ double root_inverse(double m) {
     return m == INFINITY ? 0.0 : fma(r * 0.5, fma(-m * r, r, 1.0), r);
 }
 
-/* A workgroup takes `per` rows: their positions, places and (cos, sin) go to LDS once, the heads to groups of 1 << lp_log
- * lanes in turn, AHEAD of them loaded at once.  UN: units a lane takes at most. */
+/* Heads of all rows in order, one to each group of 1 << lp_log lanes: positions, places, cos and sin of the few rows that a
+ * workgroup touches go to LDS, while its heads are loaded.  UN: units a lane takes at most. */
 template <bool BF16, int E, int UN, bool PAIRS>
 __global__ __launch_bounds__(NT) void k_rope_rows(RopeArgs a) {
-    constexpr int AHEAD = UN == 1 ? 4 : 2;
-    __shared__ __attribute__((aligned(16))) float tc[MAX_TURNS], ts[MAX_TURNS];
+    extern __shared__ __attribute__((aligned(16))) float turns[]; /* a.turns_held of cos, then of sin */
+    float *tc = turns, *ts = turns + a.turns_held;
+    __shared__ __attribute__((aligned(16))) float gains[2 * PG_MAX_HD];
     __shared__ size_t places[MAX_ROWS];
     __shared__ int where[MAX_ROWS]; /* bit 0: a row of the batch, bit 1: with a place in the cache */
-    const int t = threadIdx.x, lanes = 1 << a.lp_log, lane = t & (lanes - 1), slot = t >> a.lp_log, slots = NT >> a.lp_log;
+    const int t = threadIdx.x, lanes = 1 << a.lp_log, lane = t & (lanes - 1), slots = NT >> a.lp_log;
     const int HD = a.b.HD, half = a.rot / 2;
-    const int n0 = (int)blockIdx.x * a.per, rows = min(a.per, a.b.N - n0), items = rows * a.heads;
-    const size_t plane = (size_t)HD << a.b.shift; /* of one KV head's part of a page */
+    const int first = (int)blockIdx.x * slots, x = first + (t >> a.lp_log), items = a.items;
+    const int n0 = a.by_heads.of(first), rows = a.by_heads.of(min(first + slots, items) - 1) - n0 + 1;
     const int halves = PAIRS ? 0 : a.rot / (2 * E); /* units whose chunks lie half of the turned part apart */
-
-    struct Item {
-        int row, kind, h; /* kind: 0 q, 1 k, 2 v; -1: none */
-    };
-    auto item = [&](int x) {
-        Item it = {0, -1, 0};
-        if (x < items) {
-            it.row = a.by_heads.of(x);
-            it.h = x - it.row * a.heads;
-            it.kind = it.h < a.NH ? 0 : it.h < a.NH + a.NK ? 1 : 2;
-            it.h -= it.kind == 0 ? 0 : it.kind == 1 ? a.NH : a.NH + a.NK;
-        }
-        return it;
-    };
     auto at = [&](int i, int j) { /* of the lane's unit i, chunk j: its place in a head */
         const int u = lane + (i << a.lp_log);
         return u < halves ? E * u + (j ? half : 0) : 2 * E * u + (j ? E : 0);
     };
-    Chunk<BF16, E> raw[AHEAD][UN][2];
-    auto fetch = [&](int k, const Item& it) {
-        if (it.kind < 0) return;
-        const void* src = it.kind == 0 ? a.q : it.kind == 1 ? a.k : a.v;
-        const size_t from = (size_t)(n0 + it.row) * (it.kind == 0 ? a.ldq : it.kind == 1 ? a.ldk : a.ldv) + (size_t)it.h * HD;
+
+    const int n = a.by_heads.of(min(x, items - 1));
+    int h = x - n * a.heads;
+    const int kind = h < a.NH ? 0 : h < a.NH + a.NK ? 1 : 2; /* q, k, v */
+    h -= kind == 0 ? 0 : kind == 1 ? a.NH : a.NH + a.NK;
+    Chunk<BF16, E> raw[UN][2];
+    if (x < items) {
+        const void* src = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+        const size_t from = (size_t)n * (kind == 0 ? a.ldq : kind == 1 ? a.ldk : a.ldv) + (size_t)h * HD;
 #pragma unroll
         for (int i = 0; i < UN; i++)
 #pragma unroll
             for (int j = 0; j < 2; j++)
-                if (lane + (i << a.lp_log) < a.units) raw[k][i][j] = *(const Chunk<BF16, E>*)((const char*)src + (from + at(i, j)) * (BF16 ? 2 : 4));
-    };
-    Item its[AHEAD];
-#pragma unroll
-    for (int k = 0; k < AHEAD; k++) {
-        its[k] = item(slot + k * slots);
-        fetch(k, its[k]);
+                if (lane + (i << a.lp_log) < a.units) raw[i][j] = *(const Chunk<BF16, E>*)((const char*)src + (from + at(i, j)) * (BF16 ? 2 : 4));
     }
 
-    /* position of each row for its pairs, and (once) its place */
-    for (int x = t; x < rows * max(half, 1); x += NT) {
-        const int row = half ? a.by_half.of(x) : x, pair = x - row * half, n = n0 + row;
+    if (a.gain)
+        for (int i = t; i < 2 * HD; i += NT) gains[i] = a.gain[i];
+    for (int i = t; i < rows * max(half, 1); i += NT) {
+        const int row = half ? a.by_half.of(i) : i, pair = i - row * half;
         int p, in = 1;
         if (a.pos) {
-            p = a.pos[n];
+            p = a.pos[n0 + row];
         } else {
-            const int s = a.b.seq_of(n);
+            const int s = a.b.seq_of(n0 + row);
             in = s >= 0;
-            p = in ? a.b.pos_of(s, n) : 0;
-            if (half == 0 || pair == 0) {
+            p = in ? a.b.pos_of(s, n0 + row) : 0;
+            if (half == 0 || pair == 0) { /* once */
                 const int pg = in ? a.b.page_of(s, p) : -1;
                 places[row] = pg >= 0 ? a.b.base(pg, 0, 0) + (size_t)(p & ((1 << a.b.shift) - 1)) * HD : 0;
                 in |= pg >= 0 ? 2 : 0;
@@ -186,82 +173,84 @@ __global__ __launch_bounds__(NT) void k_rope_rows(RopeArgs a) {
             const unsigned long long turn = (unsigned long long)(long long)p * a.turns[pair];
             float c, s;
             cos_sin((unsigned int)(turn >> 32), &c, &s);
-            tc[x] = c * a.mscale;
-            ts[x] = s * a.mscale;
+            tc[i] = c * a.mscale;
+            ts[i] = s * a.mscale;
         }
     }
     __syncthreads();
 
-    for (int x0 = slot; x0 < items; x0 += AHEAD * slots) {
+    const int row = n - n0, flags = where[row];
+    const bool cached = kind == 2 || (kind == 1 && !a.ko);
+    if (x >= items || !(flags & 1) || (cached && !(flags & 2))) return;
+    float y[UN][2][E];
 #pragma unroll
-        for (int k = 0; k < AHEAD; k++) {
-            const Item it = its[k];
-            if (it.kind < 0) continue;
-            const int flags = where[it.row];
-            const bool cached = it.kind == 2 || (it.kind == 1 && !a.ko);
-            if (!(flags & 1) || (cached && !(flags & 2))) continue;
-            void* dst = it.kind == 0 ? a.qo : cached ? a.cache : a.ko;
-            const size_t to = it.kind == 0 ? (size_t)(n0 + it.row) * a.ldqo + (size_t)it.h * HD
-                              : !cached    ? (size_t)(n0 + it.row) * a.ldko + (size_t)it.h * HD
-                                           : places[it.row] + (size_t)(it.h + (it.kind == 2 ? a.b.NKV : 0)) * plane;
-            float y[UN][2][E];
+    for (int i = 0; i < UN; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int e = 0; e < E; e++) y[i][j][e] = lane + (i << a.lp_log) < a.units ? value<BF16, E>(raw[i][j], e) : 0.0f;
+    if (a.gain && kind < 2) { /* squares and their sum in 64 bits: heads past 2^64 or under 2^-64 need no care */
+        double sum = 0;
+#pragma unroll
+        for (int i = 0; i < UN; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int e = 0; e < E; e++) sum = fma((double)y[i][j][e], (double)y[i][j][e], sum);
+        const double inv = root_inverse(group_sum(sum, lanes) * a.by_hd + (double)a.eps);
+        const float f = (float)inv;
+        if (__builtin_expect(__any(f < 0x1p-100f), 0)) { /* a factor under 2^-126 has not all of fp32's bits */
 #pragma unroll
             for (int i = 0; i < UN; i++)
 #pragma unroll
                 for (int j = 0; j < 2; j++)
 #pragma unroll
-                    for (int e = 0; e < E; e++) y[i][j][e] = lane + (i << a.lp_log) < a.units ? value<BF16, E>(raw[k][i][j], e) : 0.0f;
-            if (a.gain && it.kind < 2) { /* squares and their sum in 64 bits: heads past 2^64 or under 2^-64 need no care */
-                const float* gain = a.gain + (it.kind == 1 ? HD : 0);
-                double sum = 0;
-#pragma unroll
-                for (int i = 0; i < UN; i++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++)
-#pragma unroll
-                        for (int e = 0; e < E; e++) sum = fma((double)y[i][j][e], (double)y[i][j][e], sum);
-                const double inv = root_inverse(group_sum(sum, lanes) * a.by_hd + (double)a.eps);
-                const float f = (float)inv;
-                const bool tiny = f < 0x1p-100f; /* the last bits of a factor under 2^-126 are not fp32's */
-#pragma unroll
-                for (int i = 0; i < UN; i++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++)
-#pragma unroll
-                        for (int e = 0; e < E; e++)
-                            if (lane + (i << a.lp_log) < a.units)
-                                y[i][j][e] = (tiny ? (float)((double)y[i][j][e] * inv) : y[i][j][e] * f) * gain[at(i, j) + e];
-            }
-#pragma unroll
-            for (int i = 0; i < UN; i++) {
-                const int u = lane + (i << a.lp_log);
-                if (u >= a.units) continue;
-                if (it.kind < 2 && 2 * E * u < a.rot) {
-                    const float *c = tc + it.row * half + E * u, *s = ts + it.row * half + E * u;
-                    float cs[E], sn[E];
-                    __builtin_memcpy(cs, __builtin_assume_aligned(c, E * 4 < 16 ? E * 4 : 16), sizeof cs);
-                    __builtin_memcpy(sn, __builtin_assume_aligned(s, E * 4 < 16 ? E * 4 : 16), sizeof sn);
-#pragma unroll
-                    for (int e = 0; e < E; e++) { /* pair E u + e: element e of both chunks, or neighbours along them */
-                        float &x0 = PAIRS ? y[i][2 * e / E][2 * e % E] : y[i][0][e];
-                        float &x1 = PAIRS ? y[i][(2 * e + 1) / E][(2 * e + 1) % E] : y[i][1][e];
-                        /* spelt out, so that every form gives the same bits */
-                        const float y0 = fmaf(x0, cs[e], -(x1 * sn[e])), y1 = fmaf(x0, sn[e], x1 * cs[e]);
-                        x0 = y0;
-                        x1 = y1;
+                    for (int e = 0; e < E; e++) {
+                        asm volatile(""); /* a branch, not a choice between two values */
+                        y[i][j][e] = f < 0x1p-100f ? (float)((double)y[i][j][e] * inv) : y[i][j][e] * f;
                     }
-                }
+        } else {
 #pragma unroll
-                for (int j = 0; j < 2; j++) store<BF16, E>(dst, to + at(i, j), y[i][j]);
+            for (int i = 0; i < UN; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int e = 0; e < E; e++) y[i][j][e] *= f;
+        }
+#pragma unroll
+        for (int i = 0; i < UN; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float g[E];
+                __builtin_memcpy(g, __builtin_assume_aligned(gains + (kind == 1 ? HD : 0) + min(at(i, j), HD - E), E * 4 < 8 ? 4 : 8), sizeof g);
+#pragma unroll
+                for (int e = 0; e < E; e++) y[i][j][e] *= g[e];
+            }
+    }
+    void* dst = kind == 0 ? a.qo : cached ? a.cache : a.ko;
+    const size_t to = kind == 0 ? (size_t)n * a.ldqo + (size_t)h * HD
+                      : !cached ? (size_t)n * a.ldko + (size_t)h * HD
+                                : places[row] + ((size_t)(h + (kind == 2 ? a.b.NKV : 0)) * HD << a.b.shift);
+#pragma unroll
+    for (int i = 0; i < UN; i++) {
+        const int u = lane + (i << a.lp_log);
+        if (u >= a.units) continue;
+        if (kind < 2 && 2 * E * u < a.rot) {
+            float cs[E], sn[E];
+            __builtin_memcpy(cs, __builtin_assume_aligned(tc + row * half + E * u, E * 4 < 16 ? E * 4 : 16), sizeof cs);
+            __builtin_memcpy(sn, __builtin_assume_aligned(ts + row * half + E * u, E * 4 < 16 ? E * 4 : 16), sizeof sn);
+#pragma unroll
+            for (int e = 0; e < E; e++) { /* pair E u + e: element e of both chunks, or neighbours along them */
+                float &x0 = PAIRS ? y[i][2 * e / E][2 * e % E] : y[i][0][e];
+                float &x1 = PAIRS ? y[i][(2 * e + 1) / E][(2 * e + 1) % E] : y[i][1][e];
+                /* spelt out, so that every form gives the same bits */
+                const float y0 = fmaf(x0, cs[e], -(x1 * sn[e])), y1 = fmaf(x0, sn[e], x1 * cs[e]);
+                x0 = y0;
+                x1 = y1;
             }
         }
-        if (x0 + AHEAD * slots < items) {
 #pragma unroll
-            for (int k = 0; k < AHEAD; k++) {
-                its[k] = item(x0 + (AHEAD + k) * slots);
-                fetch(k, its[k]);
-            }
-        }
+        for (int j = 0; j < 2; j++) store<BF16, E>(dst, to + at(i, j), y[i][j]);
     }
 }
 
@@ -270,18 +259,18 @@ int launch(RopeArgs& a, hipStream_t stream) {
     a.units = a.b.HD / (2 * E);
     a.lp_log = 0;
     while ((UN << a.lp_log) < a.units) a.lp_log++;
-    /* rows of a workgroup: as many as give its lanes one head each, or up to four where there are more workgroups than the
-     * chip holds (a row's cos and sin serve all its heads whatever that is) */
-    const int slots = NT >> a.lp_log, half = a.rot / 2;
-    const int least = std::max(1, slots / a.heads), most = std::max(1, 4 * slots / a.heads);
-    a.per = std::min(std::max(a.b.N / 1024, least), most);
-    a.per = std::min({a.per, MAX_ROWS, MAX_TURNS / std::max(half, 1)});
     a.by_heads = div_by(a.heads);
-    a.by_half = div_by(std::max(half, 1));
+    a.by_half = div_by(std::max(a.rot / 2, 1));
     a.by_hd = 1.0 / a.b.HD;
-    const dim3 grid((a.b.N + a.per - 1) / a.per);
-    if (a.pairs) hipLaunchKernelGGL((k_rope_rows<BF16, E, UN, true>), grid, dim3(NT), 0, stream, a);
-    else hipLaunchKernelGGL((k_rope_rows<BF16, E, UN, false>), grid, dim3(NT), 0, stream, a);
+    /* a workgroup's heads lie in whole rows and a part of one at either end; LDS for no more than those, so that it does not
+     * keep workgroups off a CU */
+    const int slots = NT >> a.lp_log, rows = (slots - 1) / a.heads + 2;
+    static_assert(NT + 1 <= MAX_ROWS, "");
+    a.turns_held = (rows * (a.rot / 2) + 3) & ~3;
+    const size_t bytes = (size_t)a.turns_held * 8;
+    const dim3 grid(((unsigned int)a.items + slots - 1) / slots);
+    if (a.pairs) hipLaunchKernelGGL((k_rope_rows<BF16, E, UN, true>), grid, dim3(NT), bytes, stream, a);
+    else hipLaunchKernelGGL((k_rope_rows<BF16, E, UN, false>), grid, dim3(NT), bytes, stream, a);
     BMK_LAUNCH_CHECK();
     return 0;
 }
@@ -296,9 +285,10 @@ int run(const bmk_launch_t* l, RopeArgs& a, bool bf16, int layout, int turns_at,
                     l->bytes[turns_at], a.rot, (size_t)a.rot * 4);
         BMK_REQUIRE(((uintptr_t)l->dev[turns_at] & 7) == 0, "%s: turns lie off an 8-byte boundary", what);
     }
-    BMK_REQUIRE((int64_t)a.b.N * a.heads < (1LL << 31), "%s: %d rows of %d heads are over 2^31 heads", what, a.b.N, a.heads);
+    BMK_REQUIRE((int64_t)a.b.N * a.heads <= PG_MAX_DIM, "%s: %d rows of %d heads are over 2^30 heads", what, a.b.N, a.heads);
     a.turns = (const unsigned long long*)l->dev[turns_at];
     a.pairs = layout;
+    a.items = a.b.N * a.heads;
     /* Chunks of up to 16 bytes: as many elements as divide every stride and address, the turned part's halves and the rest
      * of a head. */
     const size_t esz = bf16 ? 2 : 4;
