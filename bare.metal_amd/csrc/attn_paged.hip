@@ -48,6 +48,7 @@ constexpr int KT = 32;           /* keys of a tile */
 constexpr float SLACK = 8.0f;    /* in powers of two: how far a score may pass the running maximum before that moves */
 constexpr int MAX_SPLIT = 128;   /* parts of a unit's keys */
 constexpr int LEAST = 4;         /* tiles a part, at least: one a wave */
+constexpr int MANY_LEAST = 8;    /* of more than 32 rows */
 constexpr int CUS = 256, ROUNDS = 4, ROUND_TILES = 32;
 
 /* The scratch memory begins with arrival counters, each on a line of its own, that are zero between launches of any
@@ -119,15 +120,6 @@ __device__ __attribute__((aligned(16))) const unsigned int pg_nans[8 * PG_MAX_HD
 /* bits 15 and 31: the half below is an infinity or NaN (an exponent of ones carries) */
 __device__ __forceinline__ unsigned int no_numbers(unsigned int two) {
     return ((two & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-}
-
-__device__ __forceinline__ void agent_store2(float* p, float x, float y) {
-    const unsigned long long u = ((unsigned long long)__float_as_uint(y) << 32) | __float_as_uint(x);
-    __hip_atomic_store((unsigned long long*)p, u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ f32x2 agent_load2(const float* p) {
-    const unsigned long long u = __hip_atomic_load((const unsigned long long*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    return f32x2{__uint_as_float((unsigned int)u), __uint_as_float((unsigned int)(u >> 32))};
 }
 
 /* two values' bf16, rounded to nearest even */
@@ -244,7 +236,11 @@ struct Plan {
         return q;
     }
     __device__ __forceinline__ Seq chunk(int c) const { return c ? seq(c + lane) : first; }
-    __device__ __forceinline__ unsigned int parts(const Seq& q) const { return max(1, (q.T + per - 1) / per); }
+    /* of a unit of q; of more rows than one wave's, no more than pay for their records (3 parts of 128 rows of 64: 3 us) */
+    __device__ __forceinline__ unsigned int parts(const Seq& q) const {
+        const int p = (q.T + per - 1) / per;
+        return max(1, q.n * a.R > 32 ? min(p, q.T / MANY_LEAST) : p);
+    }
     __device__ __forceinline__ Sums own(const Seq& q) const {
         const unsigned int p = parts(q);
         return Sums{q.units * p * a.b.NKV, p > 1 ? (unsigned int)q.n * a.R * p * a.b.NKV : 0, p > 1 ? q.units * a.b.NKV : 0};
@@ -396,7 +392,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
         /* tiles of keys that some row of the unit sees, and this part's */
         const int lo = seen(a, p0 + tok0, it.len).first, hi = min(seen(a, p0 + tok1, it.len).last + 1, room);
         const int t0 = lo / KT, t1 = hi > lo ? (hi + KT - 1) / KT : t0;
-        const int parts = max(1, (t1 - t0 + plan.per - 1) / plan.per), per = (t1 - t0 + parts - 1) / parts; /* as even as they go */
+        const int parts = max(1, min(it.parts, (t1 - t0 + plan.per - 1) / plan.per)), per = (t1 - t0 + parts - 1) / parts; /* as even as they go */
         if (it.part >= parts) return;
         const int kt0 = t0 + it.part * per, kt1 = min(kt0 + per, t1);
         /* waves side by side on rows, the rest in turns on the keys, 32 at a time */
@@ -938,21 +934,27 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
             }
             return;
         }
-        /* Records cross XCDs: they are written and read with agent-scope accesses, past the XCDs' own L2s, and each wave
-         * waits for its stores before the barrier, so a part is counted only after its record has arrived.  A unit's
-         * records: [part][row]{HDP values, maximum, sum}, from the unit's rows and KV heads before it. */
-        constexpr int REC = HDP + 2;
-        float* recs = a.rec + ((size_t)it.rec + (size_t)it.parts * ((size_t)rows_all * it.kh + r0)) * REC;
+        /* Records cross XCDs: they are written and read past the XCDs' own L2s (sc1), and each wave waits for its stores before
+         * the barrier, so a part is counted only after its record has arrived.  A unit's records: of each part, four
+         * dimensions of all rows side by side, then all rows' maxima and sums, 16 bytes each. */
+        constexpr int REC = HDP + 4, SC1 = 16;
+        const int part_bytes = nrows * REC * 4;
+        const auto recs = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)scalar((const char*)(a.rec + ((size_t)it.rec + (size_t)it.parts * ((size_t)rows_all * it.kh + r0)) * REC)), 0,
+            scalar(parts * part_bytes), 0x00027000);
         if (writes) {
-            float* rec = recs + ((size_t)it.part * nrows + (r - r0)) * REC;
+            const int at = it.part * part_bytes + (r - r0) * 16;
+            auto put = [&](int quad, float x, float y, float z, float w) {
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{x, y, z, w}), recs, at + quad * nrows * 16, 0, SC1);
+            };
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    const int dim = 32 * d + 8 * (e >> 2) + 4 * half + (e & 3);
-                    if (dim < HD) agent_store2(rec + dim, acc[d][e], acc[d][e + 1]);
+                for (int e = 0; e < 16; e += 4) {
+                    const int dim = 32 * d + 2 * e + 4 * half;
+                    if (dim < HD) put(dim >> 2, acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]);
                 }
-            if (half == 0) agent_store2(rec + HDP, m, l);
+            if (half == 0) put(HDP / 4, m, l, 0.0f, 0.0f);
         }
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
         __builtin_amdgcn_s_waitcnt(0);
@@ -966,60 +968,82 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
         }
         __syncthreads();
         if (!last_one) return;
-        /* Each four outputs from their records, by as many lanes as there are for them (up to 64, side by side), each lane
-         * reading 8 records at once. */
+        /* Four outputs at a time from their records, eight of which a lane reads at once: of U outputs where a unit has few
+         * parts; by 1 << by_log lanes side by side, up to 64, where there are more lanes than outputs. */
         const int outs = nrows * (HD / 4);
         int by_log = 0;
         while (by_log < 6 && outs << (by_log + 1) <= NT && 4 << by_log < parts) by_log++;
-        for (int x0 = 0; x0 < outs; x0 += NT >> by_log) {
-            const int x = x0 + (t >> by_log), row = min(x, outs - 1) / (HD / 4), dim = 4 * (min(x, outs - 1) - row * (HD / 4));
-            float o[4] = {0, 0, 0, 0}, mx = -INFINITY, sum = 0.0f;
-            for (int i = t & ((1 << by_log) - 1); i < parts; i += 8 << by_log) {
-                f32x2 y[8][3];
+        auto join = [&](auto us) __attribute__((always_inline)) {
+            constexpr int U = decltype(us)::value, P = 8 / U;
+            const int step = NT >> by_log, sub = t & ((1 << by_log) - 1);
+            for (int x0 = 0; x0 < outs; x0 += U * step) {
+                int row[U], quad[U];
+                f32x4 o[U];
+                float mx[U], sum[U];
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int part = i + (e << by_log);
-                    const float* rec = recs + ((size_t)part * nrows + row) * REC;
-                    y[e][0] = y[e][1] = f32x2{0, 0};
-                    y[e][2] = f32x2{-INFINITY, 0};
-                    if (part >= parts) continue;
-                    y[e][2] = agent_load2(rec + HDP);
-                    y[e][0] = agent_load2(rec + dim);
-                    y[e][1] = agent_load2(rec + dim + 2);
+                for (int u = 0; u < U; u++) {
+                    const int x = min(x0 + u * step + (t >> by_log), outs - 1);
+                    quad[u] = x / nrows;
+                    row[u] = x - quad[u] * nrows;
+                    o[u] = f32x4{0, 0, 0, 0};
+                    mx[u] = -INFINITY;
+                    sum[u] = 0.0f;
                 }
-                float mn = mx;
+                for (int i = sub; i < parts; i += P << by_log) {
+                    f32x4 y[U][P], ml[U][P];
 #pragma unroll
-                for (int e = 0; e < 8; e++) mn = fmaxf(mn, y[e][2][0]);
-                const float f = mx > -INFINITY ? __builtin_amdgcn_exp2f(mx - mn) : 1.0f;
-                sum *= f;
+                    for (int u = 0; u < U; u++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) o[j] *= f;
+                        for (int e = 0; e < P; e++) { /* past the parts: the descriptor's end, zeros */
+                            const int at = (i + (e << by_log)) * part_bytes + row[u] * 16;
+                            ml[u][e] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(recs, at + HDP / 4 * nrows * 16, 0, SC1));
+                            y[u][e] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(recs, at + quad[u] * nrows * 16, 0, SC1));
+                        }
 #pragma unroll
-                for (int e = 0; e < 8; e++) { /* a part without a finite score has 0 or NaN */
-                    const float g = y[e][2][0] > -INFINITY ? __builtin_amdgcn_exp2f(y[e][2][0] - mn) : 1.0f;
-                    sum = fmaf(g, y[e][2][1], sum);
+                    for (int u = 0; u < U; u++) {
+                        float mn = mx[u];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) o[j] = fmaf(g, y[e][j >> 1][j & 1], o[j]);
+                        for (int e = 0; e < P; e++) {
+                            if (i + (e << by_log) >= parts) ml[u][e] = f32x4{-INFINITY, 0, 0, 0};
+                            mn = fmaxf(mn, ml[u][e][0]);
+                        }
+                        const float f = mx[u] > -INFINITY ? __builtin_amdgcn_exp2f(mx[u] - mn) : 1.0f;
+                        sum[u] *= f;
+                        o[u] *= f;
+#pragma unroll
+                        for (int e = 0; e < P; e++) { /* a part without a finite score has 0 or NaN */
+                            const float g = ml[u][e][0] > -INFINITY ? __builtin_amdgcn_exp2f(ml[u][e][0] - mn) : 1.0f;
+                            sum[u] = fmaf(g, ml[u][e][1], sum[u]);
+#pragma unroll
+                            for (int j = 0; j < 4; j++) o[u][j] = fmaf(g, y[u][e][j], o[u][j]);
+                        }
+                        mx[u] = mn;
+                    }
                 }
-                mx = mn;
-            }
-            for (int k = 0; k < by_log; k++) {
-                const float m1 = __shfl_xor(mx, 1 << k), mn = fmaxf(mx, m1);
-                const float f = mx > -INFINITY ? __builtin_amdgcn_exp2f(mx - mn) : 1.0f;
-                const float g = m1 > -INFINITY ? __builtin_amdgcn_exp2f(m1 - mn) : 1.0f;
-                sum = sum * f + __shfl_xor(sum, 1 << k) * g;
 #pragma unroll
-                for (int j = 0; j < 4; j++) o[j] = o[j] * f + __shfl_xor(o[j], 1 << k) * g;
-                mx = mn;
-            }
-            if (x >= outs || (t & ((1 << by_log) - 1))) continue;
-            const int rr = r0 + row, rtok = a.by_r.of(rr);
-            const Seen s = seen(a, p0 + rtok, it.len);
-            const bool none = s.last < s.first, gone = s.last >= room;
+                for (int u = 0; u < U; u++) {
+                    for (int k = 0; k < by_log; k++) {
+                        const float m1 = __shfl_xor(mx[u], 1 << k), mn = fmaxf(mx[u], m1);
+                        const float f = mx[u] > -INFINITY ? __builtin_amdgcn_exp2f(mx[u] - mn) : 1.0f;
+                        const float g = m1 > -INFINITY ? __builtin_amdgcn_exp2f(m1 - mn) : 1.0f;
+                        sum[u] = sum[u] * f + __shfl_xor(sum[u], 1 << k) * g;
 #pragma unroll
-            for (int j = 0; j < 4; j++) o[j] = none ? 0.0f : gone ? NAN : o[j] / sum;
-            store4<BF16>(a, (size_t)(n0 + rtok) * a.ldo + (size_t)(it.kh * R + rr - rtok * R) * HD, dim, o);
-        }
+                        for (int j = 0; j < 4; j++) o[u][j] = o[u][j] * f + __shfl_xor(o[u][j], 1 << k) * g;
+                        mx[u] = mn;
+                    }
+                    if (x0 + u * step + (t >> by_log) >= outs || sub) continue;
+                    const int rr = r0 + row[u], rtok = a.by_r.of(rr);
+                    const Seen s = seen(a, p0 + rtok, it.len);
+                    const bool none = s.last < s.first, gone = s.last >= room;
+                    float out[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) out[j] = none ? 0.0f : gone ? NAN : o[u][j] / sum[u];
+                    store4<BF16>(a, (size_t)(n0 + rtok) * a.ldo + (size_t)(it.kh * R + rr - rtok * R) * HD, 4 * quad[u], out);
+                }
+            }
+        };
+        if (parts <= 4 && outs > NT) join(std::integral_constant<int, 2>{});
+        else join(std::integral_constant<int, 1>{});
     }
 #endif
 }
@@ -1029,7 +1053,7 @@ int start(PaArgs& a, const bmk_launch_t* l) {
     typedef Shape<BF16, HDP> W;
     a.most = 0;
     if (l->scratch_bytes > DONE_BYTES)
-        a.most = (unsigned int)std::min<size_t>((l->scratch_bytes - DONE_BYTES) / ((HDP + 2) * 4), 1u << 30);
+        a.most = (unsigned int)std::min<size_t>((l->scratch_bytes - DONE_BYTES) / ((HDP + 4) * 4), 1u << 30);
     a.done = (unsigned int*)l->scratch;
     a.rec = (float*)((char*)l->scratch + DONE_BYTES);
     a.slots = W::SLOTS;
