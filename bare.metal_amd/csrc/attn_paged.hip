@@ -89,11 +89,16 @@ template <int FORM, int HDP> struct Tile {
     static constexpr int BYTES = 2 * PLANES * PLANE;
 };
 
-/* Chunk c of row r lies at c ^ key: K is read 8 rows of one chunk at a time, V 4 rows of two neighbouring chunks (fp32: two
- * rows 4 apart of eight), each set on all banks. */
-__device__ __forceinline__ int k_place(int r, int c) { return c ^ (r & 7); }
-template <int FORM>
-__device__ __forceinline__ int v_place(int r, int c) { return FORM == AS_F32 ? c ^ (2 * (r & 4)) : c ^ (2 * (r & 3)); }
+/* Chunk c of row r lies at c ^ key, so that what lanes read at once lies on all 64 banks, 256 bytes: of K one chunk of 16
+ * rows; of V two neighbouring chunks of 4 rows and the two after them (fp32: eight of a row and of the row 4 on).  Rows of
+ * 128 bytes lie in two halves of the banks already.  (2048 rows over 16384 keys, keys of 8 rows in place of 16 and V's halves
+ * on the same banks: half of LDS' cycles were conflicts.) */
+template <int CPR>
+__device__ __forceinline__ int k_place(int r, int c) { return c ^ (CPR == 8 ? r >> 1 & 7 : r & 15); }
+template <int FORM, int CPR>
+__device__ __forceinline__ int v_place(int r, int c) {
+    return c ^ (FORM == AS_F32 ? 2 * (r & 4) : CPR == 8 ? 2 * (r & 3) : 4 * (r & 3));
+}
 
 /* A workgroup's waves and LDS: every wave has a tile of its own while it goes alone, and where rows fill the waves all have
  * a ring of four (bf16) or two (fp32, in terms; heads over 128 have no such form: their registers spill). */
@@ -132,10 +137,10 @@ __device__ __forceinline__ unsigned int pack_top(float x, float y) {
 }
 __device__ __forceinline__ float top(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 
-/* x's three terms of two values each, packed; of an infinity or NaN the first alone */
+/* Two values' three terms, packed.  An infinity's others are NaN, which leaves what sees it no number, as it should. */
 __device__ __forceinline__ void split2(float x, float y, unsigned int* t) {
     t[0] = pack_top(x, y);
-    const float rx = __builtin_isfinite(x) ? x - top(x) : 0.0f, ry = __builtin_isfinite(y) ? y - top(y) : 0.0f;
+    const float rx = x - top(x), ry = y - top(y);
     t[1] = pack_top(rx, ry);
     t[2] = pack_top(rx - top(rx), ry - top(ry));
 }
@@ -467,7 +472,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
         constexpr int KG = !BF16 && HDP == 256 ? 1 : 2, VG = BF16 && HDP != 64 ? 2 : 1;
         auto block = [&](auto form, const unsigned char* buf, int k0) __attribute__((always_inline)) {
             constexpr int FORM = decltype(form)::value, PLANES = Tile<FORM, HDP>::PLANES, PLANE = Tile<FORM, HDP>::PLANE;
-            constexpr int ROWB = Tile<FORM, HDP>::ROWB;
+            constexpr int ROWB = Tile<FORM, HDP>::ROWB, CPR = Tile<FORM, HDP>::CPR;
             f32x16 sc;
 #pragma unroll
             for (int e = 0; e < 16; e++) sc[e] = 0.0f;
@@ -482,11 +487,11 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                     if constexpr (FORM == AS_F32) {
 #pragma unroll
                         for (int i = 0; i < 2; i++)
-                            kw[g & 1][s][i] = *(const f32x4*)(buf + row * ROWB + 16 * k_place(row, 4 * at + 2 * half + i));
+                            kw[g & 1][s][i] = *(const f32x4*)(buf + row * ROWB + 16 * k_place<CPR>(row, 4 * at + 2 * half + i));
                     } else {
 #pragma unroll
                         for (int x = 0; x < PLANES; x++)
-                            kf[g & 1][s][x] = *(const bf16x8*)(buf + x * PLANE + row * ROWB + 16 * k_place(row, 2 * at + half));
+                            kf[g & 1][s][x] = *(const bf16x8*)(buf + x * PLANE + row * ROWB + 16 * k_place<CPR>(row, 2 * at + half));
                     }
                 }
             };
@@ -500,7 +505,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                     for (int s = 0; s < 2; s++) {
                         if constexpr (FORM == AS_F32) {
                             const int vr = 16 * s + 4 * half, dim = 32 * (g * VG + d) + col;
-                            const unsigned char* at = buf + PLANE + vr * ROWB + 16 * v_place<FORM>(vr, dim >> 2) + 4 * (dim & 3);
+                            const unsigned char* at = buf + PLANE + vr * ROWB + 16 * v_place<FORM, CPR>(vr, dim >> 2) + 4 * (dim & 3);
 #pragma unroll
                             for (int e = 0; e < 8; e++) vw[g & 1][d][s][e] = *(const float*)(at + ((e & 3) + 2 * (e & 4)) * ROWB);
                         } else {
@@ -508,7 +513,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                             const int dim = 32 * (g * VG + d) + (lane & 16) + 4 * (lane & 3);
 #pragma unroll
                             for (int x = 0; x < PLANES; x++) {
-                                const unsigned char* at = buf + (PLANES + x) * PLANE + vr * ROWB + 16 * v_place<FORM>(vr, dim >> 3) + 2 * (dim & 4);
+                                const unsigned char* at = buf + (PLANES + x) * PLANE + vr * ROWB + 16 * v_place<FORM, CPR>(vr, dim >> 3) + 2 * (dim & 4);
                                 s16x4 y[2]; /* the second set lies 8 rows on, in the same place of its row */
                                 y[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(lvoid*)at);
                                 y[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(lvoid*)(at + 8 * ROWB));
@@ -708,16 +713,16 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
          * NaN. */
         constexpr int ESZ = BF16 ? 2 : 4;
         typedef Tile<W::ALONE, HDP> T;
-        constexpr int RPI = T::RPI, CPR = T::CPR, PLANE = T::PLANE, KINDS = 8 / RPI;
+        constexpr int RPI = T::RPI, CPR = T::CPR, PLANE = T::PLANE, KINDS = 16 / RPI; /* loads whose places differ */
         const int end = min(hi, kt1 * KT), rowb = HD * ESZ;
         const size_t page_bytes = (size_t)b.NKV * kv * (2 * ESZ), kh_bytes = (size_t)it.kh * kv * ESZ;
         auto page_of = [&](int key) { /* key: a multiple of 8, or within them; wave-uniform */
             return ((const __attribute__((address_space(4))) int*)table)[__builtin_amdgcn_readfirstlane(max(min(key, hi - 1), 0) >> b.shift)];
         };
-        /* a lane's place in the rows of a load whose first row is `first` mod 8, of keys and of values */
+        /* a lane's place in the rows of a load whose first row is `first` mod 16, of keys and of values */
         auto lane_place = [&](int first, int& k, int& v) {
             const int row = lane / CPR, place = lane % CPR;
-            const int kc = k_place(first + row, place), vc = v_place<W::ALONE>(first + row, place); /* their own inverses */
+            const int kc = k_place<CPR>(first + row, place), vc = v_place<W::ALONE, CPR>(first + row, place); /* their own inverses */
             k = 16 * kc < rowb ? row * rowb + 16 * kc : 1 << 30;
             v = 16 * vc < rowb ? row * rowb + 16 * vc : 1 << 30;
         };
@@ -738,8 +743,9 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
             if constexpr (W::ARRAYS == 4) buf = wave == 0 ? lds0 : wave == 1 ? lds1 : wave == 2 ? lds2 : lds3;
             else buf = lds0 + wave * T::BYTES;
             int k_off[KINDS], v_off[KINDS];
+            if constexpr (KINDS <= 8)
 #pragma unroll
-            for (int i = 0; i < KINDS; i++) lane_place(i * RPI, k_off[i], v_off[i]);
+                for (int i = 0; i < KINDS; i++) lane_place(i * RPI, k_off[i], v_off[i]);
             int pg[4]; /* of eight rows each */
             auto pages = [&](int kt) {
 #pragma unroll
@@ -751,7 +757,11 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                     for (int g = 0; g < 4; g++) {
                         const int key = kt * KT + 8 * g, p = page_of(key);
 #pragma unroll
-                        for (int i = 0; i < 8; i++) load(p, key + i, buf + (8 * g + i) * 1024, k_off[i], v_off[i]);
+                        for (int i = 0; i < 8; i++) {
+                            int k, v;
+                            lane_place(8 * g + i, k, v);
+                            load(p, key + i, buf + (8 * g + i) * 1024, k, v);
+                        }
                     }
                     return;
                 }
@@ -778,17 +788,17 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
             __builtin_amdgcn_s_waitcnt(0x0F70); /* none under way */
         } else if constexpr (BF16) {
             /* Load i of a wave fills rows (i NW + wave) RPI .. + RPI - 1. */
-            constexpr int NI = PLANE / 1024 / NW;
-            static_assert(NW % KINDS == 0, "a wave's loads begin at the same row of eight");
-            int k_off, v_off, pg[NI];
-            lane_place(wave * RPI & 7, k_off, v_off);
+            constexpr int NI = PLANE / 1024 / NW, KN = NW * RPI < 16 ? 16 / (NW * RPI) : 1;
+            int k_off[KN], v_off[KN], pg[NI];
+#pragma unroll
+            for (int i = 0; i < KN; i++) lane_place((i * NW + wave) * RPI, k_off[i], v_off[i]);
             auto pages = [&](int kt) {
 #pragma unroll
                 for (int i = 0; i < NI; i++) pg[i] = page_of(kt * KT + (i * NW + wave) * RPI);
             };
             auto request = [&](int kt, unsigned char* buf) {
 #pragma unroll
-                for (int i = 0; i < NI; i++) load(pg[i], kt * KT + (i * NW + wave) * RPI, buf + (i * NW + wave) * 1024, k_off, v_off);
+                for (int i = 0; i < NI; i++) load(pg[i], kt * KT + (i * NW + wave) * RPI, buf + (i * NW + wave) * 1024, k_off[i % KN], v_off[i % KN]);
             };
             pages(kt0);
             q_request();
@@ -856,7 +866,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                         unsigned int z[4][3];
 #pragma unroll
                         for (int e = 0; e < 4; e++) split2(src[e >> 1][2 * (e & 1)], src[e >> 1][2 * (e & 1) + 1], z[e]);
-                        unsigned char* to = buf + part * 3 * T3::PLANE + row * T3::ROWB + 16 * (part ? v_place<TERMS3>(row, c) : k_place(row, c));
+                        unsigned char* to = buf + part * 3 * T3::PLANE + row * T3::ROWB + 16 * (part ? v_place<TERMS3, C3>(row, c) : k_place<C3>(row, c));
 #pragma unroll
                         for (int y = 0; y < 3; y++) *(u32x4*)(to + y * T3::PLANE) = u32x4{z[0][y], z[1][y], z[2][y], z[3][y]};
                     }
