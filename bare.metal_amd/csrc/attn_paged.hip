@@ -89,7 +89,7 @@ template <int FORM, int HDP> struct Tile {
     static constexpr int BYTES = 2 * PLANES * PLANE;
 };
 
-/* Chunk c of row r lies at c ^ key, so that what lanes read at once lies on all 64 banks, 256 bytes: of K one chunk of 16
+/* Chunk c of row r lies at c ^ key, key < 16, so that what lanes read at once lies on all 64 banks, 256 bytes: of K one chunk of 16
  * rows; of V two neighbouring chunks of 4 rows and the two after them (fp32: eight of a row and of the row 4 on).  Rows of
  * 128 bytes lie in two halves of the banks already.  (2048 rows over 16384 keys, keys of 8 rows in place of 16 and V's halves
  * on the same banks: half of LDS' cycles were conflicts.) */
@@ -416,47 +416,61 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
         const int mask = (1 << b.shift) - 1;
         const int* table = b.pages + (size_t)it.s * b.max_pages;
 
-        bf16x8 qf[TERMS][STEPS]; /* step s: dimensions 16 s + 8 half .. + 7 of the lane's row */
+        constexpr int ESZ = BF16 ? 2 : 4;
+        /* q of step s: dimensions 16 s + 8 half .. + 7 of the lane's row; of fp32 heads over 128 as they are, for their terms'
+         * registers spill */
+        constexpr bool LATE = !BF16 && HDP == 256;
+        bf16x8 qf[TERMS][LATE ? 1 : STEPS];
         u32x4 qr[STEPS][BF16 ? 1 : 2];
+        /* No lane stays out (what it has no use for it reads from a place that is q's): the compiler has put a spill of all
+         * lanes' values between such branches' ends. */
         auto q_request = [&]() {
             const size_t at = (size_t)(n0 + min(tok, tok1)) * a.ldq + (size_t)(mine ? head : it.kh * R) * HD;
+            if (a.q_wide) {
 #pragma unroll
-            for (int s = 0; s < STEPS; s++) {
-                const int d = 16 * s + 8 * half;
+                for (int s = 0; s < STEPS; s++)
 #pragma unroll
-                for (int i = 0; i < (BF16 ? 1 : 2); i++) {
-                    qr[s][i] = u32x4{0, 0, 0, 0};
-                    if (!mine || d >= HD) continue;
-                    const char* p = (const char*)a.q + (at + d + 4 * i) * (BF16 ? 2 : 4);
-                    if (a.q_wide) {
-                        qr[s][i] = *(const u32x4*)p;
-                    } else {
+                    for (int i = 0; i < (BF16 ? 1 : 2); i++)
+                        qr[s][i] = *(const u32x4*)((const char*)a.q + (at + min(16 * s + 8 * half, HD - 8) + 4 * i) * ESZ);
+            } else {
+#pragma unroll
+                for (int s = 0; s < STEPS; s++)
+#pragma unroll
+                    for (int i = 0; i < (BF16 ? 1 : 2); i++) {
+                        const char* p = (const char*)a.q + (at + min(16 * s + 8 * half, HD - 8) + 4 * i) * ESZ;
 #pragma unroll
                         for (int e = 0; e < 4; e++)
                             qr[s][i][e] = BF16 ? ((const unsigned short*)p)[2 * e] | (unsigned int)((const unsigned short*)p)[2 * e + 1] << 16
                                                : ((const unsigned int*)p)[e];
                     }
-                }
             }
         };
-        auto q_take = [&]() {
+        auto q_terms = [&](int s, auto& z) __attribute__((always_inline)) {
+            const bool there = 16 * s + 8 * half < HD;
+            unsigned int u[TERMS][4];
 #pragma unroll
-            for (int s = 0; s < STEPS; s++) {
-                unsigned int u[TERMS][4];
+            for (int e = 0; e < 4; e++) {
+                if constexpr (BF16) {
+                    u[0][e] = there ? qr[s][0][e] ^ (a.flip >> 16 | a.flip) : 0;
+                } else {
+                    unsigned int y[3];
+                    split2(__uint_as_float(there ? qr[s][e >> 1][2 * (e & 1)] ^ a.flip : 0),
+                           __uint_as_float(there ? qr[s][e >> 1][2 * (e & 1) + 1] ^ a.flip : 0), y);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if constexpr (BF16) {
-                        u[0][e] = qr[s][0][e] ^ (a.flip >> 16 | a.flip);
-                    } else {
-                        unsigned int y[3];
-                        split2(__uint_as_float(qr[s][e >> 1][2 * (e & 1)] ^ a.flip),
-                               __uint_as_float(qr[s][e >> 1][2 * (e & 1) + 1] ^ a.flip), y);
-#pragma unroll
-                        for (int x = 0; x < TERMS; x++) u[x][e] = y[x];
-                    }
+                    for (int x = 0; x < TERMS; x++) u[x][e] = y[x];
                 }
+            }
 #pragma unroll
-                for (int x = 0; x < TERMS; x++) __builtin_memcpy(&qf[x][s], u[x], 16);
+            for (int x = 0; x < TERMS; x++) __builtin_memcpy(&z[x], u[x], 16);
+        };
+        auto q_take = [&]() __attribute__((always_inline)) {
+            if constexpr (LATE) return;
+#pragma unroll
+            for (int s = 0; s < (LATE ? 0 : STEPS); s++) {
+                bf16x8 z[TERMS];
+                q_terms(s, z);
+#pragma unroll
+                for (int x = 0; x < TERMS; x++) qf[x][s] = z[x];
             }
         };
 
@@ -469,7 +483,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
 
         /* The tile of keys k0 .. k0 + 31, in LDS at `buf`.  Reads are issued in groups ahead of the products that take
          * them, the first of V's ahead of the softmax. */
-        constexpr int KG = !BF16 && HDP == 256 ? 1 : 2, VG = BF16 && HDP != 64 ? 2 : 1;
+        constexpr int KG = !BF16 && HDP == 256 ? 1 : 2, VG = 1;
         auto block = [&](auto form, const unsigned char* buf, int k0) __attribute__((always_inline)) {
             constexpr int FORM = decltype(form)::value, PLANES = Tile<FORM, HDP>::PLANES, PLANE = Tile<FORM, HDP>::PLANE;
             constexpr int ROWB = Tile<FORM, HDP>::ROWB, CPR = Tile<FORM, HDP>::CPR;
@@ -487,11 +501,11 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                     if constexpr (FORM == AS_F32) {
 #pragma unroll
                         for (int i = 0; i < 2; i++)
-                            kw[g & 1][s][i] = *(const f32x4*)(buf + row * ROWB + 16 * k_place<CPR>(row, 4 * at + 2 * half + i));
+                            kw[g & 1][s][i] = *(const f32x4*)(buf + row * ROWB + 16 * (k_place<CPR>(row, (4 * at & 15) + 2 * half + i) + (4 * at & ~15)));
                     } else {
 #pragma unroll
                         for (int x = 0; x < PLANES; x++)
-                            kf[g & 1][s][x] = *(const bf16x8*)(buf + x * PLANE + row * ROWB + 16 * k_place<CPR>(row, 2 * at + half));
+                            kf[g & 1][s][x] = *(const bf16x8*)(buf + x * PLANE + row * ROWB + 16 * (k_place<CPR>(row, (2 * at & 15) + half) + (2 * at & ~15)));
                     }
                 }
             };
@@ -552,14 +566,22 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
 #pragma unroll
                         for (int x = 0; x < TERMS; x++) k[x] = kf[g & 1][s][x];
                     }
-                    if constexpr (!BF16) { /* the small terms first */
-                        sc = mfma(k[2], qf[0][at], sc);
-                        sc = mfma(k[0], qf[2][at], sc);
-                        sc = mfma(k[1], qf[1][at], sc);
-                        sc = mfma(k[1], qf[0][at], sc);
-                        sc = mfma(k[0], qf[1][at], sc);
+                    bf16x8 q[TERMS];
+                    if constexpr (LATE) {
+                        asm volatile("" : "+v"(qr[at][0]), "+v"(qr[at][1])); /* here, not ahead of the loop */
+                        q_terms(at, q);
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < TERMS; x++) q[x] = qf[x][at];
                     }
-                    sc = mfma(k[0], qf[0][at], sc);
+                    if constexpr (!BF16) { /* the small terms first */
+                        sc = mfma(k[2], q[0], sc);
+                        sc = mfma(k[0], q[2], sc);
+                        sc = mfma(k[1], q[1], sc);
+                        sc = mfma(k[1], q[0], sc);
+                        sc = mfma(k[0], q[1], sc);
+                    }
+                    sc = mfma(k[0], q[0], sc);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -711,7 +733,6 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
          * into a scalar register, apart from the loads' count, so that nothing waits for the tiles that are under way; what lies
          * behind this part's keys or a head's end comes as zeros by the buffer's bounds, a missing page's keys from rows of
          * NaN. */
-        constexpr int ESZ = BF16 ? 2 : 4;
         typedef Tile<W::ALONE, HDP> T;
         constexpr int RPI = T::RPI, CPR = T::CPR, PLANE = T::PLANE, KINDS = 16 / RPI; /* loads whose places differ */
         const int end = min(hi, kt1 * KT), rowb = HD * ESZ;
@@ -978,82 +999,84 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
         }
         __syncthreads();
         if (!last_one) return;
-        /* Four outputs at a time from their records, eight of which a lane reads at once: of U outputs where a unit has few
-         * parts; by 1 << by_log lanes side by side, up to 64, where there are more lanes than outputs. */
-        const int outs = nrows * (HD / 4);
+        /* Four outputs (a quad of dimensions) at a time from their records.  Where a unit has more quads than there are lanes, a
+         * lane keeps to one row and reads U of its quads' records and P parts at once (4 and 4: of 24 mixed sequences 26 us, two
+         * quads a row for each lane 28; 8 and 4 or 4 and 8 have no registers: 30 and 34); where it has fewer, 1 << by_log lanes
+         * side by side, up to 64, share a quad's parts. */
+        const int quads = HD / 4, across = NT / nrows, each = (quads + across - 1) / across;
         int by_log = 0;
-        while (by_log < 6 && outs << (by_log + 1) <= NT && 4 << by_log < parts) by_log++;
-        auto join = [&](auto us) __attribute__((always_inline)) {
-            constexpr int U = decltype(us)::value, P = 8 / U;
-            const int step = NT >> by_log, sub = t & ((1 << by_log) - 1);
-            for (int x0 = 0; x0 < outs; x0 += U * step) {
-                int row[U], quad[U];
+        while (by_log < 6 && nrows * quads << (by_log + 1) <= NT && 4 << by_log < parts) by_log++;
+        auto join = [&](auto us, auto ps) __attribute__((always_inline)) {
+            constexpr int U = decltype(us)::value, P = decltype(ps)::value;
+            const int sub = U == 1 ? t & ((1 << by_log) - 1) : 0, x = U == 1 ? t >> by_log : t;
+            const int col0 = x / nrows, row = x - col0 * nrows, apart = (NT >> by_log) / nrows; /* this lane's quads: col0, col0 + apart, .. */
+            if (col0 >= (U == 1 ? quads : across)) return;
+            for (int q0 = col0; q0 < quads; q0 += U * apart) {
                 f32x4 o[U];
-                float mx[U], sum[U];
+                float mx = -INFINITY, sum = 0.0f;
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int x = min(x0 + u * step + (t >> by_log), outs - 1);
-                    quad[u] = x / nrows;
-                    row[u] = x - quad[u] * nrows;
-                    o[u] = f32x4{0, 0, 0, 0};
-                    mx[u] = -INFINITY;
-                    sum[u] = 0.0f;
-                }
+                for (int u = 0; u < U; u++) o[u] = f32x4{0, 0, 0, 0};
                 for (int i = sub; i < parts; i += P << by_log) {
-                    f32x4 y[U][P], ml[U][P];
+                    f32x4 y[P][U], ml[P];
 #pragma unroll
-                    for (int u = 0; u < U; u++)
+                    for (int e = 0; e < P; e++) { /* past the parts: the descriptor's end, zeros */
+                        const int at = (i + (e << by_log)) * part_bytes + row * 16;
+                        ml[e] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(recs, at + HDP / 4 * nrows * 16, 0, SC1));
 #pragma unroll
-                        for (int e = 0; e < P; e++) { /* past the parts: the descriptor's end, zeros */
-                            const int at = (i + (e << by_log)) * part_bytes + row[u] * 16;
-                            ml[u][e] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(recs, at + HDP / 4 * nrows * 16, 0, SC1));
-                            y[u][e] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(recs, at + quad[u] * nrows * 16, 0, SC1));
+                        for (int u = 0; u < U; u++) {
+                            const int quad = min(q0 + u * apart, quads - 1);
+                            y[e][u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(recs, at + quad * nrows * 16, 0, SC1));
                         }
-#pragma unroll
-                    for (int u = 0; u < U; u++) {
-                        float mn = mx[u];
-#pragma unroll
-                        for (int e = 0; e < P; e++) {
-                            if (i + (e << by_log) >= parts) ml[u][e] = f32x4{-INFINITY, 0, 0, 0};
-                            mn = fmaxf(mn, ml[u][e][0]);
-                        }
-                        const float f = mx[u] > -INFINITY ? __builtin_amdgcn_exp2f(mx[u] - mn) : 1.0f;
-                        sum[u] *= f;
-                        o[u] *= f;
-#pragma unroll
-                        for (int e = 0; e < P; e++) { /* a part without a finite score has 0 or NaN */
-                            const float g = ml[u][e][0] > -INFINITY ? __builtin_amdgcn_exp2f(ml[u][e][0] - mn) : 1.0f;
-                            sum[u] = fmaf(g, ml[u][e][1], sum[u]);
-#pragma unroll
-                            for (int j = 0; j < 4; j++) o[u][j] = fmaf(g, y[u][e][j], o[u][j]);
-                        }
-                        mx[u] = mn;
                     }
+                    float mn = mx;
+#pragma unroll
+                    for (int e = 0; e < P; e++) {
+                        if (i + (e << by_log) >= parts) ml[e] = f32x4{-INFINITY, 0, 0, 0};
+                        mn = fmaxf(mn, ml[e][0]);
+                    }
+                    const float f = mx > -INFINITY ? __builtin_amdgcn_exp2f(mx - mn) : 1.0f;
+                    sum *= f;
+#pragma unroll
+                    for (int u = 0; u < U; u++) o[u] *= f;
+#pragma unroll
+                    for (int e = 0; e < P; e++) { /* a part without a finite score has 0 or NaN */
+                        const float g = ml[e][0] > -INFINITY ? __builtin_amdgcn_exp2f(ml[e][0] - mn) : 1.0f;
+                        sum = fmaf(g, ml[e][1], sum);
+#pragma unroll
+                        for (int u = 0; u < U; u++)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) o[u][j] = fmaf(g, y[e][u][j], o[u][j]);
+                    }
+                    mx = mn;
                 }
+                if constexpr (U == 1) {
+                    for (int k = 0; k < by_log; k++) {
+                        const float m1 = __shfl_xor(mx, 1 << k), mn = fmaxf(mx, m1);
+                        const float f = mx > -INFINITY ? __builtin_amdgcn_exp2f(mx - mn) : 1.0f;
+                        const float g = m1 > -INFINITY ? __builtin_amdgcn_exp2f(m1 - mn) : 1.0f;
+                        sum = sum * f + __shfl_xor(sum, 1 << k) * g;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) o[0][j] = o[0][j] * f + __shfl_xor(o[0][j], 1 << k) * g;
+                        mx = mn;
+                    }
+                    if (sub) return;
+                }
+                const int rr = r0 + row, rtok = a.by_r.of(rr);
+                const Seen s = seen(a, p0 + rtok, it.len);
+                const bool none = s.last < s.first, gone = s.last >= room;
+                const size_t to = (size_t)(n0 + rtok) * a.ldo + (size_t)(it.kh * R + rr - rtok * R) * HD;
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    for (int k = 0; k < by_log; k++) {
-                        const float m1 = __shfl_xor(mx[u], 1 << k), mn = fmaxf(mx[u], m1);
-                        const float f = mx[u] > -INFINITY ? __builtin_amdgcn_exp2f(mx[u] - mn) : 1.0f;
-                        const float g = m1 > -INFINITY ? __builtin_amdgcn_exp2f(m1 - mn) : 1.0f;
-                        sum[u] = sum[u] * f + __shfl_xor(sum[u], 1 << k) * g;
-#pragma unroll
-                        for (int j = 0; j < 4; j++) o[u][j] = o[u][j] * f + __shfl_xor(o[u][j], 1 << k) * g;
-                        mx[u] = mn;
-                    }
-                    if (x0 + u * step + (t >> by_log) >= outs || sub) continue;
-                    const int rr = r0 + row[u], rtok = a.by_r.of(rr);
-                    const Seen s = seen(a, p0 + rtok, it.len);
-                    const bool none = s.last < s.first, gone = s.last >= room;
+                    if (q0 + u * apart >= quads) break;
                     float out[4];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) out[j] = none ? 0.0f : gone ? NAN : o[u][j] / sum[u];
-                    store4<BF16>(a, (size_t)(n0 + rtok) * a.ldo + (size_t)(it.kh * R + rr - rtok * R) * HD, 4 * quad[u], out);
+                    for (int j = 0; j < 4; j++) out[j] = none ? 0.0f : gone ? NAN : o[u][j] / sum;
+                    store4<BF16>(a, to, 4 * (q0 + u * apart), out);
                 }
             }
         };
-        if (parts <= 4 && outs > NT) join(std::integral_constant<int, 2>{});
-        else join(std::integral_constant<int, 1>{});
+        if (each == 1) join(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+        else join(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
     }
 #endif
 }

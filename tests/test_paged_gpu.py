@@ -667,6 +667,21 @@ def test_attention_long_context_beside_short_ones(be, kind):
 
 
 @both
+@pytest.mark.parametrize("NH,NKV,HD", [(3, 1, 64), (5, 1, 72), (4, 2, 128), (2, 1, 200)])
+@pytest.mark.parametrize("new,total", [([11], [1500]), ([22, 9], [1300, 2000]), ([43], [1900]), ([100, 1], [1111, 1])])
+def test_attention_rows_in_parts(be, new, total, NH, NKV, HD, kind):
+    """More rows than one wave's over keys that are split: every number of rows a unit's records may lie in, at heads whose
+    outputs do and do not go round evenly in its lanes."""
+    rng = np.random.default_rng(sum(new) + HD)
+    b = Batch(be, rng, kind, new, total, 16, NKV, HD)
+    b.fill(rng)
+    q = kind.held(rng.standard_normal((b.N, NH, HD)))
+    scale = float(np.float32(HD ** -0.5))
+    want, off = attend(b, q, NH, scale)
+    compare(b, attention(be, b, q, NH, scale), want, off)
+
+
+@both
 def test_attention_a_cache_past_32_bits(be, kind):
     """Pages whose elements lie past 2^32 bytes and past 2^31 elements of the cache's start."""
     NKV, HD, page = 1, 64, 65536
