@@ -850,57 +850,56 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
             }
             __builtin_amdgcn_s_waitcnt(0x0F70); /* none under way */
         } else if constexpr (W::SHARED) {
-            /* Through registers: thread's part i of a tile is eight values, chunk c = x % C3 of row x / C3, x = i NT + t, of keys
-             * and of values, split into their terms on the way into LDS, two tiles in turn. */
+            /* Through registers: piece x = i NT + t of a tile is eight values, chunk c of a row, of keys, then of values, split
+             * into their terms on the way into LDS, two tiles in turn. */
             typedef Tile<TERMS3, HDP> T3;
-            constexpr int C3 = T3::CPR, PER = KT * C3 / NT;
-            static_assert(KT * C3 % NT == 0 && 2 * T3::BYTES <= W::BYTES, "whole parts, two tiles");
-            f32x4 kr[PER][2], vr[PER][2];
-            auto fetch = [&](int kt) {
+            constexpr int C3 = T3::CPR, HALF = KT * C3, PER = 2 * HALF / NT;
+            static_assert(2 * HALF % NT == 0 && HALF % 64 == 0 && 2 * T3::BYTES <= W::BYTES, "whole pieces, a wave's of keys or of values, two tiles");
+            constexpr int RPP = 64 / C3; /* rows of a wave's piece, in one page */
+            f32x4 raw[PER][2];
+            int pg[PER];
+            const int off = 8 * (lane % C3) < HD ? lane / C3 * rowb + 32 * (lane % C3) : 1 << 30;
+            auto row_of = [&](int i) { return (i * NT / 64 + wave) % (HALF / 64) * RPP; };
+            auto part_of = [&](int i) { return (i * NT / 64 + wave) / (HALF / 64); };
+            auto pages = [&](int kt) {
+#pragma unroll
+                for (int i = 0; i < PER; i++) pg[i] = page_of(kt * KT + row_of(i));
+            };
+            auto fetch = [&](int kt) __attribute__((always_inline)) {
 #pragma unroll
                 for (int i = 0; i < PER; i++) {
-                    const int x = i * NT + t, row = x / C3, c = x % C3, key = kt * KT + row;
-                    int pg = -2;
-                    if (key < hi) {
-                        pg = table[key >> b.shift];
-                        if (pg < 0 || pg >= b.n_pages) pg = -1;
-                    }
-                    const size_t at = b.base(max(pg, 0), 0, it.kh) + (size_t)((key & mask) * HD + 8 * c);
-                    const bool there = pg >= 0 && 8 * c < HD;
-                    const float fill = pg == -1 && 8 * c < HD ? NAN : 0.0f;
-                    const f32x4* k = (const f32x4*)((const float*)a.cache + at);
-                    const f32x4* v = (const f32x4*)((const float*)a.cache + at + (size_t)b.NKV * kv);
+                    const int key = kt * KT + row_of(i), part = part_of(i);
+                    const bool there = (unsigned int)pg[i] < (unsigned int)b.n_pages;
+                    const char* k = (const char*)a.cache + (there ? pg[i] : 0) * page_bytes + kh_bytes + (unsigned int)((key & mask) * rowb);
+                    const auto from = __builtin_amdgcn_make_buffer_rsrc((void*)scalar(part ? k + page_bytes / 2 : there ? k : (const char*)pg_nans), 0,
+                                                                        scalar(part && !there ? 0 : min(max(end - key, 0), RPP) * rowb), 0x00027000);
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        kr[i][e] = there ? k[e] : f32x4{fill, fill, fill, fill};
-                        vr[i][e] = there ? v[e] : f32x4{0, 0, 0, 0};
-                    }
+                    for (int e = 0; e < 2; e++) raw[i][e] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, off + 16 * e, 0, 0));
                 }
             };
             auto put = [&](unsigned char* buf) {
 #pragma unroll
                 for (int i = 0; i < PER; i++) {
-                    const int x = i * NT + t, row = x / C3, c = x % C3;
+                    const int part = part_of(i), row = row_of(i) + lane / C3, c = lane % C3;
+                    unsigned int z[4][3];
 #pragma unroll
-                    for (int part = 0; part < 2; part++) {
-                        const f32x4* src = part ? vr[i] : kr[i];
-                        unsigned int z[4][3];
+                    for (int e = 0; e < 4; e++) split2(raw[i][e >> 1][2 * (e & 1)], raw[i][e >> 1][2 * (e & 1) + 1], z[e]);
+                    unsigned char* to = buf + part * 3 * T3::PLANE + row * T3::ROWB + 16 * (part ? v_place<TERMS3, C3>(row, c) : k_place<C3>(row, c));
 #pragma unroll
-                        for (int e = 0; e < 4; e++) split2(src[e >> 1][2 * (e & 1)], src[e >> 1][2 * (e & 1) + 1], z[e]);
-                        unsigned char* to = buf + part * 3 * T3::PLANE + row * T3::ROWB + 16 * (part ? v_place<TERMS3, C3>(row, c) : k_place<C3>(row, c));
-#pragma unroll
-                        for (int y = 0; y < 3; y++) *(u32x4*)(to + y * T3::PLANE) = u32x4{z[0][y], z[1][y], z[2][y], z[3][y]};
-                    }
+                    for (int w = 0; w < 3; w++) *(u32x4*)(to + w * T3::PLANE) = u32x4{z[0][w], z[1][w], z[2][w], z[3][w]};
                 }
             };
+            pages(kt0);
             q_request();
-            if (kt0 < kt1) fetch(kt0);
+            fetch(kt0);
+            pages(kt0 + 1);
             q_take();
             for (int kt = kt0; kt < kt1; kt++) {
                 unsigned char* buf = lds0 + ((kt - kt0) & 1) * T3::BYTES;
                 put(buf);
                 __syncthreads(); /* the tile is there, and the one before has been read */
-                if (kt + 1 < kt1) fetch(kt + 1);
+                fetch(kt + 1); /* behind the part's last: zeros */
+                pages(kt + 2);
                 compute(std::integral_constant<int, TERMS3>{}, buf, kt);
             }
         }
