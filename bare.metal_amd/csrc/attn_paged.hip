@@ -52,9 +52,9 @@ constexpr int MANY_LEAST = 8;    /* of more than 32 rows */
 constexpr int CUS = 256, ROUNDS = 4, ROUND_TILES = 32;
 
 /* The scratch memory begins with arrival counters, each on a line of its own, that are zero between launches of any
- * kernel; the units' partial results lie behind them. */
+ * kernel; a table of the work and the units' partial results lie behind them. */
 constexpr int DONE_STRIDE = 32, MAX_UNITS = 1024;
-constexpr size_t DONE_BYTES = (size_t)DONE_STRIDE * MAX_UNITS * 4;
+constexpr size_t DONE_BYTES = (size_t)DONE_STRIDE * MAX_UNITS * 4, TABLE_BYTES = 1024;
 
 struct PaArgs {
     const void* q;
@@ -72,6 +72,7 @@ struct PaArgs {
     unsigned int flip; /* scale's sign, for q's */
     unsigned int most; /* rows' records that fit behind the counters */
     int slots; /* workgroups that run at once */
+    const struct Table* table; /* of many sequences, else NULL */
 };
 
 /* How a tile lies in LDS: keys, then values, a row behind the other, HDP elements each (the head size rounded up, with zeros
@@ -213,18 +214,25 @@ __device__ __forceinline__ int dpp_most(int v) { /* of values from 0 on */
     return __builtin_amdgcn_readlane(v, 63);
 }
 
-/* What is to be done, from the tables alone: every wave finds it for itself, 64 sequences at a time; up to 64 stay in
- * registers. */
-template <int ROWS>
-struct Plan {
-    const PaArgs& a;
-    const int lane;
-    Seq first;
+/* Sums of pieces of work, records and units in parts, over sequences. */
+struct Sums {
+    unsigned int w, recs, units;
+};
+/* Of more sequences than a wave has lanes, a kernel ahead lays out the work: here, of each 64 sequences, the sums up to their
+ * end.  (Every wave for itself, 64 sequences at a time: 128 sequences of 512 keys 18.7 us, with the table 18.2; 512 of them 93
+ * and 66, 4096 2165 and 490; up to 64, where the registers hold all, the launch would cost more than it gives.) */
+struct Table {
     int per;            /* tiles a part */
-    unsigned int total; /* pieces of work; 0 where the tables are none */
-    struct Sums { /* of pieces, records and units in parts, over a chunk's sequences up to the lane's */
-        unsigned int w, recs, units;
-    } sums;
+    unsigned int total; /* pieces of work */
+    Sums upto[PG_MAX_SEQS / 64];
+};
+static_assert(sizeof(Table) <= TABLE_BYTES && PG_MAX_SEQS == 64 * 64, "a lane of a wave for each 64 sequences");
+
+/* How sequences are cut into units of ROWS rows and those into parts of keys. */
+template <int ROWS>
+struct Cut {
+    const PaArgs& a;
+    int per; /* tiles a part */
 
     __device__ __forceinline__ Seq seq(int s) const {
         Seq q = {};
@@ -240,8 +248,8 @@ struct Plan {
         }
         return q;
     }
-    __device__ __forceinline__ Seq chunk(int c) const { return c ? seq(c + lane) : first; }
-    /* of a unit of q; of more rows than one wave's, no more than pay for their records (3 parts of 128 rows of 64: 3 us) */
+    /* of a unit of q; of more rows than one wave's, no more than pay for their records (24 mixed sequences, parts of 8 tiles on
+     * 26 us, of 4 or 6 27, of 12 or 16 33) */
     __device__ __forceinline__ unsigned int parts(const Seq& q) const {
         const int p = (q.T + per - 1) / per;
         return max(1, q.n * a.R > 32 ? min(p, q.T / MANY_LEAST) : p);
@@ -250,46 +258,52 @@ struct Plan {
         const unsigned int p = parts(q);
         return Sums{q.units * p * a.b.NKV, p > 1 ? (unsigned int)q.n * a.R * p * a.b.NKV : 0, p > 1 ? q.units * a.b.NKV : 0};
     }
-    __device__ __forceinline__ Sums up_to(const Sums& m) const { return Sums{dpp_sums(m.w), dpp_sums(m.recs), dpp_sums(m.units)}; }
-
-    __device__ __forceinline__ Plan(const PaArgs& args) : a(args), lane(threadIdx.x & 63) {
-        first = seq(lane);
-        float tiles = 0, units = 0, rows = 0;
-        int longest = 0;
-        for (int c = 0; c < a.b.S; c += 64) {
-            const Seq q = chunk(c);
-            tiles += (float)q.units * (float)q.T;
-            units += (float)q.units;
-            rows += (float)q.n;
-            longest = max(longest, q.T);
-        }
-        tiles = lane_of(dpp_sums(tiles), 63) * a.b.NKV;
-        units = lane_of(dpp_sums(units), 63) * a.b.NKV;
-        rows = lane_of(dpp_sums(rows), 63);
-        longest = dpp_most(longest);
+    static __device__ __forceinline__ Sums up_to(const Sums& m) { return Sums{dpp_sums(m.w), dpp_sums(m.recs), dpp_sums(m.units)}; }
+    /* from the sums over all sequences: of units times their tiles and of units, and the most tiles of one */
+    __device__ __forceinline__ void begin(float tiles, float units, int longest) {
+        tiles *= a.b.NKV;
+        units *= a.b.NKV;
         const float want = a.slots * fminf(fmaxf(tiles / (a.slots * ROUND_TILES), 1.0f), ROUNDS);
         per = max(max((int)(tiles / fmaxf(want - 0.5f * units, 0.25f * want)) + 1, LEAST), (longest + MAX_SPLIT - 1) / MAX_SPLIT);
-        if (!a.most) per = max(longest, 1);
-        per = __builtin_amdgcn_readfirstlane(per);
+        per = scalar(per);
+    }
+    /* whether the records and counters do; else the parts are longer; ends at one part a unit */
+    __device__ __forceinline__ bool fits(float recs, float units, int longest) {
+        if (per >= longest || (recs * 1.0001f < (float)a.most && units <= (float)MAX_UNITS)) return true;
+        per = scalar(per > longest / 2 ? longest : 2 * per);
+        return false;
+    }
+    /* no batch: sequences that overlap */
+    __device__ __forceinline__ bool overlap(float rows) const { return rows > (float)a.b.N * 1.0001f; }
+};
+
+/* What is to be done: of up to 64 sequences every wave finds it for itself, a sequence a lane; of more, from the table. */
+template <int ROWS>
+struct Plan {
+    Cut<ROWS> cut;
+    const PaArgs& a;
+    const int lane;
+    Seq first;
+    unsigned int total; /* pieces of work; 0 where the tables are none */
+    Sums sums;          /* over the sequences up to the lane's; over the table's entries up to the lane's */
+
+    __device__ __forceinline__ Plan(const PaArgs& args) : cut{args, 0}, a(args), lane(threadIdx.x & 63) {
+        if (a.table) {
+            cut.per = a.table->per;
+            total = a.table->total;
+            sums = a.table->upto[lane];
+            return;
+        }
+        first = cut.seq(lane);
+        const int longest = dpp_most(first.T);
+        cut.begin(lane_of(dpp_sums((float)first.units * (float)first.T), 63), lane_of(dpp_sums((float)first.units), 63), longest);
         total = 0;
-        if (rows > (float)a.b.N * 1.0001f) return; /* sequences that overlap: no batch */
-        for (;;) { /* parts as long as their records and counters need; ends at one part a unit */
-            float recs = 0;
-            units = 0;
-            for (int c = 0; c < a.b.S; c += 64) {
-                const Sums m = own(chunk(c));
-                recs += (float)m.recs;
-                units += (float)m.units;
-                if (c == 0) {
-                    sums = up_to(m);
-                    total = 0;
-                }
-                total += c == 0 ? lane_of(sums.w, 63) : lane_of(dpp_sums(m.w), 63);
-            }
-            recs = lane_of(dpp_sums(recs), 63);
-            units = lane_of(dpp_sums(units), 63);
-            if (per >= longest || (recs * 1.0001f < (float)a.most && units <= (float)MAX_UNITS)) return;
-            per = __builtin_amdgcn_readfirstlane(per > longest / 2 ? longest : 2 * per);
+        if (cut.overlap(lane_of(dpp_sums((float)first.n), 63))) return;
+        for (;;) {
+            const Sums m = cut.own(first);
+            sums = cut.up_to(m);
+            total = lane_of(sums.w, 63);
+            if (cut.fits(lane_of(dpp_sums((float)m.recs), 63), lane_of(dpp_sums((float)m.units), 63), longest)) return;
         }
     }
 
@@ -301,36 +315,98 @@ struct Plan {
     /* piece w < total of the work: within a sequence the KV heads side by side, the last units, which see the most keys, first */
     __device__ __forceinline__ Item item(unsigned int w) const {
         Item it = {};
-        unsigned int recs = 0, units = 0;
-        for (int c = 0; c < a.b.S; c += 64) {
-            const Seq q = chunk(c);
-            const Sums m = own(q), up = c ? up_to(m) : sums;
-            const unsigned long long past = __ballot(up.w > w);
-            if (past) {
-                const int l = __builtin_ctzll(past);
-                it.s = c + l;
-                it.start = lane_of(q.start, l);
-                it.n = lane_of(q.n, l);
-                it.len = lane_of(q.len, l);
-                it.parts = (int)lane_of(parts(q), l);
-                const unsigned int local = w - lane_of(up.w - m.w, l), nu = lane_of(q.units, l);
-                const int rest = a.by_kv.of(local);
-                it.kh = (int)local - rest * a.b.NKV;
-                const int back = it.parts == 1 ? rest : rest / it.parts;
-                it.part = rest - back * it.parts;
-                it.unit = (int)nu - 1 - back;
-                it.rec = recs + lane_of(up.recs - m.recs, l);
-                it.done = units + lane_of(up.units - m.units, l) + it.unit * a.b.NKV + it.kh;
-                return it;
-            }
-            w -= lane_of(up.w, 63);
-            recs += lane_of(up.recs, 63);
-            units += lane_of(up.units, 63);
-        }
         it.s = -1;
+        Sums before = {};
+        int c = 0;
+        Seq q = first;
+        Sums m, up = sums;
+        if (a.table) {
+            c = __builtin_ctzll(__ballot(sums.w > w) | 1ull << 63);
+            if (c) before = Sums{lane_of(sums.w, c - 1), lane_of(sums.recs, c - 1), lane_of(sums.units, c - 1)};
+            q = cut.seq(64 * c + lane);
+            up = cut.up_to(cut.own(q));
+            w -= before.w;
+        }
+        m = cut.own(q);
+        const unsigned long long past = __ballot(up.w > w);
+        if (!past) return it;
+        const int l = __builtin_ctzll(past);
+        it.s = 64 * c + l;
+        it.start = lane_of(q.start, l);
+        it.n = lane_of(q.n, l);
+        it.len = lane_of(q.len, l);
+        it.parts = (int)lane_of(cut.parts(q), l);
+        const unsigned int local = w - lane_of(up.w - m.w, l), nu = lane_of(q.units, l);
+        const int rest = a.by_kv.of(local);
+        it.kh = (int)local - rest * a.b.NKV;
+        const int back = it.parts == 1 ? rest : rest / it.parts;
+        it.part = rest - back * it.parts;
+        it.unit = (int)nu - 1 - back;
+        it.rec = before.recs + lane_of(up.recs - m.recs, l);
+        it.done = before.units + lane_of(up.units - m.units, l) + it.unit * a.b.NKV + it.kh;
         return it;
     }
 };
+
+/* The table, by one workgroup: a wave has every sixteenth 64 sequences, in registers. */
+template <int ROWS>
+__global__ __launch_bounds__(1024) void k_attn_paged_plan(PaArgs a, Table* table) {
+    constexpr int WAVES = 16, MINE = PG_MAX_SEQS / 64 / WAVES;
+    __shared__ float sum[2][3][WAVES];
+    __shared__ int most[WAVES];
+    __shared__ Sums of64[PG_MAX_SEQS / 64];
+    const int t = threadIdx.x, wave = scalar(t >> 6), lane = t & 63;
+    Cut<ROWS> cut{a, 0};
+    Seq q[MINE];
+    float tiles = 0, units = 0, rows = 0;
+    int longest = 0;
+#pragma unroll
+    for (int i = 0; i < MINE; i++) {
+        q[i] = cut.seq(64 * (wave + WAVES * i) + lane);
+        tiles += (float)q[i].units * (float)q[i].T;
+        units += (float)q[i].units;
+        rows += (float)q[i].n;
+        longest = max(longest, q[i].T);
+    }
+    auto all = [&](int turn, float x, float y, float z) __attribute__((always_inline)) { /* over the workgroup, in x, y, z's places */
+        const float v[3] = {lane_of(dpp_sums(x), 63), lane_of(dpp_sums(y), 63), lane_of(dpp_sums(z), 63)};
+        if (lane == 0)
+            for (int k = 0; k < 3; k++) sum[turn][k][wave] = v[k];
+        __syncthreads();
+    };
+    auto total = [&](int turn, int k) {
+        float v = 0;
+        for (int i = 0; i < WAVES; i++) v += sum[turn][k][i];
+        return v;
+    };
+    longest = dpp_most(longest);
+    if (lane == 0) most[wave] = longest;
+    all(0, tiles, units, rows);
+    for (int i = 0; i < WAVES; i++) longest = max(longest, most[i]);
+    cut.begin(total(0, 0), total(0, 1), longest);
+    const bool none = cut.overlap(total(0, 2));
+    for (int turn = 1;; turn ^= 1) {
+        float recs = 0;
+        units = 0;
+#pragma unroll
+        for (int i = 0; i < MINE; i++) {
+            const Sums m = cut.own(q[i]), up = cut.up_to(m);
+            recs += (float)m.recs;
+            units += (float)m.units;
+            if (lane == 63) of64[wave + WAVES * i] = up;
+        }
+        all(turn, recs, units, 0.0f);
+        if (cut.fits(total(turn, 0), total(turn, 1), longest)) break;
+        __syncthreads(); /* of64 has not been read; sum[turn] is not written before the next turn's barrier */
+    }
+    if (wave) return;
+    const Sums up = cut.up_to(of64[lane]);
+    table->upto[lane] = up;
+    if (lane == 63) {
+        table->per = cut.per;
+        table->total = none ? 0 : up.w;
+    }
+}
 
 /* keys that a row at position p sees: first .. last */
 struct Seen {
@@ -397,7 +473,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
         /* tiles of keys that some row of the unit sees, and this part's */
         const int lo = seen(a, p0 + tok0, it.len).first, hi = min(seen(a, p0 + tok1, it.len).last + 1, room);
         const int t0 = lo / KT, t1 = hi > lo ? (hi + KT - 1) / KT : t0;
-        const int parts = max(1, min(it.parts, (t1 - t0 + plan.per - 1) / plan.per)), per = (t1 - t0 + parts - 1) / parts; /* as even as they go */
+        const int parts = max(1, min(it.parts, (t1 - t0 + plan.cut.per - 1) / plan.cut.per)), per = (t1 - t0 + parts - 1) / parts; /* as even as they go */
         if (it.part >= parts) return;
         const int kt0 = t0 + it.part * per, kt1 = min(kt0 + per, t1);
         /* waves side by side on rows, the rest in turns on the keys, 32 at a time */
@@ -1083,12 +1159,17 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
 template <bool BF16, int HDP>
 int start(PaArgs& a, const bmk_launch_t* l) {
     typedef Shape<BF16, HDP> W;
-    a.most = 0;
-    if (l->scratch_bytes > DONE_BYTES)
-        a.most = (unsigned int)std::min<size_t>((l->scratch_bytes - DONE_BYTES) / ((HDP + 4) * 4), 1u << 30);
+    BMK_REQUIRE(l->scratch_bytes > DONE_BYTES + TABLE_BYTES, "attention_forward_paged: %zu bytes of scratch memory", l->scratch_bytes);
+    a.most = (unsigned int)std::min<size_t>((l->scratch_bytes - DONE_BYTES - TABLE_BYTES) / ((HDP + 4) * 4), 1u << 30);
     a.done = (unsigned int*)l->scratch;
-    a.rec = (float*)((char*)l->scratch + DONE_BYTES);
+    a.rec = (float*)((char*)l->scratch + DONE_BYTES + TABLE_BYTES);
     a.slots = W::SLOTS;
+    if (a.b.S > 64) {
+        Table* table = (Table*)((char*)l->scratch + DONE_BYTES);
+        hipLaunchKernelGGL((k_attn_paged_plan<W::ROWS>), dim3(1), dim3(1024), 0, l->stream, a, table);
+        BMK_LAUNCH_CHECK();
+        a.table = table;
+    }
     /* A workgroup a piece: no more than a unit for every sequence with new tokens and every ROWS rows, each in one part more
      * than the tiles' share of the plan's want (the 8: sums rounded in fp32). */
     const int64_t units = a.b.NKV * (std::min<int64_t>(a.b.N, a.b.S) + (int64_t)a.b.N * a.R / W::ROWS);

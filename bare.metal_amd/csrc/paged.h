@@ -12,7 +12,7 @@ namespace bmk {
 
 /* Rows, sequences and strides a launch takes at most, so that row and column indexes stay inside an int. */
 constexpr int PG_MAX_DIM = 1 << 30;
-constexpr int PG_MAX_HD = 256, PG_MAX_SEQS = 1 << 20;
+constexpr int PG_MAX_HD = 256, PG_MAX_SEQS = 4096;
 
 /* x / d for x below 2^31 by one product */
 struct Div {

@@ -18,7 +18,7 @@
  * boundary; page a power of two from 8 to 65536, max_pages * page at most 2^30,
  * n_pages * page at most 2^38, NKV at most 4096.
  * A layer's cache goes in by its buffer's offset.
- * The batch: S sequences, at most 2^20; start int32 [S + 1], not falling: the new tokens
+ * The batch: S sequences, at most 4096; start int32 [S + 1], not falling: the new tokens
  * of sequence s are rows start[s] .. start[s + 1] - 1 of N; len int32 [S]:
  * its keys, the new tokens' own included; pages int32 [S][max_pages]: the
  * pages of its keys in order.  Row i of a sequence with n new tokens stands

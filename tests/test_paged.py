@@ -103,7 +103,7 @@ NAMES = {
     "attn_paged": "N S NH NKV HD ldq ldo page n_pages max_pages causal window".split(),
 }
 BAD = {
-    "N": [-1, (1 << 30) + 1], "S": [-1, (1 << 30) + 1], "NH": [-1, (1 << 30) + 1], "NKV": [0, -1, 4097],
+    "N": [-1, (1 << 30) + 1], "S": [-1, 4097, (1 << 30) + 1], "NH": [-1, (1 << 30) + 1], "NKV": [0, -1, 4097],
     "HD": [0, -8, 258, 264, 7], "rot": [-2, 3, 18], "layout": [-1, 2], "page": [0, -8, 1, 4, 12, 131072],
     "n_pages": [0, -1, (1 << 31) - 1], "max_pages": [0, -1, (1 << 30)], "norm": [-1, 2], "causal": [-1, 2], "window": [-1],
 }

@@ -652,6 +652,64 @@ def test_attention_many_sequences(be, kind):
 
 
 @both
+@pytest.mark.parametrize("S,long", [(63, 0), (64, 0), (65, 0), (128, 900), (129, 4000), (1000, 2500), (4096, 0)])
+def test_attention_of_as_many_sequences_as_a_batch_takes(be, S, long, kind):
+    """Up to a wave's lanes and more than them, in 64s that are whole, empty and not; with some long sequences, among them the
+    first and the last, whose keys are split."""
+    rng = np.random.default_rng(S)
+    new = [int(x) for x in rng.choice([0, 1, 1, 1, 2], S)]
+    if S >= 1000:
+        new[128:192] = [0] * 64
+    total = [n + int(rng.integers(0, 40)) if n else 0 for n in new]
+    if long:
+        for s in (0, S // 2, S - 1):
+            new[s], total[s] = 1 + s % 3, long + s
+    b = Batch(be, rng, kind, new, total, 16, 1, 32, 0, 3)
+    b.fill(rng)
+    q = kind.held(rng.standard_normal((b.N, 2, 32)))
+    want, off = attend(b, q, 2, 0.2)
+    first = attention(be, b, q, 2, 0.2)
+    compare(b, first, want, off)
+    assert np.array_equal(attention(be, b, q, 2, 0.2), first)
+
+
+@pytest.mark.parametrize("S", [3, 200])
+@pytest.mark.parametrize("how", ["falling", "overlapping", "negative", "past", "huge", "far"])
+def test_attention_tables_that_are_no_batch(be, S, how):
+    """Whatever start and len hold, rows outside N are not written and the call ends; the next call has its own results."""
+    kind, rng = KINDS[1], np.random.default_rng(5)
+    b = Batch(be, rng, kind, [2] * S, [40] * S, 16, 1, 64)
+    b.fill(rng)
+    q = kind.held(rng.standard_normal((b.N, 2, 64)))
+    want, off = attend(b, q, 2, 0.125)
+    start, length = b.start.copy(), b.len.copy()
+    if how == "falling":
+        start = start[::-1].copy()
+    elif how == "overlapping":
+        start[:-1] = 0
+        start[1::2] = b.N
+    elif how == "negative":
+        start -= b.N // 2
+        length[::2] = -7
+    elif how == "past":
+        start += b.N // 2
+    elif how == "huge":
+        start[1:] = 2 ** 31 - 1
+        length[:] = 2 ** 31 - 1
+    else:
+        length[:] = 2 ** 31 - 1
+    room, past = b.N * 128 * kind.size, 1 << 16
+    out = marked(be, room + past)
+    tables = [be.upload(start), be.upload(length), be.upload(b.pages)]
+    assert be.dispatch("attention_forward_paged_bf16", [be.upload(kind.raw(q)), be.upload(kind.raw(b.cache)), out] + tables + [
+        be.params(b.N, b.S, 2, 1, 64, 128, 128, 16, b.count, b.width, 1, 0), floats(be, 0.125)], (b.N,), (256,)) == 0
+    be.synchronize()
+    mark = marked(be, past).read(np.uint8)
+    assert np.array_equal(out.read(np.uint8)[room:], mark)
+    compare(b, attention(be, b, q, 2, 0.125), want, off)
+
+
+@both
 def test_attention_long_context_beside_short_ones(be, kind):
     """One long sequence (joined from parts where the work is split) among short ones; the same bits every time."""
     rng = np.random.default_rng(13)

@@ -30,6 +30,9 @@ def kernels(name, path):
 def test_attention_keeps_everything_in_registers(tmp_path):
     forms = {}
     for n, u in kernels("attn_paged.hip", str(tmp_path / "a.o")).items():
+        if "k_attn_paged_plan" in n:
+            assert u[1:] == (0, 0)
+            continue
         m = re.match(r"\S*k_attn_pagedILb(\d)ELi(\d+)E", n)
         forms[bool(int(m.group(1))), int(m.group(2))] = u
     assert {f: u[0] for f, u in forms.items()} == {(True, 64): 3, (True, 128): 2, (True, 256): 1, (False, 64): 2,
