@@ -6,20 +6,34 @@
  * in one pass over the keys with the running maximum and sum (fp32) of the
  * softmax.
  *
- * A unit of work is 128 rows (new token, query head of the group) of one
- * sequence and KV head, so that every key and value is read once for a whole
- * group of heads; a unit's keys may be split over workgroups, whose partial
- * results the last one of them joins.  A workgroup goes over its keys in tiles of
- * KT, which lie in LDS in pieces of bf16: bf16 as it is, fp32 as three terms
- * x = x0 + x1 + x2 (truncations, exact), whose products of at least 2^-24 are
- * taken, six of nine.  Each of its four waves has 32 rows; of fewer rows than that, each
- * wave takes a part of the tile's keys instead.  Per 32 keys a wave forms
+ * A unit of work is up to 128 rows (new token, query head of the group; 64 of
+ * fp32 heads over 128) of one sequence and KV head, so that every key and
+ * value is read once for a whole group of heads; a unit's keys may be split
+ * over workgroups, whose partial results the last one of them joins.  The work
+ * goes over the keys in tiles of 32, which the loads put straight into LDS (a
+ * missing page and what lies past the end by the descriptors' bounds):
+ *   up to 32 rows  each of the workgroup's waves takes tiles of its own, with no barrier
+ *   more           every wave has 32 rows of each tile, through a ring of tiles
+ * Per tile a wave forms
  *   S^T (32 keys x 32 rows) = K Q^T,   O^T (HD x 32 rows) += V^T P^T
  * with v_mfma_f32_32x32x16_bf16.  A lane holds the scores of one row (lane %
  * 32) and 16 keys, exactly those whose weights the second product wants of
  * it once its sum runs over the keys in the order of the registers, so P goes
  * from the scores to the product without moving between lanes; V comes
- * transposed out of LDS (ds_read_b64_tr_b16).
+ * transposed out of LDS (ds_read_b64_tr_b16).  fp32 goes in as three terms
+ * x = x0 + x1 + x2 of bf16 (truncations, exact), whose products of at least
+ * 2^-24 are taken, six of nine.  P is rounded to bf16 where q, K and V are
+ * (its sum is not), which is half a step of the output's own type.
+ *
+ * What bounds it (us a pass, MI355X).  One token a sequence: reading the
+ * cache; 64 sequences of 8192 keys, 8 KV heads of 128 in bf16, 233 (5.4 TB/s), 1024 of 512
+ * keys, 5 heads of 64, 124 (5.4).  Few keys: the chain of latencies (the tables 1.5, the
+ * page's number and the first keys 2.5, a tile 1.5, the waves' join 1, records and counter
+ * 1.2, the parts' join 2.5); 300 keys of one token 10 of kernel time.  Long chunks: 2048 tokens
+ * over 16384 keys, 32 heads of 128, 600-630, 515 GFLOP at 0.82-0.86 PFLOP/s: a tile
+ * takes 512 cycles of the matrix cores and some 600 of exponentials and other vector
+ * instructions, which two waves a SIMD overlap in part, at 1.7 GHz (the part's power; the
+ * library's 8192^3 product runs at 1.16 PFLOP/s).  fp32: 512 tokens over 4096 keys, 15 heads of 64, 57.
  */
 #include "paged.h"
 #include "q8_common.h"
@@ -47,9 +61,9 @@ typedef __attribute__((address_space(3))) void lvoid;
 constexpr int KT = 32;           /* keys of a tile */
 constexpr float SLACK = 8.0f;    /* in powers of two: how far a score may pass the running maximum before that moves */
 constexpr int MAX_SPLIT = 128;   /* parts of a unit's keys */
-constexpr int LEAST = 4;         /* tiles a part, at least: one a wave */
-constexpr int MANY_LEAST = 8;    /* of more than 32 rows */
-constexpr int CUS = 256, ROUNDS = 4, ROUND_TILES = 32;
+constexpr int LEAST = 4;         /* tiles a part, at least: one a wave (1 token over 300 keys, parts of 2 15.3 us, 4 15.1, 8 17.5) */
+constexpr int MANY_LEAST = 8;    /* ... of more than 32 rows (Cut::parts) */
+constexpr int CUS = 256, ROUNDS = 4, ROUND_TILES = 32; /* Cut::begin */
 
 /* The scratch memory begins with arrival counters, each on a line of its own, that are zero between launches of any
  * kernel; a table of the work and the units' partial results lie behind them. */
@@ -263,7 +277,10 @@ struct Cut {
     __device__ __forceinline__ void begin(float tiles, float units, int longest) {
         tiles *= a.b.NKV;
         units *= a.b.NKV;
-        const float want = a.slots * fminf(fmaxf(tiles / (a.slots * ROUND_TILES), 1.0f), ROUNDS);
+        /* Parts for all workgroups that run at once, or for several rounds of them, so that ragged lengths even out, where those
+         * parts still have ROUND_TILES tiles (64 ragged sequences of up to 8192 keys 265 -> 235 us); never for two or three, the
+         * last of which would be part empty (4 sequences of 64 rows over 40000 keys, 2 rounds 187 us, 1 145; 2.4 rounds 178). */
+        const float want = a.slots * (tiles >= (float)a.slots * ROUND_TILES * ROUNDS ? ROUNDS : 1.0f);
         per = max(max((int)(tiles / fmaxf(want - 0.5f * units, 0.25f * want)) + 1, LEAST), (longest + MAX_SPLIT - 1) / MAX_SPLIT);
         per = scalar(per);
     }
@@ -476,8 +493,8 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
         const int parts = max(1, min(it.parts, (t1 - t0 + plan.cut.per - 1) / plan.cut.per)), per = (t1 - t0 + parts - 1) / parts; /* as even as they go */
         if (it.part >= parts) return;
         const int kt0 = t0 + it.part * per, kt1 = min(kt0 + per, t1);
-        /* waves side by side on rows, the rest in turns on the keys, 32 at a time */
-        const int groups = nrows <= 32 ? 1 : nrows <= 64 ? 2 : NW, kparts = NW / groups;
+        /* all waves have the same 32 rows and take turns on the keys' tiles, or each has rows of its own and all tiles */
+        const int groups = nrows <= 32 ? 1 : NW, kparts = NW / groups; /* (48 rows in two groups on two parts: 5% more) */
         const int group = wave & (groups - 1), kpart = wave / groups;
         const bool active = 32 * group < nrows;
         const int r = r0 + 32 * group + col, tok = a.by_r.of(r), head = it.kh * R + (r - tok * R);
@@ -983,7 +1000,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
 
         /* the waves' parts of the keys, joined in the first one's registers */
         if (kparts > 1) {
-            const int at = (kpart - 1) * groups + group; /* 0 .. 2 */
+            const int at = kpart - 1; /* all have the same rows */
             /* up to three waves' sums at 16-byte places of the lanes */
             constexpr int SUMS = HDP * 128;
             static_assert(W::ARRAYS == 4 ? SUMS <= W::BYTES : (NW - 1) * SUMS <= W::BYTES, "");
@@ -1004,7 +1021,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
             if (active && !kpart) {
                 for (int k = 1; k < kparts; k++) {
                     /* a part without a finite score has what its scores left there: 0, or NaN */
-                    const int i = (k - 1) * groups + group;
+                    const int i = k - 1;
                     const f32x4* mem = place(i);
                     const float m1 = part_m[i][lane], mx = fmaxf(m, m1);
                     const float f0 = m > -INFINITY ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
@@ -1174,8 +1191,8 @@ int start(PaArgs& a, const bmk_launch_t* l) {
      * than the tiles' share of the plan's want (the 8: sums rounded in fp32). */
     const int64_t units = a.b.NKV * (std::min<int64_t>(a.b.N, a.b.S) + (int64_t)a.b.N * a.R / W::ROWS);
     const int64_t tiles = (a.b.room() + KT - 1) / KT;
-    const double rounds = std::min(std::max((double)units * tiles / ((double)a.slots * ROUND_TILES), 1.0), (double)ROUNDS);
-    const int64_t grid = std::min(units * std::min<int64_t>(tiles, MAX_SPLIT), units + (int64_t)(a.slots * rounds) + 8);
+    const int64_t rounds = units * tiles >= (int64_t)a.slots * ROUND_TILES * ROUNDS ? ROUNDS : 1;
+    const int64_t grid = std::min(units * std::min<int64_t>(tiles, MAX_SPLIT), units + a.slots * rounds + 8);
     hipLaunchKernelGGL((k_attn_paged<BF16, HDP>), dim3((unsigned)grid), dim3(W::NT), 0, l->stream, a);
     BMK_LAUNCH_CHECK();
     return 0;
