@@ -55,11 +55,12 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(1))) void gvoid;
 typedef __attribute__((address_space(3))) void lvoid;
 
 constexpr int KT = 32;           /* keys of a tile */
-constexpr float SLACK = 8.0f;    /* in powers of two: how far a score may pass the running maximum before that moves */
+/* in powers of two: how far a score may pass the running maximum before that moves (32 sequences of 16 tokens over 1500 keys,
+ * with 0 28.8 us, with 8 27.6); fp32's sums have room for more */
+constexpr float SLACK = 8.0f;
 constexpr int MAX_SPLIT = 128;   /* parts of a unit's keys */
 constexpr int LEAST = 4;         /* tiles a part, at least: one a wave (1 token over 300 keys, parts of 2 15.3 us, 4 15.1, 8 17.5) */
 constexpr int MANY_LEAST = 8;    /* ... of more than 32 rows (Cut::parts) */
@@ -234,7 +235,8 @@ struct Sums {
 };
 /* Of more sequences than a wave has lanes, a kernel ahead lays out the work: here, of each 64 sequences, the sums up to their
  * end.  (Every wave for itself, 64 sequences at a time: 128 sequences of 512 keys 18.7 us, with the table 18.2; 512 of them 93
- * and 66, 4096 2165 and 490; up to 64, where the registers hold all, the launch would cost more than it gives.) */
+ * and 66, 4096 2165 and 490; 65 of 16 keys 6.9 and 9.1, which is the launch, so that up to 64, where the registers hold all, there is
+ * none.) */
 struct Table {
     int per;            /* tiles a part */
     unsigned int total; /* pieces of work */
