@@ -150,6 +150,37 @@ def test_rope_rows(be, N, NH, HD, rot, layout, kind):
 
 
 @both
+@pytest.mark.parametrize("layout", [0, 1], ids=["halves", "pairs"])
+def test_rows_past_the_cache_have_the_same_bits(be, layout, kind):
+    """A call of more than 128 MB, which reads past the caches, against its rows in calls of fewer; in place as well."""
+    NH, NKV, HD, rot = 4, 2, 128, 128
+    N = (150 << 20) // ((NH + NKV) * HD * kind.size)
+    rng = np.random.default_rng(8)
+    block = kind.raw(rng.standard_normal((1 << 16) + 7).astype(np.float32))
+    q, k = np.resize(block, (N, NH * HD)), np.resize(block[::-1], (N, NKV * HD))
+    pos = (np.arange(N) % 50000).astype(np.int32)
+    table, m = turn_table(rot, "none")
+    gain = rng.standard_normal((2, HD)).astype(np.float32)
+    src, out = [be.upload(q), be.upload(k)], [marked(be, q.nbytes), marked(be, k.nbytes)]
+    rest = [be.upload(pos), be.upload(table), be.upload(gain)]
+
+    def run(src, out, first, n):
+        shift = [first * NH * HD * kind.size, first * NKV * HD * kind.size] * 2 + [first * 4, 0, 0, 0, 0]
+        assert be.dispatch("qk_norm_rope_forward" + kind.suffix, src + out + rest + [
+            be.params(n, NH, NKV, HD, rot, layout, NH * HD, NKV * HD, NH * HD, NKV * HD), floats(be, m, 1e-5)], (n,), (256,),
+            offsets=shift) == 0
+
+    for first in range(0, N, 30000):
+        run(src, out, first, min(30000, N - first))
+    want = [x.read(np.uint8) for x in out]
+    out = [marked(be, q.nbytes), marked(be, k.nbytes)]
+    run(src, out, 0, N)
+    run(src, src, 0, N)
+    for x in (out, src):
+        assert all(np.array_equal(a.read(np.uint8), w) for a, w in zip(x, want))
+
+
+@both
 def test_rope_leaves_the_rest_of_a_head(be, kind):
     """Elements from rot on come through bit for bit, infinities and NaN too, and do not touch the turned ones."""
     N, NH, HD, rot = 3, 4, 64, 32
