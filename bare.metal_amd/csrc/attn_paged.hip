@@ -283,7 +283,14 @@ struct Cut {
          * parts still have ROUND_TILES tiles (64 ragged sequences of up to 8192 keys 265 -> 235 us); never for two or three, the
          * last of which would be part empty (4 sequences of 64 rows over 40000 keys, 2 rounds 187 us, 1 145; 2.4 rounds 178). */
         const float want = a.slots * (tiles >= (float)a.slots * ROUND_TILES * ROUNDS ? ROUNDS : 1.0f);
-        per = max(max((int)(tiles / fmaxf(want - 0.5f * units, 0.25f * want)) + 1, LEAST), (longest + MAX_SPLIT - 1) / MAX_SPLIT);
+        auto over = [](float x, float y) { return x * __builtin_amdgcn_rcpf(y); };
+        int p = (int)over(tiles, fmaxf(want - 0.5f * units, 0.25f * want)) + 1;
+        /* were all as long as the longest: no parts that only just do not fit (24 sequences of 4000 keys, 8 heads of 128, in three
+         * parts 81 us, in two 72) */
+        const float alike = over(tiles, (float)max(longest, 1));
+        if (alike * ceilf(over((float)longest, (float)p) - 0.001f) > want)
+            p = (int)ceilf(over((float)longest, fmaxf(floorf(over(want, alike)), 1.0f)) - 0.001f);
+        per = max(max(p, LEAST), (longest + MAX_SPLIT - 1) / MAX_SPLIT);
         per = scalar(per);
     }
     /* whether the records and counters do; else the parts are longer; ends at one part a unit */
