@@ -291,6 +291,7 @@ struct Cut {
         if (alike * ceilf(over((float)longest, (float)p) - 0.001f) > want)
             p = (int)ceilf(over((float)longest, fmaxf(floorf(over(want, alike)), 1.0f)) - 0.001f);
         per = max(max(p, LEAST), (longest + MAX_SPLIT - 1) / MAX_SPLIT);
+        if (!a.most) per = max(longest, 1); /* no memory for records */
         per = scalar(per);
     }
     /* whether the records and counters do; else the parts are longer; ends at one part a unit */
@@ -1185,11 +1186,23 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
 template <bool BF16, int HDP>
 int start(PaArgs& a, const bmk_launch_t* l) {
     typedef Shape<BF16, HDP> W;
-    BMK_REQUIRE(l->scratch_bytes > DONE_BYTES + TABLE_BYTES, "attention_forward_paged: %zu bytes of scratch memory", l->scratch_bytes);
-    a.most = (unsigned int)std::min<size_t>((l->scratch_bytes - DONE_BYTES - TABLE_BYTES) / ((HDP + 4) * 4), 1u << 30);
+    a.most = 0;
+    if (l->scratch_bytes > DONE_BYTES + TABLE_BYTES)
+        a.most = (unsigned int)std::min<size_t>((l->scratch_bytes - DONE_BYTES - TABLE_BYTES) / ((HDP + 4) * 4), 1u << 30);
     a.done = (unsigned int*)l->scratch;
     a.rec = (float*)((char*)l->scratch + DONE_BYTES + TABLE_BYTES);
     a.slots = W::SLOTS;
+    if (a.b.S > 64 && !a.most) { /* no memory for the table */
+        PaArgs some = a;
+        for (int s = 0; s < a.b.S; s += 64) {
+            some.b.S = std::min(a.b.S - s, 64);
+            some.b.start = a.b.start + s;
+            some.b.len = a.b.len + s;
+            some.b.pages = a.b.pages + (size_t)s * a.b.max_pages;
+            if (int rc = start<BF16, HDP>(some, l)) return rc;
+        }
+        return 0;
+    }
     if (a.b.S > 64) {
         Table* table = (Table*)((char*)l->scratch + DONE_BYTES);
         hipLaunchKernelGGL((k_attn_paged_plan<W::ROWS>), dim3(1), dim3(1024), 0, l->stream, a, table);

@@ -2,6 +2,8 @@
 """Serving from a paged cache (include/bm_paged.h) through the backend's C ABI against the formulas in 64 bits.
 
 Tolerances count roundings: U32 = 2^-24 and UB16 = 2^-8, half a step relative to the value."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -873,6 +875,41 @@ def test_agrees_with_the_one_sequence_kernels(be):
     want, off = attend(b, q.reshape(1, NH, HD), NH, 0.125)
     check(KINDS[0], got, want, off)
     check(KINDS[0], out1.read(np.float32).reshape(1, NH, HD), want, off)
+
+
+class Context(ctypes.Structure):
+    """backend_ctx_t up to its scratch memory (include/backend_hip_device.h)."""
+    _fields_ = [("device", ctypes.c_void_p), ("queue", ctypes.c_void_p), ("library", ctypes.c_void_p),
+                ("supports_bf16", ctypes.c_int), ("allocated", ctypes.c_size_t), ("peak", ctypes.c_size_t),
+                ("threads", ctypes.c_int), ("memory", ctypes.c_size_t), ("most", ctypes.c_size_t), ("working", ctypes.c_size_t),
+                ("unified", ctypes.c_int), ("cus", ctypes.c_int), ("clock", ctypes.c_int), ("name", ctypes.c_char * 64),
+                ("busy", ctypes.c_double), ("buffers", ctypes.c_uint64), ("submitted", ctypes.c_uint64),
+                ("done", ctypes.c_uint64), ("events", ctypes.c_void_p * 32), ("n_events", ctypes.c_int),
+                ("last_stop", ctypes.c_void_p), ("last_stop_epoch", ctypes.c_uint64), ("scratch", ctypes.c_void_p),
+                ("scratch_bytes", ctypes.c_size_t)]
+
+
+@both
+@pytest.mark.parametrize("keep", [0, 1 << 17, (1 << 17) + 1024 + 40000], ids=["none", "counters", "little"])
+@pytest.mark.parametrize("S", [5, 150])
+def test_attention_without_memory_for_parts(S, keep, kind):
+    """A context that got no scratch memory, or next to none: the same rows, in fewer parts or unsplit."""
+    other = bmhip.Backend()
+    try:
+        c = Context.from_address(other.ctx)
+        assert c.scratch_bytes == 64 << 20 and c.scratch
+        c.scratch_bytes = keep
+        rng = np.random.default_rng(S)
+        new = [1 + s % 3 for s in range(S)]
+        total = [n + (3000 if s in (1, S - 1) else 20) for s, n in enumerate(new)]
+        new[2], total[2] = 60, 1000
+        b = Batch(other, rng, kind, new, total, 16, 2, 64)
+        b.fill(rng)
+        q = kind.held(rng.standard_normal((b.N, 6, 64)))
+        want, off = attend(b, q, 6, 0.125)
+        compare(b, attention(other, b, q, 6, 0.125), want, off)
+    finally:
+        other.close()
 
 
 def test_two_contexts_at_once(be):
