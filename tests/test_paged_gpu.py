@@ -877,6 +877,38 @@ def test_agrees_with_the_one_sequence_kernels(be):
     check(KINDS[0], out1.read(np.float32).reshape(1, NH, HD), want, off)
 
 
+@both
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.3, 1e-30, 3.0])
+@pytest.mark.parametrize("new,total,window", [([1, 3], [70, 20], 0), ([40], [90], 16), ([5, 1], [33, 1500], 0)])
+def test_attention_scales(be, new, total, window, scale, kind):
+    """No order among the keys (scale 0: the mean of the values a row sees), the smallest one first, one that takes all."""
+    rng = np.random.default_rng(len(new) + window)
+    b = Batch(be, rng, kind, new, total, 16, 2, 64)
+    b.fill(rng)
+    q = kind.held(rng.standard_normal((b.N, 4, 64)))
+    scale = float(np.float32(scale))
+    want, off = attend(b, q, 4, scale, window=window)
+    compare(b, attention(be, b, q, 4, scale, window=window), want, off)
+
+
+@both
+def test_attention_of_a_shared_prefix(be, kind):
+    """Sequences whose first pages are the same ones, as after a common prompt, and one that is the same altogether."""
+    rng = np.random.default_rng(21)
+    new, total, page = [1, 2, 1, 1, 30], [100, 90, 100, 64, 94], 16
+    b = Batch(be, rng, kind, new, total, page, 2, 64)
+    b.fill(rng)
+    for s in range(1, 5):
+        n = 6 if s == 2 else 4
+        b.pages[s, :n] = b.pages[0, :n]
+        for x in (b.K, b.V):
+            x[s][:, :min(n * page, total[s])] = x[0][:, :min(n * page, total[s])]
+    b.pages[2], b.K[2], b.V[2] = b.pages[0], b.K[0], b.V[0]
+    q = kind.held(rng.standard_normal((b.N, 6, 64)))
+    want, off = attend(b, q, 6, 0.125)
+    compare(b, attention(be, b, q, 6, 0.125), want, off)
+
+
 class Context(ctypes.Structure):
     """backend_ctx_t up to its scratch memory (include/backend_hip_device.h)."""
     _fields_ = [("device", ctypes.c_void_p), ("queue", ctypes.c_void_p), ("library", ctypes.c_void_p),
