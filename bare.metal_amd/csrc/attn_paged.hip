@@ -480,7 +480,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
     /* a ring of four arrays, not one array: reads of one then wait for no load into another */
     constexpr int REST = W::ARRAYS == 4 ? W::BYTES : 16;
     __shared__ __attribute__((aligned(16))) unsigned char lds0[W::BYTES], lds1[REST], lds2[REST], lds3[REST];
-    __shared__ float part_m[3][64], part_l[3][64];
+    __shared__ float part_m[NW][32], part_l[NW][32];
     __shared__ int last_one;
     const PgBatch& b = a.b;
     const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
@@ -1008,87 +1008,86 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
         }
         l += other_half(l);
 
-        /* the waves' parts of the keys, joined in the first one's registers */
+        constexpr int REC = HDP + 4, SC1 = 16;
+        const int part_bytes = nrows * REC * 4, quads = HD / 4;
+        const auto recs = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)scalar((const char*)(a.rec + ((size_t)it.rec + (size_t)it.parts * ((size_t)rows_all * it.kh + r0)) * REC)), 0,
+            scalar(parts * part_bytes), 0x00027000);
+        auto put = [&](int row, int quad, f32x4 x) __attribute__((always_inline)) {
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), recs, it.part * part_bytes + (quad * nrows + row) * 16, 0, SC1);
+        };
+        /* four outputs of a row, of its sums */
+        auto finish = [&](int row, int quad, f32x4 x, float sum) __attribute__((always_inline)) {
+            const int rr = r0 + row, rtok = a.by_r.of(rr);
+            const Seen s = seen(a, p0 + rtok, it.len);
+            const bool none = s.last < s.first, gone = s.last >= room;
+            float out[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) out[j] = none ? 0.0f : gone ? NAN : x[j] / sum;
+            store4<BF16>(a, (size_t)(n0 + rtok) * a.ldo + (size_t)(it.kh * R + rr - rtok * R) * HD, 4 * quad, out);
+        };
         if (kparts > 1) {
-            const int at = kpart - 1; /* all have the same rows */
-            /* up to three waves' sums at 16-byte places of the lanes */
+            /* The waves' sums of the same rows, each in its own tile's place, joined four outputs a lane. */
             constexpr int SUMS = HDP * 128;
-            static_assert(W::ARRAYS == 4 ? SUMS <= W::BYTES : (NW - 1) * SUMS <= W::BYTES, "");
-            auto place = [&](int i) {
-                return (f32x4*)(W::ARRAYS == 1 ? lds0 + i * SUMS : i == 0 ? lds0 : i == 1 ? lds1 : lds2) + lane;
+            static_assert(SUMS <= T::BYTES, "");
+            auto place = [&](int w) {
+                return (f32x4*)(W::ARRAYS == 1 ? lds0 + w * T::BYTES : w == 0 ? lds0 : w == 1 ? lds1 : w == 2 ? lds2 : lds3);
             };
-            __syncthreads();
-            if (active && kpart) {
-                f32x4* mem = place(at);
-                part_m[at][lane] = m;
-                part_l[at][lane] = l;
+            if (mine) {
+                f32x4* mem = place(wave) + col;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) mem[(4 * d + e) * 64] = f32x4{acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2], acc[d][4 * e + 3]};
-            }
-            __syncthreads();
-            if (active && !kpart) {
-                for (int k = 1; k < kparts; k++) {
-                    /* a part without a finite score has what its scores left there: 0, or NaN */
-                    const int i = k - 1;
-                    const f32x4* mem = place(i);
-                    const float m1 = part_m[i][lane], mx = fmaxf(m, m1);
-                    const float f0 = m > -INFINITY ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
-                    const float f1 = m1 > -INFINITY ? __builtin_amdgcn_exp2f(m1 - mx) : 1.0f;
-                    l = l * f0 + part_l[i][lane] * f1;
-#pragma unroll
-                    for (int d = 0; d < DT; d++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const f32x4 x = mem[(4 * d + e) * 64];
-#pragma unroll
-                            for (int j = 0; j < 4; j++) acc[d][4 * e + j] = acc[d][4 * e + j] * f0 + x[j] * f1;
-                        }
-                    m = mx;
+                    for (int e = 0; e < 16; e += 4)
+                        mem[(8 * d + e / 2 + half) * 32] = f32x4{acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]};
+                if (half == 0) {
+                    part_m[wave][col] = m;
+                    part_l[wave][col] = l;
                 }
             }
-        }
-        const bool writes = active && kpart == 0 && mine;
-        if (parts == 1) {
-            if (writes) {
-                const size_t row = (size_t)(n0 + tok) * a.ldo + (size_t)head * HD;
-                const bool none = sn.last < sn.first, gone = sn.last >= room;
+            __syncthreads();
+            for (int x = t; x < nrows * quads; x += NT) {
+                const int quad = x / nrows, row = x - quad * nrows;
+                float mx = part_m[0][row], sum = 0.0f;
+#pragma unroll
+                for (int w = 1; w < NW; w++) mx = fmaxf(mx, part_m[w][row]);
+                f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+                for (int w = 0; w < NW; w++) { /* a part without a finite score has what its scores left there: 0, or NaN */
+                    const float mw = part_m[w][row], f = mw > -INFINITY ? __builtin_amdgcn_exp2f(mw - mx) : 1.0f;
+                    const f32x4 y = place(w)[quad * 32 + row];
+                    sum = fmaf(part_l[w][row], f, sum);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) o[j] = fmaf(y[j], f, o[j]);
+                }
+                if (parts == 1) {
+                    finish(row, quad, o, sum);
+                } else {
+                    put(row, quad, o);
+                    if (quad == 0) put(row, HDP / 4, f32x4{mx, sum, 0.0f, 0.0f});
+                }
+            }
+            if (parts == 1) return;
+        } else if (parts == 1) {
+            if (mine) {
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        const int dim = 32 * d + 2 * e + 4 * half;
-                        float o[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) o[i] = none ? 0.0f : gone ? NAN : acc[d][e + i] / l;
-                        if (dim < HD) store4<BF16>(a, row, dim, o);
-                    }
+                    for (int e = 0; e < 16; e += 4)
+                        if (32 * d + 2 * e + 4 * half < HD) finish(r - r0, 8 * d + e / 2 + half, f32x4{acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]}, l);
             }
             return;
+        } else if (mine) {
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    if (32 * d + 2 * e + 4 * half < HD) put(r - r0, 8 * d + e / 2 + half, f32x4{acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]});
+            if (half == 0) put(r - r0, HDP / 4, f32x4{m, l, 0.0f, 0.0f});
         }
         /* Records cross XCDs: they are written and read past the XCDs' own L2s (sc1), and each wave waits for its stores before
          * the barrier, so a part is counted only after its record has arrived.  A unit's records: of each part, four
          * dimensions of all rows side by side, then all rows' maxima and sums, 16 bytes each. */
-        constexpr int REC = HDP + 4, SC1 = 16;
-        const int part_bytes = nrows * REC * 4;
-        const auto recs = __builtin_amdgcn_make_buffer_rsrc(
-            (void*)scalar((const char*)(a.rec + ((size_t)it.rec + (size_t)it.parts * ((size_t)rows_all * it.kh + r0)) * REC)), 0,
-            scalar(parts * part_bytes), 0x00027000);
-        if (writes) {
-            const int at = it.part * part_bytes + (r - r0) * 16;
-            auto put = [&](int quad, float x, float y, float z, float w) {
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{x, y, z, w}), recs, at + quad * nrows * 16, 0, SC1);
-            };
-#pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    const int dim = 32 * d + 2 * e + 4 * half;
-                    if (dim < HD) put(dim >> 2, acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]);
-                }
-            if (half == 0) put(HDP / 4, m, l, 0.0f, 0.0f);
-        }
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
         __builtin_amdgcn_s_waitcnt(0);
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
@@ -1105,7 +1104,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
          * lane keeps to one row and reads U of its quads' records and P parts at once (4 and 4: of 24 mixed sequences 26 us, two
          * quads a row for each lane 28; 8 and 4 or 4 and 8 have no registers: 30 and 34); where it has fewer, 1 << by_log lanes
          * side by side, up to 64, share a quad's parts. */
-        const int quads = HD / 4, across = NT / nrows, each = (quads + across - 1) / across;
+        const int across = NT / nrows, each = (quads + across - 1) / across;
         int by_log = 0;
         while (by_log < 6 && nrows * quads << (by_log + 1) <= NT && 4 << by_log < parts) by_log++;
         auto join = [&](auto us, auto ps) __attribute__((always_inline)) {
@@ -1163,17 +1162,10 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                     }
                     if (sub) return;
                 }
-                const int rr = r0 + row, rtok = a.by_r.of(rr);
-                const Seen s = seen(a, p0 + rtok, it.len);
-                const bool none = s.last < s.first, gone = s.last >= room;
-                const size_t to = (size_t)(n0 + rtok) * a.ldo + (size_t)(it.kh * R + rr - rtok * R) * HD;
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     if (q0 + u * apart >= quads) break;
-                    float out[4];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) out[j] = none ? 0.0f : gone ? NAN : o[u][j] / sum;
-                    store4<BF16>(a, to, 4 * (q0 + u * apart), out);
+                    finish(row, q0 + u * apart, o[u], sum);
                 }
             }
         };
