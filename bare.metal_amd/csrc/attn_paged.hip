@@ -27,9 +27,9 @@
  *
  * What bounds it (us a pass, MI355X).  One token a sequence: reading the
  * cache; 64 sequences of 8192 keys, 8 KV heads of 128 in bf16, 233 (5.4 TB/s), 1024 of 512
- * keys, 5 heads of 64, 124 (5.4).  Few keys: the chain of latencies (the tables 1.5, the
- * page's number and the first keys 2.5, a tile 1.5, the waves' join 1, records and counter
- * 1.2, the parts' join 2.5); 300 keys of one token 10 of kernel time.  Long chunks: 2048 tokens
+ * keys, 5 heads of 64, 124 (5.4).  Few keys: the chain of latencies (the tables 1-2, the
+ * page's number and the first keys 2.5, a tile 1.5, the waves' join 0.7, records and counter
+ * 0.9, the parts' join 2.1); 300 keys of one token 10 of kernel time.  Long chunks: 2048 tokens
  * over 16384 keys, 32 heads of 128, 600-630, 515 GFLOP at 0.82-0.86 PFLOP/s: a tile
  * takes 512 cycles of the matrix cores and some 600 of exponentials and other vector
  * instructions, which two waves a SIMD overlap in part, at 1.7 GHz (the part's power; the
