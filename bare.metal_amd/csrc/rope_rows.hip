@@ -11,7 +11,7 @@
  * output may be its input's buffer).
  *
  * HBM bounds the large calls (us, MI355X): 4096 rows of 40 heads of 128 in
- * bf16 18.8 (4.5 TB/s; chunks of 4 bytes in place of 16 32), norms of them in
+ * bf16 18.3 (4.6 TB/s; chunks of 4 bytes in place of 16 32), norms of them in
  * fp32 33 (5.1; with the norm's root and gains by every lane from memory 59),
  * 16 chunks of 32 + 16 heads to their pages 26 (3.5: heads of 256 bytes to
  * places of their own; cos and sin by every head 43).  Small ones take 2 to 4,
@@ -25,8 +25,8 @@ namespace {
 
 using namespace bmk;
 
-constexpr int NT = 256;
-constexpr int MAX_ROWS = 264; /* that a workgroup touches */
+constexpr int NT = 512;       /* (norms of 4096 rows of 40 heads of 128 in fp32: 128 46 us, 256 40, 512 39, 1024 43) */
+constexpr int MAX_ROWS = 520; /* that a workgroup touches */
 
 struct RopeArgs {
     const void *q, *k, *v;
