@@ -6,8 +6,8 @@
  * in one pass over the keys with the running maximum and sum (fp32) of the
  * softmax.
  *
- * A unit of work is up to 128 rows (new token, query head of the group; 64 of
- * fp32 heads over 128) of one sequence and KV head, so that every key and
+ * A unit of work is up to 128 rows (new token, query head of the group)
+ * of one sequence and KV head, so that every key and
  * value is read once for a whole group of heads; a unit's keys may be split
  * over workgroups, whose partial results the last one of them joins.  The work
  * goes over the keys in tiles of 32, which the loads put straight into LDS (a
@@ -120,10 +120,13 @@ __device__ __forceinline__ int v_place(int r, int c) {
 /* A workgroup's waves and LDS: every wave has a tile of its own while it goes alone, and where rows fill the waves all have
  * a ring of four (bf16) or two (fp32, in terms; heads over 128 have no such form: their registers spill). */
 template <bool BF16, int HDP> struct Shape {
-    static constexpr int NW = !BF16 && HDP == 256 ? 2 : 4, NT = 64 * NW, ROWS = 32 * NW;
+    static constexpr int NW = 4, NT = 64 * NW, ROWS = 32 * NW;
     static constexpr int ALONE = BF16 ? AS_BF16 : AS_F32;
     static constexpr bool SHARED = BF16 || HDP <= 128;
-    static constexpr int ALONE_BYTES = Tile<ALONE, HDP>::BYTES, ARRAYS = BF16 ? 4 : 1;
+    /* a wave's own tile where both halves do not fit for four waves: the values into the keys' place, once those are read (64
+     * sequences of 4000 keys, 4 heads of 256: two waves with both 689 us, four with halves 446; 512 rows of 4 heads over 4096 655 and 377) */
+    static constexpr bool HALVES = !BF16 && HDP == 256;
+    static constexpr int ALONE_BYTES = Tile<ALONE, HDP>::BYTES / (HALVES ? 2 : 1), ARRAYS = BF16 ? 4 : 1;
     static constexpr int BYTES = NW / ARRAYS * ALONE_BYTES; /* of an array */
     /* waves a SIMD, as registers (512 a lane) and LDS allow */
     static constexpr int WAVES = BF16 ? (HDP == 64 ? 3 : HDP == 128 ? 2 : 1) : HDP == 64 ? 2 : 1;
@@ -588,7 +591,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
         /* The tile of keys k0 .. k0 + 31, in LDS at `buf`.  Reads are issued in groups ahead of the products that take
          * them, the first of V's ahead of the softmax. */
         constexpr int KG = !BF16 && HDP == 256 ? 1 : 2, VG = 1;
-        auto block = [&](auto form, const unsigned char* buf, int k0) __attribute__((always_inline)) {
+        auto block = [&](auto form, const unsigned char* buf, int k0, auto behind_k) __attribute__((always_inline)) {
             constexpr int FORM = decltype(form)::value, PLANES = Tile<FORM, HDP>::PLANES, PLANE = Tile<FORM, HDP>::PLANE;
             constexpr int ROWB = Tile<FORM, HDP>::ROWB, CPR = Tile<FORM, HDP>::CPR;
             f32x16 sc;
@@ -623,7 +626,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                     for (int s = 0; s < 2; s++) {
                         if constexpr (FORM == AS_F32) {
                             const int vr = 16 * s + 4 * half, dim = 32 * (g * VG + d) + col;
-                            const unsigned char* at = buf + PLANE + vr * ROWB + 16 * v_place<FORM, CPR>(vr, dim >> 2) + 4 * (dim & 3);
+                            const unsigned char* at = buf + (W::HALVES ? 0 : PLANE) + vr * ROWB + 16 * v_place<FORM, CPR>(vr, dim >> 2) + 4 * (dim & 3);
 #pragma unroll
                             for (int e = 0; e < 8; e++) vw[g & 1][d][s][e] = *(const float*)(at + ((e & 3) + 2 * (e & 4)) * ROWB);
                         } else {
@@ -653,7 +656,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
 #pragma unroll
             for (int g = 0; g < STEPS / KG; g++) {
                 if (g + 1 < STEPS / KG) read_k(g + 1);
-                else read_v(0);
+                else if constexpr (!W::HALVES) read_v(0);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int s = 0; s < KG; s++) {
@@ -689,6 +692,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
+            behind_k();
             /* lane's score e: key k0 + 8 (e / 4) + 4 half + e % 4 */
             const bool masked = k0 < all_first || k0 + 31 > all_last;
             unsigned int sees = 0xffff; /* bit e */
@@ -747,9 +751,14 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                 for (int x = 0; x < TERMS; x++) __builtin_memcpy(&pf[x][s], u[x], 16);
             }
             __builtin_amdgcn_sched_barrier(0);
+if constexpr (W::HALVES) {
+                __builtin_amdgcn_s_waitcnt(0x0F70); /* vmcnt(0): the values are there */
+                asm volatile("" ::: "memory");
+                read_v(0);
+            }
 #pragma unroll
             for (int g = 0; g < DT / VG; g++) {
-                if (g + 1 < DT / VG) read_v(g + 1);
+                if (W::HALVES ? g > 0 : g + 1 < DT / VG) read_v(W::HALVES ? g : g + 1); /* HALVES: no registers for one ahead */
                 __builtin_amdgcn_sched_barrier(0);
                 u32x4 v[VG][TERMS][2];
 #pragma unroll
@@ -828,9 +837,9 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        auto compute = [&](auto form, const unsigned char* buf, int kt) __attribute__((always_inline)) {
+        auto compute = [&](auto form, const unsigned char* buf, int kt, auto behind_k) __attribute__((always_inline)) {
             const int k0 = kt * KT;
-            if (active && (kt & (kparts - 1)) == kpart && k0 <= any_last && k0 + 31 >= any_first && k0 < hi) block(form, buf, k0);
+            if (active && (kt & (kparts - 1)) == kpart && k0 <= any_last && k0 + 31 >= any_first && k0 < hi) block(form, buf, k0, behind_k);
         };
 
         /* Straight into LDS, 16 bytes a lane, a wave's load RPI rows, eight at most, which lie in one page.  Its number is read
@@ -851,14 +860,14 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
             k = 16 * kc < rowb ? row * rowb + 16 * kc : 1 << 30;
             v = 16 * vc < rowb ? row * rowb + 16 * vc : 1 << 30;
         };
-        auto load = [&](int pg, int key, unsigned char* to, int k_off, int v_off) {
+        auto load = [&](int pg, int key, unsigned char* to, int k_off, int v_off, bool keys = true, bool values = true) __attribute__((always_inline)) {
             const bool there = (unsigned int)pg < (unsigned int)b.n_pages;
             const int bytes = min(max(end - key, 0), RPI) * rowb;
             const char* k = (const char*)a.cache + (there ? pg : 0) * page_bytes + kh_bytes + (unsigned int)((key & mask) * rowb);
             const auto ks = __builtin_amdgcn_make_buffer_rsrc((void*)scalar(there ? k : (const char*)pg_nans), 0, scalar(bytes), 0x00027000);
             const auto vs = __builtin_amdgcn_make_buffer_rsrc((void*)scalar(k + page_bytes / 2), 0, scalar(there ? bytes : 0), 0x00027000);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(ks, (lvoid*)to, 16, k_off, 0, 0, 0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(vs, (lvoid*)(to + PLANE), 16, v_off, 0, 0, 0);
+            if (keys) __builtin_amdgcn_raw_ptr_buffer_load_lds(ks, (lvoid*)to, 16, k_off, 0, 0, 0);
+            if (values) __builtin_amdgcn_raw_ptr_buffer_load_lds(vs, (lvoid*)(to + (W::HALVES ? 0 : PLANE)), 16, v_off, 0, 0, 0);
         };
 
         if (!W::SHARED || groups == 1) {
@@ -866,7 +875,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
              * way while it computes. */
             unsigned char* buf;
             if constexpr (W::ARRAYS == 4) buf = wave == 0 ? lds0 : wave == 1 ? lds1 : wave == 2 ? lds2 : lds3;
-            else buf = lds0 + wave * T::BYTES;
+            else buf = lds0 + wave * W::ALONE_BYTES;
             int k_off[KINDS], v_off[KINDS];
             if constexpr (KINDS <= 8)
 #pragma unroll
@@ -876,8 +885,9 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
 #pragma unroll
                 for (int i = 0; i < 4; i++) pg[i] = page_of(kt * KT + 8 * i);
             };
-            auto request = [&](int kt) {
-                if constexpr (RPI == 1) { /* 32 descriptors at once spill scalar registers */
+            auto request = [&](int kt, bool values) __attribute__((always_inline)) { /* HALVES: the keys, or the values */
+                if constexpr (W::HALVES) { /* 32 descriptors at once spill scalar registers */
+                    static_assert(RPI == 1, "");
 #pragma unroll 1
                     for (int g = 0; g < 4; g++) {
                         const int key = kt * KT + 8 * g, p = page_of(key);
@@ -885,7 +895,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                         for (int i = 0; i < 8; i++) {
                             int k, v;
                             lane_place(8 * g + i, k, v);
-                            load(p, key + i, buf + (8 * g + i) * 1024, k, v);
+                            load(p, key + i, buf + (8 * g + i) * 1024, k, v, !values, values);
                         }
                     }
                     return;
@@ -898,17 +908,19 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
             q_request();
             if constexpr (!BF16 && HDP == 256) q_take(); /* no registers for both */
             __builtin_amdgcn_sched_barrier(0);
-            request(kt);
+            request(kt, false);
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (BF16 || HDP < 256) q_take();
             for (; kt < kt1; kt += kparts) {
                 pages(kt + kparts);
                 __builtin_amdgcn_s_waitcnt(0x0F70); /* vmcnt(0) */
                 asm volatile("" ::: "memory");
-                compute(std::integral_constant<int, W::ALONE>{}, buf, kt);
+                compute(std::integral_constant<int, W::ALONE>{}, buf, kt, [&]() __attribute__((always_inline)) {
+                    if constexpr (W::HALVES) request(kt, true);
+                });
                 asm volatile("" ::: "memory");
                 __builtin_amdgcn_sched_barrier(0);
-                if (kt + kparts < kt1) request(kt + kparts);
+                if (kt + kparts < kt1) request(kt + kparts, false);
             }
             __builtin_amdgcn_s_waitcnt(0x0F70); /* none under way */
         } else if constexpr (BF16) {
@@ -944,7 +956,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                 barrier();
                 request(kt + 3, before);
                 pages(kt + 4);
-                compute(std::integral_constant<int, AS_BF16>{}, buf, kt);
+                compute(std::integral_constant<int, AS_BF16>{}, buf, kt, []() {});
             };
             for (int kt = kt0; kt < kt1; kt += 4) {
                 step(kt, lds0, lds3);
@@ -1004,7 +1016,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                 __syncthreads(); /* the tile is there, and the one before has been read */
                 fetch(kt + 1); /* behind the part's last: zeros */
                 pages(kt + 2);
-                compute(std::integral_constant<int, TERMS3>{}, buf, kt);
+                compute(std::integral_constant<int, TERMS3>{}, buf, kt, []() {});
             }
         }
         l += other_half(l);
@@ -1030,9 +1042,9 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
         if (kparts > 1) {
             /* The waves' sums of the same rows, each in its own tile's place, joined four outputs a lane. */
             constexpr int SUMS = HDP * 128;
-            static_assert(SUMS <= T::BYTES, "");
+            static_assert(SUMS <= W::ALONE_BYTES, "");
             auto place = [&](int w) {
-                return (f32x4*)(W::ARRAYS == 1 ? lds0 + w * T::BYTES : w == 0 ? lds0 : w == 1 ? lds1 : w == 2 ? lds2 : lds3);
+                return (f32x4*)(W::ARRAYS == 1 ? lds0 + w * W::ALONE_BYTES : w == 0 ? lds0 : w == 1 ? lds1 : w == 2 ? lds2 : lds3);
             };
             if (mine) {
                 f32x4* mem = place(wave) + col;
