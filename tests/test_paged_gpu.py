@@ -579,7 +579,7 @@ def test_attention_weights(be, new, total, window, HD, kind):
 
 @both
 @pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf], ids=["nan", "inf", "-inf"])
-@pytest.mark.parametrize("NH,NKV,HD", [(3, 1, 64), (4, 2, 128), (2, 1, 96)])
+@pytest.mark.parametrize("NH,NKV,HD", [(3, 1, 64), (4, 2, 128), (2, 1, 96), (2, 1, 256)])
 @pytest.mark.parametrize("new,total,window", [([64], [100], 0), ([5, 1], [33, 70], 0), ([40], [90], 16), ([150], [150], 50)])
 def test_attention_masked_keys_hold_anything(be, new, total, window, NH, NKV, HD, what, kind):
     """A key or a value that is no number, at a place that only later rows (or with a window only earlier ones) see: the
@@ -614,12 +614,13 @@ def test_attention_masked_keys_hold_anything(be, new, total, window, NH, NKV, HD
 
 
 @both
-def test_attention_missing_pages(be, kind):
+@pytest.mark.parametrize("HD", [64, 104, 200])
+def test_attention_missing_pages(be, HD, kind):
     """Rows that see a key whose page is none, or lies past the table, get NaN; the others are as ever."""
     rng = np.random.default_rng(4)
-    b = Batch(be, rng, kind, [40, 1, 2], [60, 70, 33], 16, 2, 64)
+    b = Batch(be, rng, kind, [40, 1, 2], [60, 70, 33], 16, 2, HD)
     b.fill(rng)
-    q = kind.held(rng.standard_normal((b.N, 4, 64)))
+    q = kind.held(rng.standard_normal((b.N, 4, HD)))
     want, off = attend(b, q, 4, 0.125)
     for bad in (-1, b.count, -(1 << 31), (1 << 31) - 1):
         t = b.tables(be)
