@@ -205,7 +205,7 @@ __global__ __launch_bounds__(NT) void k_rope_rows(RopeArgs a) {
         for (int j = 0; j < 2; j++)
 #pragma unroll
             for (int e = 0; e < E; e++) y[i][j][e] = lane + (i << a.lp_log) < a.units ? value<BF16, E>(raw[i][j], e) : 0.0f;
-    if (a.gain && kind < 2) { /* squares and their sum in 64 bits: heads past 2^64 or under 2^-64 need no care */
+    if (a.gain && kind < 2) { /* squares and their sum in 64 bits: those of heads past 2^64 or under 2^-64 need no care */
         double sum = 0;
 #pragma unroll
         for (int i = 0; i < UN; i++)
@@ -215,7 +215,9 @@ __global__ __launch_bounds__(NT) void k_rope_rows(RopeArgs a) {
                 for (int e = 0; e < E; e++) sum = fma((double)y[i][j][e], (double)y[i][j][e], sum);
         const double inv = root_inverse(group_sum(sum, lanes) * a.by_hd + (double)a.eps);
         const float f = (float)inv;
-        if (__builtin_expect(__any(f < 0x1p-100f), 0)) { /* a factor under 2^-126 has not all of fp32's bits */
+        /* a factor under 2^-126 has not all of fp32's bits, one over 2^128 (heads under 2^-128 with an eps as small) is none */
+        const bool far = f < 0x1p-100f || f > 0x1p100f;
+        if (__builtin_expect(__any(far), 0)) {
 #pragma unroll
             for (int i = 0; i < UN; i++)
 #pragma unroll
@@ -223,7 +225,7 @@ __global__ __launch_bounds__(NT) void k_rope_rows(RopeArgs a) {
 #pragma unroll
                     for (int e = 0; e < E; e++) {
                         asm volatile(""); /* a branch, not a choice between two values */
-                        y[i][j][e] = f < 0x1p-100f ? (float)((double)y[i][j][e] * inv) : y[i][j][e] * f;
+                        y[i][j][e] = far ? (float)((double)y[i][j][e] * inv) : y[i][j][e] * f;
                     }
         } else {
 #pragma unroll

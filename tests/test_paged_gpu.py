@@ -292,6 +292,31 @@ def test_qk_norm_of_extreme_heads(be):
         assert np.isnan(got[3]).all() and np.isnan(got[4, 60]) and (got[4, :60] == 0).all()
 
 
+@both
+@pytest.mark.parametrize("HD,off0", [(64, 0), (6, 0), (64, 1)], ids=["wide", "narrow", "odd"])
+def test_qk_norm_of_the_smallest_heads(be, HD, off0, kind):
+    """Heads under 2^-128, down to the type's least number, whose factor 1 / sqrt(mean x^2) is past fp32: with eps 0 (or one as
+    small) they come out like any others, beside heads that are ordinary."""
+    size = [1.0, 2.0 ** -100, 2.0 ** -126, 2.0 ** -128, 2.0 ** -131, 2.0 ** -140, 0.0, 2.0 ** 40]
+    NH = len(size)
+    rng = np.random.default_rng(41)
+    x = kind.held(rng.standard_normal((NH, HD)) * np.array(size)[:, None])
+    x[6, 1] = 2.0 ** (-133 if kind.bf16 else -149)  # the least number alone
+    x[5, 0] = x[6, 1]  # no head of zeros, which has no norm
+    gain = (1 + 0.3 * rng.standard_normal((2, HD))).astype(np.float32)
+    one = be.upload(np.int32([0]))
+    for eps in (0.0, 2.0 ** -149):
+        src = be.upload(strided(kind, x.reshape(1, -1), NH * HD, off0))
+        out = [marked(be, (off0 + NH * HD + 3) * kind.size) for _ in range(2)]
+        assert be.dispatch("qk_norm_rope_forward" + kind.suffix, [
+            src, src] + out + [one, one, be.upload(gain), be.params(1, NH, NH, HD, 0, 0, *[NH * HD] * 4),
+                               floats(be, 1.0, eps)], (1,), (256,), offsets=[off0 * kind.size] * 4 + [0] * 5) == 0
+        for buf, g in zip(out, gain):
+            want = normed(x, g, np.float64(np.float32(eps)))
+            got = rows_of(kind, buf, 1, NH * HD, NH * HD, off0).reshape(NH, HD)
+            check(kind, got, want, 3 * U32 * np.abs(want))
+
+
 # ---------------------------------------------------------------- the cache
 
 class Batch:
