@@ -492,9 +492,10 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
     const int HD = b.HD, R = a.R;
     const Plan<ROWS> plan(a);
 
-    if (blockIdx.x >= plan.total) return;
+    const unsigned int piece = pg_group();
+    if (piece >= plan.total) return;
     {
-        const auto it = plan.item(blockIdx.x);
+        const auto it = plan.item(piece);
         if (it.s < 0) return;
         const int rows_all = it.n * R, r0 = it.unit * ROWS, nrows = min(ROWS, rows_all - r0);
         const int p0 = (int)((unsigned)it.len - (unsigned)it.n); /* position of the sequence's first new token */
@@ -1220,7 +1221,7 @@ int start(PaArgs& a, const bmk_launch_t* l) {
     const int64_t tiles = (a.b.room() + KT - 1) / KT;
     const int64_t rounds = units * tiles >= (int64_t)a.slots * ROUND_TILES * ROUNDS ? ROUNDS : 1;
     const int64_t grid = std::min(units * std::min<int64_t>(tiles, MAX_SPLIT), units + a.slots * rounds + 8);
-    hipLaunchKernelGGL((k_attn_paged<BF16, HDP>), dim3((unsigned)grid), dim3(W::NT), 0, l->stream, a);
+    hipLaunchKernelGGL((k_attn_paged<BF16, HDP>), pg_grid(grid, W::NT), dim3(W::NT), 0, l->stream, a);
     BMK_LAUNCH_CHECK();
     return 0;
 }
@@ -1285,6 +1286,13 @@ extern "C" void bmk_paged_lookup(const int* start, const int* len, const int* pa
     out[0] = b.seq_of(n);
     out[1] = out[0] < 0 ? 0 : b.pos_of(out[0], n);
     out[2] = out[0] < 0 ? -1 : b.page_of(out[0], j);
+}
+
+/* workgroups of a launch along x and y */
+extern "C" void bmk_paged_grid(long long groups, int lanes, unsigned int* xy) {
+    const dim3 g = pg_grid(groups, lanes);
+    xy[0] = g.x;
+    xy[1] = g.y;
 }
 
 extern "C" int bmk_launch_attn_paged(const bmk_launch_t* a) { return launch_attn_paged(a, false); }

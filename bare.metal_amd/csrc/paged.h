@@ -14,6 +14,14 @@ namespace bmk {
 constexpr int PG_MAX_DIM = 1 << 30;
 constexpr int PG_MAX_HD = 256, PG_MAX_SEQS = 4096;
 
+/* A launch's workgroups, side by side and in as few rows as take them: HIP has fewer than 2^32 work-items along an axis.
+ * The last row may have workgroups over, fewer than there are rows. */
+inline dim3 pg_grid(int64_t groups, int lanes) {
+    const int64_t most = ((1LL << 32) - 1) / lanes, rows = (groups + most - 1) / most;
+    return dim3((unsigned int)((groups + rows - 1) / rows), (unsigned int)rows);
+}
+__device__ __forceinline__ unsigned int pg_group() { return blockIdx.y * gridDim.x + blockIdx.x; }
+
 /* x / d for x below 2^31 by one product */
 struct Div {
     unsigned int d, mul, shift;

@@ -137,7 +137,8 @@ __global__ __launch_bounds__(NT) void k_rope_rows(RopeArgs a) {
     __shared__ int where[MAX_ROWS]; /* bit 0: a row of the batch, bit 1: with a place in the cache */
     const int t = threadIdx.x, lanes = 1 << a.lp_log, lane = t & (lanes - 1), slots = NT >> a.lp_log;
     const int HD = a.b.HD, half = a.rot / 2;
-    const int first = (int)blockIdx.x * slots, x = first + (t >> a.lp_log), items = a.items;
+    const int first = (int)pg_group() * slots, x = first + (t >> a.lp_log), items = a.items;
+    if (first >= items) return;
     const int n0 = a.by_heads.of(first), rows = a.by_heads.of(min(first + slots, items) - 1) - n0 + 1;
     const int halves = PAIRS ? 0 : a.rot / (2 * E); /* units whose chunks lie half of the turned part apart */
     auto at = [&](int i, int j) { /* of the lane's unit i, chunk j: its place in a head */
@@ -286,7 +287,7 @@ int launch(RopeArgs& a, hipStream_t stream) {
     static_assert(NT + 1 <= MAX_ROWS, "");
     a.turns_held = (rows * (a.rot / 2) + 3) & ~3;
     const size_t bytes = (size_t)a.turns_held * 8;
-    const dim3 grid(((unsigned int)a.items + slots - 1) / slots);
+    const dim3 grid = pg_grid(((int64_t)a.items + slots - 1) / slots, NT);
     constexpr bool WIDE = E * (BF16 ? 2 : 4) == 16;
     if (WIDE && a.once) {
         if (a.pairs) hipLaunchKernelGGL((k_rope_rows<BF16, E, UN, true, WIDE>), grid, dim3(NT), bytes, stream, a);

@@ -287,3 +287,26 @@ def test_lookups_stay_inside_any_table():
         n, j = int(rng.integers(0, 12)), int(rng.choice(wild))
         s, _, pg = lookup(start, length, pages, page, 5, n, j)
         assert -1 <= s < S and -1 <= pg < 5
+
+
+# ---------------------------------------------------------------- launches
+
+@pytest.mark.parametrize("lanes", [256, 512])
+def test_a_launch_stays_under_the_work_items_of_an_axis(lanes):
+    """HIP refuses 2^32 work-items or more along an axis: up to there one row of workgroups, then as few rows as take them,
+    all workgroups among them and fewer over than there are rows."""
+    fn = bmhip.lib().bmk_paged_grid
+    fn.restype, fn.argtypes = None, [ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p]
+    most = ((1 << 32) - 1) // lanes
+    # 2^30 heads by 64 lanes each; 4096 KV heads of 4096 sequences, with a part of a unit for each
+    sizes = [1, 2, 255, most - 1, most, most + 1, 2 * most, 2 * most + 1, (1 << 30) * 64 // lanes, 4096 * (4096 + 32) + 3080]
+    for groups in sizes + [random.Random(lanes).randrange(1, 1 << 28) for _ in range(200)]:
+        xy = np.zeros(2, np.uint32)
+        fn(groups, lanes, xy.ctypes.data)
+        x, y = (int(v) for v in xy)
+        assert x * lanes < 1 << 32 and groups <= x * y < groups + y and y == -(-groups // most) <= 65535, (groups, x, y)
+    for log in range(7):  # the rotation: 2^30 heads by 1 << log lanes each; the first head of any workgroup stays inside an int
+        slots = 512 >> log
+        xy = np.zeros(2, np.uint32)
+        fn((1 << 30) // slots, 512, xy.ctypes.data)
+        assert int(xy[0]) * int(xy[1]) * slots < 1 << 31

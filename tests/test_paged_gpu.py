@@ -200,6 +200,34 @@ def test_rope_leaves_the_rest_of_a_head(be, kind):
         assert np.array_equal(got[0], x[0], equal_nan=True)  # position 0: no turn
 
 
+def test_rope_of_more_work_items_than_an_axis_takes(be):
+    """Heads of 256 at odd strides take 64 lanes each: 2^26 heads and more are over 2^32 work-items.  34 GB, in place, zeros but
+    for a few rows, which the kernel itself (rot 0) puts there and takes back."""
+    kind, NH, HD, rot = KINDS[1], 1024, 256, 64
+    W = NH * HD
+    ld, N = W + 1, (1 << 16) + 9  # heads of row 2^16 on lie past the axis
+    rng = np.random.default_rng(44)
+    rows = [0, 1, 40000, (1 << 16) - 1, 1 << 16, (1 << 16) + 1, N - 1]
+    x = kind.held(rng.standard_normal((len(rows), W)))
+    pos = positions(rng, N, 1 << 20)
+    table, m = turn_table(rot, "yarn")
+    big, turns, one, factor = be.alloc(N * ld * kind.size), be.upload(table), be.upload(np.int32([0])), floats(be, m)
+    try:
+        for r, v in zip(rows, x):
+            assert be.dispatch("rope_forward_rows_bf16", [be.upload(kind.raw(v)), big, one, turns, be.params(1, NH, HD, 0, 0, W, W),
+                                                          factor], (1,), (256,), offsets=[0, r * ld * kind.size, 0, 0, 0, 0]) == 0
+        assert be.dispatch("rope_forward_rows_bf16", [big, big, be.upload(pos), turns, be.params(N, NH, HD, rot, 0, ld, ld),
+                                                      factor], (N,), (256,)) == 0
+        want, off = turned(x.reshape(len(rows), NH, HD), pos[rows], rot, 0, table, m)
+        for r, w, o in zip(rows + [2, 50000, (1 << 16) + 5], list(want) + [np.zeros((NH, HD))] * 3, list(off) + [0.0] * 3):
+            out = marked(be, W * kind.size)
+            assert be.dispatch("rope_forward_rows_bf16", [big, out, one, turns, be.params(1, NH, HD, 0, 0, W, W), factor], (1,),
+                               (256,), offsets=[r * ld * kind.size, 0, 0, 0, 0, 0]) == 0
+            check(kind, kind.values(out.read(kind.memory)).reshape(NH, HD), w, o)
+    finally:
+        big.free()
+
+
 def test_rope_keeps_lengths_and_distances(be):
     """Closed forms: a turn keeps a pair's length, and a dot product depends on the positions' difference alone."""
     NH, HD = 2, 64
@@ -822,6 +850,31 @@ def test_attention_a_cache_past_32_bits(be, kind):
     got = kind.values(out.read(kind.memory)).reshape(n, 1, HD)
     cache.free()
     check(kind, got, want, off)
+
+
+def test_attention_of_more_work_items_than_an_axis_takes(be):
+    """4096 sequences over 4096 KV heads, a workgroup each: over 2^32 work-items.  All have one page; a row that sees one key
+    has that key's value bit for bit, and one that sees eight alike keys the mean of the values."""
+    kind, S, NKV, HD, page = KINDS[1], 4096, 4096, 8, 8
+    W = NKV * HD
+    rng = np.random.default_rng(45)
+    q = np.resize(kind.raw(rng.standard_normal(1 << 16)), (S, W))
+    cache = kind.raw(rng.standard_normal((2, 2, NKV, page, HD)))
+    cache[:, 0] = cache[:, 0, :, :1]  # the keys of a head are alike
+    length = np.where(rng.random(S) < 0.5, 1, 8).astype(np.int32)
+    length[[0, -1]] = 8, 1
+    pages = rng.integers(0, 2, (S, 1)).astype(np.int32)
+    out = marked(be, S * W * kind.size)
+    assert be.dispatch("attention_forward_paged_bf16", [
+        be.upload(q), be.upload(cache), out, be.upload(np.arange(S + 1, dtype=np.int32)), be.upload(length), be.upload(pages),
+        be.params(S, S, NKV, NKV, HD, W, W, page, 2, 1, 1, 0), floats(be, HD ** -0.5)], (S,), (256,)) == 0
+    got = out.read(kind.memory).reshape(S, NKV, HD)
+    mean = kind.values(cache[:, 1]).astype(np.float64).mean(2)
+    most = np.abs(kind.values(cache[:, 1])).astype(np.float64).mean(2)  # a sum of eight in fp32, its quotient
+    for p in (0, 1):
+        one, all_ = (pages[:, 0] == p) & (length == 1), (pages[:, 0] == p) & (length == 8)
+        assert (got[one] == cache[p, 1, :, 0]).all()
+        check(kind, kind.values(got[all_]), mean[p], 12 * U32 * most[p])
 
 
 # ---------------------------------------------------------------- the operators together
