@@ -21,8 +21,10 @@
  * it once its sum runs over the keys in the order of the registers, so P goes
  * from the scores to the product without moving between lanes; V comes
  * transposed out of LDS (ds_read_b64_tr_b16).  fp32 goes in as three terms
- * x = x0 + x1 + x2 of bf16 (truncations, exact), whose products of at least
- * 2^-24 are taken, six of nine.  P is rounded to bf16 where q, K and V are
+ * x = x0 + x1 + x2 of bf16, exactly: |x1| < 2^-7 |x|, |x2| <= 2^-16 |x|, x2 of
+ * either sign.  Six of the nine products are taken; what the other three would add is at
+ * most 2^-22 of a product, 0.4 x 2^-24 in the mean and of either sign (with all terms cut off
+ * towards zero up to 2^-21, and 0.7 x 2^-24 too little in the mean).  P is rounded to bf16 where q, K and V are
  * (its sum is not), which is half a step of the output's own type.
  *
  * What bounds it (us a pass, MI355X).  One token a sequence: reading the
@@ -157,12 +159,16 @@ __device__ __forceinline__ unsigned int pack_top(float x, float y) {
 }
 __device__ __forceinline__ float top(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 
-/* Two values' three terms, packed.  An infinity's others are NaN, which leaves what sees it no number, as it should. */
+__device__ __forceinline__ float low_half(unsigned int two) { return __uint_as_float(two << 16); }
+__device__ __forceinline__ float high_half(unsigned int two) { return __uint_as_float(two & 0xffff0000u); }
+
+/* Two values' three terms, packed: the upper half, which no finite value leaves for infinity, of what is left the nearest, and
+ * the rest, exactly.  An infinity's others are NaN, which leaves what sees it no number, as it should. */
 __device__ __forceinline__ void split2(float x, float y, unsigned int* t) {
     t[0] = pack_top(x, y);
     const float rx = x - top(x), ry = y - top(y);
-    t[1] = pack_top(rx, ry);
-    t[2] = pack_top(rx - top(rx), ry - top(ry));
+    t[1] = pack_rne(rx, ry);
+    t[2] = pack_top(rx - low_half(t[1]), ry - high_half(t[1]));
 }
 
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {

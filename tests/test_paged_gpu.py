@@ -970,6 +970,29 @@ def test_attention_scales(be, new, total, window, scale, kind):
     compare(b, attention(be, b, q, 4, scale, window=window), want, off)
 
 
+def test_attention_fp32_scores_lean_to_neither_side(be):
+    """Scores of about 500, all of one sign, of keys with 24 bits beside ones with 8, whose products are whole: 65536 pairs'
+    difference, in units of 2^-24 of a score, through the weights.  Roundings to nearest of bits without a pattern, under 2 units
+    each, leave a mean within 6 * 2 / sqrt(65536) = 0.05; 0.3 has room for what the exponential and the quotient add (2^-22
+    of a weight, 0.01 units).  Terms cut off towards zero leave -0.69."""
+    kind, S, NH, HD, page = KINDS[0], 1024, 64, 16, 8
+    rng = np.random.default_rng(46)
+    q, ka = (rng.uniform(1, 2, (S, NH, HD)).astype(np.float32) for _ in range(2))
+    kb = from_bf16(to_bf16(ka))
+    cache = np.zeros((S, 2, NH, page, HD), np.float32)
+    cache[:, 0, :, 0], cache[:, 0, :, 1], cache[:, 1, :, 0] = ka, kb, 1
+    out, scale = marked(be, q.nbytes), 14.0
+    assert be.dispatch("attention_forward_paged", [
+        be.upload(q), be.upload(cache), out, be.upload(np.arange(S + 1, dtype=np.int32)), be.upload(np.full(S, 2, np.int32)),
+        be.upload(np.arange(S, dtype=np.int32)), be.params(S, S, NH, NH, HD, NH * HD, NH * HD, page, S, 1, 1, 0),
+        floats(be, scale)], (S,), (256,)) == 0
+    p = out.read(np.float32).reshape(S, NH, HD)[..., 0].astype(np.float64)
+    q, ka, kb = (x.astype(np.float64) for x in (q, ka, kb))
+    a, b = scale * (q * ka).sum(-1), scale * (q * kb).sum(-1)
+    mean = ((np.log(p / (1 - p)) - (a - b)) / (a * U32)).mean()
+    assert abs(mean) < 0.3, mean
+
+
 @both
 def test_attention_of_a_shared_prefix(be, kind):
     """Sequences whose first pages are the same ones, as after a common prompt, and one that is the same altogether."""
