@@ -11,6 +11,7 @@ import numpy as np
 import pytest
 
 import bmhip
+from paged_exactness import SIX, deviation, emulated, last_bits, last_bits_off
 
 MAX_BUFFERS = 12
 BASE = 1 << 20  # an address on a 16-byte boundary
@@ -310,3 +311,44 @@ def test_a_launch_stays_under_the_work_items_of_an_axis(lanes):
         xy = np.zeros(2, np.uint32)
         fn((1 << 30) // slots, 512, xy.ctypes.data)
         assert int(xy[0]) * int(xy[1]) * slots < 1 << 31
+
+
+# ---------------------------------------------------------------- what the fp32 attention's bound tells apart
+
+FOUR = [(1, 1), (1, 0), (0, 1), (0, 0)]
+THREE = [(1, 0), (0, 1), (0, 0)]
+
+
+@pytest.mark.parametrize("HD", [8, 40, 64, 128, 256])
+@pytest.mark.parametrize("keys", [2, 40, 300, 1500])
+def test_the_bound_on_average_error_wants_all_six_products(HD, keys):
+    """The kernel's arithmetic with all products of terms is within it; without the third terms' products, of the scores or of the
+    values, or with three products alone, the error is past four times the mean that the roundings leave."""
+    rng = np.random.default_rng(HD * 10000 + keys)
+    rows = [tuple(rng.standard_normal(s).astype(np.float32) for s in (HD, (keys, HD), (keys, HD))) for _ in range(12)]
+    scale = float(np.float32(HD ** -0.5))
+
+    def ratio(*products):
+        err = want = 0.0
+        for q, k, v in rows:
+            sc = k.astype(np.float64) @ q.astype(np.float64) * scale
+            p = np.exp(sc - sc.max())
+            err += (((p / p.sum()) @ v.astype(np.float64) - emulated(q, k, v, scale, *products)) ** 2).sum()
+            want += (deviation(q, k, v, scale) ** 2).sum()
+        return math.sqrt(err / want)
+
+    assert ratio() < 1
+    for left in (FOUR, THREE):
+        assert min(ratio(left, SIX), ratio(SIX, left)) > 4, (ratio(left, SIX), ratio(SIX, left))
+
+
+@pytest.mark.parametrize("HD", [8, 64, 256])
+def test_scores_of_last_bits_want_their_third_terms(HD):
+    rng = np.random.default_rng(HD)
+    for in_key in (0, 1):
+        worst = {0: 0.0, 1: 0.0, 2: 0.0}
+        for _ in range(40):
+            q, k, v = last_bits(rng, 1, 2 + int(rng.integers(0, 30)), HD, in_key)
+            for n, products in enumerate((SIX, FOUR, THREE)):
+                worst[n] = max(worst[n], last_bits_off(q[0], k, v, emulated(q[0], k, v, 1.0, products)))
+        assert worst[0] < 1 and worst[1] > 1000 and worst[2] > 1000, worst

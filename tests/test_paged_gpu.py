@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 
 import bmhip
+from paged_exactness import deviation, last_bits, last_bits_off
 
 pytestmark = pytest.mark.gpu
 U32, UB16 = 2.0 ** -24, 2.0 ** -8
@@ -991,6 +992,74 @@ def test_attention_fp32_scores_lean_to_neither_side(be):
     a, b = scale * (q * ka).sum(-1), scale * (q * kb).sum(-1)
     mean = ((np.log(p / (1 - p)) - (a - b)) / (a * U32)).mean()
     assert abs(mean) < 0.3, mean
+
+
+@pytest.mark.parametrize("NH,NKV,HD", [(3, 1, 8), (4, 2, 40), (15, 5, 64), (6, 2, 96), (8, 2, 128), (2, 1, 200), (4, 1, 256)])
+@pytest.mark.parametrize("new,total,page,window", [
+    ([1] * 6, [2, 40, 300, 300, 150, 77], 16, 0), ([1, 1], [1500, 1100], 64, 0), ([130], [333], 32, 0), ([70], [1300], 16, 0),
+    ([40, 1], [200, 90], 8, 33)])
+def test_attention_is_fp32_on_average(be, new, total, page, window, NH, NKV, HD):
+    """The root of the mean square error over all elements within twice that of the roundings (tests/paged_exactness.py): the
+    same arithmetic with a term of q, K, the weights or V missing is past four times."""
+    rng = np.random.default_rng(sum(total) * 31 + HD)
+    b = Batch(be, rng, KINDS[0], new, total, page, NKV, HD)
+    b.fill(rng)
+    q = rng.standard_normal((b.N, NH, HD)).astype(np.float32)
+    scale = float(np.float32(HD ** -0.5))
+    want, _ = attend(b, q, NH, scale, 1, window)
+    err = want - attention(be, b, q, NH, scale, 1, window)
+    allowed = np.zeros_like(want)
+    for n in range(b.N):
+        s, last = b.seq[n], b.pos[n]
+        first = max(0, last - window + 1) if window else 0
+        for h in range(NH):
+            allowed[n, h] = deviation(q[n, h], *(x[s][h // (NH // NKV), first:last + 1] for x in (b.K, b.V)), scale)
+    assert np.sqrt((err ** 2).mean() / (allowed ** 2).mean()) < 2
+
+
+@pytest.mark.parametrize("NH,HD", [(1, 8), (3, 64), (2, 96), (1, 128), (2, 200), (1, 256)])
+@pytest.mark.parametrize("new,ahead", [(1, 0), (5, 0), (8, 40), (8, 1200), (128, 30)])
+def test_attention_gives_a_value_back_bit_for_bit(be, new, ahead, NH, HD):
+    """fp32: a row whose weights are 1 for one key and 0 for all others has that key's value, all 24 bits of it: the three terms'
+    sum, smallest first, is exact."""
+    rng = np.random.default_rng(HD + new + ahead)
+    total = ahead + new
+    b = Batch(be, rng, KINDS[0], [new], [total], 16, 1, HD)
+    b.K = [np.zeros((1, total, HD), np.float32)]
+    b.V = [(rng.standard_normal((1, total, HD)) * np.exp2(rng.integers(-40, 100, (1, total, 1)))).astype(np.float32)]
+    b.V[0][0, ::3] = 1 + rng.integers(0, 1 << 23, b.V[0][0, ::3].shape).astype(np.float32) * np.float32(2.0 ** -23)
+    # keys are unit vectors, which repeat after HD; a row's q is one of the last HD keys that it sees: a score of 512, whose exponent
+    # is exact, the others 0, and one of -512 for the earlier keys of the same direction
+    q = np.zeros((new, NH, HD), np.float32)
+    own = np.zeros((new, NH), int)
+    for j in range(total):
+        b.K[0][0, j, j % HD] = -16 if j < total - min(HD, total) else 16
+    for i in range(new):
+        for h in range(NH):
+            lo = max(0, total - HD)
+            own[i, h] = j = int(rng.integers(lo, ahead + i + 1)) if ahead + i >= lo else -1
+            q[i, h, j % HD] = 32
+    b.set(0, b.K[0], b.V[0])
+    got = attention(be, b, q, NH, 1.0)
+    for i in range(new):
+        for h in range(NH):
+            if own[i, h] >= 0:
+                assert np.array_equal(got[i, h], b.V[0][0, own[i, h]]), (i, h)
+
+
+@pytest.mark.parametrize("in_key", [0, 1], ids=["q", "key"])
+@pytest.mark.parametrize("HD", [8, 64, 128, 256])
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_scores_have_all_their_bits(be, new, HD, in_key):
+    """fp32 scores that are a number's last 8 bits, what a form without some third terms has nothing of."""
+    rng = np.random.default_rng(HD + new)
+    q, k, v = last_bits(rng, new, 2 * new, HD, in_key)
+    b = Batch(be, rng, KINDS[0], [new], [2 * new], 16, 1, HD, fill=0.0)
+    b.K, b.V = [k[None]], [v[None]]
+    b.set(0, b.K[0], b.V[0])
+    got = attention(be, b, q[:, None], 1, 1.0)
+    for i in range(new):
+        assert last_bits_off(q[i], k[:new + i + 1], v[:new + i + 1], got[i, 0]) <= 1, i
 
 
 @both
