@@ -64,6 +64,12 @@ constexpr int KT = 32;           /* keys of a tile */
 /* in powers of two: how far a score may pass the running maximum before that moves (32 sequences of 16 tokens over 1500 keys,
  * with 0 28.8 us, with 8 27.6); fp32's sums have room for more */
 constexpr float SLACK = 8.0f;
+/* A row's weights are exp2(fma(score, scale2, -m)) with m = score * scale2 of its largest score, rounded, so that score's own
+ * exponent is what the rounding left: up to 32 where m is under FAR, which all weights of the row have in common, but past fp32's
+ * range from 2^31 on.  From FAR on the scores of a row, numbers of 24 bits, lie 64 apart or are equal: the largest takes all, also
+ * with the power of two at or over scale2 in its place, whose products with them are exact.  (The rest of m as a second number,
+ * carried to the joins: 2048 rows over 16384 keys 2% slower, 24 mixed sequences 4%.) */
+constexpr float FAR = 0x1p30f;
 constexpr int MAX_SPLIT = 128;   /* parts of a unit's keys */
 constexpr int LEAST = 4;         /* tiles a part, at least: one a wave (1 token over 300 keys, parts of 2 15.3 us, 4 15.1, 8 17.5) */
 constexpr int MANY_LEAST = 8;    /* ... of more than 32 rows (Cut::parts) */
@@ -86,7 +92,7 @@ struct PaArgs {
     int q_wide; /* q's heads begin on 16-byte boundaries */
     int causal, window;
     size_t ldq, ldo;
-    float scale2; /* |scale| * log2(e) */
+    float scale2, far_scale2; /* |scale| * log2(e); the power of two from there on */
     unsigned int flip; /* scale's sign, for q's */
     unsigned int most; /* rows' records that fit behind the counters */
     int slots; /* workgroups that run at once */
@@ -594,6 +600,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[d][e] = 0.0f;
         float m = -INFINITY, l = 0.0f; /* in powers of two, of the row; this lane's keys' sum */
+        float scale2 = a.scale2;       /* the row's: far_scale2 where m is far */
 
         /* The tile of keys k0 .. k0 + 31, in LDS at `buf`.  Reads are issued in groups ahead of the products that take
          * them, the first of V's ahead of the softmax. */
@@ -716,11 +723,12 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
             float cm = sc[0];
 #pragma unroll
             for (int e = 1; e < 16; e++) cm = fmaxf(cm, sc[e]);
-            cm *= a.scale2; /* -infinity times 0 is NaN, which moves nothing */
-            if (__any(cm > m + SLACK)) {
+            if (__any(cm * scale2 > m + SLACK)) { /* -infinity times 0 is NaN, which moves nothing */
                 cm = fmaxf(cm, other_half(cm));
                 /* of its own scores alone: what another row of the wave sees does not touch a row's roundings */
-                const float mn = cm > m + SLACK ? cm : m, f = mn > -INFINITY ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+                const bool moves = cm * scale2 > m + SLACK;
+                if (moves) scale2 = fabsf(cm * a.scale2) >= FAR ? a.far_scale2 : a.scale2;
+                const float mn = moves ? cm * scale2 : m, f = mn > -INFINITY ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
                 l *= f;
 #pragma unroll
                 for (int d = 0; d < DT; d++) acc[d] *= f;
@@ -729,7 +737,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
             const float ms = m > -INFINITY ? m : 0.0f;
             float p[16];
 #pragma unroll
-            for (int e = 0; e < 16; e++) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale2, -ms));
+            for (int e = 0; e < 16; e++) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], scale2, -ms));
             if (masked) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) p[e] = sees >> e & 1 ? p[e] : 0.0f;
@@ -1271,6 +1279,8 @@ int launch_attn_paged(const bmk_launch_t* l, bool bf16) {
     const float scale = bmk_pf(l, 7, 0);
     a.flip = std::signbit(scale) ? 0x80000000u : 0u;
     a.scale2 = fabsf(scale) * 1.44269504088896341f;
+    int two;
+    a.far_scale2 = a.scale2 < INFINITY && frexpf(a.scale2, &two) > 0.5f ? ldexpf(1.0f, two) : a.scale2; /* 0 and the powers of two are their own */
     if (HD <= 64) return bf16 ? start<true, 64>(a, l) : start<false, 64>(a, l);
     if (HD <= 128) return bf16 ? start<true, 128>(a, l) : start<false, 128>(a, l);
     return bf16 ? start<true, 256>(a, l) : start<false, 256>(a, l);

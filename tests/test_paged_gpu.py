@@ -726,6 +726,48 @@ def test_attention_scores_far_apart(be, kind):
 
 
 @both
+@pytest.mark.parametrize("HD", [64, 128, 256])
+@pytest.mark.parametrize("new,total", [([1, 2], [1500, 40]), ([40], [900]), ([130, 1], [333, 20])])
+@pytest.mark.parametrize("at", [25, 29, 30, 31, 40, 100, "mixed"])
+def test_attention_scores_past_what_tells_them_apart(be, at, new, total, HD, kind):
+    """Scores of 2^at and a few steps of the type more, to 2^100, or of both signs from 1 to 2^34: q and K have one dimension, so a
+    score is exact, and the answer is the softmax of those numbers: the largest takes all, or its equals share, or the steps are small
+    enough for weights between.
+
+    The exponent is one rounding of its own size and one of the row's base, which is a step of the score, up to 2^9 where that
+    still lets a second weight live; the scale's rounding, the exponential, a rounding a key in the sums."""
+    mixed, at = at == "mixed", 34 if at == "mixed" else at
+    rng = np.random.default_rng(at * 1000 + HD + sum(new))
+    step = 2.0 ** (-7 if kind.bf16 else -23)
+    for sign, scale in ((1, 1.0), (-1, 1.0), (1, 0.7), (1, -1.0)):
+        scale = float(np.float32(scale))
+        b = Batch(be, rng, kind, new, total, 16, 1, HD, fill=0.0)
+        b.fill(rng)
+        d = int(rng.integers(0, HD))
+        for s in range(b.S):
+            k = np.zeros((1, total[s], HD), np.float32)
+            k[0, :, d] = 2.0 ** (at // 2) * (1 + step * rng.integers(0, 5, total[s]))
+            if mixed:  # rising from far below 0 to far above in the order of the keys, here and there the other way
+                k[0, :, d] *= np.exp2(-rng.integers(0, 35, total[s])) * np.where(rng.random(total[s]) < 0.99, -1, 1)
+                k[0, :total[s] // 2, d] = -np.abs(k[0, :total[s] // 2, d])
+            b.K[s] = k
+            b.set(s, k, b.V[s])
+        q = np.zeros((b.N, 3, HD), np.float32)
+        q[..., d] = sign * 2.0 ** (at - at // 2)
+        got = attention(be, b, q, 3, scale)
+        for n in range(b.N):
+            s, seen = b.seq[n], b.pos[n] + 1
+            k, v = (x[s][0, :seen].astype(np.float64) for x in (b.K, b.V))
+            away = k[:, d] * q[n, 0, d] * scale
+            away -= away.max()
+            p = np.exp(away)
+            p /= p.sum()
+            e = (3 * np.abs(away) + min(2.0 ** (at - 22), 512.0) + 32 + seen + 64) * U32
+            off = 2 * (p * e) @ np.abs(v)
+            check(kind, got[n], np.broadcast_to(p @ v, (3, HD)), off + kind.step * (p @ np.abs(v)))
+
+
+@both
 def test_attention_many_sequences(be, kind):
     """More sequences than lanes, some without tokens, some without keys."""
     rng = np.random.default_rng(12)
