@@ -41,6 +41,7 @@ constexpr int AT_MAX_SPLIT = 64; /* records the merge holds weights for in LDS *
  * the counters stay zero between launches of any shape. */
 constexpr int AT_DONE_STRIDE = 32, AT_MAX_GROUPS = 1024;
 constexpr size_t AT_DONE_BYTES = (size_t)AT_DONE_STRIDE * AT_MAX_GROUPS * 4;
+static_assert(AT_DONE_BYTES <= BMK_SCRATCH_COUNTERS, "");
 constexpr size_t AT_SCRATCH_BYTES = (size_t)8 << 20; /* as much of it as the splits are cut for */
 
 /* Keys a wave takes per tile: each load instruction covers 256 / HD keys (16

@@ -79,6 +79,7 @@ constexpr int CUS = 256, ROUNDS = 4, ROUND_TILES = 32; /* Cut::begin */
  * kernel; a table of the work and the units' partial results lie behind them. */
 constexpr int DONE_STRIDE = 32, MAX_UNITS = 1024;
 constexpr size_t DONE_BYTES = (size_t)DONE_STRIDE * MAX_UNITS * 4, TABLE_BYTES = 1024;
+static_assert(DONE_BYTES <= BMK_SCRATCH_COUNTERS, "");
 
 struct PaArgs {
     const void* q;

@@ -15,6 +15,7 @@
 #include <stdint.h>
 
 #define BMK_MAX_BUFFERS 12
+#define BMK_SCRATCH_COUNTERS ((size_t)128 << 10) /* bytes at the scratch memory's start that are zero between launches */
 
 typedef struct {
     hipStream_t stream;

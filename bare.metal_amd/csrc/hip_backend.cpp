@@ -62,7 +62,16 @@ static bool hip_ok(hipError_t e, const char* what, const char* file, int line) {
     return false;
 }
 
-#define BMK_SCRATCH_BYTES ((size_t)64 << 20)
+/* A context's scratch memory: as much as attention over pages cuts its work for, or where the device has not that much left, as
+ * attention_forward does; 0 and NULL where it has neither.  The failed tries leave no error for the next launch's check. */
+extern "C" size_t bmk_scratch_alloc(void** p, hipError_t (*alloc)(void**, size_t)) {
+    for (size_t bytes : {(size_t)64 << 20, (size_t)8 << 20}) {
+        if (alloc(p, bytes) == hipSuccess) return bytes;
+        (void)hipGetLastError();
+    }
+    *p = nullptr;
+    return 0;
+}
 
 static inline hipStream_t ctx_stream(backend_ctx_t* ctx) { return (hipStream_t)ctx->queue; }
 
@@ -133,14 +142,13 @@ extern "C" backend_ctx_t* backend_create(void) {
         return NULL;
     }
     /* a context's launches run in the order of its one stream, so they share one scratch memory; without
-     * it the kernels that would split their work run unsplit */
-    if (hipMalloc(&ctx->scratch, BMK_SCRATCH_BYTES) == hipSuccess &&
-        hipMemsetAsync(ctx->scratch, 0, BMK_SCRATCH_BYTES, s) == hipSuccess) {
-        ctx->scratch_bytes = BMK_SCRATCH_BYTES;
-    } else {
+     * it the kernels that would split their work run unsplit.  The counters that it begins with are zero between launches. */
+    ctx->scratch_bytes = bmk_scratch_alloc(&ctx->scratch, [](void** p, size_t n) { return hipMalloc(p, n); });
+    if (ctx->scratch && hipMemsetAsync(ctx->scratch, 0, BMK_SCRATCH_COUNTERS, s) != hipSuccess) {
         (void)hipGetLastError();
-        BMK_WARN("backend_create: no scratch memory, kernels run unsplit");
+        ctx->scratch_bytes = 0;
     }
+    if (!ctx->scratch_bytes) BMK_WARN("backend_create: no scratch memory, kernels run unsplit");
     ctx->device = (void*)(intptr_t)dev;
     ctx->queue = (void*)s;
     ctx->library = (void*)bmk_table;

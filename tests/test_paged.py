@@ -313,6 +313,26 @@ def test_a_launch_stays_under_the_work_items_of_an_axis(lanes):
         assert int(xy[0]) * int(xy[1]) * slots < 1 << 31
 
 
+@pytest.mark.parametrize("room,want,tries", [(1 << 40, 64, 1), (64, 64, 1), (63, 8, 2), (8, 8, 2), (7, 0, 2), (0, 0, 2)])
+def test_scratch_memory_of_a_full_device(room, want, tries):
+    """64 MiB, or where there is not that much the 8 that attention_forward cuts its work for, or none."""
+    asked = []
+    hook = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.POINTER(ctypes.c_void_p), ctypes.c_size_t)
+
+    def alloc(p, n):
+        asked.append(n)
+        if n > room << 20:
+            return 2  # out of memory
+        p[0] = 4096
+        return 0
+
+    fn = bmhip.lib().bmk_scratch_alloc
+    fn.restype, fn.argtypes = ctypes.c_size_t, [ctypes.c_void_p, hook]
+    p = ctypes.c_void_p(7)
+    assert fn(ctypes.byref(p), hook(alloc)) == want << 20 and len(asked) == tries
+    assert p.value == (4096 if want else None)
+
+
 # ---------------------------------------------------------------- what the fp32 attention's bound tells apart
 
 FOUR = [(1, 1), (1, 0), (0, 1), (0, 0)]

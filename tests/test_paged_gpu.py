@@ -1217,3 +1217,40 @@ def test_scratch_is_left_for_the_next_kernel(be):
         assert np.array_equal(x, seen[0][0]) and np.array_equal(y, seen[0][1])
     want, off = attend(b, q2, NH, 0.125)
     check(KINDS[0], seen[0][1].reshape(2, NH, HD), want, off)
+
+
+@pytest.mark.parametrize("size", [64 << 20, 8 << 20])
+def test_scratch_memory_holds_anything_but_counters(be, size):
+    """What lies in a context's scratch memory behind its counters does not matter, and attention_forward cuts its work alike in one of
+    8 MiB: its results have the same bits."""
+    rng = np.random.default_rng(47)
+    NH, NKV, HD, S = 15, 5, 64, 2048
+    kv = rng.standard_normal((2, S, NKV * HD)).astype(np.float32)
+    q = rng.standard_normal((1, NH * HD)).astype(np.float32)
+
+    def flat(c):
+        out = marked(c, q.nbytes)
+        assert c.dispatch("attention_forward", [c.upload(q), c.upload(kv), out, c.params(NH, HD, NKV, NKV * HD, S, 3, 0, S),
+                                                floats(c, 0.125)], (NH,), (64,)) == 0
+        return out.read(np.float32)
+
+    other = bmhip.Backend()
+    try:
+        c = Context.from_address(other.ctx)
+        c.scratch_bytes = size
+        hip = ctypes.CDLL("libamdhip64.so")
+        hip.hipMemset.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t]
+        other.synchronize()
+        assert hip.hipMemset(c.scratch + (128 << 10), 0xFF, size - (128 << 10)) == 0 and hip.hipDeviceSynchronize() == 0
+        for S_ in (3, 200):
+            new = [1 + s % 2 for s in range(S_)]
+            total = [n + (3000 if s in (0, S_ - 1) else 20) for s, n in enumerate(new)]
+            for kind in KINDS:
+                b = Batch(other, rng, kind, new, total, 16, 2, 64)
+                b.fill(rng)
+                x = kind.held(rng.standard_normal((b.N, 6, 64)))
+                want, off = attend(b, x, 6, 0.125)
+                compare(b, attention(other, b, x, 6, 0.125), want, off)
+        assert np.array_equal(flat(other), flat(be))
+    finally:
+        other.close()
