@@ -489,6 +489,72 @@ def test_kv_append_skips_what_has_no_place(be, kind):
                 assert (raw[pg, :, j].copy().view(np.uint8) == MARK).all(), (pg, j)
 
 
+@both
+@pytest.mark.parametrize("S", [65, 1000, 4096])
+def test_kv_append_of_many_sequences(be, S, kind):
+    """As many sequences as a batch takes, some without tokens, in a call of more rows than a workgroup has: every row is in its place."""
+    rng = np.random.default_rng(S)
+    new = [int(x) for x in rng.choice([0, 0, 1, 1, 2, 3], S)]
+    total = [n + int(rng.integers(0, 30)) for n in new]
+    NH, NKV, HD, page = 2, 1, 16, 8
+    b = Batch(be, rng, kind, new, total, page, NKV, HD, 1, 2)
+    q, k, v = (kind.held(rng.standard_normal((b.N, w * HD))) for w in (NH, NKV, NKV))
+    table, m = turn_table(HD, "none")
+    cache = marked(be, b.cache.size * kind.size)
+    out = marked(be, b.N * NH * HD * kind.size)
+    assert be.dispatch("kv_append_paged" + kind.suffix, [be.upload(kind.raw(x)) for x in (q, k, v)] + [out, cache] + b.tables(be) + [
+        be.upload(table), be.upload(table), be.params(b.N, S, NH, NKV, HD, HD, 0, NH * HD, HD, HD, NH * HD, page, b.count, b.width, 0),
+        floats(be, m, 0.0)], (b.N,), (256,)) == 0
+    at = np.flatnonzero(b.seq >= 0)
+    want, off = turned(q.reshape(b.N, NH, HD), b.pos, HD, 0, table, m)
+    got = rows_of(kind, out, b.N, NH * HD, NH * HD, 0, b.seq >= 0).reshape(b.N, NH, HD)
+    check(kind, got[at], want[at], off[at])
+    raw = cache.read(kind.memory, b.cache.size).reshape(b.cache.shape)
+    want, off = turned(k.reshape(b.N, NKV, HD), b.pos, HD, 0, table, m)
+    pg, j = b.pages[b.seq[at], b.pos[at] // page], b.pos[at] % page
+    check(kind, kind.values(raw[pg, 0, :, j]), want[at], off[at])
+    assert np.array_equal(kind.values(raw[pg, 1, :, j]).reshape(-1, HD), v[at])
+    raw[pg, :, :, j] = np.full(1, MARK, np.uint8).repeat(kind.size).view(kind.memory)[0]
+    assert (raw.view(np.uint8) == MARK).all()  # nothing else was written
+
+
+@both
+@pytest.mark.parametrize("norm", [0, 1], ids=["plain", "norm"])
+def test_kv_append_past_the_cache_has_the_same_bits(be, norm, kind):
+    """A call of more than 128 MB, which reads past the caches, against its rows in calls of fewer, each behind what is there."""
+    NH, NKV, HD, page, S = 4, 2, 128, 64, 3
+    W = (NH + 2 * NKV) * HD
+    N = (150 << 20) // (W * kind.size) // S * S
+    n = N // S
+    rng = np.random.default_rng(51)
+    block = kind.raw(rng.standard_normal((1 << 16) + 7).astype(np.float32))
+    width = -(-n // page)
+    qkv = be.upload(np.resize(block, (N, W)))
+    pages = be.upload(rng.permutation(S * width).astype(np.int32).reshape(S, width))
+    table, m = turn_table(HD, "none")
+    rest = [be.upload(table), be.upload(rng.standard_normal((2, HD)).astype(np.float32))]
+
+    def run(cache, out, start, length, first, rows):
+        shift = first * W * kind.size
+        assert be.dispatch("kv_append_paged" + kind.suffix, [
+            qkv, qkv, qkv, out, cache, be.upload(np.int32(start)), be.upload(np.int32(length)), pages] + rest + [
+            be.params(rows, S, NH, NKV, HD, HD, 0, W, W, W, NH * HD, page, S * width, width, norm), floats(be, m, 1e-5)], (rows,),
+            (256,), offsets=[shift, shift + NH * HD * kind.size, shift + (NH + NKV) * HD * kind.size,
+                             first * NH * HD * kind.size] + [0] * 8) == 0
+
+    def buffers():
+        return be.alloc(S * width * 2 * NKV * page * HD * kind.size), marked(be, N * NH * HD * kind.size)
+
+    whole, parts = buffers(), buffers()
+    run(*whole, [0, n, 2 * n, N], [n] * S, 0, N)
+    for s in range(S):
+        for a in range(0, n, 5000):
+            c = min(5000, n - a)
+            run(*parts, [0] * (s + 1) + [c] * (S - s), [a + c if x == s else 0 for x in range(S)], s * n + a, c)
+    for x, y in zip(whole, parts):
+        assert np.array_equal(x.read(np.uint8), y.read(np.uint8))
+
+
 # ---------------------------------------------------------------- attention
 
 def attend(b, q, NH, scale, causal=1, window=0):
@@ -837,6 +903,38 @@ def test_attention_tables_that_are_no_batch(be, S, how):
     mark = marked(be, past).read(np.uint8)
     assert np.array_equal(out.read(np.uint8)[room:], mark)
     compare(b, attention(be, b, q, 2, 0.125), want, off)
+
+
+@both
+@pytest.mark.parametrize("NH,NKV,HD", [(6, 2, 64), (4, 1, 128), (2, 1, 256)])
+@pytest.mark.parametrize("new,total,causal,window", [([1], [3000], 0, 0), ([50], [2500], 0, 0), ([140, 1, 9], [2100, 1800, 40], 0, 0),
+                                                     ([1, 2], [3000, 1700], 1, 700), ([50, 3], [2500, 900], 1, 33),
+                                                     ([140, 1, 9], [2100, 1800, 40], 1, 700), ([70], [1500], 1, (1 << 31) - 1)])
+def test_attention_masks_over_keys_in_parts(be, causal, window, new, total, NH, NKV, HD, kind):
+    """Every mask where the keys that rows see are many enough to be split, and where a window leaves few of many."""
+    rng = np.random.default_rng(sum(new) + HD)
+    b = Batch(be, rng, kind, new, total, 16, NKV, HD)
+    b.fill(rng)
+    q = kind.held(rng.standard_normal((b.N, NH, HD)))
+    scale = float(np.float32(HD ** -0.5))
+    want, off = attend(b, q, NH, scale, causal, window)
+    compare(b, attention(be, b, q, NH, scale, causal, window), want, off)
+
+
+@both
+@pytest.mark.parametrize("causal,window", [(0, 0), (1, 300)])
+def test_attention_masks_of_many_sequences(be, causal, window, kind):
+    """The same for more sequences than lanes, a few of them long."""
+    rng = np.random.default_rng(50)
+    new = [int(x) for x in rng.choice([0, 1, 1, 2], 150)]
+    total = [n + int(rng.integers(0, 50)) for n in new]
+    for s, n, t in ((0, 1, 2500), (70, 40, 1500), (149, 3, 900)):
+        new[s], total[s] = n, t
+    b = Batch(be, rng, kind, new, total, 16, 1, 64, 2, 3)
+    b.fill(rng)
+    q = kind.held(rng.standard_normal((b.N, 3, 64)))
+    want, off = attend(b, q, 3, 0.125, causal, window)
+    compare(b, attention(be, b, q, 3, 0.125, causal, window), want, off)
 
 
 @both
