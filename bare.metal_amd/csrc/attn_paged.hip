@@ -24,8 +24,11 @@
  * x = x0 + x1 + x2 of bf16, exactly: |x1| < 2^-7 |x|, |x2| <= 2^-16 |x|, x2 of
  * either sign.  Six of the nine products are taken; what the other three would add is at
  * most 2^-22 of a product, 0.4 x 2^-24 in the mean and of either sign (with all terms cut off
- * towards zero up to 2^-21, and 0.7 x 2^-24 too little in the mean).  P is rounded to bf16 where q, K and V are
- * (its sum is not), which is half a step of the output's own type.
+ * towards zero up to 2^-21, and 0.7 x 2^-24 too little in the mean).  In bf16
+ * P goes in as two terms, 2^-17 of it, where waves go alone, which the reads hide; where rows
+ * fill the waves it is rounded to bf16, half a step of the output's own type (its sum is
+ * not): 1.9 to 2.1e-3 from the exact result in place of the 1.66e-3 of the output's rounding,
+ * but 2048 tokens over 16384 keys in 635 us in place of 760.
  *
  * What bounds it (us a pass, MI355X).  One token a sequence: reading the
  * cache; 64 sequences of 8192 keys, 8 KV heads of 128 in bf16, 233 (5.4 TB/s), 1024 of 512
@@ -606,7 +609,8 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
         /* The tile of keys k0 .. k0 + 31, in LDS at `buf`.  Reads are issued in groups ahead of the products that take
          * them, the first of V's ahead of the softmax. */
         constexpr int KG = !BF16 && HDP == 256 ? 1 : 2, VG = 1;
-        auto block = [&](auto form, const unsigned char* buf, int k0, auto behind_k) __attribute__((always_inline)) {
+        auto block = [&](auto form, auto weights, const unsigned char* buf, int k0, auto behind_k) __attribute__((always_inline)) {
+            constexpr int PT = decltype(weights)::value; /* terms of the weights */
             constexpr int FORM = decltype(form)::value, PLANES = Tile<FORM, HDP>::PLANES, PLANE = Tile<FORM, HDP>::PLANE;
             constexpr int ROWB = Tile<FORM, HDP>::ROWB, CPR = Tile<FORM, HDP>::CPR;
             f32x16 sc;
@@ -747,15 +751,16 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
 #pragma unroll
             for (int e = 0; e < 4; e++) s4[e] = (p[e] + p[e + 4]) + (p[e + 8] + p[e + 12]);
             l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
-            bf16x8 pf[TERMS][2];
+            bf16x8 pf[PT][2];
 #pragma unroll
             for (int s = 0; s < 2; s++) {
-                unsigned int u[TERMS][4];
+                unsigned int u[PT][4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const float x = p[8 * s + 2 * e], y = p[8 * s + 2 * e + 1];
                     if constexpr (BF16) {
                         u[0][e] = pack_rne(x, y);
+                        if constexpr (PT == 2) u[1][e] = pack_rne(x - low_half(u[0][e]), y - high_half(u[0][e]));
                     } else {
                         unsigned int z[3];
                         split2(x, y, z);
@@ -764,7 +769,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                     }
                 }
 #pragma unroll
-                for (int x = 0; x < TERMS; x++) __builtin_memcpy(&pf[x][s], u[x], 16);
+                for (int x = 0; x < PT; x++) __builtin_memcpy(&pf[x][s], u[x], 16);
             }
             __builtin_amdgcn_sched_barrier(0);
 if constexpr (W::HALVES) {
@@ -847,15 +852,17 @@ if constexpr (W::HALVES) {
                             o = mfma(y[1], pf[1][s], o);
                             o = mfma(y[1], pf[0][s], o);
                             o = mfma(y[0], pf[1][s], o);
+                        } else if constexpr (PT == 2) {
+                            o = mfma(y[0], pf[1][s], o);
                         }
                         o = mfma(y[0], pf[0][s], o);
                     }
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        auto compute = [&](auto form, const unsigned char* buf, int kt, auto behind_k) __attribute__((always_inline)) {
+        auto compute = [&](auto form, auto weights, const unsigned char* buf, int kt, auto behind_k) __attribute__((always_inline)) {
             const int k0 = kt * KT;
-            if (active && (kt & (kparts - 1)) == kpart && k0 <= any_last && k0 + 31 >= any_first && k0 < hi) block(form, buf, k0, behind_k);
+            if (active && (kt & (kparts - 1)) == kpart && k0 <= any_last && k0 + 31 >= any_first && k0 < hi) block(form, weights, buf, k0, behind_k);
         };
 
         /* Straight into LDS, 16 bytes a lane, a wave's load RPI rows, eight at most, which lie in one page.  Its number is read
@@ -931,7 +938,7 @@ if constexpr (W::HALVES) {
                 pages(kt + kparts);
                 __builtin_amdgcn_s_waitcnt(0x0F70); /* vmcnt(0) */
                 asm volatile("" ::: "memory");
-                compute(std::integral_constant<int, W::ALONE>{}, buf, kt, [&]() __attribute__((always_inline)) {
+                compute(std::integral_constant<int, W::ALONE>{}, std::integral_constant<int, BF16 ? 2 : 3>{}, buf, kt, [&]() __attribute__((always_inline)) {
                     if constexpr (W::HALVES) request(kt, true);
                 });
                 asm volatile("" ::: "memory");
@@ -972,7 +979,7 @@ if constexpr (W::HALVES) {
                 barrier();
                 request(kt + 3, before);
                 pages(kt + 4);
-                compute(std::integral_constant<int, AS_BF16>{}, buf, kt, []() {});
+                compute(std::integral_constant<int, AS_BF16>{}, std::integral_constant<int, 1>{}, buf, kt, []() {});
             };
             for (int kt = kt0; kt < kt1; kt += 4) {
                 step(kt, lds0, lds3);
@@ -1032,7 +1039,7 @@ if constexpr (W::HALVES) {
                 __syncthreads(); /* the tile is there, and the one before has been read */
                 fetch(kt + 1); /* behind the part's last: zeros */
                 pages(kt + 2);
-                compute(std::integral_constant<int, TERMS3>{}, buf, kt, []() {});
+                compute(std::integral_constant<int, TERMS3>{}, std::integral_constant<int, 3>{}, buf, kt, []() {});
             }
         }
         l += other_half(l);

@@ -589,6 +589,13 @@ def attend(b, q, NH, scale, causal=1, window=0):
     return out, off
 
 
+def attend_values(b, NH, q, scale, window=0):
+    """softmax(..) |V|, which the weights' rounding in `attend` is relative to."""
+    c = Batch.__new__(Batch)
+    c.__dict__.update(b.__dict__, V=[np.abs(v) for v in b.V])
+    return attend(c, q, NH, scale, 1, window)[0]
+
+
 def attention(be, b, q, NH, scale, causal=1, window=0, ldq=None, ldo=None, lead=0, cache=None, tables=None, out=None):
     """One call; the rows of out, checked to hold the mark wherever no sequence has a row."""
     kind, W = b.kind, NH * b.HD
@@ -1155,6 +1162,22 @@ def test_attention_is_fp32_on_average(be, new, total, page, window, NH, NKV, HD)
         for h in range(NH):
             allowed[n, h] = deviation(q[n, h], *(x[s][h // (NH // NKV), first:last + 1] for x in (b.K, b.V)), scale)
     assert np.sqrt((err ** 2).mean() / (allowed ** 2).mean()) < 2
+
+
+@pytest.mark.parametrize("NH,NKV,HD", [(3, 1, 8), (15, 5, 64), (32, 1, 64), (8, 2, 128), (4, 1, 200), (4, 1, 256)])
+@pytest.mark.parametrize("new,total,window", [([1] * 5, [2, 40, 300, 150, 77], 0), ([1, 1], [1500, 1100], 0), ([1, 1], [600, 90], 33),
+                                              ([1] * 70, [30] * 69 + [900], 0)])
+def test_attention_of_few_rows_rounds_once_in_bf16(be, new, total, window, NH, NKV, HD):
+    """Up to 32 rows of a KV head (single tokens): the weights go into the second product as two terms of bf16, 2^-17 of each, so
+    that the result is off by its own rounding and fp32 steps alone."""
+    rng = np.random.default_rng(sum(total) * 31 + HD)
+    b = Batch(be, rng, KINDS[1], new, total, 16, NKV, HD)
+    b.fill(rng)
+    q = b.kind.held(rng.standard_normal((b.N, NH, HD)))
+    scale = float(np.float32(HD ** -0.5))
+    want, off = attend(b, q, NH, scale, 1, window)
+    most = attend_values(b, NH, q, scale, window)
+    check(b.kind, attention(be, b, q, NH, scale, 1, window), want, off + (2.0 ** -17 - b.kind.step) * most)
 
 
 @pytest.mark.parametrize("NH,HD", [(1, 8), (3, 64), (2, 96), (1, 128), (2, 200), (1, 256)])
