@@ -89,8 +89,8 @@ __device__ __forceinline__ void store(void* p, size_t i, const float* x) {
 }
 
 /* cos and sin of t / 2^32 of a turn: the nearest quarter taken off, the
- * Taylor series of what is left (at most pi / 4 to either side), whose next
- * terms are under 2e-9. */
+ * Taylor series of what is left (at most pi / 4 to either side, fp32: up to
+ * 2^-26.3 of a turn off), whose next terms are under 2e-9; 1.7 x 2^-24 off in all. */
 __device__ __forceinline__ void cos_sin(unsigned int t, float* c, float* s) {
     const unsigned int quarter = (t + 0x20000000u) >> 30;
     const float x = (float)(int)(t - (quarter << 30)) * 1.46291807926715968e-9f; /* 2 pi / 2^32 */

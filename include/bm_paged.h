@@ -7,8 +7,9 @@
  *
  * Named kernels, bound like any other through backend_encode_dispatch (the
  * grid and threadgroup sizes are not looked at).  A _bf16 name takes and
- * gives bf16 where "T" stands, the plain name f32; arithmetic is fp32 and
- * results are rounded once.  Rows of a matrix lie ld elements apart, on an
+ * gives bf16 where "T" stands, the plain name f32; sums and norms are held in
+ * fp32 or more and results rounded once (what attention_forward_paged rounds
+ * besides stands with it).  Rows of a matrix lie ld elements apart, on an
  * element's boundary; a row holds its heads one after another, HD elements
  * each (HD even and at most 256; a multiple of 8 where there is a cache).
  * Row counts may be 0 (nothing is done).  Outputs may not overlap inputs but
@@ -32,10 +33,10 @@
  * i + rot/2 (layout 0, halves) or 2i and 2i + 1 (layout 1, neighbours), is
  * turned at position p by a = 2 pi (p * turns[i] mod 2^64) / 2^64 and
  * multiplied by mscale: (x0, x1) -> mscale (x0 cos a - x1 sin a, x0 sin a + x1
- * cos a).  turns u64 [rot/2] on an 8-byte boundary comes from bm_rope_turns; the angle is off by at
- * most 2^-32 of a turn at any position, where rope_forward's fp32 product loses
- * the fraction of far ones (so the two differ by up to about p * 2^-24 in the
- * angle).  Elements from rot on pass unturned.  rot 0: no rotation (bind any
+ * cos a).  turns u64 [rot/2] on an 8-byte boundary comes from bm_rope_turns; the product's fraction of a
+ * turn is kept to 2^-32 (and the table's rounding, 2^-64 a position) at any position, where rope_forward's
+ * fp32 product loses the fraction of far ones (so the two differ by up to about p * 2^-24 in the
+ * angle).  cos and sin of it are fp32's, within 2 x 2^-24.  Elements from rot on pass unturned.  rot 0: no rotation (bind any
  * buffer as turns).
  *
  *   "rope_forward_rows", "rope_forward_rows_bf16"
@@ -69,6 +70,13 @@
  *                         What masked keys, values and the rest of a page hold does not matter,
  *                         infinities and NaN included; a value that a row sees and that is not
  *                         finite makes that element of the row not finite, a key its whole row
+ *                         (but in bf16 a key whose score is -infinity has weight 0).
+ *                         Roundings: scores and sums are fp32.  f32: operands of the products as
+ *                         three terms of bf16, six products of nine, which leaves out at most 2^-22 of a
+ *                         product; multiples of 2^-133 remain of an element.  bf16: of a sequence with up to 32 rows
+ *                         for a KV head (new tokens x query heads) the weights keep 2^-17 of each, with
+ *                         more they are rounded to bf16 (of long random sums, 2.1e-3 from the exact result in the mean
+ *                         square in place of 1.7e-3).  Finite for scores up to 2^125 with values up to 2^56
  */
 #ifndef BM_PAGED_H
 #define BM_PAGED_H

@@ -201,6 +201,28 @@ def test_rope_leaves_the_rest_of_a_head(be, kind):
         assert np.array_equal(got[0], x[0], equal_nan=True)  # position 0: no turn
 
 
+def test_cos_and_sin_of_any_turn(be):
+    """A million fractions of a turn, the quarters' borders among them: x = (1, 0) comes out as (cos, sin), within 2 units of 2^-24 and
+    the 2^-32 of a turn that the fraction is kept to."""
+    N, HD = 8192, 256
+    rng = np.random.default_rng(52)
+    table = rng.integers(0, 1 << 64, HD // 2, dtype=np.uint64)
+    table[:16] = [(k << 61) + d & ((1 << 64) - 1) for k in range(8) for d in (0, -1)]
+    pos = rng.integers(-(1 << 31), 1 << 31, N).astype(np.int32)
+    pos[:4] = [0, 1, -1, 3]
+    x = np.zeros((N, HD), np.float32)
+    x[:, :HD // 2] = 1
+    out = marked(be, x.nbytes)
+    assert be.dispatch("rope_forward_rows", [be.upload(x), out, be.upload(pos), be.upload(table), be.params(N, 1, HD, HD, 0, HD, HD),
+                                             floats(be, 1.0)], (N,), (256,)) == 0
+    got = out.read(np.float32).reshape(N, 2, HD // 2).astype(np.float64)
+    with np.errstate(over="ignore"):
+        turn = pos.astype(np.int64).view(np.uint64)[:, None] * table
+    a = turn.astype(np.float64) * (2 * np.pi / 2.0 ** 64)
+    off = 2 * U32 + 2 * np.pi * 2.0 ** -32 + 1e-15
+    assert np.abs(got[:, 0] - np.cos(a)).max() <= off and np.abs(got[:, 1] - np.sin(a)).max() <= off
+
+
 def test_rope_of_more_work_items_than_an_axis_takes(be):
     """Heads of 256 at odd strides take 64 lanes each: 2^26 heads and more are over 2^32 work-items.  34 GB, in place, zeros but
     for a few rows, which the kernel itself (rot 0) puts there and takes back."""
