@@ -66,15 +66,16 @@ typedef __attribute__((address_space(3))) void lvoid;
 constexpr int KT = 32;           /* keys of a tile */
 /* in powers of two: how far a score may pass the running maximum before that moves (32 sequences of 16 tokens over 1500 keys,
  * with 0 28.8 us, with 8 27.6); fp32's sums have room for more */
-constexpr float SLACK = 8.0f;
+[[maybe_unused]] constexpr float SLACK = 8.0f;
 /* A row's weights are exp2(fma(score, scale2, -m)) with m = score * scale2 of its largest score, rounded, so that score's own
- * exponent is what the rounding left: up to 32 where m is under FAR, which all weights of the row have in common, but past fp32's
- * range from 2^31 on.  From FAR on the scores of a row, numbers of 24 bits, lie 64 apart or are equal: the largest takes all, also
- * with the power of two at or over scale2 in its place, whose products with them are exact.  (The rest of m as a second number,
- * carried to the joins: 2048 rows over 16384 keys 2% slower, 24 mixed sequences 4%.) */
-constexpr float FAR = 0x1p30f;
+ * exponent is what the rounding left: up to 32 where m is under FAR, which all weights of the row have in common, but past
+ * fp32's range from 2^31 on.  From FAR on the scores of a row, numbers of 24 bits, lie 64 apart or are equal: the largest takes
+ * all, also with the power of two at or over scale2 in its place, whose products with them are exact.  (The rest of m as a second
+ * number, carried to the joins: 2048 rows over 16384 keys 2% slower, 24 mixed sequences 4%.) */
+[[maybe_unused]] constexpr float FAR = 0x1p30f;
 constexpr int MAX_SPLIT = 128;   /* parts of a unit's keys */
-constexpr int LEAST = 4;         /* tiles a part, at least: one a wave (1 token over 300 keys, parts of 2 15.3 us, 4 15.1, 8 17.5) */
+/* tiles a part, at least: one a wave (1 token over 300 keys, parts of 2 15.3 us, 4 15.1, 8 17.5) */
+constexpr int LEAST = 4;
 constexpr int MANY_LEAST = 8;    /* ... of more than 32 rows (Cut::parts) */
 constexpr int CUS = 256, ROUNDS = 4, ROUND_TILES = 32; /* Cut::begin */
 
@@ -118,8 +119,8 @@ template <int FORM, int HDP> struct Tile {
     static constexpr int BYTES = 2 * PLANES * PLANE;
 };
 
-/* Chunk c of row r lies at c ^ key, key < 16, so that what lanes read at once lies on all 64 banks, 256 bytes: of K one chunk of 16
- * rows; of V two neighbouring chunks of 4 rows and the two after them (fp32: eight of a row and of the row 4 on).  Rows of
+/* Chunk c of row r lies at c ^ key, key < 16, so that what lanes read at once lies on all 64 banks, 256 bytes: of K one chunk
+ * of 16 rows; of V two neighbouring chunks of 4 rows and the two after them (fp32: eight of a row and of the row 4 on).  Rows of
  * 128 bytes lie in two halves of the banks already.  (2048 rows over 16384 keys, keys of 8 rows in place of 16 and V's halves
  * on the same banks: half of LDS' cycles were conflicts.) */
 template <int CPR>
@@ -136,7 +137,8 @@ template <bool BF16, int HDP> struct Shape {
     static constexpr int ALONE = BF16 ? AS_BF16 : AS_F32;
     static constexpr bool SHARED = BF16 || HDP <= 128;
     /* a wave's own tile where both halves do not fit for four waves: the values into the keys' place, once those are read (64
-     * sequences of 4000 keys, 4 heads of 256: two waves with both 689 us, four with halves 446; 512 rows of 4 heads over 4096 655 and 377) */
+     * sequences of 4000 keys, 4 heads of 256: two waves with both 689 us, four with halves 446; 512 rows of 4 heads over 4096
+     * 655 and 377) */
     static constexpr bool HALVES = !BF16 && HDP == 256;
     static constexpr int ALONE_BYTES = Tile<ALONE, HDP>::BYTES / (HALVES ? 2 : 1), ARRAYS = BF16 ? 4 : 1;
     static constexpr int BYTES = NW / ARRAYS * ALONE_BYTES; /* of an array */
@@ -149,7 +151,7 @@ template <bool BF16, int HDP> struct Shape {
 #define N4 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u
 #define N64 N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4, N4
 #define N512 N64, N64, N64, N64, N64, N64, N64, N64
-__device__ __attribute__((aligned(16))) const unsigned int pg_nans[8 * PG_MAX_HD] = {N512, N512, N512, N512};
+[[maybe_unused]] __device__ __attribute__((aligned(16))) const unsigned int pg_nans[8 * PG_MAX_HD] = {N512, N512, N512, N512};
 #undef N512
 #undef N64
 #undef N4
@@ -185,12 +187,20 @@ __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-/* of all lanes alike: in scalar registers, where a descriptor has to be (the compiler loops over the lanes' descriptors otherwise) */
+/* of all lanes alike: in scalar registers, where a descriptor has to be (the compiler loops over the lanes' descriptors
+ * otherwise) */
 __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ const char* scalar(const char* p) {
     const unsigned long long u = (unsigned long long)p;
     return (const char*)((unsigned long long)(unsigned int)scalar((int)(u >> 32)) << 32 | (unsigned int)scalar((int)u));
 }
+
+/* a descriptor of `bytes` bytes from p on, past whose end a load gives zeros and a store is dropped */
+#ifdef __HIP_DEVICE_COMPILE__ /* no type of the host's */
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const char* p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)scalar(p), 0, scalar(bytes), 0x00027000);
+}
+#endif
 
 /* all waves of the workgroup; memory accesses stay on their side of it */
 __device__ __forceinline__ void barrier() {
@@ -255,8 +265,8 @@ struct Sums {
 };
 /* Of more sequences than a wave has lanes, a kernel ahead lays out the work: here, of each 64 sequences, the sums up to their
  * end.  (Every wave for itself, 64 sequences at a time: 128 sequences of 512 keys 18.7 us, with the table 18.2; 512 of them 93
- * and 66, 4096 2165 and 490; 65 of 16 keys 6.9 and 9.1, which is the launch, so that up to 64, where the registers hold all, there is
- * none.) */
+ * and 66, 4096 2165 and 490; 65 of 16 keys 6.9 and 9.1, which is the launch, so that up to 64, where the registers hold all,
+ * there is none.) */
 struct Table {
     int per;            /* tiles a part */
     unsigned int total; /* pieces of work */
@@ -294,7 +304,9 @@ struct Cut {
         const unsigned int p = parts(q);
         return Sums{q.units * p * a.b.NKV, p > 1 ? (unsigned int)q.n * a.R * p * a.b.NKV : 0, p > 1 ? q.units * a.b.NKV : 0};
     }
-    static __device__ __forceinline__ Sums up_to(const Sums& m) { return Sums{dpp_sums(m.w), dpp_sums(m.recs), dpp_sums(m.units)}; }
+    static __device__ __forceinline__ Sums up_to(const Sums& m) {
+        return Sums{dpp_sums(m.w), dpp_sums(m.recs), dpp_sums(m.units)};
+    }
     /* from the sums over all sequences: of units times their tiles and of units, and the most tiles of one */
     __device__ __forceinline__ void begin(float tiles, float units, int longest) {
         tiles *= a.b.NKV;
@@ -305,8 +317,8 @@ struct Cut {
         const float want = a.slots * (tiles >= (float)a.slots * ROUND_TILES * ROUNDS ? ROUNDS : 1.0f);
         auto over = [](float x, float y) { return x * __builtin_amdgcn_rcpf(y); };
         int p = (int)over(tiles, fmaxf(want - 0.5f * units, 0.25f * want)) + 1;
-        /* were all as long as the longest: no parts that only just do not fit (24 sequences of 4000 keys, 8 heads of 128, in three
-         * parts 81 us, in two 72) */
+        /* were all as long as the longest: no parts that only just do not fit (24 sequences of 4000 keys, 8 heads of 128, in
+         * three parts 81 us, in two 72) */
         const float alike = over(tiles, (float)max(longest, 1));
         if (alike * ceilf(over((float)longest, (float)p) - 0.001f) > want)
             p = (int)ceilf(over((float)longest, fmaxf(floorf(over(want, alike)), 1.0f)) - 0.001f);
@@ -415,7 +427,8 @@ __global__ __launch_bounds__(1024) void k_attn_paged_plan(PaArgs a, Table* table
         rows += (float)q[i].n;
         longest = max(longest, q[i].T);
     }
-    auto all = [&](int turn, float x, float y, float z) __attribute__((always_inline)) { /* over the workgroup, in x, y, z's places */
+    /* over the workgroup, in x, y, z's places */
+    auto all = [&](int turn, float x, float y, float z) __attribute__((always_inline)) {
         const float v[3] = {lane_of(dpp_sums(x), 63), lane_of(dpp_sums(y), 63), lane_of(dpp_sums(z), 63)};
         if (lane == 0)
             for (int k = 0; k < 3; k++) sum[turn][k][wave] = v[k];
@@ -521,7 +534,8 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
         /* tiles of keys that some row of the unit sees, and this part's */
         const int lo = seen(a, p0 + tok0, it.len).first, hi = min(seen(a, p0 + tok1, it.len).last + 1, room);
         const int t0 = lo / KT, t1 = hi > lo ? (hi + KT - 1) / KT : t0;
-        const int parts = max(1, min(it.parts, (t1 - t0 + plan.cut.per - 1) / plan.cut.per)), per = (t1 - t0 + parts - 1) / parts; /* as even as they go */
+        const int parts = max(1, min(it.parts, (t1 - t0 + plan.cut.per - 1) / plan.cut.per));
+        const int per = (t1 - t0 + parts - 1) / parts; /* as even as they go */
         if (it.part >= parts) return;
         const int kt0 = t0 + it.part * per, kt1 = min(kt0 + per, t1);
         /* all waves have the same 32 rows and take turns on the keys' tiles, or each has rows of its own and all tiles */
@@ -532,7 +546,8 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
         const bool mine = r < r0 + nrows;
         const Seen sn = mine ? seen(a, p0 + tok, it.len) : Seen{0, -1};
         /* of the wave's rows: keys from all_first to all_last are seen by all, outside any_first .. any_last by none */
-        const int gtok0 = a.by_r.of(min(r0 + 32 * group, r0 + nrows - 1)), gtok1 = a.by_r.of(min(r0 + 32 * group + 31, r0 + nrows - 1));
+        const int gtok0 = a.by_r.of(min(r0 + 32 * group, r0 + nrows - 1));
+        const int gtok1 = a.by_r.of(min(r0 + 32 * group + 31, r0 + nrows - 1));
         const Seen sa = seen(a, p0 + gtok0, it.len), sz = seen(a, p0 + gtok1, it.len);
         const int any_first = sa.first, any_last = sz.last, all_first = sz.first, all_last = sa.last;
 
@@ -563,9 +578,10 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                     for (int i = 0; i < (BF16 ? 1 : 2); i++) {
                         const char* p = (const char*)a.q + (at + min(16 * s + 8 * half, HD - 8) + 4 * i) * ESZ;
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            qr[s][i][e] = BF16 ? ((const unsigned short*)p)[2 * e] | (unsigned int)((const unsigned short*)p)[2 * e + 1] << 16
-                                               : ((const unsigned int*)p)[e];
+                        for (int e = 0; e < 4; e++) {
+                            const unsigned short* two = (const unsigned short*)p + 2 * e;
+                            qr[s][i][e] = BF16 ? two[0] | (unsigned int)two[1] << 16 : ((const unsigned int*)p)[e];
+                        }
                     }
             }
         };
@@ -609,7 +625,8 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
         /* The tile of keys k0 .. k0 + 31, in LDS at `buf`.  Reads are issued in groups ahead of the products that take
          * them, the first of V's ahead of the softmax. */
         constexpr int KG = !BF16 && HDP == 256 ? 1 : 2, VG = 1;
-        auto block = [&](auto form, auto weights, const unsigned char* buf, int k0, auto behind_k) __attribute__((always_inline)) {
+        auto block = [&](auto form, auto weights, const unsigned char* buf, int k0,
+                         auto behind_k) __attribute__((always_inline)) {
             constexpr int PT = decltype(weights)::value; /* terms of the weights */
             constexpr int FORM = decltype(form)::value, PLANES = Tile<FORM, HDP>::PLANES, PLANE = Tile<FORM, HDP>::PLANE;
             constexpr int ROWB = Tile<FORM, HDP>::ROWB, CPR = Tile<FORM, HDP>::CPR;
@@ -626,12 +643,15 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                     const int at = g * KG + s;
                     if constexpr (FORM == AS_F32) {
 #pragma unroll
-                        for (int i = 0; i < 2; i++)
-                            kw[g & 1][s][i] = *(const f32x4*)(buf + row * ROWB + 16 * (k_place<CPR>(row, (4 * at & 15) + 2 * half + i) + (4 * at & ~15)));
+                        for (int i = 0; i < 2; i++) {
+                            const int place = k_place<CPR>(row, (4 * at & 15) + 2 * half + i) + (4 * at & ~15);
+                            kw[g & 1][s][i] = *(const f32x4*)(buf + row * ROWB + 16 * place);
+                        }
                     } else {
+                        const int place = k_place<CPR>(row, (2 * at & 15) + half) + (2 * at & ~15);
 #pragma unroll
                         for (int x = 0; x < PLANES; x++)
-                            kf[g & 1][s][x] = *(const bf16x8*)(buf + x * PLANE + row * ROWB + 16 * (k_place<CPR>(row, (2 * at & 15) + half) + (2 * at & ~15)));
+                            kf[g & 1][s][x] = *(const bf16x8*)(buf + x * PLANE + row * ROWB + 16 * place);
                     }
                 }
             };
@@ -645,7 +665,8 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                     for (int s = 0; s < 2; s++) {
                         if constexpr (FORM == AS_F32) {
                             const int vr = 16 * s + 4 * half, dim = 32 * (g * VG + d) + col;
-                            const unsigned char* at = buf + (W::HALVES ? 0 : PLANE) + vr * ROWB + 16 * v_place<FORM, CPR>(vr, dim >> 2) + 4 * (dim & 3);
+                            const unsigned char* at =
+                                buf + (W::HALVES ? 0 : PLANE) + vr * ROWB + 16 * v_place<FORM, CPR>(vr, dim >> 2) + 4 * (dim & 3);
 #pragma unroll
                             for (int e = 0; e < 8; e++) vw[g & 1][d][s][e] = *(const float*)(at + ((e & 3) + 2 * (e & 4)) * ROWB);
                         } else {
@@ -653,7 +674,8 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                             const int dim = 32 * (g * VG + d) + (lane & 16) + 4 * (lane & 3);
 #pragma unroll
                             for (int x = 0; x < PLANES; x++) {
-                                const unsigned char* at = buf + (PLANES + x) * PLANE + vr * ROWB + 16 * v_place<FORM, CPR>(vr, dim >> 3) + 2 * (dim & 4);
+                                const unsigned char* at = buf + (PLANES + x) * PLANE + vr * ROWB +
+                                                          16 * v_place<FORM, CPR>(vr, dim >> 3) + 2 * (dim & 4);
                                 s16x4 y[2]; /* the second set lies 8 rows on, in the same place of its row */
                                 y[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(lvoid*)at);
                                 y[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(lvoid*)(at + 8 * ROWB));
@@ -772,7 +794,7 @@ __global__ __launch_bounds__((Shape<BF16, HDP>::NT), (Shape<BF16, HDP>::WAVES)) 
                 for (int x = 0; x < PT; x++) __builtin_memcpy(&pf[x][s], u[x], 16);
             }
             __builtin_amdgcn_sched_barrier(0);
-if constexpr (W::HALVES) {
+            if constexpr (W::HALVES) {
                 __builtin_amdgcn_s_waitcnt(0x0F70); /* vmcnt(0): the values are there */
                 asm volatile("" ::: "memory");
                 read_v(0);
@@ -860,9 +882,11 @@ if constexpr (W::HALVES) {
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        auto compute = [&](auto form, auto weights, const unsigned char* buf, int kt, auto behind_k) __attribute__((always_inline)) {
+        auto compute = [&](auto form, auto weights, const unsigned char* buf, int kt,
+                           auto behind_k) __attribute__((always_inline)) {
             const int k0 = kt * KT;
-            if (active && (kt & (kparts - 1)) == kpart && k0 <= any_last && k0 + 31 >= any_first && k0 < hi) block(form, weights, buf, k0, behind_k);
+            if (active && (kt & (kparts - 1)) == kpart && k0 <= any_last && k0 + 31 >= any_first && k0 < hi)
+                block(form, weights, buf, k0, behind_k);
         };
 
         /* Straight into LDS, 16 bytes a lane, a wave's load RPI rows, eight at most, which lie in one page.  Its number is read
@@ -874,21 +898,22 @@ if constexpr (W::HALVES) {
         const int end = min(hi, kt1 * KT), rowb = HD * ESZ;
         const size_t page_bytes = (size_t)b.NKV * kv * (2 * ESZ), kh_bytes = (size_t)it.kh * kv * ESZ;
         auto page_of = [&](int key) { /* key: a multiple of 8, or within them; wave-uniform */
-            return ((const __attribute__((address_space(4))) int*)table)[__builtin_amdgcn_readfirstlane(max(min(key, hi - 1), 0) >> b.shift)];
+            return ((const __attribute__((address_space(4))) int*)table)[scalar(max(min(key, hi - 1), 0) >> b.shift)];
         };
         /* a lane's place in the rows of a load whose first row is `first` mod 16, of keys and of values */
         auto lane_place = [&](int first, int& k, int& v) {
             const int row = lane / CPR, place = lane % CPR;
-            const int kc = k_place<CPR>(first + row, place), vc = v_place<W::ALONE, CPR>(first + row, place); /* their own inverses */
+            /* their own inverses */
+            const int kc = k_place<CPR>(first + row, place), vc = v_place<W::ALONE, CPR>(first + row, place);
             k = 16 * kc < rowb ? row * rowb + 16 * kc : 1 << 30;
             v = 16 * vc < rowb ? row * rowb + 16 * vc : 1 << 30;
         };
-        auto load = [&](int pg, int key, unsigned char* to, int k_off, int v_off, bool keys = true, bool values = true) __attribute__((always_inline)) {
+        auto load = [&](int pg, int key, unsigned char* to, int k_off, int v_off, bool keys = true,
+                        bool values = true) __attribute__((always_inline)) {
             const bool there = (unsigned int)pg < (unsigned int)b.n_pages;
             const int bytes = min(max(end - key, 0), RPI) * rowb;
             const char* k = (const char*)a.cache + (there ? pg : 0) * page_bytes + kh_bytes + (unsigned int)((key & mask) * rowb);
-            const auto ks = __builtin_amdgcn_make_buffer_rsrc((void*)scalar(there ? k : (const char*)pg_nans), 0, scalar(bytes), 0x00027000);
-            const auto vs = __builtin_amdgcn_make_buffer_rsrc((void*)scalar(k + page_bytes / 2), 0, scalar(there ? bytes : 0), 0x00027000);
+            const auto ks = rsrc(there ? k : (const char*)pg_nans, bytes), vs = rsrc(k + page_bytes / 2, there ? bytes : 0);
             if (keys) __builtin_amdgcn_raw_ptr_buffer_load_lds(ks, (lvoid*)to, 16, k_off, 0, 0, 0);
             if (values) __builtin_amdgcn_raw_ptr_buffer_load_lds(vs, (lvoid*)(to + (W::HALVES ? 0 : PLANE)), 16, v_off, 0, 0, 0);
         };
@@ -924,7 +949,8 @@ if constexpr (W::HALVES) {
                     return;
                 }
 #pragma unroll
-                for (int i = 0; i < KT / RPI; i++) load(pg[i * RPI / 8], kt * KT + i * RPI, buf + i * 1024, k_off[i % KINDS], v_off[i % KINDS]);
+                for (int i = 0; i < KT / RPI; i++)
+                    load(pg[i * RPI / 8], kt * KT + i * RPI, buf + i * 1024, k_off[i % KINDS], v_off[i % KINDS]);
             };
             int kt = kt0 + ((kpart - kt0) & (kparts - 1)); /* tiles kpart mod kparts, as compute takes them */
             pages(kt);
@@ -938,9 +964,10 @@ if constexpr (W::HALVES) {
                 pages(kt + kparts);
                 __builtin_amdgcn_s_waitcnt(0x0F70); /* vmcnt(0) */
                 asm volatile("" ::: "memory");
-                compute(std::integral_constant<int, W::ALONE>{}, std::integral_constant<int, BF16 ? 2 : 3>{}, buf, kt, [&]() __attribute__((always_inline)) {
+                auto values = [&]() __attribute__((always_inline)) {
                     if constexpr (W::HALVES) request(kt, true);
-                });
+                };
+                compute(std::integral_constant<int, W::ALONE>{}, std::integral_constant<int, BF16 ? 2 : 3>{}, buf, kt, values);
                 asm volatile("" ::: "memory");
                 __builtin_amdgcn_sched_barrier(0);
                 if (kt + kparts < kt1) request(kt + kparts, false);
@@ -958,7 +985,8 @@ if constexpr (W::HALVES) {
             };
             auto request = [&](int kt, unsigned char* buf) {
 #pragma unroll
-                for (int i = 0; i < NI; i++) load(pg[i], kt * KT + (i * NW + wave) * RPI, buf + (i * NW + wave) * 1024, k_off[i % KN], v_off[i % KN]);
+                for (int i = 0; i < NI; i++)
+                    load(pg[i], kt * KT + (i * NW + wave) * RPI, buf + (i * NW + wave) * 1024, k_off[i % KN], v_off[i % KN]);
             };
             pages(kt0);
             q_request();
@@ -993,7 +1021,8 @@ if constexpr (W::HALVES) {
              * into their terms on the way into LDS, two tiles in turn. */
             typedef Tile<TERMS3, HDP> T3;
             constexpr int C3 = T3::CPR, HALF = KT * C3, PER = 2 * HALF / NT;
-            static_assert(2 * HALF % NT == 0 && HALF % 64 == 0 && 2 * T3::BYTES <= W::BYTES, "whole pieces, a wave's of keys or of values, two tiles");
+            static_assert(2 * HALF % NT == 0 && HALF % 64 == 0 && 2 * T3::BYTES <= W::BYTES,
+                          "whole pieces, a wave's of keys or of values, two tiles");
             constexpr int RPP = 64 / C3; /* rows of a wave's piece, in one page */
             f32x4 raw[PER][2];
             int pg[PER];
@@ -1009,11 +1038,13 @@ if constexpr (W::HALVES) {
                 for (int i = 0; i < PER; i++) {
                     const int key = kt * KT + row_of(i), part = part_of(i);
                     const bool there = (unsigned int)pg[i] < (unsigned int)b.n_pages;
-                    const char* k = (const char*)a.cache + (there ? pg[i] : 0) * page_bytes + kh_bytes + (unsigned int)((key & mask) * rowb);
-                    const auto from = __builtin_amdgcn_make_buffer_rsrc((void*)scalar(part ? k + page_bytes / 2 : there ? k : (const char*)pg_nans), 0,
-                                                                        scalar(part && !there ? 0 : min(max(end - key, 0), RPP) * rowb), 0x00027000);
+                    const char* k = (const char*)a.cache + (there ? pg[i] : 0) * page_bytes + kh_bytes +
+                                    (unsigned int)((key & mask) * rowb);
+                    const auto from = rsrc(part ? k + page_bytes / 2 : there ? k : (const char*)pg_nans,
+                                           part && !there ? 0 : min(max(end - key, 0), RPP) * rowb);
 #pragma unroll
-                    for (int e = 0; e < 2; e++) raw[i][e] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, off + 16 * e, 0, 0));
+                    for (int e = 0; e < 2; e++)
+                        raw[i][e] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, off + 16 * e, 0, 0));
                 }
             };
             auto put = [&](unsigned char* buf) {
@@ -1023,7 +1054,8 @@ if constexpr (W::HALVES) {
                     unsigned int z[4][3];
 #pragma unroll
                     for (int e = 0; e < 4; e++) split2(raw[i][e >> 1][2 * (e & 1)], raw[i][e >> 1][2 * (e & 1) + 1], z[e]);
-                    unsigned char* to = buf + part * 3 * T3::PLANE + row * T3::ROWB + 16 * (part ? v_place<TERMS3, C3>(row, c) : k_place<C3>(row, c));
+                    unsigned char* to = buf + part * 3 * T3::PLANE + row * T3::ROWB +
+                                        16 * (part ? v_place<TERMS3, C3>(row, c) : k_place<C3>(row, c));
 #pragma unroll
                     for (int w = 0; w < 3; w++) *(u32x4*)(to + w * T3::PLANE) = u32x4{z[0][w], z[1][w], z[2][w], z[3][w]};
                 }
@@ -1046,11 +1078,14 @@ if constexpr (W::HALVES) {
 
         constexpr int REC = HDP + 4, SC1 = 16;
         const int part_bytes = nrows * REC * 4, quads = HD / 4;
-        const auto recs = __builtin_amdgcn_make_buffer_rsrc(
-            (void*)scalar((const char*)(a.rec + ((size_t)it.rec + (size_t)it.parts * ((size_t)rows_all * it.kh + r0)) * REC)), 0,
-            scalar(parts * part_bytes), 0x00027000);
+        const auto recs = rsrc((const char*)(a.rec + ((size_t)it.rec + (size_t)it.parts * ((size_t)rows_all * it.kh + r0)) * REC),
+                               parts * part_bytes);
+        auto four = [&](int d, int e) __attribute__((always_inline)) {
+            return f32x4{acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]};
+        };
         auto put = [&](int row, int quad, f32x4 x) __attribute__((always_inline)) {
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), recs, it.part * part_bytes + (quad * nrows + row) * 16, 0, SC1);
+            const int at = it.part * part_bytes + (quad * nrows + row) * 16;
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), recs, at, 0, SC1);
         };
         /* four outputs of a row, of its sums */
         auto finish = [&](int row, int quad, f32x4 x, float sum) __attribute__((always_inline)) {
@@ -1067,7 +1102,11 @@ if constexpr (W::HALVES) {
             constexpr int SUMS = HDP * 128;
             static_assert(SUMS <= W::ALONE_BYTES, "");
             auto place = [&](int w) {
-                return (f32x4*)(W::ARRAYS == 1 ? lds0 + w * W::ALONE_BYTES : w == 0 ? lds0 : w == 1 ? lds1 : w == 2 ? lds2 : lds3);
+                return (f32x4*)(W::ARRAYS == 1 ? lds0 + w * W::ALONE_BYTES
+                                : w == 0       ? lds0
+                                : w == 1       ? lds1
+                                : w == 2       ? lds2
+                                               : lds3);
             };
             if (mine) {
                 f32x4* mem = place(wave) + col;
@@ -1075,7 +1114,7 @@ if constexpr (W::HALVES) {
                 for (int d = 0; d < DT; d++)
 #pragma unroll
                     for (int e = 0; e < 16; e += 4)
-                        mem[(8 * d + e / 2 + half) * 32] = f32x4{acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]};
+                        mem[(8 * d + e / 2 + half) * 32] = four(d, e);
                 if (half == 0) {
                     part_m[wave][col] = m;
                     part_l[wave][col] = l;
@@ -1110,7 +1149,7 @@ if constexpr (W::HALVES) {
                 for (int d = 0; d < DT; d++)
 #pragma unroll
                     for (int e = 0; e < 16; e += 4)
-                        if (32 * d + 2 * e + 4 * half < HD) finish(r - r0, 8 * d + e / 2 + half, f32x4{acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]}, l);
+                        if (32 * d + 2 * e + 4 * half < HD) finish(r - r0, 8 * d + e / 2 + half, four(d, e), l);
             }
             return;
         } else if (mine) {
@@ -1118,7 +1157,7 @@ if constexpr (W::HALVES) {
             for (int d = 0; d < DT; d++)
 #pragma unroll
                 for (int e = 0; e < 16; e += 4)
-                    if (32 * d + 2 * e + 4 * half < HD) put(r - r0, 8 * d + e / 2 + half, f32x4{acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]});
+                    if (32 * d + 2 * e + 4 * half < HD) put(r - r0, 8 * d + e / 2 + half, four(d, e));
             if (half == 0) put(r - r0, HDP / 4, f32x4{m, l, 0.0f, 0.0f});
         }
         /* Records cross XCDs: they are written and read past the XCDs' own L2s (sc1), and each wave waits for its stores before
@@ -1143,10 +1182,14 @@ if constexpr (W::HALVES) {
         const int across = NT / nrows, each = (quads + across - 1) / across;
         int by_log = 0;
         while (by_log < 6 && nrows * quads << (by_log + 1) <= NT && 4 << by_log < parts) by_log++;
+        auto take = [&](int at) __attribute__((always_inline)) {
+            return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(recs, at, 0, SC1));
+        };
         auto join = [&](auto us, auto ps) __attribute__((always_inline)) {
             constexpr int U = decltype(us)::value, P = decltype(ps)::value;
             const int sub = U == 1 ? t & ((1 << by_log) - 1) : 0, x = U == 1 ? t >> by_log : t;
-            const int col0 = x / nrows, row = x - col0 * nrows, apart = (NT >> by_log) / nrows; /* this lane's quads: col0, col0 + apart, .. */
+            /* this lane's quads: col0, col0 + apart, .. */
+            const int col0 = x / nrows, row = x - col0 * nrows, apart = (NT >> by_log) / nrows;
             if (col0 >= (U == 1 ? quads : across)) return;
             for (int q0 = col0; q0 < quads; q0 += U * apart) {
                 f32x4 o[U];
@@ -1158,11 +1201,11 @@ if constexpr (W::HALVES) {
 #pragma unroll
                     for (int e = 0; e < P; e++) { /* past the parts: the descriptor's end, zeros */
                         const int at = (i + (e << by_log)) * part_bytes + row * 16;
-                        ml[e] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(recs, at + HDP / 4 * nrows * 16, 0, SC1));
+                        ml[e] = take(at + HDP / 4 * nrows * 16);
 #pragma unroll
                         for (int u = 0; u < U; u++) {
                             const int quad = min(q0 + u * apart, quads - 1);
-                            y[e][u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(recs, at + quad * nrows * 16, 0, SC1));
+                            y[e][u] = take(at + quad * nrows * 16);
                         }
                     }
                     float mn = mx;
@@ -1288,7 +1331,8 @@ int launch_attn_paged(const bmk_launch_t* l, bool bf16) {
     a.flip = std::signbit(scale) ? 0x80000000u : 0u;
     a.scale2 = fabsf(scale) * 1.44269504088896341f;
     int two;
-    a.far_scale2 = a.scale2 < INFINITY && frexpf(a.scale2, &two) > 0.5f ? ldexpf(1.0f, two) : a.scale2; /* 0 and the powers of two are their own */
+    /* 0 and the powers of two are their own */
+    a.far_scale2 = a.scale2 < INFINITY && frexpf(a.scale2, &two) > 0.5f ? ldexpf(1.0f, two) : a.scale2;
     if (HD <= 64) return bf16 ? start<true, 64>(a, l) : start<false, 64>(a, l);
     if (HD <= 128) return bf16 ? start<true, 128>(a, l) : start<false, 128>(a, l);
     return bf16 ? start<true, 256>(a, l) : start<false, 256>(a, l);
