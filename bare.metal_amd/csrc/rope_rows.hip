@@ -254,7 +254,13 @@ __global__ __launch_bounds__(NT) void k_rope_rows(RopeArgs a) {
     for (int i = 0; i < UN; i++) {
         const int u = lane + (i << a.lp_log);
         if (u >= a.units) continue;
-        if (kind < 2 && 2 * E * u < a.rot) {
+        const bool turned = kind < 2 && 2 * E * u < a.rot;
+        if (BF16 && !turned && (kind == 2 || !a.gain)) { /* every bit of it: a conversion would make other NaNs */
+#pragma unroll
+            for (int j = 0; j < 2; j++) *(Chunk<BF16, E>*)((char*)dst + (to + at(i, j)) * 2) = raw[i][j];
+            continue;
+        }
+        if (turned) {
             float cs[E], sn[E];
             __builtin_memcpy(cs, __builtin_assume_aligned(tc + row * half + E * u, E * 4 < 16 ? E * 4 : 16), sizeof cs);
             __builtin_memcpy(sn, __builtin_assume_aligned(ts + row * half + E * u, E * 4 < 16 ? E * 4 : 16), sizeof sn);

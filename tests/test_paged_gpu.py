@@ -512,6 +512,37 @@ def test_kv_append_skips_what_has_no_place(be, kind):
 
 
 @both
+@pytest.mark.parametrize("norm", [0, 1], ids=["plain", "norm"])
+@pytest.mark.parametrize("HD,rot,layout,ld", [(64, 32, 0, 64), (64, 32, 1, 64), (8, 0, 0, 8), (40, 8, 0, 41), (256, 64, 1, 258)])
+def test_what_passes_unturned_keeps_every_bit(be, HD, rot, layout, ld, norm, kind):
+    """v, and without the norm q's and k's elements from rot on, of every pattern of bits that bf16 has (and as many of fp32),
+    NaNs that signal among them."""
+    rng = np.random.default_rng(HD)
+    n, page = 65536 // HD + 5, 64
+    turn = np.arange(HD) < rot
+    bits = np.resize(rng.permutation(1 << 16).astype(np.uint16), n * HD).reshape(n, HD)
+    if not kind.bf16:
+        bits = bits.astype(np.uint32) << 16 | rng.integers(0, 1 << 16, (n, HD)).astype(np.uint32)
+    x = np.where(turn, kind.raw(rng.standard_normal((n, HD))).view(bits.dtype), bits)
+    table, m = turn_table(rot, "none")
+    src = np.zeros((n, ld), bits.dtype)
+    src[:, :HD] = x
+    vsrc = np.zeros((n, ld), bits.dtype)
+    vsrc[:, :HD] = bits
+    width = -(-n // page)
+    cache, out = be.alloc(width * 2 * page * HD * kind.size), be.alloc(n * ld * kind.size)
+    assert be.dispatch("kv_append_paged" + kind.suffix, [
+        be.upload(src), be.upload(src), be.upload(vsrc), out, cache, be.upload(np.int32([0, n])), be.upload(np.int32([n])),
+        be.upload(np.arange(width, dtype=np.int32)), be.upload(table), be.upload(np.ones((2, HD), np.float32)),
+        be.params(n, 1, 1, 1, HD, rot, layout, ld, ld, ld, ld, page, width, width, norm), floats(be, m, 1e-5)], (n,), (256,)) == 0
+    raw = cache.read(bits.dtype).reshape(width, 2, page, HD)
+    assert np.array_equal(raw[:, 1].reshape(-1, HD)[:n], bits)
+    if not norm:
+        assert np.array_equal(raw[:, 0].reshape(-1, HD)[:n, ~turn], bits[:, ~turn])
+        assert np.array_equal(out.read(bits.dtype).reshape(n, ld)[:, :HD][:, ~turn], bits[:, ~turn])
+
+
+@both
 @pytest.mark.parametrize("S", [65, 1000, 4096])
 def test_kv_append_of_many_sequences(be, S, kind):
     """As many sequences as a batch takes, some without tokens, in a call of more rows than a workgroup has: every row is in its place."""
