@@ -35,11 +35,11 @@
  * keys, 5 heads of 64, 124 (5.4).  Few keys: the chain of latencies (the tables 1-2, the
  * page's number and the first keys 2.5, a tile 1.5, the waves' join 0.7, records and counter
  * 0.9, the parts' join 2.1); 300 keys of one token 10 of kernel time.  Long chunks: 2048 tokens
- * over 16384 keys, 32 heads of 128, 605-640, 515 GFLOP at 0.80-0.85 PFLOP/s: a tile
- * takes 512 cycles of the matrix cores and some 600 of exponentials and other vector
- * instructions, which two waves a SIMD overlap in part, at 1.7 GHz (the part's power; the
- * library's 8192^3 product runs at 1.16 PFLOP/s).  fp32: 512 tokens over 4096 keys, 15 heads of 64,
- * 57-64: 43 thousand cycles a SIMD of the matrix cores, 44 thousand of vector instructions.
+ * over 16384 keys, 32 heads of 128, 605-640, 515 GFLOP at 0.80-0.85 PFLOP/s (the
+ * library's 8192^3 product runs at 1.16): a tile takes 512 cycles of the matrix cores and
+ * some 600 of exponentials and other vector instructions, one after the other in a wave, which
+ * two waves a SIMD overlap in part (35% and 45% busy).  fp32: 512 tokens over 4096 keys, 15 heads of 64,
+ * 59-66: 43 thousand cycles a SIMD of the matrix cores, 44 thousand of vector instructions.
  */
 #include "paged.h"
 #include "q8_common.h"

@@ -11,11 +11,11 @@
  * output may be its input's buffer).
  *
  * HBM bounds the large calls (us, MI355X): 4096 rows of 40 heads of 128 in
- * bf16 18.3 (4.6 TB/s; chunks of 4 bytes in place of 16 32), norms of them in
- * fp32 33 (5.1; with the norm's root and gains by every lane from memory 59),
- * 16 chunks of 32 + 16 heads to their pages 26 (3.5: heads of 256 bytes to
- * places of their own; cos and sin by every head 43).  Small ones take 2 to 4,
- * a launch and two loads on end.
+ * bf16 15.1 (5.6 TB/s; chunks of 4 bytes in place of 16 32), norms of them in
+ * fp32 33 (5.1; with the norm's root and gains by every lane from memory 59).
+ * 16 chunks of 32 + 16 heads to their pages take 24.6 (3.8 TB/s; cos and sin by
+ * every head 43): 17.4 the turning, 2 to 3 the norms, 2 each the lookups of
+ * sequences and of pages.  Small ones take 2 to 4, a launch and two loads on end.
  */
 #include "paged.h"
 
