@@ -154,6 +154,14 @@ def test_rope_rows(be, N, NH, HD, rot, layout, kind):
 
 @both
 @pytest.mark.parametrize("layout", [0, 1], ids=["halves", "pairs"])
+@pytest.mark.parametrize("N,NH,HD,rot", [(3, 5000, 2, 2), (2, 3000, 64, 32)])
+def test_rope_rows_of_many_heads(be, N, NH, HD, rot, layout, kind):
+    """Rows that several workgroups share."""
+    test_rope_rows(be, N, NH, HD, rot, layout, kind)
+
+
+@both
+@pytest.mark.parametrize("layout", [0, 1], ids=["halves", "pairs"])
 def test_rows_past_the_cache_have_the_same_bits(be, layout, kind):
     """A call of more than 128 MB, which reads past the caches, against its rows in calls of fewer; in place as well."""
     NH, NKV, HD, rot = 4, 2, 128, 128
@@ -979,6 +987,22 @@ def test_attention_masks_over_keys_in_parts(be, causal, window, new, total, NH, 
     scale = float(np.float32(HD ** -0.5))
     want, off = attend(b, q, NH, scale, causal, window)
     compare(b, attention(be, b, q, NH, scale, causal, window), want, off)
+
+
+@both
+@pytest.mark.parametrize("NH,NKV,HD", [(129, 1, 64), (300, 1, 8), (1100, 1, 128), (1200, 300, 8), (4096, 4096, 8)])
+@pytest.mark.parametrize("new,total,window", [([1], [40], 0), ([3, 1], [130, 20], 0), ([2, 2], [700, 9], 60)])
+def test_attention_of_many_heads(be, new, total, window, NH, NKV, HD, kind):
+    """Groups of more heads than a unit has rows, so that a token's lie in several of them, and as many KV heads as there may be."""
+    rng = np.random.default_rng(NH + sum(total))
+    if NKV > 1000:
+        new, total = new[:1], [min(total[0], 60)]
+    b = Batch(be, rng, kind, new, total, 16, NKV, HD)
+    b.fill(rng)
+    q = kind.held(rng.standard_normal((b.N, NH, HD)))
+    scale = float(np.float32(HD ** -0.5))
+    want, off = attend(b, q, NH, scale, 1, window)
+    compare(b, attention(be, b, q, NH, scale, 1, window), want, off)
 
 
 @both
